@@ -13,6 +13,7 @@ source is newer than the output, unless force=True.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -25,15 +26,21 @@ PKG = os.path.join(HERE, "kernel_opt")
 LIBDIR = os.path.join(PKG, "lib")
 INCLUDE = os.path.join(REPO, "include")
 
-CAPI_SOURCES = ["k1_capi.cu", "k1_kernels.cuh", "k1_common.cuh", "k1_ring.cuh", "k1_fwd_sm.cuh",
-                "k1_lmhead.cuh"]
+# translation units of the C-ABI library and the headers each includes
+CAPI_UNITS = {
+    "k1_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_tc.cuh", "k1_kernels.cuh",
+                   "k1_ring.cuh", "k1_fwd_sm.cuh", "k1_lmhead.cuh"],
+    "k1_decode_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_tc.cuh",
+                          "k1_norm.cuh", "k1_fp8_linear.cuh", "k1_sample.cuh"],
+}
+OBJDIR = os.path.join(HERE, "build")
 CAPI_LIB = os.path.join(LIBDIR, "libk1_b200.so")
 BINDING_SOURCE = "k1_torch_binding.cpp"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -57,16 +64,28 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"build step failed: {' '.join(cmd[:3])} ... (exit {r.returncode})")
 
 
-def build_capi(force: bool = False, verbose_ptxas: bool = False) -> str:
-    srcs = [os.path.join(CSRC, s) for s in CAPI_SOURCES] + [os.path.join(INCLUDE, "k1_logprob.h")]
-    if force or _stale(CAPI_LIB, srcs):
-        os.makedirs(LIBDIR, exist_ok=True)
-        cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, os.path.join(CSRC, "k1_capi.cu"),
-               "-o", CAPI_LIB]
-        if verbose_ptxas:
-            cmd.insert(1, "-Xptxas=-v")
-        _run(cmd)
-    return CAPI_LIB
+def _build_lib(out: str, tag: str, flags: list[str], force: bool) -> str:
+    """Compile the stale translation units (in parallel) and link them into `out`."""
+    header = os.path.join(INCLUDE, "k1_logprob.h")
+    os.makedirs(LIBDIR, exist_ok=True)
+    os.makedirs(OBJDIR, exist_ok=True)
+    cmds, objs = [], []
+    for unit, headers in CAPI_UNITS.items():
+        obj = os.path.join(OBJDIR, f"{os.path.splitext(unit)[0]}{tag}.o")
+        objs.append(obj)
+        srcs = [os.path.join(CSRC, s) for s in (unit, *headers)] + [header]
+        if force or _stale(obj, srcs):
+            cmds.append([_nvcc(), *NVCC_FLAGS, *flags, "-c", "-I", INCLUDE,
+                         os.path.join(CSRC, unit), "-o", obj])
+    if cmds or _stale(out, objs):
+        with concurrent.futures.ThreadPoolExecutor(len(cmds) or 1) as pool:
+            list(pool.map(_run, cmds))
+        _run([_nvcc(), *NVCC_FLAGS, "-shared", *objs, "-o", out])
+    return out
+
+
+def build_capi(force: bool = False) -> str:
+    return _build_lib(CAPI_LIB, "", [], force)
 
 
 # The wait-timeout test library: the same C ABI built with short wait limits and the
@@ -78,12 +97,7 @@ WAIT_TEST_FLAGS = ["-DK1_WAIT_TEST", "-DK1_RING_MAX_TRIES=16", "-DK1_SM_MAX_POLL
 
 
 def build_wait_test_lib(force: bool = False) -> str:
-    srcs = [os.path.join(CSRC, s) for s in CAPI_SOURCES] + [os.path.join(INCLUDE, "k1_logprob.h")]
-    if force or _stale(WAIT_TEST_LIB, srcs):
-        os.makedirs(LIBDIR, exist_ok=True)
-        _run([_nvcc(), *NVCC_FLAGS, *WAIT_TEST_FLAGS, "-I", INCLUDE,
-              os.path.join(CSRC, "k1_capi.cu"), "-o", WAIT_TEST_LIB])
-    return WAIT_TEST_LIB
+    return _build_lib(WAIT_TEST_LIB, "_waittest", WAIT_TEST_FLAGS, force)
 
 
 def binding_path() -> str:
@@ -118,9 +132,12 @@ def build_binding(force: bool = False) -> str:
 
 
 def build(force: bool = False) -> None:
-    build_capi(force=force)
+    # the two libraries compile side by side
+    with concurrent.futures.ThreadPoolExecutor(2) as pool:
+        libs = [pool.submit(build_capi, force), pool.submit(build_wait_test_lib, force)]
+        for lib in libs:
+            lib.result()
     build_binding(force=force)
-    build_wait_test_lib(force=force)
 
 
 if __name__ == "__main__":

@@ -20,51 +20,21 @@
 #include <utility>
 
 #include "k1_fwd_sm.cuh"
+#include "k1_host.cuh"
 #include "k1_lmhead.cuh"
 
 namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int code, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    g_last_error = buf;
+}  // namespace
+
+int k1_host_fail(int code, const char* message) {
+    g_last_error = message;
     return code;
 }
 
-#ifndef K1_PDL
-#define K1_PDL 1
-#endif
-
-// Launch with programmatic stream serialization (see pdl_wait / pdl_trigger): the grid
-// may be scheduled while the previous kernel of the stream drains; it waits for that
-// kernel's completion on the device before touching memory.
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), int64_t grid, int block, size_t smem,
-                   cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = K1_PDL ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-int check_launch(const char* what) {
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess)
-        return fail(K1_ERR_CUDA, "%s: kernel launch failed: %s", what, cudaGetErrorString(e));
-    return K1_OK;
-}
+namespace {
 
 #ifndef K1_FWD_THREADS
 #define K1_FWD_THREADS 256
@@ -93,7 +63,6 @@ constexpr bool kRingFwd = K1_RING_FWD != 0; // bulk-copy ring forward on the vec
 constexpr int kRingWarps = K1_RING_WARPS;   // consumer warps per block (+1 producer warp)
 constexpr int kRingStages = K1_RING_STAGES;
 constexpr int kRingBytes = K1_RING_BYTES;   // bytes per ring stage
-constexpr int kMaxDevices = 64;
 constexpr int kMaxBlocksPerSm = 8;   // grid cap
 // Forward dynamic tail: the last (1 - K1_FWD_STATIC_NUM / K1_FWD_STATIC_DEN) of the units
 // are cut into chunks that blocks take once their static piece is done -- whole rows,
@@ -174,28 +143,6 @@ template <bool SCALED>
 constexpr bool kSmPrefetch = SCALED ? (K1_SM_PREFETCH_SCALED != 0) : (K1_SM_PREFETCH != 0);
 constexpr int64_t kMinUnitsPerBlockVec = (int64_t)kThreads * kUnroll;
 constexpr int64_t kMinUnitsPerBlockScalar = (int64_t)kThreads * 64;
-
-int elem_size(int dtype) { return dtype == K1_DTYPE_F32 ? 4 : 2; }
-
-int current_device(int* dev) {
-    cudaError_t e = cudaGetDevice(dev);
-    if (e != cudaSuccess) return fail(K1_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
-    if (*dev < 0 || *dev >= kMaxDevices) return fail(K1_ERR_CUDA, "device ordinal %d out of range", *dev);
-    return K1_OK;
-}
-
-int sm_count(int dev, int* out) {
-    static std::atomic<int> cache[kMaxDevices];
-    int v = cache[dev].load(std::memory_order_relaxed);
-    if (v == 0) {
-        cudaError_t e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-        if (e != cudaSuccess)
-            return fail(K1_ERR_CUDA, "cudaDeviceGetAttribute(SM count): %s", cudaGetErrorString(e));
-        cache[dev].store(v, std::memory_order_relaxed);
-    }
-    *out = v;
-    return K1_OK;
-}
 
 // Resident blocks per SM of one kernel instance, cached per (device, kernel).  Kernels
 // with more than 48 KB of dynamic shared memory get the opt-in attribute set here, once
@@ -565,29 +512,6 @@ int check_common(const char* fn, const void* logits, int dtype, const Rows& L) {
 // ---------------------------------------------------------------------------------------
 // LM head fused with K1 (k1_lmhead.cuh): tensor maps, work split, launches
 // ---------------------------------------------------------------------------------------
-using TmapEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled from the driver, looked up through the runtime (no link-time
-// dependency on libcuda).
-int tmap_encoder(TmapEncodeFn* out) {
-    static std::once_flag once;
-    static TmapEncodeFn fn = nullptr;
-    std::call_once(once, [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<TmapEncodeFn>(f);
-    });
-    if (!fn) return fail(K1_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    *out = fn;
-    return K1_OK;
-}
-
 // Row-major bf16 [rows, cols] matrix read in boxes of box_rows x 64 with 128-byte swizzle.
 int make_tmap(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows,
               const char* what) {
@@ -895,6 +819,9 @@ int k1_ring_status(unsigned* out) {
     unsigned v = 0, zero = 0;
     cudaError_t e = cudaMemcpyFromSymbol(&v, k1::k1_ring_error, sizeof v);
     if (e == cudaSuccess) e = cudaMemcpyToSymbol(k1::k1_ring_error, &zero, sizeof zero);
+    unsigned more = 0;
+    if (e == cudaSuccess) e = k1_decode_wait_status(&more);
+    v |= more;
     if (e != cudaSuccess) return fail(K1_ERR_CUDA, "k1_ring_status: %s", cudaGetErrorString(e));
     if (out) *out = v;
     return K1_OK;
@@ -1266,6 +1193,7 @@ int k1_lm_head_shard_backward(const void* hidden, const void* weight_shard, int6
 int k1_test_set_knobs(long long withhold, long long skip_grab) {
     cudaError_t e = cudaMemcpyToSymbol(k1::k1_test_withhold, &withhold, sizeof withhold);
     if (e == cudaSuccess) e = cudaMemcpyToSymbol(k1::k1_test_skip_grab, &skip_grab, sizeof skip_grab);
+    if (e == cudaSuccess) e = k1_decode_set_withhold(withhold);
     if (e != cudaSuccess) return fail(K1_ERR_CUDA, "k1_test_set_knobs: %s", cudaGetErrorString(e));
     return K1_OK;
 }

@@ -1,0 +1,548 @@
+// k1_decode_capi.cu -- extern "C" entry points of the decoding-step operators (declared in
+// include/k1_logprob.h): residual RMS norm, 8-bit product, token sampling.  Argument
+// validation, kernel choice, launches.
+#include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
+#include <utility>
+
+#include "k1_fp8_linear.cuh"
+#include "k1_host.cuh"
+#include "k1_norm.cuh"
+#include "k1_sample.cuh"
+
+cudaError_t k1_decode_wait_status(unsigned* bits) {
+    unsigned zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(bits, k1::k1_ring_error, sizeof *bits);
+    if (e == cudaSuccess) e = cudaMemcpyToSymbol(k1::k1_ring_error, &zero, sizeof zero);
+    return e;
+}
+
+#ifdef K1_WAIT_TEST
+cudaError_t k1_decode_set_withhold(long long withhold) {
+    return cudaMemcpyToSymbol(k1::k1_test_withhold, &withhold, sizeof withhold);
+}
+#endif
+
+namespace {
+
+bool known_dtype(int d) { return d == K1_DTYPE_F32 || d == K1_DTYPE_F16 || d == K1_DTYPE_BF16; }
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Opt in to `smem` bytes of dynamic shared memory, once per device and kernel (the largest
+// asked for so far).
+template <typename Kernel>
+int allow_smem(Kernel kernel, int dev, size_t smem) {
+    static std::mutex mu;
+    static std::map<std::pair<int, const void*>, size_t> cache;
+    std::lock_guard<std::mutex> lock(mu);
+    size_t& have = cache[std::make_pair(dev, reinterpret_cast<const void*>(kernel))];
+    if (smem <= have) return K1_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(K1_ERR_CUDA, "cudaFuncSetAttribute(smem): %s", cudaGetErrorString(e));
+    have = smem;
+    return K1_OK;
+}
+
+// `launch` with a cluster of `cluster` blocks along x.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, int cluster,
+                           cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = K1_PDL ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+int launched(const char* fn, cudaError_t e) {
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(K1_ERR_CUDA, "%s: kernel launch failed: %s", fn, cudaGetErrorString(e));
+    }
+    return K1_OK;
+}
+
+// ---------------------------------------------------------------------------------------
+// Residual RMS norm
+// ---------------------------------------------------------------------------------------
+// Threads and pieces per thread of a row of `hidden` elements; nv is one of the kernel's
+// instances (vectors: 1, 2, 4 or 8; single elements: 4 or 32).
+struct NormShape {
+    bool vec;
+    int nv, threads;
+};
+
+NormShape norm_shape(int hidden, int es, bool vec) {
+    const int pieces = vec ? hidden * es / 16 : hidden;
+    NormShape s;
+    s.vec = vec;
+    if (vec) {
+        s.nv = 1;
+        while (s.nv < 8 && pieces > 256 * s.nv && (s.nv < 2 || pieces > 512 * s.nv)) s.nv *= 2;
+    } else {
+        s.nv = pieces <= 4 * k1::norm::kMaxThreads ? 4 : 32;
+    }
+    // whole groups of 128 threads, so that single elements' blocks of 128 are whole warps
+    const int unit = vec ? 32 : 128;
+    s.threads = std::max(unit, (pieces + s.nv - 1) / s.nv);
+    s.threads = (s.threads + unit - 1) / unit * unit;
+    return s;
+}
+
+// Blocks that fill the device: as many as are resident at 2048 threads per SM, or the
+// rows if there are fewer.
+int64_t norm_grid(int64_t n, int threads, int sms, int most_per_sm) {
+    const int per_sm = std::max(1, std::min(most_per_sm, 2048 / threads));
+    return std::min<int64_t>(n, (int64_t)sms * per_sm);
+}
+
+template <typename T, int OUT>
+cudaError_t norm_launch(const k1::norm::FwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
+    using namespace k1::norm;
+    if (!s.vec)
+        return s.nv == 4 ? launch(k1_rmsnorm_kernel<T, false, 4, OUT>, grid, s.threads, 0, st, p)
+                         : launch(k1_rmsnorm_kernel<T, false, 32, OUT>, grid, s.threads, 0, st, p);
+    switch (s.nv) {
+        case 1: return launch(k1_rmsnorm_kernel<T, true, 1, OUT>, grid, s.threads, 0, st, p);
+        case 2: return launch(k1_rmsnorm_kernel<T, true, 2, OUT>, grid, s.threads, 0, st, p);
+        case 4: return launch(k1_rmsnorm_kernel<T, true, 4, OUT>, grid, s.threads, 0, st, p);
+        default:
+            if constexpr (sizeof(T) == 4)
+                return launch(k1_rmsnorm_kernel<T, true, 8, OUT>, grid, s.threads, 0, st, p);
+            return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T>
+cudaError_t norm_bwd_launch(const k1::norm::BwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
+    using namespace k1::norm;
+    if (!s.vec)
+        return s.nv == 4 ? launch(k1_rmsnorm_bwd_kernel<T, false, 4>, grid, s.threads, 0, st, p)
+                         : launch(k1_rmsnorm_bwd_kernel<T, false, 32>, grid, s.threads, 0, st, p);
+    switch (s.nv) {
+        case 1: return launch(k1_rmsnorm_bwd_kernel<T, true, 1>, grid, s.threads, 0, st, p);
+        case 2: return launch(k1_rmsnorm_bwd_kernel<T, true, 2>, grid, s.threads, 0, st, p);
+        case 4: return launch(k1_rmsnorm_bwd_kernel<T, true, 4>, grid, s.threads, 0, st, p);
+        default:
+            if constexpr (sizeof(T) == 4)
+                return launch(k1_rmsnorm_bwd_kernel<T, true, 8>, grid, s.threads, 0, st, p);
+            return cudaErrorInvalidValue;
+    }
+}
+
+int norm_check(const char* fn, int dtype, int weight_dtype, int64_t n_rows, int64_t hidden) {
+    if (!known_dtype(dtype))
+        return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: dtype must be bf16, fp16, or fp32", fn);
+    if (weight_dtype != dtype && weight_dtype != K1_DTYPE_F32)
+        return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: the weight must have the inputs' dtype or fp32", fn);
+    if (n_rows < 0) return fail(K1_ERR_INVALID_ARGUMENT, "%s: n_rows must be >= 0", fn);
+    if (hidden < 1 || hidden > k1::norm::kMaxHidden)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: hidden must be in [1, %d], got %lld", fn,
+                    k1::norm::kMaxHidden, (long long)hidden);
+    return K1_OK;
+}
+
+// Whether the rows of a matrix are whole 16-byte vectors at 16-byte addresses.
+bool rows_vec(const void* p, int64_t stride, int64_t n, int es) {
+    return !p || (aligned(p, 16) && (n <= 1 || (stride * es) % 16 == 0));
+}
+
+// What the backward's grid takes of the SM: three streams of vectors in flight per thread
+// and as few partial rows of dw as keep the loads going.
+constexpr int kBwdBlocksPerSm = 4;
+
+int64_t norm_bwd_grid(int64_t n, int threads, int sms) { return norm_grid(n, threads, sms, kBwdBlocksPerSm); }
+
+int norm_forward(const char* fn, int out, const void* x, int64_t x_stride, const void* r, int64_t r_stride,
+                 const void* w, int weight_dtype, int dtype, int64_t n, int64_t hidden, float eps, void* s,
+                 void* y, float* scales, float* rstd, cudaStream_t st) {
+    const bool only = out == k1::norm::FP8_ONLY;
+    int rc = norm_check(fn, dtype, only ? dtype : weight_dtype, n, hidden);
+    if (rc) return rc;
+    if (!only && (!(eps > 0.f) || !std::isfinite(eps)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: eps must be positive and finite", fn);
+    if (n == 0) return K1_OK;
+    if (!x || !y || (!only && !w) || (r && !s) || (out != k1::norm::SAME && !scales))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: NULL pointer argument", fn);
+    const int es = elem_size(dtype);
+    if (n > 1 && (x_stride < 0 || (r && r_stride < 0)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: strides must be >= 0", fn);
+    if (!aligned(x, es) || !aligned(r, es) || !aligned(s, es) || (out == k1::norm::SAME && !aligned(y, es)) ||
+        (w && !aligned(w, weight_dtype == K1_DTYPE_F32 ? 4 : es)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element size", fn);
+    int dev = 0, sms = 0;
+    rc = current_device(&dev);
+    if (!rc) rc = sm_count(dev, &sms);
+    if (rc) return rc;
+    const bool vec = (hidden * es) % 16 == 0 && rows_vec(x, x_stride, n, es) && rows_vec(r, r_stride, n, es) &&
+                     aligned(w, 16) && aligned(s, 16) && aligned(y, 16);
+    const NormShape sh = norm_shape((int)hidden, es, vec);
+    k1::norm::FwdParams p = {};
+    p.x = x;
+    p.r = r;
+    p.w = w;
+    p.s = s;
+    p.y = y;
+    p.scales = scales;
+    p.rstd = rstd;
+    p.n = n;
+    p.x_stride = x_stride;
+    p.r_stride = r_stride;
+    p.h = (int)hidden;
+    p.w32 = weight_dtype == K1_DTYPE_F32;
+    p.eps = eps;
+    const int64_t grid = norm_grid(n, sh.threads, sms, 8);
+    auto go = [&](auto tag) {
+        using T = decltype(tag);
+        if (out == k1::norm::SAME) return norm_launch<T, k1::norm::SAME>(p, sh, grid, st);
+        if (out == k1::norm::FP8) return norm_launch<T, k1::norm::FP8>(p, sh, grid, st);
+        return norm_launch<T, k1::norm::FP8_ONLY>(p, sh, grid, st);
+    };
+    return launched(fn, dtype == K1_DTYPE_BF16  ? go(__nv_bfloat16{})
+                        : dtype == K1_DTYPE_F16 ? go(__half{})
+                                                : go(float{}));
+}
+
+// ---------------------------------------------------------------------------------------
+// 8-bit product
+// ---------------------------------------------------------------------------------------
+// Row-major 8-bit [rows, cols] matrix, rows `stride` bytes apart, read in boxes of
+// box_rows x 128 with 128-byte swizzle; what lies beyond it reads as zero.
+int make_tmap8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, int box_rows,
+               const char* what) {
+    TmapEncodeFn enc = nullptr;
+    int rc = tmap_encoder(&enc);
+    if (rc) return rc;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)k1::fp8::BK, (cuuint32_t)box_rows};
+    const cuuint32_t es[2] = {1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(K1_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed: %d", what, (int)r);
+    return K1_OK;
+}
+
+// Largest inner dimension: the few-token kernel keeps its scales (64 tokens) in shared memory.
+constexpr int64_t kMaxInner = 32768;
+
+template <int TN, typename OutT>
+int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
+           int64_t inner, int sms, int dev, cudaStream_t st) {
+    using S = k1::fp8::Skinny<TN>;
+    CUtensorMap tx, tw;
+    int rc = make_tmap8(&tx, x, p.m, inner, ldx, TN, "x");
+    if (!rc) rc = make_tmap8(&tw, w, p.n, inner, ldw, k1::fp8::BM, "weight");
+    if (rc) return rc;
+    const int64_t tiles = (p.n + 127) / 128, tok = (p.m + TN - 1) / TN;
+    // split K while the blocks do not fill the SMs twice and every part keeps two blocks of K
+    int split = 1;
+    while (split < 8 && tiles * tok * split < 2 * sms && p.kb_total >= 4 * split) split *= 2;
+    auto kern = k1::fp8::k1_fp8_skinny_kernel<TN, OutT>;
+    const size_t smem = S::smem((p.kb_total + split - 1) / split);
+    rc = allow_smem(kern, dev, smem);
+    if (rc) return rc;
+    const dim3 grid((unsigned)(tiles * split), (unsigned)tok);
+    return launched(fn, launch_cluster(kern, grid, S::THREADS, smem, split, st, tx, tw, p, split));
+}
+
+template <typename OutT>
+int wide(const char* fn, k1::fp8::Params p, const void* x, int64_t ldx, const void* w, int64_t ldw,
+         int64_t inner, int sms, int dev, cudaStream_t st) {
+    using S = k1::fp8::Wide;
+    CUtensorMap tx, tw;
+    int rc = make_tmap8(&tx, x, p.m, inner, ldx, k1::fp8::BM, "x");
+    if (!rc) rc = make_tmap8(&tw, w, p.n, inner, ldw, S::BN, "weight");
+    if (rc) return rc;
+    p.m_blocks = (int)((p.m + 127) / 128);
+    p.n_tiles = (int)((p.n + S::BN - 1) / S::BN);
+    auto kern = k1::fp8::k1_fp8_wide_kernel<OutT>;
+    rc = allow_smem(kern, dev, S::SMEM);
+    if (rc) return rc;
+    const int64_t grid = std::min<int64_t>(sms, (int64_t)p.m_blocks * p.n_tiles);
+    return launched(fn, launch(kern, grid, S::THREADS, (size_t)S::SMEM, st, tx, tw, p));
+}
+
+template <typename OutT>
+int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
+           int64_t inner, int sms, int dev, cudaStream_t st) {
+    if (p.m <= 16) return skinny<16, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+    if (p.m <= 32) return skinny<32, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+    const int64_t wide_tiles = (p.m + 127) / 128 * ((p.n + 255) / 256);
+    if (p.m <= 64 || wide_tiles < sms / 2)
+        return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+    return wide<OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+}
+
+// ---------------------------------------------------------------------------------------
+// Sampling
+// ---------------------------------------------------------------------------------------
+template <typename T>
+int sample_launch(const char* fn, k1::sample::Params p, int sms, int dev, cudaStream_t st) {
+    using namespace k1::sample;
+    constexpr int E = k1::DT<T>::kEPV;
+    // two blocks per SM while a row's part leaves room for them; a lone block takes up to
+    // kLone; a row that is longer still stays in global memory
+    constexpr int64_t kShared = 76 * 1024, kLone = 184 * 1024, kLeast = 8 * 1024;
+    const int64_t row_bytes = ((p.vocab + E - 1) / E + 1) * 16;  // one more for the shift
+    int cluster = 1;
+    while (cluster < kMaxCluster && row_bytes > cluster * kShared) cluster *= 2;
+    // few rows: more blocks per row, so that the SMs share the load
+    while (cluster < kMaxCluster && p.n_rows * cluster < sms && row_bytes > 2 * cluster * kLeast) cluster *= 2;
+    const int64_t vecs = (row_bytes / 16 + cluster - 1) / cluster;
+    if (vecs > (int64_t)1 << 30) return fail(K1_ERR_INVALID_ARGUMENT, "%s: vocab too large", fn);
+    p.cluster = cluster;
+    p.slice_vecs = (int)vecs;
+    const bool resident = vecs * 16 <= kLone;
+    const size_t base = (sizeof(Smem) + 15) & ~(size_t)15;
+    const size_t smem = base + (resident ? (size_t)vecs * 16 : 0);
+    auto kern = resident ? k1_sample_kernel<T, true> : k1_sample_kernel<T, false>;
+    int rc = allow_smem(kern, dev, smem);
+    if (rc) return rc;
+    const dim3 grid((unsigned)(p.n_rows * cluster));
+    return launched(fn, launch_cluster(kern, grid, THREADS, smem, cluster, st, p));
+}
+
+}  // namespace
+
+extern "C" {
+
+int k1_residual_rmsnorm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                        const void* weight, int weight_dtype, int dtype, int64_t n_rows, int64_t hidden,
+                        float eps, void* stream_out, void* y, float* rstd, void* stream) {
+    return norm_forward("k1_residual_rmsnorm", k1::norm::SAME, x, x_stride, residual, residual_stride, weight,
+                        weight_dtype, dtype, n_rows, hidden, eps, stream_out, y, nullptr, rstd,
+                        reinterpret_cast<cudaStream_t>(stream));
+}
+
+int k1_residual_rmsnorm_fp8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                            const void* weight, int weight_dtype, int dtype, int64_t n_rows, int64_t hidden,
+                            float eps, void* stream_out, void* q, float* scales, void* stream) {
+    return norm_forward("k1_residual_rmsnorm_fp8", k1::norm::FP8, x, x_stride, residual, residual_stride, weight,
+                        weight_dtype, dtype, n_rows, hidden, eps, stream_out, q, scales, nullptr,
+                        reinterpret_cast<cudaStream_t>(stream));
+}
+
+int k1_quantize_fp8_rows(const void* x, int64_t x_stride, int dtype, int64_t n_rows, int64_t hidden, void* q,
+                         float* scales, void* stream) {
+    return norm_forward("k1_quantize_fp8_rows", k1::norm::FP8_ONLY, x, x_stride, nullptr, 0, nullptr, dtype, dtype,
+                        n_rows, hidden, 0.f, nullptr, q, scales, nullptr, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int k1_quantize_fp8_blocks(const void* w, int64_t w_stride, int dtype, int64_t rows, int64_t cols, void* q,
+                           float* scales, void* stream) {
+    static const char* fn = "k1_quantize_fp8_blocks";
+    if (!known_dtype(dtype))
+        return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: dtype must be bf16, fp16, or fp32", fn);
+    if (rows < 0 || cols < 1) return fail(K1_ERR_INVALID_ARGUMENT, "%s: rows must be >= 0 and cols >= 1", fn);
+    if (rows > (int64_t)65535 * 128 || cols > (int64_t)65535 * 128)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: at most %lld rows and columns", fn, (long long)65535 * 128);
+    if (rows == 0) return K1_OK;
+    if (!w || !q || !scales) return fail(K1_ERR_INVALID_ARGUMENT, "%s: NULL pointer argument", fn);
+    if (w_stride < 0) return fail(K1_ERR_INVALID_ARGUMENT, "%s: strides must be >= 0", fn);
+    if (!aligned(w, elem_size(dtype)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element size", fn);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((cols + 127) / 128), (unsigned)((rows + 127) / 128));
+    cfg.blockDim = dim3(256);
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    auto go = [&](auto tag) {
+        using T = decltype(tag);
+        return cudaLaunchKernelEx(&cfg, k1::norm::k1_quantize_blocks_kernel<T>, reinterpret_cast<const T*>(w),
+                                  w_stride, rows, cols, reinterpret_cast<uint8_t*>(q), scales);
+    };
+    return launched(fn, dtype == K1_DTYPE_BF16  ? go(__nv_bfloat16{})
+                        : dtype == K1_DTYPE_F16 ? go(__half{})
+                                                : go(float{}));
+}
+
+size_t k1_residual_rmsnorm_workspace_bytes(int64_t n_rows, int64_t hidden, int device) {
+    int sms = 0;
+    if (n_rows < 0 || hidden < 1 || hidden > k1::norm::kMaxHidden || device < 0 || device >= kMaxDevices ||
+        sm_count(device, &sms) != K1_OK)
+        return 0;
+    return (size_t)std::min<int64_t>(std::max<int64_t>(n_rows, 1), (int64_t)sms * kBwdBlocksPerSm) *
+           (size_t)hidden * sizeof(float);
+}
+
+int k1_residual_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void* g_stream,
+                                 int64_t g_stream_stride, const void* stream_in, int64_t stream_stride,
+                                 const float* rstd, const void* weight, int weight_dtype, int dtype,
+                                 int64_t n_rows, int64_t hidden, void* d_x, void* d_weight, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    static const char* fn = "k1_residual_rmsnorm_backward";
+    int rc = norm_check(fn, dtype, weight_dtype, n_rows, hidden);
+    if (rc) return rc;
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int es = elem_size(dtype), ws = elem_size(weight_dtype);
+    if (n_rows == 0) {
+        if (d_weight) {
+            cudaError_t e = cudaMemsetAsync(d_weight, 0, (size_t)hidden * ws, st);
+            if (e != cudaSuccess) return fail(K1_ERR_CUDA, "%s: %s", fn, cudaGetErrorString(e));
+        }
+        return K1_OK;
+    }
+    if (!g_y || !stream_in || !rstd || !weight)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: NULL pointer argument", fn);
+    if (!d_x && !d_weight) return K1_OK;
+    if (n_rows > 1 && (g_y_stride < 0 || stream_stride < 0 || (g_stream && g_stream_stride < 0)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: strides must be >= 0", fn);
+    if (!aligned(g_y, es) || !aligned(g_stream, es) || !aligned(stream_in, es) || !aligned(d_x, es) ||
+        !aligned(weight, ws) || !aligned(d_weight, ws))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element size", fn);
+    int dev = 0, sms = 0;
+    rc = current_device(&dev);
+    if (!rc) rc = sm_count(dev, &sms);
+    if (rc) return rc;
+    const bool vec = (hidden * es) % 16 == 0 && rows_vec(g_y, g_y_stride, n_rows, es) &&
+                     rows_vec(g_stream, g_stream_stride, n_rows, es) &&
+                     rows_vec(stream_in, stream_stride, n_rows, es) && aligned(weight, 16) && aligned(d_x, 16);
+    const NormShape sh = norm_shape((int)hidden, es, vec);
+    const int64_t grid = norm_bwd_grid(n_rows, sh.threads, sms);
+    if (d_weight && (!workspace || !aligned(workspace, 16) ||
+                     workspace_bytes < (size_t)grid * hidden * sizeof(float)))
+        return fail(K1_ERR_WORKSPACE, "%s: the weight's gradient needs %zu bytes of 16-byte aligned workspace", fn,
+                    k1_residual_rmsnorm_workspace_bytes(n_rows, hidden, dev));
+    k1::norm::BwdParams p = {};
+    p.gy = g_y;
+    p.gs = g_stream;
+    p.s = stream_in;
+    p.rstd = rstd;
+    p.w = weight;
+    p.ds = d_x;
+    p.dw = d_weight ? reinterpret_cast<float*>(workspace) : nullptr;
+    p.n = n_rows;
+    p.gy_stride = g_y_stride;
+    p.gs_stride = g_stream_stride;
+    p.s_stride = stream_stride;
+    p.h = (int)hidden;
+    p.w32 = weight_dtype == K1_DTYPE_F32;
+    rc = launched(fn, dtype == K1_DTYPE_BF16  ? norm_bwd_launch<__nv_bfloat16>(p, sh, grid, st)
+                      : dtype == K1_DTYPE_F16 ? norm_bwd_launch<__half>(p, sh, grid, st)
+                                              : norm_bwd_launch<float>(p, sh, grid, st));
+    if (rc || !d_weight) return rc;
+    const int64_t blocks = (hidden + 31) / 32;
+    auto sum = [&](auto tag) {
+        using W = decltype(tag);
+        return launch(k1::norm::k1_rmsnorm_dw_kernel<W>, blocks, 512, 0, st, (const float*)p.dw, (int)grid,
+                      (int)hidden, reinterpret_cast<W*>(d_weight));
+    };
+    return launched(fn, weight_dtype == K1_DTYPE_BF16  ? sum(__nv_bfloat16{})
+                        : weight_dtype == K1_DTYPE_F16 ? sum(__half{})
+                                                       : sum(float{}));
+}
+
+int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const void* weight,
+                  int64_t weight_stride, const float* weight_scales, int64_t tokens, int64_t inner,
+                  int64_t outer, void* y, int64_t y_stride, int out_dtype, void* stream) {
+    static const char* fn = "k1_fp8_linear";
+    if (!known_dtype(out_dtype))
+        return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: the output's dtype must be bf16, fp16, or fp32", fn);
+    if (tokens < 0 || outer < 0) return fail(K1_ERR_INVALID_ARGUMENT, "%s: tokens and outer must be >= 0", fn);
+    if (inner < 16 || inner % 16 != 0 || inner > kMaxInner)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: inner must be a multiple of 16 in [16, %lld], got %lld", fn,
+                    (long long)kMaxInner, (long long)inner);
+    if (tokens > (int64_t)65535 * 64 || outer > (int64_t)1 << 27)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: tokens or outer too large", fn);
+    if (tokens == 0 || outer == 0) return K1_OK;
+    if (!x || !x_scales || !weight || !weight_scales || !y)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: NULL pointer argument", fn);
+    if (!aligned(x, 16) || !aligned(weight, 16) || x_stride % 16 != 0 || weight_stride % 16 != 0 ||
+        x_stride < inner || weight_stride < inner)
+        return fail(K1_ERR_INVALID_ARGUMENT,
+                    "%s: x and weight rows must start at multiples of 16 bytes and not overlap", fn);
+    if (y_stride < outer) return fail(K1_ERR_INVALID_ARGUMENT, "%s: y_stride must be >= outer", fn);
+    if (!aligned(y, elem_size(out_dtype)) || !aligned(x_scales, 4) || !aligned(weight_scales, 4))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element size", fn);
+    int dev = 0, sms = 0;
+    int rc = current_device(&dev);
+    if (!rc) rc = sm_count(dev, &sms);
+    if (rc) return rc;
+    k1::fp8::Params p = {};
+    p.xs = x_scales;
+    p.ws = weight_scales;
+    p.y = y;
+    p.m = tokens;
+    p.n = outer;
+    p.ldy = y_stride;
+    p.kb_total = (int)((inner + 127) / 128);
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (out_dtype) {
+        case K1_DTYPE_BF16:
+            return linear<__nv_bfloat16>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
+        case K1_DTYPE_F16:
+            return linear<__half>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
+        default:
+            return linear<float>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
+    }
+}
+
+int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                     const float* u, const k1_sampling* s, int64_t* token, float* logprob,
+                     float* kept_logprob, void* stream) {
+    static const char* fn = "k1_sample_tokens";
+    if (!known_dtype(dtype))
+        return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: logits dtype must be bf16, fp16, or fp32", fn);
+    if (n_rows < 0) return fail(K1_ERR_INVALID_ARGUMENT, "%s: n_rows must be >= 0", fn);
+    if (vocab < 1 || vocab > INT32_MAX)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: vocab must be in [1, 2^31)", fn);
+    if (n_rows > (INT32_MAX / k1::sample::kMaxCluster))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: too many rows", fn);
+    if (!s) return fail(K1_ERR_INVALID_ARGUMENT, "%s: NULL settings", fn);
+    if (!s->temperature_rows && !(s->temperature >= 0.0 && std::isfinite(s->temperature)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: temperature must be finite and >= 0", fn);
+    if (!s->top_p_rows && !(s->top_p >= 0.f))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: top_p must be >= 0", fn);
+    if (!s->min_p_rows && !(s->min_p >= 0.f && s->min_p <= 1.f))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: min_p must be in [0, 1]", fn);
+    if (n_rows == 0) return K1_OK;
+    if (!logits || !u || !token || !logprob || !kept_logprob)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: NULL pointer argument", fn);
+    if (n_rows > 1 && row_stride < 0) return fail(K1_ERR_INVALID_ARGUMENT, "%s: strides must be >= 0", fn);
+    if (!aligned(logits, elem_size(dtype)))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: logits not aligned to its element size", fn);
+    int dev = 0, sms = 0;
+    int rc = current_device(&dev);
+    if (!rc) rc = sm_count(dev, &sms);
+    if (rc) return rc;
+    k1::sample::Params p = {};
+    p.logits = logits;
+    p.n_rows = n_rows;
+    p.vocab = vocab;
+    p.row_stride = row_stride;
+    p.u = u;
+    p.temperature = s->temperature_rows;
+    p.top_k = s->top_k_rows;
+    p.top_p = s->top_p_rows;
+    p.min_p = s->min_p_rows;
+    p.temperature0 = s->temperature;
+    p.top_k0 = s->top_k;
+    p.top_p0 = s->top_p;
+    p.min_p0 = s->min_p;
+    p.token = token;
+    p.logprob = logprob;
+    p.kept_logprob = kept_logprob;
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case K1_DTYPE_BF16: return sample_launch<__nv_bfloat16>(fn, p, sms, dev, st);
+        case K1_DTYPE_F16: return sample_launch<__half>(fn, p, sms, dev, st);
+        default: return sample_launch<float>(fn, p, sms, dev, st);
+    }
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@
 #pragma once
 
 #include "k1_kernels.cuh"
+#include "k1_sync.cuh"
 
 #ifndef K1_RING_MINB
 #define K1_RING_MINB 1
@@ -33,71 +34,9 @@
 #define K1_RING_EARLY 0
 #endif
 
-// Polls of a bounded mbarrier wait before it gives up (each poll suspends for at most
-// kSuspendHintNs).  The wait-timeout test library is built with a small value.
-#ifndef K1_RING_MAX_TRIES
-#define K1_RING_MAX_TRIES 4096
-#endif
-
 namespace k1 {
 
-__device__ unsigned k1_ring_error;
-
-#ifdef K1_WAIT_TEST
-// Test-only knob (compiled into the wait-timeout test library only): block 0's producer
-// issues no copy from its chunk number k1_test_withhold on, so the consumers' waits for
-// that chunk run out.  -1: off.
-__device__ long long k1_test_withhold = -1;
-#endif
-
 namespace ring {
-
-constexpr int kMaxTries = K1_RING_MAX_TRIES;  // x up to 1 ms suspend hint per poll
-constexpr uint32_t kSuspendHintNs = 1000000;
-
-__device__ __forceinline__ uint32_t saddr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void fence_init() {
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-}
-__device__ __forceinline__ void arrive_expect(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(b)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(b)) : "memory");
-}
-__device__ __forceinline__ bool try_wait(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(saddr(b)), "r"(parity), "r"(kSuspendHintNs)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait for the phase of parity `parity`; false (and the error word set) if it
-// did not complete in time.
-__device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) {
-    for (int i = 0; i < kMaxTries; ++i)
-        if (try_wait(b, parity)) return true;
-    atomicOr(&k1_ring_error, 1u);
-    return false;
-}
-__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-            "r"(saddr(dst)),
-        "l"(src), "r"(bytes), "r"(saddr(bar))
-        : "memory");
-}
 
 // The chunk sequence of one block: its flattened vector range [start, end) walked row by
 // row, each row segment cut into chunks of at most SV vectors.  Producer and consumers

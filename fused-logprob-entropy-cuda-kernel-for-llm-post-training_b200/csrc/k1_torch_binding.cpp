@@ -16,6 +16,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 #include <map>
@@ -507,6 +508,199 @@ void lm_head_shard_backward(at::Tensor hidden, at::Tensor weight, at::Tensor tar
         d_logits.data_ptr(), d_logits.stride(0), at::cuda::getCurrentCUDAStream().stream()));
 }
 
+// ---------------------------------------------------------------------------------------
+// The tail of a decoding step: residual RMS norm, 8-bit product, token sampling
+// ---------------------------------------------------------------------------------------
+void check_matrix(const at::Tensor& t, const at::Tensor& like, const char* what) {
+    TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), what, " must be on the inputs' CUDA device");
+    TORCH_CHECK(t.dim() == 2 && t.sizes() == like.sizes() && t.scalar_type() == like.scalar_type(), what,
+                " must have the inputs' shape [N, H] and dtype");
+    TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, what, " must be contiguous along the last dimension");
+}
+
+int norm_inputs(const at::Tensor& x, const c10::optional<at::Tensor>& residual, const at::Tensor& weight) {
+    TORCH_CHECK(x.is_cuda(), "x must be CUDA");
+    TORCH_CHECK(x.dim() == 2, "x must be [N, H]");
+    const int dt = dtype_code(x);
+    TORCH_CHECK(dt >= 0, "x dtype must be bf16, fp16, or fp32");
+    check_matrix(x, x, "x");
+    if (residual.has_value()) check_matrix(*residual, x, "residual");
+    TORCH_CHECK(weight.is_cuda() && weight.get_device() == x.get_device() && weight.is_contiguous() &&
+                    weight.numel() == x.size(1),
+                "weight must be a contiguous CUDA tensor with one value per column, on x's device");
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
+                "weight must have x's dtype or fp32");
+    return dt;
+}
+
+// (y, stream, rstd); stream is x itself without a residual.
+std::vector<at::Tensor> residual_rmsnorm(at::Tensor x, c10::optional<at::Tensor> residual, at::Tensor weight,
+                                         double eps) {
+    const int dt = norm_inputs(x, residual, weight);
+    const int64_t N = x.size(0), H = x.size(1);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor y = at::empty({N, H}, x.options());
+    at::Tensor s = residual.has_value() ? at::empty({N, H}, x.options()) : x;
+    at::Tensor rstd = at::empty({N}, x.options().dtype(at::kFloat));
+    check_launch(k1_residual_rmsnorm(
+        x.data_ptr(), x.stride(0), residual.has_value() ? residual->data_ptr() : nullptr,
+        residual.has_value() ? residual->stride(0) : 0, weight.data_ptr(), dtype_code(weight), dt, N, H, (float)eps,
+        residual.has_value() ? s.data_ptr() : nullptr, y.data_ptr(), rstd.data_ptr<float>(),
+        at::cuda::getCurrentCUDAStream().stream()));
+    return {y, s, rstd};
+}
+
+// (q, scales, stream)
+std::vector<at::Tensor> residual_rmsnorm_fp8(at::Tensor x, c10::optional<at::Tensor> residual,
+                                             at::Tensor weight, double eps) {
+    const int dt = norm_inputs(x, residual, weight);
+    const int64_t N = x.size(0), H = x.size(1);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor q = at::empty({N, H}, x.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scales = at::empty({N, (H + 127) / 128}, x.options().dtype(at::kFloat));
+    at::Tensor s = residual.has_value() ? at::empty({N, H}, x.options()) : x;
+    check_launch(k1_residual_rmsnorm_fp8(
+        x.data_ptr(), x.stride(0), residual.has_value() ? residual->data_ptr() : nullptr,
+        residual.has_value() ? residual->stride(0) : 0, weight.data_ptr(), dtype_code(weight), dt, N, H, (float)eps,
+        residual.has_value() ? s.data_ptr() : nullptr, q.data_ptr(), scales.data_ptr<float>(),
+        at::cuda::getCurrentCUDAStream().stream()));
+    return {q, scales, s};
+}
+
+// (d_x or None, d_weight or None)
+std::vector<c10::optional<at::Tensor>> residual_rmsnorm_backward(at::Tensor g_y,
+                                                                 c10::optional<at::Tensor> g_stream,
+                                                                 at::Tensor stream_in, at::Tensor rstd,
+                                                                 at::Tensor weight, bool need_x, bool need_w) {
+    const int dt = norm_inputs(stream_in, g_stream, weight);
+    check_matrix(g_y, stream_in, "g_y");
+    const int64_t N = stream_in.size(0), H = stream_in.size(1);
+    TORCH_CHECK(rstd.is_cuda() && rstd.get_device() == stream_in.get_device() &&
+                    rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == N,
+                "rstd must be contiguous fp32 with one entry per row");
+    c10::cuda::CUDAGuard guard(stream_in.device());
+    c10::optional<at::Tensor> dx, dw;
+    if (need_x) dx = at::empty({N, H}, stream_in.options());
+    at::Tensor ws;
+    size_t ws_bytes = 0;
+    if (need_w) {
+        dw = at::empty(weight.sizes(), weight.options());
+        ws_bytes = k1_residual_rmsnorm_workspace_bytes(N, H, stream_in.get_device());
+        ws = at::empty({(int64_t)ws_bytes}, stream_in.options().dtype(at::kByte));
+    }
+    check_launch(k1_residual_rmsnorm_backward(
+        g_y.data_ptr(), g_y.stride(0), g_stream.has_value() ? g_stream->data_ptr() : nullptr,
+        g_stream.has_value() ? g_stream->stride(0) : 0, stream_in.data_ptr(), stream_in.stride(0),
+        rstd.data_ptr<float>(), weight.data_ptr(), dtype_code(weight), dt, N, H, need_x ? dx->data_ptr() : nullptr,
+        need_w ? dw->data_ptr() : nullptr, need_w ? ws.data_ptr() : nullptr, ws_bytes,
+        at::cuda::getCurrentCUDAStream().stream()));
+    return {dx, dw};
+}
+
+// (q, scales): rows in 8 bits, one scale per row and 128 columns
+std::vector<at::Tensor> quantize_fp8_rows(at::Tensor x) {
+    TORCH_CHECK(x.is_cuda(), "x must be CUDA");
+    TORCH_CHECK(x.dim() == 2, "x must be [N, H]");
+    const int dt = dtype_code(x);
+    TORCH_CHECK(dt >= 0, "x dtype must be bf16, fp16, or fp32");
+    check_matrix(x, x, "x");
+    const int64_t N = x.size(0), H = x.size(1);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor q = at::empty({N, H}, x.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scales = at::empty({N, (H + 127) / 128}, x.options().dtype(at::kFloat));
+    check_launch(k1_quantize_fp8_rows(x.data_ptr(), x.stride(0), dt, N, H, q.data_ptr(), scales.data_ptr<float>(),
+                                      at::cuda::getCurrentCUDAStream().stream()));
+    return {q, scales};
+}
+
+// (q, scales): a weight in 8 bits, one scale per block of 128 x 128
+std::vector<at::Tensor> quantize_fp8_blocks(at::Tensor w) {
+    TORCH_CHECK(w.is_cuda(), "weight must be CUDA");
+    TORCH_CHECK(w.dim() == 2, "weight must be [O, H]");
+    const int dt = dtype_code(w);
+    TORCH_CHECK(dt >= 0, "weight dtype must be bf16, fp16, or fp32");
+    check_matrix(w, w, "weight");
+    const int64_t N = w.size(0), H = w.size(1);
+    c10::cuda::CUDAGuard guard(w.device());
+    at::Tensor q = at::empty({N, H}, w.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scales = at::empty({(N + 127) / 128, (H + 127) / 128}, w.options().dtype(at::kFloat));
+    check_launch(k1_quantize_fp8_blocks(w.data_ptr(), w.stride(0), dt, N, H, q.data_ptr(),
+                                        scales.data_ptr<float>(), at::cuda::getCurrentCUDAStream().stream()));
+    return {q, scales};
+}
+
+void fp8_linear(at::Tensor x, at::Tensor x_scales, at::Tensor weight, at::Tensor weight_scales, at::Tensor y) {
+    TORCH_CHECK(x.is_cuda() && weight.is_cuda(), "x and weight must be CUDA");
+    TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && weight.scalar_type() == at::kFloat8_e4m3fn,
+                "x and weight must be float8_e4m3fn");
+    TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1),
+                "x [N, H] and weight [O, H] expected");
+    const int64_t M = x.size(0), K = x.size(1), N = weight.size(0), KB = (K + 127) / 128;
+    TORCH_CHECK(x.stride(1) == 1 && weight.stride(1) == 1,
+                "x and weight must be contiguous along the last dimension");
+    for (const at::Tensor* t : {&x_scales, &weight_scales, &weight, &y})
+        TORCH_CHECK(t->is_cuda() && t->get_device() == x.get_device(), "all tensors must be on the same device");
+    TORCH_CHECK(x_scales.scalar_type() == at::kFloat && x_scales.is_contiguous() && x_scales.dim() == 2 &&
+                    x_scales.size(0) == M && x_scales.size(1) == KB,
+                "x_scales must be contiguous fp32 [N, ceil(H / 128)]");
+    TORCH_CHECK(weight_scales.scalar_type() == at::kFloat && weight_scales.is_contiguous() &&
+                    weight_scales.dim() == 2 && weight_scales.size(0) == (N + 127) / 128 &&
+                    weight_scales.size(1) == KB,
+                "weight_scales must be contiguous fp32 [ceil(O / 128), ceil(H / 128)]");
+    const int dt = dtype_code(y);
+    TORCH_CHECK(dt >= 0, "the output's dtype must be bf16, fp16, or fp32");
+    TORCH_CHECK(y.dim() == 2 && y.size(0) == M && y.size(1) == N && (N <= 1 || y.stride(1) == 1),
+                "the output must be [N, O], contiguous along the last dimension");
+    c10::cuda::CUDAGuard guard(x.device());
+    check_launch(k1_fp8_linear(x.data_ptr(), M > 1 ? x.stride(0) : K, x_scales.data_ptr<float>(), weight.data_ptr(),
+                               N > 1 ? weight.stride(0) : K, weight_scales.data_ptr<float>(), M, K, N,
+                               y.data_ptr(), M > 1 ? y.stride(0) : N, dt,
+                               at::cuda::getCurrentCUDAStream().stream()));
+}
+
+// A sampling setting: one number, or a tensor with one entry per row.
+const void* setting_rows(const c10::optional<at::Tensor>& t, at::ScalarType type, const at::Tensor& logits,
+                         const char* what) {
+    if (!t.has_value()) return nullptr;
+    TORCH_CHECK(t->is_cuda() && t->get_device() == logits.get_device() && t->scalar_type() == type &&
+                    t->is_contiguous() && t->numel() == logits.size(0),
+                what, " must be a number or a contiguous ", type, " tensor with one entry per row, on the logits' device");
+    return t->data_ptr();
+}
+
+// (token, logprob, kept_logprob)
+std::vector<at::Tensor> sample_tokens(at::Tensor logits, at::Tensor u, double temperature, int64_t top_k,
+                                      double top_p, double min_p, c10::optional<at::Tensor> temperature_rows,
+                                      c10::optional<at::Tensor> top_k_rows, c10::optional<at::Tensor> top_p_rows,
+                                      c10::optional<at::Tensor> min_p_rows) {
+    TORCH_CHECK(logits.is_cuda(), "logits must be CUDA");
+    const int dt = dtype_code(logits);
+    TORCH_CHECK(dt >= 0, "logits dtype must be bf16, fp16, or fp32");
+    TORCH_CHECK(logits.dim() == 2, "logits must be [N, V]");
+    TORCH_CHECK(logits.size(1) <= 1 || logits.stride(1) == 1, "logits must be contiguous along the vocab dimension");
+    TORCH_CHECK(u.is_cuda() && u.get_device() == logits.get_device() && u.scalar_type() == at::kFloat &&
+                    u.is_contiguous() && u.numel() == logits.size(0),
+                "u must be contiguous fp32 with one entry per row, on the logits' device");
+    const int64_t N = logits.size(0), V = logits.size(1);
+    k1_sampling s = {};
+    s.temperature_rows = (const float*)setting_rows(temperature_rows, at::kFloat, logits, "temperature");
+    s.top_k_rows = (const int*)setting_rows(top_k_rows, at::kInt, logits, "top_k");
+    s.top_p_rows = (const float*)setting_rows(top_p_rows, at::kFloat, logits, "top_p");
+    s.min_p_rows = (const float*)setting_rows(min_p_rows, at::kFloat, logits, "min_p");
+    s.temperature = temperature;
+    s.top_k = (int)std::min<int64_t>(std::max<int64_t>(top_k, 0), INT32_MAX);
+    s.top_p = (float)top_p;
+    s.min_p = (float)min_p;
+    c10::cuda::CUDAGuard guard(logits.device());
+    at::Tensor token = at::empty({N}, logits.options().dtype(at::kLong));
+    at::Tensor logprob = at::empty({N}, logits.options().dtype(at::kFloat));
+    at::Tensor kept = at::empty({N}, logits.options().dtype(at::kFloat));
+    check_launch(k1_sample_tokens(logits.data_ptr(), dt, N, V, logits.stride(0), u.data_ptr<float>(), &s,
+                                  token.data_ptr<int64_t>(), logprob.data_ptr<float>(), kept.data_ptr<float>(),
+                                  at::cuda::getCurrentCUDAStream().stream()));
+    return {token, logprob, kept};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -563,6 +757,29 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           pybind11::arg("vocab_offset"), pybind11::arg("lse"), pybind11::arg("entropy"),
           pybind11::arg("g_logp"), pybind11::arg("g_ent"), pybind11::arg("g_lse"),
           pybind11::arg("d_logits"), pybind11::arg("scale"));
+    m.def("residual_rmsnorm", &residual_rmsnorm,
+          "stream = x + residual, y = its RMS norm times the weight: (y, stream, rstd).",
+          pybind11::arg("x"), pybind11::arg("residual"), pybind11::arg("weight"), pybind11::arg("eps"));
+    m.def("residual_rmsnorm_fp8", &residual_rmsnorm_fp8,
+          "residual_rmsnorm with y in 8 bits, one scale per row and 128 columns: (q, scales, stream).",
+          pybind11::arg("x"), pybind11::arg("residual"), pybind11::arg("weight"), pybind11::arg("eps"));
+    m.def("residual_rmsnorm_backward", &residual_rmsnorm_backward,
+          "Gradients of residual_rmsnorm: (d_x = d_residual, d_weight).", pybind11::arg("g_y"),
+          pybind11::arg("g_stream"), pybind11::arg("stream"), pybind11::arg("rstd"), pybind11::arg("weight"),
+          pybind11::arg("need_x"), pybind11::arg("need_weight"));
+    m.def("quantize_fp8_rows", &quantize_fp8_rows, "Rows in 8 bits: (q, scales [N, ceil(H / 128)]).",
+          pybind11::arg("x"));
+    m.def("quantize_fp8_blocks", &quantize_fp8_blocks,
+          "A weight in 8 bits: (q, scales [ceil(O / 128), ceil(H / 128)]).", pybind11::arg("weight"));
+    m.def("fp8_linear", &fp8_linear, "y = x weight^T of 8-bit operands with a scale per block of 128.",
+          pybind11::arg("x"), pybind11::arg("x_scales"), pybind11::arg("weight"),
+          pybind11::arg("weight_scales"), pybind11::arg("y"));
+    m.def("sample_tokens", &sample_tokens,
+          "One token per row from given uniform numbers: (token, logprob, kept_logprob).",
+          pybind11::arg("logits"), pybind11::arg("u"), pybind11::arg("temperature"), pybind11::arg("top_k"),
+          pybind11::arg("top_p"), pybind11::arg("min_p"), pybind11::arg("temperature_rows") = pybind11::none(),
+          pybind11::arg("top_k_rows") = pybind11::none(), pybind11::arg("top_p_rows") = pybind11::none(),
+          pybind11::arg("min_p_rows") = pybind11::none());
     m.def("abi_version", &k1_abi_version, "C ABI version of the loaded libk1_b200.so.");
     m.def(
         "ring_status",

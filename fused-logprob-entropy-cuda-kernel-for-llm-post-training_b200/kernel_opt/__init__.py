@@ -5,7 +5,8 @@ Drop-in for the reference package of the same name (python/kernel_opt/__init__.p
 the same public functions, the same `_C` binding names, and the lazily imported
 `KernelOptGRPOTrainer` (needs `trl`).  Multi-GPU helpers live in `kernel_opt.parallel`,
 the GRPO completion-window node in `kernel_opt.grpo`, the LM head fused with K1 in
-`kernel_opt.lm_head`.
+`kernel_opt.lm_head`.  The operators of a decoding step's tail, which produce the tokens that
+K1 scores, are in `kernel_opt.norm`, `kernel_opt.fp8` and `kernel_opt.sampling`.
 """
 import torch  # noqa: F401  (loads libc10 / libtorch before the extension)
 
@@ -23,6 +24,9 @@ from .ops import (  # noqa: F401
     fused_logprob_entropy_scaled,
 )
 from .lm_head import fused_linear_logprob_entropy  # noqa: F401
+from .norm import fused_residual_rmsnorm, fused_residual_rmsnorm_fp8  # noqa: F401
+from .fp8 import fp8_linear, quantize_fp8_blocks, quantize_fp8_rows  # noqa: F401
+from .sampling import sample_tokens  # noqa: F401
 
 
 def set_check_waits(on: bool = True) -> None:

@@ -1,0 +1,59 @@
+"""Tokens from logits, with temperature, top-k, top-p and min-p and given random numbers.
+
+One kernel over the rows of [..., V] logits (csrc/k1_sample.cuh), which reads them once.  The
+random numbers are inputs, and the sums that decide a token are accurate to about 1e-11, so
+the same logits and numbers give the same token whatever batch the row is in.  The returned
+`logprob` is K1's log-probability of the drawn token (at the sampling temperature, over the
+whole vocabulary): the old-policy value that GRPO's ratio needs.  No counterpart in the
+reference, whose generation runs in another library.
+"""
+from __future__ import annotations
+
+import torch
+
+from kernel_opt import _C
+
+
+def _setting(v, dtype, lead, name):
+    """(number, rows): one of the two is in use."""
+    if isinstance(v, torch.Tensor):
+        if v.dim() != 0 and v.shape != lead:
+            raise ValueError(f"{name} must be a number or a tensor shaped like the rows "
+                             f"{tuple(lead)}, got {tuple(v.shape)}")
+        return 0, v.to(dtype).expand(lead).reshape(-1)
+    return v, None
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0):
+    """(tokens, logprobs, kept_logprobs), each shaped like `u`.
+
+    logits: [..., V] bf16 / fp16 / fp32; u: [...] fp32 in [0, 1).  temperature, top_k, top_p,
+    min_p: numbers, or tensors shaped like u (one setting per row).
+
+    Logits are divided by the temperature (multiplied by fp32(1/T)); top-k keeps the k most
+    likely tokens (the lower id among equals), top-p the shortest prefix of those with at
+    least that share of their probability, min-p those at least min_p times as likely as the
+    first; the first always stays.  The token is the first kept id at which the kept
+    probability up to it, in the order of ids, exceeds u.  top_k <= 0, top_p >= 1 and min_p = 0
+    are off; temperature 0 takes the first largest logit.
+
+    logprobs: of the token in the whole distribution at this temperature (at 0: at 1);
+    kept_logprobs: in the filtered, renormalised one.  A row with a NaN or +inf, or nothing
+    above -inf (or, per row, a temperature that is negative or not finite), gives token -1 and
+    NaN."""
+    if not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    lead = logits.shape[:-1]
+    if u.shape != lead:
+        raise ValueError(f"u must be shaped like the rows {tuple(lead)}, got {tuple(u.shape)}")
+    t, t_rows = _setting(temperature, torch.float32, lead, "temperature")
+    k, k_rows = _setting(top_k, torch.int32, lead, "top_k")
+    p, p_rows = _setting(top_p, torch.float32, lead, "top_p")
+    q, q_rows = _setting(min_p, torch.float32, lead, "min_p")
+    x = logits.reshape(u.numel(), logits.shape[-1])
+    token, logprob, kept = _C.sample_tokens(
+        x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous(),
+        u.to(torch.float32).reshape(-1), float(t), int(k), float(p), float(q), t_rows, k_rows,
+        p_rows, q_rows)
+    return token.view(lead), logprob.view(lead), kept.view(lead)

@@ -313,6 +313,108 @@ int k1_lm_head_shard_backward(const void* hidden, const void* weight_shard, int6
                               const float* entropy, const float* g_logp, const float* g_ent,
                               const float* g_lse, void* d_logits, int64_t d_stride, void* stream);
 
+/*
+ * The tail of a decoding step: the operators that produce the tokens K1 scores.  No
+ * counterpart in the reference.
+ *
+ * Residual RMS norm.  Over n_rows x hidden matrices of `dtype` (unit stride inside a row,
+ * rows *_stride elements apart; hidden in [1, 16384]):
+ *     stream_out = dtype(x + residual)             (stored; the next layer reads it too)
+ *     rstd       = 1 / sqrt(mean(stream^2) + eps)  (fp32, one per row)
+ *     y          = dtype(stream * rstd * weight)
+ * The norm reads the stream as stored.  residual = NULL: the stream is x and stream_out is
+ * not written.  weight: hidden values of dtype or fp32.  stream_out and y are contiguous
+ * (stream_out may be x or residual if that is contiguous).  rstd may be NULL (no backward).
+ */
+int k1_residual_rmsnorm(const void* x, int64_t x_stride, const void* residual,
+                        int64_t residual_stride, const void* weight, int weight_dtype, int dtype,
+                        int64_t n_rows, int64_t hidden, float eps, void* stream_out, void* y,
+                        float* rstd, void* stream);
+
+/*
+ * The same with the output in 8 bits: q (e4m3, n_rows x hidden) and scales (fp32, n_rows x
+ * ceil(hidden / 128)), scale = max(|y| over the 128 columns, 1e-30) / 448 and q =
+ * e4m3(y / scale) from the fp32 y, not rounded in between.  A NaN makes its block's scale
+ * NaN; an infinity makes it infinite (its block then reads as NaN).
+ */
+int k1_residual_rmsnorm_fp8(const void* x, int64_t x_stride, const void* residual,
+                            int64_t residual_stride, const void* weight, int weight_dtype,
+                            int dtype, int64_t n_rows, int64_t hidden, float eps, void* stream_out,
+                            void* q, float* scales, void* stream);
+
+/* Rows in 8 bits without the norm (same layout and scales). */
+int k1_quantize_fp8_rows(const void* x, int64_t x_stride, int dtype, int64_t n_rows,
+                         int64_t hidden, void* q, float* scales, void* stream);
+
+/*
+ * A weight in 8 bits: q (e4m3, rows x cols, contiguous) and scales (fp32, ceil(rows / 128) x
+ * ceil(cols / 128)), one scale per block of 128 x 128.
+ */
+int k1_quantize_fp8_blocks(const void* w, int64_t w_stride, int dtype, int64_t rows, int64_t cols,
+                           void* q, float* scales, void* stream);
+
+/* Workspace bytes of the backward's weight gradient; 0 for invalid arguments. */
+size_t k1_residual_rmsnorm_workspace_bytes(int64_t n_rows, int64_t hidden, int device);
+
+/*
+ * Backward of k1_residual_rmsnorm: d_x = dtype(dL/dstream) (which is the gradient of x and of
+ * the residual alike) and d_weight (the weight's dtype, summed over the rows in fp32 in a
+ * fixed order), from g_y = dL/dy, g_stream = dL/dstream_out (NULL: none), the stored stream
+ * and rstd.  d_x or d_weight may be NULL (not computed); the workspace is only needed for
+ * d_weight.
+ */
+int k1_residual_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void* g_stream,
+                                 int64_t g_stream_stride, const void* stream_in,
+                                 int64_t stream_stride, const float* rstd, const void* weight,
+                                 int weight_dtype, int dtype, int64_t n_rows, int64_t hidden,
+                                 void* d_x, void* d_weight, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/*
+ * 8-bit matrix product on the tensor cores (tcgen05):
+ *     y[t, o] = sum_b x_scales[t, b] weight_scales[o / 128, b] sum_{k in block b} x[t, k] weight[o, k]
+ * with b over the blocks of 128 of `inner`.  x: tokens x inner e4m3, weight: outer x inner
+ * e4m3, rows x_stride / weight_stride bytes apart (multiples of 16, 16-byte aligned); scales
+ * fp32, contiguous; inner a multiple of 16, at most 32768.  Blocks are summed in fp32; y
+ * (out_dtype, rows y_stride elements apart) is rounded once.
+ */
+int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const void* weight,
+                  int64_t weight_stride, const float* weight_scales, int64_t tokens, int64_t inner,
+                  int64_t outer, void* y, int64_t y_stride, int out_dtype, void* stream);
+
+/*
+ * One token per row of logits.  A *_rows pointer (n_rows values on the device) takes the
+ * place of the single value; temperature 0 takes the first largest logit, top_k <= 0, top_p
+ * >= 1 and min_p = 0 are off.
+ */
+typedef struct k1_sampling {
+    const float* temperature_rows;
+    const int* top_k_rows;
+    const float* top_p_rows;
+    const float* min_p_rows;
+    double temperature;
+    int top_k;
+    float top_p;
+    float min_p;
+} k1_sampling;
+
+/*
+ *     y_i = x_i * fp32(1 / temperature), w_i = exp(y_i - max y)
+ *     top-k keeps the k first (larger y first, the lower index among equals), top-p of those
+ *     the shortest prefix with at least top_p of their mass, min-p what has w_i >= min_p; the
+ *     first always stays
+ *     token = the first kept index at which the kept mass up to it (in index order) exceeds
+ *     u * (kept mass), u in [0, 1)
+ *     logprob = log(w_token / sum of all w), kept_logprob = log(w_token / kept mass)
+ * (at temperature 0: logprob at temperature 1, kept_logprob 0).  Sums are accurate to about
+ * 1e-11, so a token does not depend on how the work is split.  A row with a NaN or +inf, with
+ * nothing above -inf, or with a temperature that is negative or not finite gives token -1
+ * and NaN log-probabilities.  logits: n_rows rows of `vocab` elements, row_stride apart.
+ */
+int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
+                     int64_t row_stride, const float* u, const k1_sampling* settings,
+                     int64_t* token, float* logprob, float* kept_logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
