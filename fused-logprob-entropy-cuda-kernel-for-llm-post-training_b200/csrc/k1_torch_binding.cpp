@@ -511,191 +511,271 @@ void lm_head_shard_backward(at::Tensor hidden, at::Tensor weight, at::Tensor tar
 // ---------------------------------------------------------------------------------------
 // The tail of a decoding step: residual RMS norm, 8-bit product, token sampling
 // ---------------------------------------------------------------------------------------
-void check_matrix(const at::Tensor& t, const at::Tensor& like, const char* what) {
-    TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), what, " must be on the inputs' CUDA device");
-    TORCH_CHECK(t.dim() == 2 && t.sizes() == like.sizes() && t.scalar_type() == like.scalar_type(), what,
-                " must have the inputs' shape [N, H] and dtype");
-    TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, what, " must be contiguous along the last dimension");
+// [..., H] as [N, H] with unit stride inside a row; a view where the layout allows it.
+at::Tensor rows2d(const at::Tensor& t) {
+    TORCH_CHECK_VALUE(t.dim() >= 1, "a tensor with a hidden dimension is expected");
+    at::Tensor r = t;
+    if (t.dim() != 2) {
+        const int64_t H = t.size(-1);
+        r = t.reshape({H ? t.numel() / H : 0, H});
+    }
+    return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
 
-int norm_inputs(const at::Tensor& x, const c10::optional<at::Tensor>& residual, const at::Tensor& weight) {
-    TORCH_CHECK(x.is_cuda(), "x must be CUDA");
-    TORCH_CHECK(x.dim() == 2, "x must be [N, H]");
+int float_dtype(const at::Tensor& x, const char* what) {
+    TORCH_CHECK_VALUE(x.is_cuda(), what, " must be a CUDA tensor");
     const int dt = dtype_code(x);
-    TORCH_CHECK(dt >= 0, "x dtype must be bf16, fp16, or fp32");
-    check_matrix(x, x, "x");
-    if (residual.has_value()) check_matrix(*residual, x, "residual");
-    TORCH_CHECK(weight.is_cuda() && weight.get_device() == x.get_device() && weight.is_contiguous() &&
-                    weight.numel() == x.size(1),
-                "weight must be a contiguous CUDA tensor with one value per column, on x's device");
-    TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
-                "weight must have x's dtype or fp32");
+    TORCH_CHECK(dt >= 0, what, " dtype must be bf16, fp16, or fp32");
     return dt;
 }
 
-// (y, stream, rstd); stream is x itself without a residual.
-std::vector<at::Tensor> residual_rmsnorm(at::Tensor x, c10::optional<at::Tensor> residual, at::Tensor weight,
-                                         double eps) {
-    const int dt = norm_inputs(x, residual, weight);
-    const int64_t N = x.size(0), H = x.size(1);
+int norm_inputs(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, double eps) {
+    const int dt = float_dtype(x, "x");
+    if (residual.defined())
+        TORCH_CHECK_VALUE(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type() &&
+                              residual.device() == x.device(),
+                          "residual must match x in shape, dtype and device, got ", residual.sizes(), " ",
+                          residual.scalar_type(), " for ", x.sizes(), " ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 1 && weight.size(0) == x.size(-1),
+                      "weight must have one value per column of x, got ", weight.sizes(), " for ", x.sizes());
+    TORCH_CHECK_VALUE(weight.device() == x.device(), "weight must be on x's device");
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
+                "weight must have x's dtype or fp32");
+    TORCH_CHECK_VALUE(eps > 0, "eps must be positive, got ", eps);
+    return dt;
+}
+
+struct NormOut {
+    at::Tensor y, stream, rstd, scales, weight;  // as rows [N, H]; stream is x without a residual
+};
+
+// The forward on rows; rstd only for a backward, scales only in 8 bits.
+NormOut norm_run(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, double eps, bool fp8,
+                 bool want_rstd) {
+    const int dt = norm_inputs(x, residual, weight, eps);
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty({N, H}, x.options());
-    at::Tensor s = residual.has_value() ? at::empty({N, H}, x.options()) : x;
-    at::Tensor rstd = at::empty({N}, x.options().dtype(at::kFloat));
-    check_launch(k1_residual_rmsnorm(
-        x.data_ptr(), x.stride(0), residual.has_value() ? residual->data_ptr() : nullptr,
-        residual.has_value() ? residual->stride(0) : 0, weight.data_ptr(), dtype_code(weight), dt, N, H, (float)eps,
-        residual.has_value() ? s.data_ptr() : nullptr, y.data_ptr(), rstd.data_ptr<float>(),
-        at::cuda::getCurrentCUDAStream().stream()));
-    return {y, s, rstd};
+    const at::Tensor x2 = rows2d(x);
+    const at::Tensor r2 = residual.defined() ? rows2d(residual) : at::Tensor();
+    NormOut o;
+    o.weight = weight.contiguous();
+    const int64_t N = x2.size(0), H = x2.size(1);
+    o.y = fp8 ? at::empty({N, H}, x.options().dtype(at::kFloat8_e4m3fn)) : at::empty({N, H}, x.options());
+    o.stream = r2.defined() ? at::empty({N, H}, x.options()) : x2;
+    void* r = r2.defined() ? r2.data_ptr() : nullptr;
+    const int64_t rs = r2.defined() ? r2.stride(0) : 0;
+    void* so = r2.defined() ? o.stream.data_ptr() : nullptr;
+    cudaStream_t st = at::cuda::getCurrentCUDAStream().stream();
+    if (fp8) {
+        o.scales = at::empty({N, (H + 127) / 128}, x.options().dtype(at::kFloat));
+        check_launch(k1_residual_rmsnorm_fp8(x2.data_ptr(), x2.stride(0), r, rs, o.weight.data_ptr(),
+                                             dtype_code(weight), dt, N, H, (float)eps, so, o.y.data_ptr(),
+                                             o.scales.data_ptr<float>(), st));
+    } else {
+        if (want_rstd) o.rstd = at::empty({N}, x.options().dtype(at::kFloat));
+        check_launch(k1_residual_rmsnorm(x2.data_ptr(), x2.stride(0), r, rs, o.weight.data_ptr(), dtype_code(weight),
+                                         dt, N, H, (float)eps, so, o.y.data_ptr(),
+                                         want_rstd ? o.rstd.data_ptr<float>() : nullptr, st));
+    }
+    return o;
+}
+
+at::Tensor shaped(const at::Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
+
+// The differentiable norm: y alone without a residual, else y and the stream.
+struct ResidualRmsnorm : public torch::autograd::Function<ResidualRmsnorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                  const c10::optional<at::Tensor>& residual_,
+                                                  const at::Tensor& weight, double eps) {
+        const at::Tensor residual = residual_.has_value() ? *residual_ : at::Tensor();
+        NormOut o = norm_run(x, residual, weight, eps, false, true);
+        const at::Tensor y = shaped(o.y, x.sizes());
+        const at::Tensor stream = residual.defined() ? shaped(o.stream, x.sizes()) : at::Tensor();
+        // without a residual the stream is the caller's x: saved as the input it is
+        ctx->save_for_backward({residual.defined() ? stream : x, o.rstd, weight});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["residual"] = residual.defined();
+        if (residual.defined()) return {y, stream};
+        return {y};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "the residual RMS norm has no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &stream = saved[0], &rstd = saved[1], &weight = saved[2];
+        // counted over the tensors that were given
+        const bool has_r = ctx->saved_data["residual"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_r = has_r && ctx->needs_input_grad(1),
+                   need_w = ctx->needs_input_grad(has_r ? 2 : 1);
+        const at::Tensor g_y = grads[0];
+        const at::Tensor g_s = grads.size() > 1 ? grads[1] : at::Tensor();
+        const at::Tensor none;
+        if (!g_y.defined())  // only the stream was used: the addition's own gradient
+            return {need_x ? g_s : none, need_r ? g_s : none, none, none};
+        c10::cuda::CUDAGuard guard(stream.device());
+        const at::Tensor s2 = rows2d(stream), gy2 = rows2d(g_y);
+        const at::Tensor gs2 = g_s.defined() ? rows2d(g_s) : at::Tensor();
+        const at::Tensor w = weight.contiguous();
+        const int64_t N = s2.size(0), H = s2.size(1);
+        at::Tensor d, dw, ws;
+        size_t ws_bytes = 0;
+        if (need_x || need_r) d = at::empty({N, H}, stream.options());
+        if (need_w) {
+            dw = at::empty(weight.sizes(), weight.options());
+            ws_bytes = k1_residual_rmsnorm_workspace_bytes(N, H, stream.get_device());
+            ws = at::empty({(int64_t)ws_bytes}, stream.options().dtype(at::kByte));
+        }
+        check_launch(k1_residual_rmsnorm_backward(
+            gy2.data_ptr(), gy2.stride(0), gs2.defined() ? gs2.data_ptr() : nullptr,
+            gs2.defined() ? gs2.stride(0) : 0, s2.data_ptr(), s2.stride(0), rstd.data_ptr<float>(), w.data_ptr(),
+            dtype_code(weight), dtype_code(stream), N, H, d.defined() ? d.data_ptr() : nullptr,
+            dw.defined() ? dw.data_ptr() : nullptr, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes,
+            at::cuda::getCurrentCUDAStream().stream()));
+        if (d.defined()) d = shaped(d, stream.sizes());
+        return {need_x ? d : none, need_r ? d : none, dw, none};
+    }
+};
+
+// (y, stream); differentiable in x, residual and weight.
+std::tuple<at::Tensor, at::Tensor> residual_rmsnorm(const at::Tensor& x, const c10::optional<at::Tensor>& residual_,
+                                                    const at::Tensor& weight, double eps) {
+    const at::Tensor residual = residual_.has_value() ? *residual_ : at::Tensor();
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || weight.requires_grad() || (residual.defined() && residual.requires_grad()))) {
+        norm_inputs(x, residual, weight, eps);
+        auto out = ResidualRmsnorm::apply(x, residual_, weight, eps);
+        return {out[0], residual.defined() ? out[1] : x};
+    }
+    NormOut o = norm_run(x, residual, weight, eps, false, false);
+    return {shaped(o.y, x.sizes()), residual.defined() ? shaped(o.stream, x.sizes()) : x};
+}
+
+// Sizes of x with the last one replaced.
+at::Tensor lead_shaped(const at::Tensor& t, const at::Tensor& x) {
+    if (x.dim() == 2) return t;
+    std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = t.size(1);
+    return t.view(sizes);
 }
 
 // (q, scales, stream)
-std::vector<at::Tensor> residual_rmsnorm_fp8(at::Tensor x, c10::optional<at::Tensor> residual,
-                                             at::Tensor weight, double eps) {
-    const int dt = norm_inputs(x, residual, weight);
-    const int64_t N = x.size(0), H = x.size(1);
-    c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor q = at::empty({N, H}, x.options().dtype(at::kFloat8_e4m3fn));
-    at::Tensor scales = at::empty({N, (H + 127) / 128}, x.options().dtype(at::kFloat));
-    at::Tensor s = residual.has_value() ? at::empty({N, H}, x.options()) : x;
-    check_launch(k1_residual_rmsnorm_fp8(
-        x.data_ptr(), x.stride(0), residual.has_value() ? residual->data_ptr() : nullptr,
-        residual.has_value() ? residual->stride(0) : 0, weight.data_ptr(), dtype_code(weight), dt, N, H, (float)eps,
-        residual.has_value() ? s.data_ptr() : nullptr, q.data_ptr(), scales.data_ptr<float>(),
-        at::cuda::getCurrentCUDAStream().stream()));
-    return {q, scales, s};
-}
-
-// (d_x or None, d_weight or None)
-std::vector<c10::optional<at::Tensor>> residual_rmsnorm_backward(at::Tensor g_y,
-                                                                 c10::optional<at::Tensor> g_stream,
-                                                                 at::Tensor stream_in, at::Tensor rstd,
-                                                                 at::Tensor weight, bool need_x, bool need_w) {
-    const int dt = norm_inputs(stream_in, g_stream, weight);
-    check_matrix(g_y, stream_in, "g_y");
-    const int64_t N = stream_in.size(0), H = stream_in.size(1);
-    TORCH_CHECK(rstd.is_cuda() && rstd.get_device() == stream_in.get_device() &&
-                    rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == N,
-                "rstd must be contiguous fp32 with one entry per row");
-    c10::cuda::CUDAGuard guard(stream_in.device());
-    c10::optional<at::Tensor> dx, dw;
-    if (need_x) dx = at::empty({N, H}, stream_in.options());
-    at::Tensor ws;
-    size_t ws_bytes = 0;
-    if (need_w) {
-        dw = at::empty(weight.sizes(), weight.options());
-        ws_bytes = k1_residual_rmsnorm_workspace_bytes(N, H, stream_in.get_device());
-        ws = at::empty({(int64_t)ws_bytes}, stream_in.options().dtype(at::kByte));
-    }
-    check_launch(k1_residual_rmsnorm_backward(
-        g_y.data_ptr(), g_y.stride(0), g_stream.has_value() ? g_stream->data_ptr() : nullptr,
-        g_stream.has_value() ? g_stream->stride(0) : 0, stream_in.data_ptr(), stream_in.stride(0),
-        rstd.data_ptr<float>(), weight.data_ptr(), dtype_code(weight), dt, N, H, need_x ? dx->data_ptr() : nullptr,
-        need_w ? dw->data_ptr() : nullptr, need_w ? ws.data_ptr() : nullptr, ws_bytes,
-        at::cuda::getCurrentCUDAStream().stream()));
-    return {dx, dw};
+std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_rmsnorm_fp8(const at::Tensor& x,
+                                                                    const c10::optional<at::Tensor>& residual_,
+                                                                    const at::Tensor& weight, double eps) {
+    const at::Tensor residual = residual_.has_value() ? *residual_ : at::Tensor();
+    NormOut o = norm_run(x, residual, weight, eps, true, false);
+    return {lead_shaped(o.y, x), lead_shaped(o.scales, x), residual.defined() ? lead_shaped(o.stream, x) : x};
 }
 
 // (q, scales): rows in 8 bits, one scale per row and 128 columns
-std::vector<at::Tensor> quantize_fp8_rows(at::Tensor x) {
-    TORCH_CHECK(x.is_cuda(), "x must be CUDA");
-    TORCH_CHECK(x.dim() == 2, "x must be [N, H]");
-    const int dt = dtype_code(x);
-    TORCH_CHECK(dt >= 0, "x dtype must be bf16, fp16, or fp32");
-    check_matrix(x, x, "x");
-    const int64_t N = x.size(0), H = x.size(1);
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_rows(const at::Tensor& x) {
+    const int dt = float_dtype(x, "x");
     c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor x2 = rows2d(x);
+    const int64_t N = x2.size(0), H = x2.size(1);
     at::Tensor q = at::empty({N, H}, x.options().dtype(at::kFloat8_e4m3fn));
     at::Tensor scales = at::empty({N, (H + 127) / 128}, x.options().dtype(at::kFloat));
-    check_launch(k1_quantize_fp8_rows(x.data_ptr(), x.stride(0), dt, N, H, q.data_ptr(), scales.data_ptr<float>(),
+    check_launch(k1_quantize_fp8_rows(x2.data_ptr(), x2.stride(0), dt, N, H, q.data_ptr(), scales.data_ptr<float>(),
                                       at::cuda::getCurrentCUDAStream().stream()));
-    return {q, scales};
+    return {lead_shaped(q, x), lead_shaped(scales, x)};
 }
 
 // (q, scales): a weight in 8 bits, one scale per block of 128 x 128
-std::vector<at::Tensor> quantize_fp8_blocks(at::Tensor w) {
-    TORCH_CHECK(w.is_cuda(), "weight must be CUDA");
-    TORCH_CHECK(w.dim() == 2, "weight must be [O, H]");
-    const int dt = dtype_code(w);
-    TORCH_CHECK(dt >= 0, "weight dtype must be bf16, fp16, or fp32");
-    check_matrix(w, w, "weight");
-    const int64_t N = w.size(0), H = w.size(1);
+std::tuple<at::Tensor, at::Tensor> quantize_fp8_blocks(const at::Tensor& w) {
+    const int dt = float_dtype(w, "weight");
+    TORCH_CHECK_VALUE(w.dim() == 2, "weight must be [O, H]");
     c10::cuda::CUDAGuard guard(w.device());
+    const at::Tensor w2 = rows2d(w);
+    const int64_t N = w2.size(0), H = w2.size(1);
     at::Tensor q = at::empty({N, H}, w.options().dtype(at::kFloat8_e4m3fn));
     at::Tensor scales = at::empty({(N + 127) / 128, (H + 127) / 128}, w.options().dtype(at::kFloat));
-    check_launch(k1_quantize_fp8_blocks(w.data_ptr(), w.stride(0), dt, N, H, q.data_ptr(),
+    check_launch(k1_quantize_fp8_blocks(w2.data_ptr(), w2.stride(0), dt, N, H, q.data_ptr(),
                                         scales.data_ptr<float>(), at::cuda::getCurrentCUDAStream().stream()));
     return {q, scales};
 }
 
-void fp8_linear(at::Tensor x, at::Tensor x_scales, at::Tensor weight, at::Tensor weight_scales, at::Tensor y) {
-    TORCH_CHECK(x.is_cuda() && weight.is_cuda(), "x and weight must be CUDA");
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
+                      const at::Tensor& weight_scales, at::ScalarType out_dtype, const c10::optional<at::Tensor>& out) {
+    TORCH_CHECK_VALUE(x.is_cuda() && weight.is_cuda(), "x and weight must be CUDA tensors");
     TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && weight.scalar_type() == at::kFloat8_e4m3fn,
                 "x and weight must be float8_e4m3fn");
-    TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1),
+    TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
                 "x [N, H] and weight [O, H] expected");
-    const int64_t M = x.size(0), K = x.size(1), N = weight.size(0), KB = (K + 127) / 128;
-    TORCH_CHECK(x.stride(1) == 1 && weight.stride(1) == 1,
-                "x and weight must be contiguous along the last dimension");
-    for (const at::Tensor* t : {&x_scales, &weight_scales, &weight, &y})
-        TORCH_CHECK(t->is_cuda() && t->get_device() == x.get_device(), "all tensors must be on the same device");
-    TORCH_CHECK(x_scales.scalar_type() == at::kFloat && x_scales.is_contiguous() && x_scales.dim() == 2 &&
-                    x_scales.size(0) == M && x_scales.size(1) == KB,
-                "x_scales must be contiguous fp32 [N, ceil(H / 128)]");
-    TORCH_CHECK(weight_scales.scalar_type() == at::kFloat && weight_scales.is_contiguous() &&
-                    weight_scales.dim() == 2 && weight_scales.size(0) == (N + 127) / 128 &&
-                    weight_scales.size(1) == KB,
-                "weight_scales must be contiguous fp32 [ceil(O / 128), ceil(H / 128)]");
-    const int dt = dtype_code(y);
-    TORCH_CHECK(dt >= 0, "the output's dtype must be bf16, fp16, or fp32");
-    TORCH_CHECK(y.dim() == 2 && y.size(0) == M && y.size(1) == N && (N <= 1 || y.stride(1) == 1),
-                "the output must be [N, O], contiguous along the last dimension");
+    TORCH_CHECK_VALUE(x_scales.dim() == x.dim() && x_scales.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                      "x_scales must have x's leading dimensions, got ", x_scales.sizes(), " for ", x.sizes());
+    for (const at::Tensor* t : {&x_scales, &weight_scales, &weight})
+        TORCH_CHECK(t->device() == x.device(), "all tensors must be on the same device");
     c10::cuda::CUDAGuard guard(x.device());
-    check_launch(k1_fp8_linear(x.data_ptr(), M > 1 ? x.stride(0) : K, x_scales.data_ptr<float>(), weight.data_ptr(),
-                               N > 1 ? weight.stride(0) : K, weight_scales.data_ptr<float>(), M, K, N,
-                               y.data_ptr(), M > 1 ? y.stride(0) : N, dt,
-                               at::cuda::getCurrentCUDAStream().stream()));
+    const at::Tensor x2 = rows2d(x), w2 = rows2d(weight);
+    const int64_t M = x2.size(0), K = x2.size(1), N = w2.size(0), KB = (K + 127) / 128;
+    TORCH_CHECK(x_scales.scalar_type() == at::kFloat && x_scales.size(-1) == KB,
+                "x_scales must be fp32 [N, ceil(H / 128)]");
+    TORCH_CHECK(weight_scales.scalar_type() == at::kFloat && weight_scales.dim() == 2 &&
+                    weight_scales.size(0) == (N + 127) / 128 && weight_scales.size(1) == KB,
+                "weight_scales must be fp32 [ceil(O / 128), ceil(H / 128)]");
+    const at::Tensor xs = x_scales.contiguous(), ws = weight_scales.contiguous();
+    at::Tensor y;
+    if (out.has_value()) {
+        y = *out;
+        TORCH_CHECK(y.dim() == 2 && y.size(0) == M && y.size(1) == N && (N <= 1 || y.stride(1) == 1) &&
+                        y.device() == x.device(),
+                    "the output must be [N, O] on x's device, contiguous along the last dimension");
+        TORCH_CHECK(dtype_code(y) >= 0, "the output's dtype must be bf16, fp16, or fp32");
+    } else {
+        TORCH_CHECK_VALUE(out_dtype == at::kBFloat16 || out_dtype == at::kHalf || out_dtype == at::kFloat,
+                          "out_dtype must be bf16, fp16, or fp32, got ", out_dtype);
+        y = at::empty({M, N}, x.options().dtype(out_dtype));
+    }
+    check_launch(k1_fp8_linear(x2.data_ptr(), M > 1 ? x2.stride(0) : K, xs.data_ptr<float>(), w2.data_ptr(),
+                               N > 1 ? w2.stride(0) : K, ws.data_ptr<float>(), M, K, N, y.data_ptr(),
+                               M > 1 ? y.stride(0) : N, dtype_code(y), at::cuda::getCurrentCUDAStream().stream()));
+    return out.has_value() ? y : lead_shaped(y, x);
 }
 
-// A sampling setting: one number, or a tensor with one entry per row.
-const void* setting_rows(const c10::optional<at::Tensor>& t, at::ScalarType type, const at::Tensor& logits,
-                         const char* what) {
-    if (!t.has_value()) return nullptr;
-    TORCH_CHECK(t->is_cuda() && t->get_device() == logits.get_device() && t->scalar_type() == type &&
-                    t->is_contiguous() && t->numel() == logits.size(0),
-                what, " must be a number or a contiguous ", type, " tensor with one entry per row, on the logits' device");
-    return t->data_ptr();
+// A sampling setting: a number, or a tensor with one entry per row (kept alive in `rows`).
+template <typename V>
+const V* setting(const pybind11::object& v, at::ScalarType type, const at::Tensor& u, const char* what, double* number,
+                 at::Tensor& rows) {
+    if (!THPVariable_Check(v.ptr())) {
+        *number = v.cast<double>();
+        return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(v.ptr());
+    TORCH_CHECK_VALUE(t.dim() == 0 || t.sizes() == u.sizes(), what,
+                      " must be a number or a tensor shaped like the rows ", u.sizes(), ", got ", t.sizes());
+    rows = t.to(u.device(), type).expand(u.sizes()).contiguous();
+    return rows.const_data_ptr<V>();
 }
 
-// (token, logprob, kept_logprob)
-std::vector<at::Tensor> sample_tokens(at::Tensor logits, at::Tensor u, double temperature, int64_t top_k,
-                                      double top_p, double min_p, c10::optional<at::Tensor> temperature_rows,
-                                      c10::optional<at::Tensor> top_k_rows, c10::optional<at::Tensor> top_p_rows,
-                                      c10::optional<at::Tensor> min_p_rows) {
-    TORCH_CHECK(logits.is_cuda(), "logits must be CUDA");
-    const int dt = dtype_code(logits);
-    TORCH_CHECK(dt >= 0, "logits dtype must be bf16, fp16, or fp32");
-    TORCH_CHECK(logits.dim() == 2, "logits must be [N, V]");
-    TORCH_CHECK(logits.size(1) <= 1 || logits.stride(1) == 1, "logits must be contiguous along the vocab dimension");
-    TORCH_CHECK(u.is_cuda() && u.get_device() == logits.get_device() && u.scalar_type() == at::kFloat &&
-                    u.is_contiguous() && u.numel() == logits.size(0),
-                "u must be contiguous fp32 with one entry per row, on the logits' device");
-    const int64_t N = logits.size(0), V = logits.size(1);
-    k1_sampling s = {};
-    s.temperature_rows = (const float*)setting_rows(temperature_rows, at::kFloat, logits, "temperature");
-    s.top_k_rows = (const int*)setting_rows(top_k_rows, at::kInt, logits, "top_k");
-    s.top_p_rows = (const float*)setting_rows(top_p_rows, at::kFloat, logits, "top_p");
-    s.min_p_rows = (const float*)setting_rows(min_p_rows, at::kFloat, logits, "min_p");
-    s.temperature = temperature;
-    s.top_k = (int)std::min<int64_t>(std::max<int64_t>(top_k, 0), INT32_MAX);
-    s.top_p = (float)top_p;
-    s.min_p = (float)min_p;
+// (token, logprob, kept_logprob), each shaped like u
+std::tuple<at::Tensor, at::Tensor, at::Tensor> sample_tokens(const at::Tensor& logits, const at::Tensor& u,
+                                                             const pybind11::object& temperature,
+                                                             const pybind11::object& top_k,
+                                                             const pybind11::object& top_p,
+                                                             const pybind11::object& min_p) {
+    const int dt = float_dtype(logits, "logits");
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && u.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                      "u must be shaped like the rows of logits ", logits.sizes(), ", got ", u.sizes());
+    TORCH_CHECK_VALUE(u.device() == logits.device(), "u must be on the logits' device");
     c10::cuda::CUDAGuard guard(logits.device());
-    at::Tensor token = at::empty({N}, logits.options().dtype(at::kLong));
-    at::Tensor logprob = at::empty({N}, logits.options().dtype(at::kFloat));
-    at::Tensor kept = at::empty({N}, logits.options().dtype(at::kFloat));
-    check_launch(k1_sample_tokens(logits.data_ptr(), dt, N, V, logits.stride(0), u.data_ptr<float>(), &s,
+    const int64_t N = u.numel(), V = logits.size(-1);
+    at::Tensor x = logits.dim() == 2 ? logits : logits.reshape({N, V});
+    if (x.stride(1) != 1 && V > 1) x = x.contiguous();
+    const at::Tensor uu = u.to(at::kFloat).contiguous();
+    k1_sampling s = {};
+    at::Tensor t_rows, k_rows, p_rows, q_rows;
+    double k = 0, p = 1, q = 0;
+    s.temperature_rows = setting<float>(temperature, at::kFloat, u, "temperature", &s.temperature, t_rows);
+    s.top_k_rows = setting<int>(top_k, at::kInt, u, "top_k", &k, k_rows);
+    s.top_p_rows = setting<float>(top_p, at::kFloat, u, "top_p", &p, p_rows);
+    s.min_p_rows = setting<float>(min_p, at::kFloat, u, "min_p", &q, q_rows);
+    s.top_k = (int)std::min(std::max(k, 0.0), (double)INT32_MAX);
+    s.top_p = (float)p;
+    s.min_p = (float)q;
+    at::Tensor token = at::empty(u.sizes(), logits.options().dtype(at::kLong));
+    at::Tensor logprob = at::empty(u.sizes(), logits.options().dtype(at::kFloat));
+    at::Tensor kept = at::empty(u.sizes(), logits.options().dtype(at::kFloat));
+    check_launch(k1_sample_tokens(x.data_ptr(), dt, N, V, x.stride(0), uu.data_ptr<float>(), &s,
                                   token.data_ptr<int64_t>(), logprob.data_ptr<float>(), kept.data_ptr<float>(),
                                   at::cuda::getCurrentCUDAStream().stream()));
     return {token, logprob, kept};
@@ -758,28 +838,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           pybind11::arg("g_logp"), pybind11::arg("g_ent"), pybind11::arg("g_lse"),
           pybind11::arg("d_logits"), pybind11::arg("scale"));
     m.def("residual_rmsnorm", &residual_rmsnorm,
-          "stream = x + residual, y = its RMS norm times the weight: (y, stream, rstd).",
+          "stream = x + residual, y = its RMS norm times the weight: (y, stream), differentiable.",
           pybind11::arg("x"), pybind11::arg("residual"), pybind11::arg("weight"), pybind11::arg("eps"));
     m.def("residual_rmsnorm_fp8", &residual_rmsnorm_fp8,
           "residual_rmsnorm with y in 8 bits, one scale per row and 128 columns: (q, scales, stream).",
           pybind11::arg("x"), pybind11::arg("residual"), pybind11::arg("weight"), pybind11::arg("eps"));
-    m.def("residual_rmsnorm_backward", &residual_rmsnorm_backward,
-          "Gradients of residual_rmsnorm: (d_x = d_residual, d_weight).", pybind11::arg("g_y"),
-          pybind11::arg("g_stream"), pybind11::arg("stream"), pybind11::arg("rstd"), pybind11::arg("weight"),
-          pybind11::arg("need_x"), pybind11::arg("need_weight"));
     m.def("quantize_fp8_rows", &quantize_fp8_rows, "Rows in 8 bits: (q, scales [N, ceil(H / 128)]).",
           pybind11::arg("x"));
     m.def("quantize_fp8_blocks", &quantize_fp8_blocks,
           "A weight in 8 bits: (q, scales [ceil(O / 128), ceil(H / 128)]).", pybind11::arg("weight"));
     m.def("fp8_linear", &fp8_linear, "y = x weight^T of 8-bit operands with a scale per block of 128.",
           pybind11::arg("x"), pybind11::arg("x_scales"), pybind11::arg("weight"),
-          pybind11::arg("weight_scales"), pybind11::arg("y"));
+          pybind11::arg("weight_scales"), pybind11::arg("out_dtype"), pybind11::arg("out"));
     m.def("sample_tokens", &sample_tokens,
           "One token per row from given uniform numbers: (token, logprob, kept_logprob).",
           pybind11::arg("logits"), pybind11::arg("u"), pybind11::arg("temperature"), pybind11::arg("top_k"),
-          pybind11::arg("top_p"), pybind11::arg("min_p"), pybind11::arg("temperature_rows") = pybind11::none(),
-          pybind11::arg("top_k_rows") = pybind11::none(), pybind11::arg("top_p_rows") = pybind11::none(),
-          pybind11::arg("min_p_rows") = pybind11::none());
+          pybind11::arg("top_p"), pybind11::arg("min_p"));
     m.def("abi_version", &k1_abi_version, "C ABI version of the loaded libk1_b200.so.");
     m.def(
         "ring_status",

@@ -14,16 +14,6 @@ import torch
 from kernel_opt import _C
 
 
-def _setting(v, dtype, lead, name):
-    """(number, rows): one of the two is in use."""
-    if isinstance(v, torch.Tensor):
-        if v.dim() != 0 and v.shape != lead:
-            raise ValueError(f"{name} must be a number or a tensor shaped like the rows "
-                             f"{tuple(lead)}, got {tuple(v.shape)}")
-        return 0, v.to(dtype).expand(lead).reshape(-1)
-    return v, None
-
-
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
                   min_p=0.0):
     """(tokens, logprobs, kept_logprobs), each shaped like `u`.
@@ -42,18 +32,4 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     kept_logprobs: in the filtered, renormalised one.  A row with a NaN or +inf, or nothing
     above -inf (or, per row, a temperature that is negative or not finite), gives token -1 and
     NaN."""
-    if not logits.is_cuda:
-        raise ValueError("logits must be a CUDA tensor")
-    lead = logits.shape[:-1]
-    if u.shape != lead:
-        raise ValueError(f"u must be shaped like the rows {tuple(lead)}, got {tuple(u.shape)}")
-    t, t_rows = _setting(temperature, torch.float32, lead, "temperature")
-    k, k_rows = _setting(top_k, torch.int32, lead, "top_k")
-    p, p_rows = _setting(top_p, torch.float32, lead, "top_p")
-    q, q_rows = _setting(min_p, torch.float32, lead, "min_p")
-    x = logits.reshape(u.numel(), logits.shape[-1])
-    token, logprob, kept = _C.sample_tokens(
-        x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous(),
-        u.to(torch.float32).reshape(-1), float(t), int(k), float(p), float(q), t_rows, k_rows,
-        p_rows, q_rows)
-    return token.view(lead), logprob.view(lead), kept.view(lead)
+    return _C.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
