@@ -292,13 +292,14 @@ int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
 // ---------------------------------------------------------------------------------------
 // Sampling
 // ---------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, bool FILTER>
 int sample_launch(const char* fn, k1::sample::Params p, int sms, int dev, cudaStream_t st) {
     using namespace k1::sample;
     constexpr int E = k1::DT<T>::kEPV;
-    // two blocks per SM while a row's part leaves room for them; a lone block takes up to
-    // kLone; a row that is longer still stays in global memory
-    constexpr int64_t kShared = 76 * 1024, kLone = 184 * 1024, kLeast = 8 * 1024;
+    // Bytes of a row's part in one block: what lets two blocks with lists, or three without,
+    // share an SM; a lone block takes up to kLone; a row that is longer still stays in global
+    // memory.
+    constexpr int64_t kShared = (FILTER ? 92 : K1_SP_KB) * 1024, kLone = 184 * 1024, kLeast = 8 * 1024;
     const int64_t row_bytes = ((p.vocab + E - 1) / E + 1) * 16;  // one more for the shift
     int cluster = 1;
     while (cluster < kMaxCluster && row_bytes > cluster * kShared) cluster *= 2;
@@ -309,13 +310,20 @@ int sample_launch(const char* fn, k1::sample::Params p, int sms, int dev, cudaSt
     p.cluster = cluster;
     p.slice_vecs = (int)vecs;
     const bool resident = vecs * 16 <= kLone;
-    const size_t base = (sizeof(Smem) + 15) & ~(size_t)15;
-    const size_t smem = base + (resident ? (size_t)vecs * 16 : 0);
-    auto kern = resident ? k1_sample_kernel<T, true> : k1_sample_kernel<T, false>;
+    const size_t smem = smem_header<FILTER>() + (resident ? (size_t)vecs * 16 : 0);
+    auto kern = resident ? k1_sample_kernel<T, true, FILTER> : k1_sample_kernel<T, false, FILTER>;
     int rc = allow_smem(kern, dev, smem);
     if (rc) return rc;
     const dim3 grid((unsigned)(p.n_rows * cluster));
-    return launched(fn, launch_cluster(kern, grid, THREADS, smem, cluster, st, p));
+    return launched(fn, launch_cluster(kern, grid, FILTER ? kFilterThreads : kPlainThreads, smem, cluster, st, p));
+}
+
+template <typename T>
+int sample(const char* fn, const k1::sample::Params& p, int sms, int dev, cudaStream_t st) {
+    // settings that may cut the distribution of some row (temperature 0 does)
+    const bool filter = p.temperature || p.top_k || p.top_p || p.min_p || p.greedy0 || p.top_p0 < 1.f ||
+                        (p.top_k0 > 0 && p.top_k0 < p.vocab) || p.min_p0 > 0.f;
+    return filter ? sample_launch<T, true>(fn, p, sms, dev, st) : sample_launch<T, false>(fn, p, sms, dev, st);
 }
 
 }  // namespace
@@ -530,7 +538,8 @@ int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t voca
     p.top_k = s->top_k_rows;
     p.top_p = s->top_p_rows;
     p.min_p = s->min_p_rows;
-    p.temperature0 = s->temperature;
+    p.greedy0 = s->temperature == 0.0;
+    p.scale0 = p.greedy0 ? 1.f : (float)(1.0 / s->temperature);
     p.top_k0 = s->top_k;
     p.top_p0 = s->top_p;
     p.min_p0 = s->min_p;
@@ -539,9 +548,9 @@ int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t voca
     p.kept_logprob = kept_logprob;
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case K1_DTYPE_BF16: return sample_launch<__nv_bfloat16>(fn, p, sms, dev, st);
-        case K1_DTYPE_F16: return sample_launch<__half>(fn, p, sms, dev, st);
-        default: return sample_launch<float>(fn, p, sms, dev, st);
+        case K1_DTYPE_BF16: return sample<__nv_bfloat16>(fn, p, sms, dev, st);
+        case K1_DTYPE_F16: return sample<__half>(fn, p, sms, dev, st);
+        default: return sample<float>(fn, p, sms, dev, st);
     }
 }
 

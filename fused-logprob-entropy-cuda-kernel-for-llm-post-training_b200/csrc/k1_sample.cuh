@@ -23,8 +23,8 @@
 //   short lists             Each thread keeps the maxima of four groups of its elements.  A
 //                           histogram of those maxima gives a bound that at least K elements
 //                           reach, and few more; only groups that reach it are read again,
-//                           and their elements go to a list in the first block, which sorts
-//                           it and applies the filters.  Serves top-k up to kListK and every
+//                           and their elements go to a list in the first block, which applies
+//                           the filters to it.  Serves top-k up to kListK and every
 //                           top-p whose nucleus lies within the list.
 //   selection               Otherwise the threshold is found by histograms over all elements:
 //                           bins of equal width in y (counts for top-k, masses for top-p,
@@ -39,11 +39,27 @@
 #include "k1_common.cuh"
 #include "k1_sync.cuh"
 
+#include <type_traits>
+
 namespace k1 {
 namespace sample {
 
-constexpr int THREADS = 512;
-constexpr int WARPS = THREADS / 32;
+// Threads per block.  With filters the passes after the first are many and short, so a block
+// brings more threads; without, a thread's fixed work (the exchanges) counts, and fewer
+// threads with more elements each win.
+constexpr int kFilterThreads = 512;
+#ifndef K1_SP_TH
+#define K1_SP_TH 256
+#endif
+#ifndef K1_SP_MINB
+#define K1_SP_MINB 5
+#endif
+#ifndef K1_SP_KB
+#define K1_SP_KB 48
+#endif
+constexpr int kPlainThreads = K1_SP_TH;
+constexpr int kMaxWarps = 16;
+constexpr int THREADS = kFilterThreads;  // of the code that only filters use
 constexpr int NB = THREADS;        // histogram bins, one per thread
 constexpr int NG = 4;              // groups of elements per thread
 constexpr int kListCap = 2048;     // entries of the list
@@ -60,7 +76,8 @@ struct Params {
     const int* top_k;
     const float* top_p;
     const float* min_p;
-    double temperature0;
+    float scale0;      // fp32(1 / temperature), 1 at temperature 0
+    bool greedy0;      // temperature 0
     float top_p0, min_p0;
     int top_k0;
     int64_t* token;
@@ -77,23 +94,36 @@ struct Xch {
     unsigned n, pad;
 };
 
+// What every row needs of shared memory, and what only filters need.
 struct Smem {
-    uint64_t list[kListCap];
-    double scan[kListCap];
-    unsigned hist[NB];
-    Xch slot[2];
-    Xch all;              // the exchange's result
-    double before;        // sum of `a` over the blocks of lower rank
-    unsigned n_before;    // sum of `n` over the blocks of lower rank
-    double wsum[WARPS];
-    double wsum_b[WARPS];
-    unsigned wn[WARPS];
-    float wlo[WARPS], whi[WARPS];
-    unsigned list_n;
-    int pick;             // a block-wide choice
-    int64_t ilim;
-    float tau;
+    Xch slot[2][kMaxCluster];  // every block's contribution, written by its owner
+    double wsum[kMaxWarps];    // the warps' parts of an exchange
+    double wsum_b[kMaxWarps];
+    unsigned wn[kMaxWarps];
+    float wlo[kMaxWarps], whi[kMaxWarps];
 };
+struct FilterSmem : Smem {
+    uint64_t list[kListCap];
+    uint64_t sums[NB];    // histogram of the list
+    unsigned hist[NB];    // histogram of the block's elements
+    double wscan[kMaxWarps];
+    uint64_t wsum64[kMaxWarps];
+    uint64_t few_key[32], few_word[32];
+    unsigned few_n;
+    uint64_t entry;       // block-wide values
+    uint64_t above;
+    unsigned found;
+    unsigned list_n;
+    int pick;
+    float tau;            // the threshold, told by the block that finds it
+    int told;
+    int64_t ilim;
+};
+
+template <bool FILTER>
+__host__ __device__ constexpr size_t smem_header() {
+    return ((FILTER ? sizeof(FilterSmem) : sizeof(Smem)) + 15) & ~(size_t)15;
+}
 
 // ------------------------------------------------------------------------------------
 // A row's part in one block
@@ -101,52 +131,76 @@ struct Smem {
 // The row is widened to 16-byte boundaries: virtual index v = i + shift, shift = elements
 // between the boundary at or below the row's start and the start.  Elements outside the row
 // read as -inf, which no pass counts.
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T* row, int64_t i0, int64_t vocab) {
+    constexpr int E = DT<T>::kEPV;
+    uint4 v;
+    T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int64_t i = i0 + k;
+        if (i >= 0 && i < vocab)
+            e[k] = row[i];
+        else
+            DT<T>::store1(e + k, -INFINITY);
+    }
+    return v;
+}
+
 template <typename T, bool RES>
 struct Slice {
     static constexpr int E = DT<T>::kEPV;
     const T* row;
-    uint4* buf;        // RES: the slice in shared memory
+    const uint4* base;  // the boundary at or below the block's first element (vectors in
+                        // [whole0, whole1) alone may be read through it)
+    uint4* buf;         // RES: the slice in shared memory
     int64_t vocab;
-    int shift;
-    int64_t vec0;      // the block's first vector
-    int nvec;          // its vectors
-    int w0, w1;        // the warp's vectors: contiguous, lanes interleaved
+    int64_t i0;         // index of the first vector's first element (negative: before the row)
+    int nvec;           // the block's vectors
+    int whole0, whole1; // those that lie inside the row
+    int w0, w1;         // the warp's vectors: contiguous, lanes interleaved
 
-    __device__ __forceinline__ uint4 load_global(int64_t vec) const {
-        const int64_t i0 = vec * E - shift;
-        if (i0 >= 0 && i0 + E <= vocab) return ldg_stream(row + i0);
-        uint4 v;
-        T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const int64_t i = i0 + k;
-            if (i >= 0 && i < vocab)
-                e[k] = row[i];
-            else
-                DT<T>::store1(e + k, -INFINITY);
-        }
-        return v;
+    __device__ __forceinline__ void init(const T* r, int64_t v, int64_t vec0, int slice_vecs) {
+        row = r;
+        vocab = v;
+        const int shift = (int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+        i0 = vec0 * E - shift;
+        base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(r) & ~(uintptr_t)15) + vec0;
+        const int64_t left = v - i0;  // elements from the first vector to the row's end
+        nvec = left <= 0 ? 0 : (int)min((int64_t)slice_vecs, (left + E - 1) / E);
+        whole0 = i0 < 0 ? 1 : 0;
+        whole1 = left <= 0 ? 0 : (int)min((int64_t)nvec, left / E);
+    }
+    __device__ __forceinline__ uint4 load_global(int j) const {
+        if (j >= whole0 && j < whole1) return ldg_stream(base + j);
+        return load_edge<T>(row, i0 + (int64_t)j * E, vocab);
     }
     __device__ __forceinline__ uint4 vec(int j) const {
         if constexpr (RES)
             return buf[j];
         else
-            return load_global(vec0 + j);
+            return load_global(j);
     }
-    __device__ __forceinline__ int64_t index(int j, int e) const { return (vec0 + j) * E + e - shift; }
+    __device__ __forceinline__ int64_t index(int j, int e) const { return i0 + (int64_t)j * E + e; }
 };
 
 template <typename T>
 __device__ __forceinline__ void unpack(uint4 v, float s, float (&y)[DT<T>::kEPV]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            y[i] = __uint_as_float(w[i]) * s;
-        } else {
-            const float2 f = DT<T>::to_f2(w[i]);
-            y[2 * i] = f.x * s;
-            y[2 * i + 1] = f.y * s;
+        for (int i = 0; i < 4; i += 2) {
+            const float2 f =
+                mul2(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), splat(s));
+            y[i] = f.x;
+            y[i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = mul2(DT<T>::to_f2(w[i]), splat(s));
+            y[2 * i] = f.x;
+            y[2 * i + 1] = f.y;
         }
     }
 }
@@ -164,33 +218,34 @@ __device__ __forceinline__ float vec_max(uint4 v) {
 }
 
 // Exact running sum of weights in [0, 1]: multiples of 2^-13 add exactly in fp32 (up to 2^11
-// per thread and fold), the rests of one vector go to fp64.
+// of them), the rests of one vector go to fp64.  Two weights per instruction.
 struct Mass {
-    float hi = 0.f;
+    float2 hi = make_float2(0.f, 0.f);
     double sum = 0.0;
     int folds = 0;
     template <int E>
     __device__ __forceinline__ void add(const float (&w)[E]) {
-        float lo = 0.f;
+        float2 lo = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float h = __fadd_rn(__fadd_rn(w[i], 1536.f), -1536.f);
-            hi += h;
-            lo += w[i] - h;
+        for (int i = 0; i < E; i += 2) {
+            const float2 x = make_float2(w[i], w[i + 1]);
+            const float2 h = add2(add2(x, splat(1536.f)), splat(-1536.f));
+            hi = add2(hi, h);
+            lo = add2(lo, diff2(x, h));
         }
-        sum += (double)lo;
-        if (++folds == 128) {
-            sum += (double)hi;
-            hi = 0.f;
+        sum += (double)(lo.x + lo.y);
+        if (++folds == 256) {  // 256 vectors of at most 4 weights per half
+            sum += (double)hi.x + (double)hi.y;
+            hi = make_float2(0.f, 0.f);
             folds = 0;
         }
     }
-    __device__ __forceinline__ double total() const { return sum + (double)hi; }
+    __device__ __forceinline__ double total() const { return sum + ((double)hi.x + (double)hi.y); }
 };
 
-// Order-preserving key of a float (larger value, larger key).
+// Order-preserving key of a float (larger value, larger key; -0 and +0 are one).
 __device__ __forceinline__ uint32_t key_of(float y) {
-    const uint32_t b = __float_as_uint(y);
+    const uint32_t b = __float_as_uint(y + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
@@ -215,12 +270,15 @@ struct Bins {
         const uint32_t range = key_of(top) - key_of(bottom);
         return Bins{top, 0.f, key_of(top), max(0, 32 - __clz(range) - 9)};  // NB = 2^9
     }
-    __device__ __forceinline__ int of(float y) const {
-        return shift < 0 ? (int)fminf((top - y) * per_unit, (float)(NB - 1))
-                         : (int)((key_top - key_of(y)) >> shift);
+    // equal width: the bin is this, rounded to the nearest whole number
+    __device__ __forceinline__ float place(float y) const {
+        return fminf((top - y) * per_unit, (float)(NB - 1));
     }
-    // the largest y of bin b (up to rounding)
-    __device__ __forceinline__ float top_of(int b) const {
+    __device__ __forceinline__ int of(float y) const {
+        return shift < 0 ? __float2int_rn(place(y)) : (int)((key_top - key_of(y)) >> shift);
+    }
+    // the y that weights of bin b are taken relative to: its middle (equal width), or its top
+    __device__ __forceinline__ float base_of(int b) const {
         return shift < 0 ? top - (float)b / per_unit : value_of(key_top - ((uint32_t)b << shift));
     }
 };
@@ -236,86 +294,111 @@ __device__ __forceinline__ V warp_add(V v) {
     return v;
 }
 
-__device__ __forceinline__ void ld_remote(Xch* dst, const Xch* slot, int rank) {
-    const uint32_t a = ring::mapa(ring::saddr(slot), rank);
-    uint64_t w[sizeof(Xch) / 8];
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(Xch) / 8); ++i)
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w[i]) : "r"(a + 8 * i) : "memory");
-    memcpy(dst, w, sizeof(Xch));
-}
+// What an exchange carries.
+enum Carry : int { A = 1, B = 2, N = 4, RANGE = 8 };
 
-// Adds a, b, n and joins lo (min), hi (max) over all threads of all blocks of the row;
-// the result is in sm.all (and sm.before, sm.n_before) for every thread on return.  NaN in
-// hi survives.  Sums run in a fixed order.  `phase` alternates between calls, so that a
-// block may write its next contribution while another still reads the last one.
-__device__ __forceinline__ void exchange(Smem& sm, int& phase, int cluster, int rank, double a, double b,
-                                         unsigned n, float lo, float hi) {
+struct Joined {
+    double a, b;
+    double before;      // sum of a over the blocks of lower rank
+    unsigned n;
+    unsigned n_before;
+    float lo, hi;
+};
+
+// Adds a, b, n and joins lo (min) and hi (max, NaN survives) over all threads of all blocks of
+// the row, in a fixed order; every thread gets the result.  The warps' parts of a and n stay
+// in sm.wsum and sm.wn.  Each block writes its contribution into every block's shared memory,
+// so that after one cluster barrier all are at hand.  `phase` alternates between calls: a block
+// may write its next contribution while another still reads the last one, and the barrier in
+// between keeps it from getting further ahead.
+template <int WHAT, int WARPS>
+__device__ __forceinline__ Joined exchange(Smem& sm, int& phase, int cluster, int rank, double a, double b,
+                                           unsigned n, float lo, float hi) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    a = warp_add(a);
-    b = warp_add(b);
-    n = warp_add(n);
+    if (WHAT & A) a = warp_add(a);
+    if (WHAT & B) b = warp_add(b);
+    if (WHAT & N) n = __reduce_add_sync(0xffffffffu, n);
+    if (WHAT & RANGE) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = warp_max_nan(hi);
+        for (int o = 16; o > 0; o >>= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = warp_max_nan(hi);
+    }
     if (lane == 0) {
-        sm.wsum[warp] = a;
-        sm.wsum_b[warp] = b;
-        sm.wn[warp] = n;
-        sm.wlo[warp] = lo;
-        sm.whi[warp] = hi;
+        if (WHAT & A) sm.wsum[warp] = a;
+        if (WHAT & B) sm.wsum_b[warp] = b;
+        if (WHAT & N) sm.wn[warp] = n;
+        if (WHAT & RANGE) {
+            sm.wlo[warp] = lo;
+            sm.whi[warp] = hi;
+        }
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        Xch x = {0.0, 0.0, INFINITY, -INFINITY, 0, 0};
-        for (int i = 0; i < WARPS; ++i) {
-            x.a += sm.wsum[i];
-            x.b += sm.wsum_b[i];
-            x.n += sm.wn[i];
-            x.lo = fminf(x.lo, sm.wlo[i]);
-            x.hi = fmax_nan(x.hi, sm.whi[i]);
+    if (warp == 0) {
+        const int i = lane & (WARPS - 1);  // every WARPS lanes hold all parts
+        if (WHAT & A) a = sm.wsum[i];
+        if (WHAT & B) b = sm.wsum_b[i];
+        if (WHAT & N) n = sm.wn[i];
+        if (WHAT & RANGE) {
+            lo = sm.wlo[i];
+            hi = sm.whi[i];
         }
-        sm.slot[phase] = x;
-    }
-    ring::cluster_sync();
-    if (threadIdx.x == 0) {
-        Xch t = {0.0, 0.0, INFINITY, -INFINITY, 0, 0};
-        Xch x[kMaxCluster];
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r)
-            if (r < cluster) ld_remote(&x[r], &sm.slot[phase], r);
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-            if (r < cluster) {
-                if (r == rank) {
-                    sm.before = t.a;
-                    sm.n_before = t.n;
-                }
-                t.a += x[r].a;
-                t.b += x[r].b;
-                t.n += x[r].n;
-                t.lo = fminf(t.lo, x[r].lo);
-                t.hi = fmax_nan(t.hi, x[r].hi);
+        for (int o = WARPS / 2; o > 0; o >>= 1) {
+            if (WHAT & A) a += __shfl_xor_sync(0xffffffffu, a, o);
+            if (WHAT & B) b += __shfl_xor_sync(0xffffffffu, b, o);
+            if (WHAT & N) n += __shfl_xor_sync(0xffffffffu, n, o);
+            if (WHAT & RANGE) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
             }
         }
-        sm.all = t;
+        if (lane < cluster) {
+            const uint32_t to = ring::mapa(ring::saddr(&sm.slot[phase][rank]), lane);
+            if (WHAT & A)
+                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(a) : "memory");
+            if (WHAT & B)
+                asm volatile("st.shared::cluster.f64 [%0 + 8], %1;" ::"r"(to), "d"(b) : "memory");
+            if (WHAT & RANGE)
+                asm volatile("st.shared::cluster.v2.f32 [%0 + 16], {%1, %2};" ::"r"(to), "f"(lo), "f"(hi)
+                             : "memory");
+            if (WHAT & N) asm volatile("st.shared::cluster.u32 [%0 + 24], %1;" ::"r"(to), "r"(n) : "memory");
+        }
     }
-    __syncthreads();
+    ring::cluster_sync();
+    Joined t = {0.0, 0.0, 0.0, 0, 0, INFINITY, -INFINITY};
+#pragma unroll 4
+    for (int r = 0; r < cluster; ++r) {
+        const Xch& x = sm.slot[phase][r];
+        if (r == rank) {
+            t.before = t.a;
+            t.n_before = t.n;
+        }
+        if (WHAT & A) t.a += x.a;
+        if (WHAT & B) t.b += x.b;
+        if (WHAT & N) t.n += x.n;
+        if (WHAT & RANGE) {
+            t.lo = fminf(t.lo, x.lo);
+            t.hi = fmax_nan(t.hi, x.hi);
+        }
+    }
     phase ^= 1;
+    return t;
 }
 
-// Adds the blocks' histograms: thread b returns bin b of the row.  Ends with no block still
-// reading another's.
-__device__ __forceinline__ unsigned row_bin(Smem& sm, int cluster) {
+// Adds the blocks' histograms: thread b returns bin b of the row.  A block may write its
+// histogram again after the next exchange.
+__device__ __forceinline__ unsigned row_bin(FilterSmem& sm, int cluster) {
     ring::cluster_sync();
     unsigned v = 0;
     const uint32_t a = ring::saddr(&sm.hist[threadIdx.x]);
-    for (int r = 0; r < cluster; ++r) {
-        unsigned x;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(ring::mapa(a, r)) : "memory");
-        v += x;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+        if (r < cluster) {
+            unsigned x;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(ring::mapa(a, r)) : "memory");
+            v += x;
+        }
     }
-    ring::cluster_sync();
     return v;
 }
 
@@ -332,84 +415,155 @@ __device__ __forceinline__ V block_scan(V v, V* warp_sums) {
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
     V base = 0;
-    for (int i = 0; i < warp; ++i) base += warp_sums[i];
+#pragma unroll
+    for (int i = 0; i < THREADS / 32 - 1; ++i) base += i < warp ? warp_sums[i] : V(0);
     return base + v;
 }
 
-// The first thread whose (inclusive, nondecreasing) prefix satisfies `hit`; the last thread
-// if none does.
-__device__ __forceinline__ int first_thread(Smem& sm, bool hit) {
-    if (threadIdx.x == 0) sm.pick = NB - 1;
+// The smallest value of `v` among the block's threads that hit, `none` without one.
+__device__ __forceinline__ int first_of(FilterSmem& sm, bool hit, int v, int none) {
+    if (threadIdx.x == 0) sm.pick = none;
     __syncthreads();
-    if (hit) atomicMin(&sm.pick, (int)threadIdx.x);
+    if (hit) atomicMin(&sm.pick, v);
     __syncthreads();
-    const int v = sm.pick;
+    v = sm.pick;
     __syncthreads();
     return v;
 }
 
-// Append to the list in the row's first block.
-__device__ __forceinline__ void append(Smem& sm, float y, int64_t index) {
-    const uint32_t cnt = ring::mapa(ring::saddr(&sm.list_n), 0);
-    unsigned pos;
-    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(pos) : "r"(cnt) : "memory");
-    if (pos < (unsigned)kListCap) {
-        const uint64_t k = ((uint64_t)key_of(y) << 32) | (uint32_t)~(uint32_t)index;
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ring::mapa(ring::saddr(&sm.list[0]), 0) + pos * 8),
-                     "l"(k)
+// ------------------------------------------------------------------------------------
+// The list: entries of the row (key of y, ~index), in the row's first block
+// ------------------------------------------------------------------------------------
+constexpr int PER = kListCap / THREADS;  // entries per thread
+static_assert(PER == 4, "block sums of a list's words add four");
+
+__device__ __forceinline__ uint64_t entry(float y, int64_t index) {
+    return ((uint64_t)key_of(y) << 32) | (uint32_t)~(uint32_t)index;
+}
+__device__ __forceinline__ float entry_value(uint64_t e) { return value_of((uint32_t)(e >> 32)); }
+__device__ __forceinline__ int64_t entry_index(uint64_t e) { return (int64_t)(uint32_t)~(uint32_t)e; }
+
+// The elements of vector j that `hits` marks, one bit each, into this block's own list, one
+// atomic per warp (whose lanes all call) and round; entries past the list's end are only
+// counted.  f(y) for each.
+template <int E, typename F>
+__device__ __forceinline__ void append(FilterSmem& sm, unsigned hits, const float (&y)[E], int64_t index, F f) {
+    const unsigned lane = threadIdx.x & 31;
+    for (unsigned some; (some = __ballot_sync(0xffffffffu, hits != 0)) != 0; hits &= hits - 1) {
+        unsigned pos = 0;
+        if (lane == 0) pos = atomicAdd(&sm.list_n, (unsigned)__popc(some));
+        pos = __shfl_sync(0xffffffffu, pos, 0) + __popc(some & ((1u << lane) - 1));
+        if (hits) {
+            const int at = __ffs(hits) - 1;
+            float v = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v = at == e ? y[e] : v;
+            if (pos < (unsigned)kListCap) sm.list[pos] = entry(v, index + at);
+            f(v);
+        }
+    }
+}
+
+// The blocks' lists (n_before entries in lower ranks, kListCap in all at most) joined in the
+// first block.
+__device__ __forceinline__ void join_lists(FilterSmem& sm, int rank, unsigned n_before) {
+    if (rank > 0) {
+        const uint32_t to = ring::mapa(ring::saddr(&sm.list[0]), 0) + n_before * 8;
+        for (unsigned i = threadIdx.x; i < sm.list_n; i += THREADS)
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + i * 8), "l"(sm.list[i]) : "memory");
+    }
+    ring::cluster_sync();
+}
+
+// One thread tells every block of the row the threshold; they read it after a cluster barrier.
+__device__ __forceinline__ void tell(FilterSmem& sm, int cluster, float tau, int64_t ilim) {
+    for (int r = 0; r < cluster; ++r) {
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(ring::mapa(ring::saddr(&sm.tau), r)), "f"(tau)
+                     : "memory");
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ring::mapa(ring::saddr(&sm.told), r)), "r"(1)
+                     : "memory");
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ring::mapa(ring::saddr(&sm.ilim), r)), "l"(ilim)
                      : "memory");
     }
 }
 
-// Bitonic sort of keys[0, n), n <= kListCap, largest first (this block's threads).
-__device__ __forceinline__ void sort_list(uint64_t* keys, int n) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += THREADS) keys[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1) {
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int t = threadIdx.x; t < size / 2; t += THREADS) {
-                const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-                const uint64_t a = keys[i], b = keys[i + j];
-                if ((a < b) == ((i & k) == 0)) {
-                    keys[i] = b;
-                    keys[i + j] = a;
-                }
-            }
-            __syncthreads();
-        }
-    }
+// A weight (or a count of one) and the number of entries in one word: 2^-40 units of weight
+// above 12 bits of count, so sums over a list fit 63 bits and do not depend on their order.
+constexpr int kCountBits = 12;
+constexpr float kUnit = 1099511627776.f;  // 2^40
+__device__ __forceinline__ uint64_t weight_word(float w) {
+    return ((uint64_t)__float2ull_rn(w * kUnit) << kCountBits) | 1u;
 }
+__device__ __forceinline__ uint64_t word_weight(uint64_t v) { return v >> kCountBits; }
 
-// scan[i] = sum of weight(i') for i' <= i < n, in fp64 (this block's threads).
-template <typename F>
-__device__ __forceinline__ void scan_list(Smem& sm, int n, F weight) {
-    double base = 0.0;
-    for (int i0 = 0; i0 < n; i0 += THREADS) {
-        const int i = i0 + threadIdx.x;
-        const double v = block_scan(i < n ? weight(i) : 0.0, sm.wsum) + base;
-        if (i < n) sm.scan[i] = v;
-        __syncthreads();
-        base = sm.scan[min(n, i0 + THREADS) - 1];
-    }
+__device__ __forceinline__ uint64_t block_sum64(FilterSmem& sm, uint64_t v) {
+    v = warp_add(v);
     __syncthreads();
-}
-
-// The first i in [0, n) with test(i) (a test that stays true once true); n - 1 if none.
-template <typename F>
-__device__ __forceinline__ int first_in_list(Smem& sm, int n, F test) {
-    if (threadIdx.x == 0) sm.pick = n - 1;
+    if ((threadIdx.x & 31) == 0) sm.wsum64[threadIdx.x >> 5] = v;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += THREADS)
-        if (test(i)) {
-            atomicMin(&sm.pick, i);
-            break;
-        }
-    __syncthreads();
-    const int v = sm.pick;
-    __syncthreads();
+    v = 0;
+    for (int i = 0; i < kFilterThreads / 32; ++i) v += sm.wsum64[i];
     return v;
+}
+
+// Of the block's entries (PER to a thread, distinct keys, a word of 0 for none), largest key
+// first: the key at which the weight added up so far first reaches `target` (> 0); the entries'
+// keys lie in [lo, hi], and their whole weight is at least `target`.  Each round adds the
+// words up in 512 bins of the remaining key range and keeps the crossing bin, until that
+// holds few entries: one round for spread keys, 64 / 9 at most.
+__device__ __forceinline__ uint64_t select_entry(FilterSmem& sm, const uint64_t (&key)[PER],
+                                                 const uint64_t (&word)[PER], uint64_t lo, uint64_t hi,
+                                                 uint64_t target) {
+    uint64_t above = 0;
+    for (;;) {
+        const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
+        sm.sums[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+            if (word[r] && key[r] >= lo && key[r] <= hi)
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sm.sums[(hi - key[r]) >> shift]),
+                          (unsigned long long)word[r]);
+        __syncthreads();
+        const uint64_t mine = sm.sums[threadIdx.x];
+        const uint64_t upto = block_scan(mine, sm.wsum64);
+        // the one bin that holds entries and crosses
+        const uint64_t before = above + word_weight(upto - mine);
+        if (mine && before < target && above + word_weight(upto) >= target) {
+            sm.pick = threadIdx.x;
+            sm.above = before;
+            sm.found = (unsigned)(mine & ((1u << kCountBits) - 1));
+        }
+        __syncthreads();
+        const uint64_t top = hi - ((uint64_t)sm.pick << shift);
+        const uint64_t bottom = top - (((uint64_t)1 << shift) - 1);
+        lo = bottom > top || bottom < lo ? lo : bottom;
+        hi = top;
+        above = sm.above;
+        if (sm.found <= 32) break;
+        __syncthreads();
+    }
+    // the bin's entries, one to a lane, against one another
+#pragma unroll
+    for (int r = 0; r < PER; ++r)
+        if (word[r] && key[r] >= lo && key[r] <= hi) {
+            const unsigned i = atomicAdd(&sm.few_n, 1u);
+            sm.few_key[i] = key[r];
+            sm.few_word[i] = word_weight(word[r]);
+        }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const unsigned n = sm.found, lane = threadIdx.x;
+        const uint64_t k = lane < n ? sm.few_key[lane] : 0, w = lane < n ? sm.few_word[lane] : 0;
+        uint64_t before = above;
+        for (unsigned i = 0; i < n; ++i) before += sm.few_key[i] > k ? sm.few_word[i] : 0;
+        if (w && before < target && before + w >= target) sm.entry = k;
+    }
+    __syncthreads();
+    const uint64_t e = sm.entry;
+    if (threadIdx.x == 0) sm.few_n = 0;
+    __syncthreads();
+    return e;
 }
 
 // ------------------------------------------------------------------------------------
@@ -420,18 +574,17 @@ struct Keep {
     float tau;
     int64_t ilim;
     float min_p;  // a weight's lower limit, 0: off
-    __device__ __forceinline__ bool ranked(float y, int64_t i) const {
-        return y > tau || (y == tau && i <= ilim);
-    }
-    __device__ __forceinline__ bool holds(float y, float w, int64_t i) const {
-        return w >= min_p && ranked(y, i);
+    // Whether y >= tau is kept (of equals, those up to ilim).
+    template <typename SL>
+    __device__ __forceinline__ bool allows(float y, const SL& sl, int j, int e) const {
+        return y != tau || sl.index(j, e) <= ilim;
     }
 };
 
-template <typename T, bool RES>
+template <typename T, bool RES, int TH>
 struct Row {
     static constexpr int E = DT<T>::kEPV;
-    Smem& sm;
+    static constexpr int WARPS = TH / 32;
     Slice<T, RES> sl;
     float s, m;
     int cluster, rank, phase;
@@ -446,62 +599,87 @@ struct Row {
         }
     }
 
-    // Mass of what is kept (`all`: of everything) over the row; the warps' parts stay in
-    // sm.wsum, the lower ranks' in sm.before.
-    __device__ __forceinline__ double kept_mass(const Keep& k, bool all) {
+    // The same with all lanes of a warp at every step, for what they do together, and the
+    // vector as it is; past the part's end it holds -inf.
+    template <typename F>
+    __device__ __forceinline__ void each_vector(F f) const {
+        constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u
+                                   : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
+        for (int j0 = sl.w0; j0 < sl.w1; j0 += 32) {
+            const int j = j0 + (threadIdx.x & 31);
+            f(j, j < sl.w1 ? sl.vec(j) : make_uint4(kNone, kNone, kNone, kNone));
+        }
+    }
+
+    // The weights of vector j that are kept (ALL: all of them).
+    template <bool ALL>
+    __device__ __forceinline__ void weights(const Keep& k, int j, const float (&y)[E], float (&w)[E]) const {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float2 d = add2(make_float2(y[e], y[e + 1]), splat(-m));
+            w[e] = expf(d.x);
+            w[e + 1] = expf(d.y);
+        }
+        if (!ALL) {
+            bool tie = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                tie |= y[e] == k.tau;
+                if (!(y[e] >= k.tau && w[e] >= k.min_p)) w[e] = 0.f;
+            }
+            if (tie) {  // rare: the threshold itself, kept up to an index
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (y[e] == k.tau && sl.index(j, e) > k.ilim) w[e] = 0.f;
+            }
+        }
+    }
+
+    // Mass of what is kept over the row; the warps' parts stay in sm.wsum.
+    template <bool ALL>
+    __device__ __forceinline__ Joined kept_mass(Smem& sm, const Keep& k) {
         Mass mass;
         each([&](int j, float (&y)[E]) {
             float w[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                w[e] = expf(y[e] - m);
-                if (!all && !k.holds(y[e], w[e], sl.index(j, e))) w[e] = 0.f;
-            }
+            weights<ALL>(k, j, y, w);
             mass.add(w);
         });
-        exchange(sm, phase, cluster, rank, mass.total(), 0.0, 0, 0.f, 0.f);
-        return sm.all.a;
+        return exchange<A, WARPS>(sm, phase, cluster, rank, mass.total(), 0.0, 0, 0.f, 0.f);
     }
 
-    // The token at mass `target` of what is kept, in index order, found by the warp that
-    // holds it.  Follows kept_mass (whose partial sums it reads) directly.
-    __device__ __forceinline__ void draw(const Keep& k, bool all, double target, double total, double sum,
-                                         const Params& p, int64_t row) {
-        // the block, then the warp, whose prefix first exceeds the target; the last one with
-        // any mass if rounding leaves none
+    // The token at mass `target` of what is kept, in index order: the block, then its warp's
+    // part, then the vector and the element whose prefix first exceeds the target (where
+    // rounding leaves none, the last with any mass).  Follows the kept_mass that gave `c`,
+    // whose parts in sm.wsum it reads.
+    template <bool ALL>
+    __device__ __forceinline__ void draw(Smem& sm, const Keep& k, const Joined& c, double target, double sum,
+                                         const Params& p, int64_t row) const {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        double base = sm.before, blk = 0.0;
-        for (int i = 0; i < WARPS; ++i) blk += sm.wsum[i];  // as exchange added them
-        if (blk <= 0.0) return;
-        const bool last_block = !(base + blk < total);
-        if (target < base || !(target < base + blk || last_block)) return;
-        int pick = -1;
-        double pick_base = base, run = base;
+        const double end = rank + 1 < cluster ? c.before + sm.slot[phase ^ 1][rank].a : c.a;
+        const double blk = sm.slot[phase ^ 1][rank].a;
+        if (!(blk > 0.0) || target < c.before || !(target < end || !(end < c.a))) return;
+        int part = 0;
+        double base = c.before, run = c.before;
         for (int i = 0; i < WARPS; ++i) {
             const double w = sm.wsum[i];
             if (w > 0.0) {
-                pick = i;
-                pick_base = run;
+                part = i;
+                base = run;
                 run += w;
                 if (run > target) break;
             }
         }
-        if (warp != pick) return;
-        run = pick_base;
-        int64_t found = -1;
-        float yf = 0.f;
-        for (int j0 = sl.w0; j0 < sl.w1; j0 += 32) {
-            const int j = j0 + lane;
+        const int per = (sl.nvec + WARPS - 1) / WARPS;
+        const int j1 = min(sl.nvec, (part + 1) * per);
+        for (int j0 = part * per; j0 < j1; j0 += TH) {
+            const int j = j0 + threadIdx.x;
             float y[E], w[E];
             double mass = 0.0;
-            if (j < sl.w1) {
+            if (j < j1) {
                 unpack<T>(sl.vec(j), s, y);
+                weights<ALL>(k, j, y, w);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    w[e] = expf(y[e] - m);
-                    if (!all && !k.holds(y[e], w[e], sl.index(j, e))) w[e] = 0.f;
-                    mass += (double)w[e];
-                }
+                for (int e = 0; e < E; ++e) mass += (double)w[e];
             }
             double incl = mass;
 #pragma unroll
@@ -509,41 +687,57 @@ struct Row {
                 const double t = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += t;
             }
-            const bool over = mass > 0.0 && run + incl > target;
-            const unsigned any = __ballot_sync(0xffffffffu, over);
-            const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0);
-            // the crossing lane; without one, the last lane with mass holds the candidate
-            const int at = any ? __ffs(any) - 1 : some ? 31 - __clz(some) : -1;
-            if (at == lane) {
-                double c = run + incl - mass;
+            __syncthreads();  // sm.wsum and sm.wsum_b have been read
+            if (lane == 31) sm.wsum_b[warp] = incl;
+            __syncthreads();
+            double before = base, all = base;
+            int last = 0;  // the last warp with any mass
+            for (int i = 0; i < WARPS; ++i) {
+                if (i == warp) before = all;
+                if (sm.wsum_b[i] > 0.0) last = i;
+                all += sm.wsum_b[i];
+            }
+            const bool crossed = all > target;
+            // one warp holds it: the first whose end exceeds the target; until one does, the
+            // last with any mass stands in (and is written over)
+            const double wend = before + __shfl_sync(0xffffffffu, incl, 31);
+            if (all > base && (crossed ? wend > target && !(before > target) : warp == last)) {
+                const unsigned over = __ballot_sync(0xffffffffu, mass > 0.0 && before + incl > target);
+                const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0);
+                const int at = over ? __ffs(over) - 1 : 31 - __clz(some);
+                if (lane == at) {
+                    double cum = before + incl - mass;
+                    int64_t token = -1;
+                    float d = 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (w[e] > 0.f && !(any && c > target)) {
-                        c += (double)w[e];
-                        found = sl.index(j, e);
-                        yf = y[e];
-                    }
+                    for (int e = 0; e < E; ++e)
+                        if (w[e] > 0.f && !(over && cum > target)) {
+                            cum += (double)w[e];
+                            token = sl.index(j, e);
+                            d = y[e] - m;
+                        }
+                    p.token[row] = token;
+                    p.logprob[row] = (float)((double)d - log(sum));
+                    p.kept_logprob[row] = (float)((double)d - log(c.a));
+                }
             }
-            if (at >= 0) {
-                found = __shfl_sync(0xffffffffu, found, at);
-                yf = __shfl_sync(0xffffffffu, yf, at);
-            }
-            if (any) break;
-            run += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (lane == 0) {
-            p.token[row] = found;
-            p.logprob[row] = (float)((double)(yf - m) - log(sum));
-            p.kept_logprob[row] = (float)((double)(yf - m) - log(total));
+            if (crossed) return;
+            base = all;
         }
     }
 };
 
-template <typename T, bool RES>
-__global__ void __launch_bounds__(THREADS, 2) k1_sample_kernel(Params p) {
+// FILTER: top-k, top-p or min-p may be in use (else rows draw from the whole distribution,
+// and the kernel needs no list or histogram).
+template <typename T, bool RES, bool FILTER>
+__global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTER ? 2 : K1_SP_MINB)
+    k1_sample_kernel(Params p) {
     constexpr int E = DT<T>::kEPV;
+    constexpr int TH = FILTER ? kFilterThreads : kPlainThreads;
+    constexpr int WARPS = TH / 32;
+    using SM = std::conditional_t<FILTER, FilterSmem, Smem>;
     extern __shared__ __align__(16) unsigned char sp_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(sp_raw);
+    SM& sm = *reinterpret_cast<SM*>(sp_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cluster = p.cluster;
     const int rank = blockIdx.x % cluster;
@@ -552,28 +746,14 @@ __global__ void __launch_bounds__(THREADS, 2) k1_sample_kernel(Params p) {
     pdl_wait();
     pdl_trigger();
 
-    // the row's settings
-    const double temp = p.temperature ? (double)p.temperature[row] : p.temperature0;
-    const bool greedy = temp == 0.0;
-    int top_k = greedy ? 1 : p.top_k ? p.top_k[row] : p.top_k0;
-    if (top_k <= 0 || top_k >= p.vocab) top_k = 0;
-    const float top_p = greedy ? 1.f : p.top_p ? p.top_p[row] : p.top_p0;
-    const bool use_p = top_p < 1.f;
-    const float min_p = greedy ? 0.f : fminf(p.min_p ? p.min_p[row] : p.min_p0, 1.f);
-
-    Row<T, RES> R{sm};
+    Row<T, RES, TH> R;
     R.cluster = cluster;
     R.rank = rank;
     R.phase = 0;
-    R.s = greedy ? 1.f : (float)(1.0 / temp);
     Slice<T, RES>& sl = R.sl;
-    sl.row = reinterpret_cast<const T*>(p.logits) + row * p.row_stride;
-    sl.buf = reinterpret_cast<uint4*>(sp_raw + ((sizeof(Smem) + 15) & ~(size_t)15));
-    sl.vocab = p.vocab;
-    sl.shift = (int)((reinterpret_cast<uintptr_t>(sl.row) & 15) / sizeof(T));
-    sl.vec0 = (int64_t)rank * p.slice_vecs;
-    const int64_t row_vecs = (p.vocab + sl.shift + E - 1) / E;
-    sl.nvec = (int)max((int64_t)0, min((int64_t)p.slice_vecs, row_vecs - sl.vec0));
+    sl.buf = reinterpret_cast<uint4*>(sp_raw + smem_header<FILTER>());
+    sl.init(reinterpret_cast<const T*>(p.logits) + row * p.row_stride, p.vocab, (int64_t)rank * p.slice_vecs,
+            p.slice_vecs);
     const int per_warp = (sl.nvec + WARPS - 1) / WARPS;
     sl.w0 = min(sl.nvec, warp * per_warp);
     sl.w1 = min(sl.nvec, sl.w0 + per_warp);
@@ -582,302 +762,385 @@ __global__ void __launch_bounds__(THREADS, 2) k1_sample_kernel(Params p) {
     float g[NG];
 #pragma unroll
     for (int q = 0; q < NG; ++q) g[q] = -INFINITY;
-    sm.hist[threadIdx.x] = 0;
-    if (threadIdx.x == 0) sm.list_n = 0;
-    for (int j = sl.w0 + lane; j < sl.w1; j += 32 * NG) {
+    if constexpr (FILTER) {
+        sm.hist[threadIdx.x] = 0;
+        if (threadIdx.x == 0) {
+            sm.list_n = 0;
+            sm.few_n = 0;
+            sm.told = 0;
+        }
+    }
+    int j = sl.w0 + lane;
+    for (; j + 32 * (NG - 1) < sl.w1; j += 32 * NG) {
         uint4 v[NG];
 #pragma unroll
-        for (int q = 0; q < NG; ++q)
-            if (j + 32 * q < sl.w1) v[q] = sl.load_global(sl.vec0 + j + 32 * q);
-#pragma unroll
-        for (int q = 0; q < NG; ++q)
-            if (j + 32 * q < sl.w1) {
-                if constexpr (RES) sl.buf[j + 32 * q] = v[q];
-                g[q] = fmax_nan(g[q], vec_max<T>(v[q]));
-            }
-    }
-    {
-        float hi = -INFINITY, lo = INFINITY;
+        for (int q = 0; q < NG; ++q) v[q] = sl.load_global(j + 32 * q);
 #pragma unroll
         for (int q = 0; q < NG; ++q) {
-            g[q] *= R.s;
-            hi = fmax_nan(hi, g[q]);
-            if (g[q] > -INFINITY) lo = fminf(lo, g[q]);
+            if constexpr (RES) sl.buf[j + 32 * q] = v[q];
+            g[q] = fmax_nan(g[q], vec_max<T>(v[q]));
         }
-        exchange(sm, R.phase, cluster, rank, 0.0, 0.0, 0, lo, hi);
     }
-    const float m = sm.all.hi;
-    const float floor = m - kFloor;
+#pragma unroll
+    for (int q = 0; q < NG; ++q)
+        if (j + 32 * q < sl.w1) {
+            const uint4 v = sl.load_global(j + 32 * q);
+            if constexpr (RES) sl.buf[j + 32 * q] = v;
+            g[q] = fmax_nan(g[q], vec_max<T>(v));
+        }
+    // the row's temperature
+    const float temp = p.temperature ? p.temperature[row] : 1.f;
+    const bool greedy = p.temperature ? temp == 0.f : p.greedy0;
+    R.s = !p.temperature ? p.scale0 : greedy ? 1.f : (float)(1.0 / (double)temp);
+    float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+        g[q] *= R.s;
+        hi = fmax_nan(hi, g[q]);
+        if (FILTER && g[q] > -INFINITY) lo = fminf(lo, g[q]);
+    }
+    const Joined range = exchange<RANGE, WARPS>(sm, R.phase, cluster, rank, 0.0, 0.0, 0, lo, hi);
+    const float m = range.hi;
     R.m = m;
     // NaN, +inf, or nothing above -inf; or a temperature that is negative or no number
-    if (!(m > -INFINITY && m < INFINITY) || !(temp >= 0.0 && R.s > 0.f)) {
+    if (!(m > -INFINITY && m < INFINITY) || !(temp >= 0.f && R.s > 0.f)) {
         if (leader && threadIdx.x == 0) {
             p.token[row] = -1;
             p.logprob[row] = p.kept_logprob[row] = __int_as_float(0x7fc00000);
         }
-        ring::cluster_sync();  // no block leaves while its shared memory may be read
         return;
     }
-
-    // ---- the whole mass ----
-    const bool try_list = top_k ? top_k <= min(kListK, cluster * THREADS) : use_p;
-    Bins bins = Bins::linear(m, fmaxf(sm.all.lo, floor));
-    if (try_list) {
-#pragma unroll
-        for (int q = 0; q < NG; ++q)
-            if (g[q] >= floor) atomicAdd(&sm.hist[bins.of(g[q])], 1u);
-    }
-    Keep keep = {-INFINITY, 0, 0.f};
-    const double S = R.kept_mass(keep, true);
     const double u = (double)p.u[row];
+    Keep keep = {-INFINITY, 0, 0.f};
 
-    if (!top_k && !use_p && !(min_p > 0.f)) {
-        R.draw(keep, true, u * S, S, S, p, row);
-        ring::cluster_sync();
-        return;
-    }
+    if constexpr (!FILTER) {
+        const Joined S = R.template kept_mass<true>(sm, keep);
+        R.template draw<true>(sm, keep, S, u * S.a, S.a, p, row);
+    } else {
+        int top_k = greedy ? 1 : p.top_k ? p.top_k[row] : p.top_k0;
+        if (top_k <= 0 || top_k >= p.vocab) top_k = 0;
+        const float top_p = greedy ? 1.f : p.top_p ? p.top_p[row] : p.top_p0;
+        const bool use_p = top_p < 1.f;
+        const float min_p = greedy ? 0.f : fminf(p.min_p ? p.min_p[row] : p.min_p0, 1.f);
+        const float floor = m - kFloor;
 
-    // ---- a short list ----
-    if (try_list) {
-        const unsigned want = top_k ? top_k : kNucleusK;
-        const unsigned upto = block_scan(row_bin(sm, cluster), sm.wn);
-        const int b = first_thread(sm, upto >= want);
-        double mass = 0.0;
-        unsigned n = 0;
+        // ---- the whole mass ----
+        const bool try_list = top_k ? top_k <= min(kListK, cluster * THREADS) : use_p;
+        // twice the groups' range: the elements below the lowest group maximum spread too
+        Bins bins = Bins::linear(m, fmaxf(m - 2.f * (m - range.lo), floor));
+        if (try_list) {
 #pragma unroll
-        for (int q = 0; q < NG; ++q) {
-            if (!(g[q] >= floor && bins.of(g[q]) <= b)) continue;
-            for (int j = sl.w0 + lane + 32 * q; j < sl.w1; j += 32 * NG) {
-                float y[E];
-                unpack<T>(sl.vec(j), R.s, y);
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (y[e] >= floor && bins.of(y[e]) <= b) {
-                        mass += (double)expf(y[e] - m);
-                        append(sm, y[e], sl.index(j, e));
-                        ++n;
-                    }
-            }
+            for (int q = 0; q < NG; ++q)
+                if (g[q] >= floor) atomicAdd(&sm.hist[bins.of(g[q])], 1u);
         }
-        exchange(sm, R.phase, cluster, rank, mass, 0.0, n, 0.f, 0.f);
-        const int count = (int)sm.all.n;
-        if (count <= kListCap && (top_k || sm.all.a >= (double)top_p * S)) {
-            if (leader) {
-                sort_list(sm.list, count);
-                auto weight = [&](int i) { return (double)expf(value_of((uint32_t)(sm.list[i] >> 32)) - m); };
-                scan_list(sm, count, weight);
-                int kept = top_k ? min(top_k, count) : count;
-                if (use_p) {
-                    const double target = (double)top_p * (top_k ? sm.scan[kept - 1] : S);
-                    kept = first_in_list(sm, kept, [&](int i) { return sm.scan[i] >= target; }) + 1;
-                }
-                if (min_p > 0.f) {
-                    const int lowest = first_in_list(sm, kept, [&](int i) { return weight(i) < (double)min_p; });
-                    if (weight(lowest) < (double)min_p) kept = max(1, lowest);
-                    __syncthreads();
-                }
-                // index order: keys (~index, value) sorted largest first
-                for (int i = threadIdx.x; i < kept; i += THREADS)
-                    sm.list[i] = (sm.list[i] << 32) | (sm.list[i] >> 32);
-                __syncthreads();
-                sort_list(sm.list, kept);
-                scan_list(sm, kept, [&](int i) { return (double)expf(value_of((uint32_t)sm.list[i]) - m); });
-                const double C = sm.scan[kept - 1], target = u * C;
-                const int at = first_in_list(sm, kept, [&](int i) { return sm.scan[i] > target; });
-                if (threadIdx.x == 0) {
-                    const double d = (double)(value_of((uint32_t)sm.list[at]) - m);
-                    p.token[row] = (int64_t)(uint32_t)~(uint32_t)(sm.list[at] >> 32);
-                    p.logprob[row] = (float)(d - log(S));
-                    p.kept_logprob[row] = (float)(d - log(C));
-                }
-            }
-            ring::cluster_sync();
+        const Joined whole = R.template kept_mass<true>(sm, keep);
+        const double S = whole.a;
+
+        if (!top_k && !use_p && !(min_p > 0.f)) {
+            R.template draw<true>(sm, keep, whole, u * S, S, p, row);
             return;
         }
-    }
 
-    // ---- selection over all elements: top-k, then top-p ----
-    double Z = S;
-    for (int what = 0; what < 2; ++what) {
-        const bool by_mass = what == 1;
-        if (!(by_mass ? use_p : top_k > 0)) continue;
-        const double target = by_mass ? (double)top_p * Z : (double)top_k;
-        // the crossing element (the last one kept) lies in y of [ylo, yhi]; `above` is what
-        // is ranked before that interval
-        float ylo = floor, yhi = m;
-        double above = 0.0;
-        for (;;) {
-            // histogram of the interval: counts, or weights relative to the bin's largest
-            // one in steps of 2^-14 (larger ones for vocabularies above 2^18, so that a bin
-            // that holds every element fits 32 bits)
-            const float step = by_mass ? fminf(16384.f, 4294967040.f / (float)p.vocab) : 1.f;
-            sm.hist[threadIdx.x] = 0;
-            __syncthreads();
-            R.each([&](int j, float (&y)[E]) {
+        // ---- a short list ----
+        if (try_list) {
+            const unsigned want = top_k ? top_k : kNucleusK;
+            const unsigned upto = block_scan(row_bin(sm, cluster), sm.wn);
+            const int b = first_of(sm, upto >= want, threadIdx.x, NB - 1);
+            // about the lower edge of bin b; whether at least `want` elements reach it is
+            // seen from their number
+            const float least = b == NB - 1 ? floor : fmaxf(floor, m - ((float)b + 0.5f) / bins.per_unit);
+            double mass = 0.0;
+            unsigned n = 0;
+            R.each_vector([&](int j, uint4 v) {
+                if (!__any_sync(0xffffffffu, vec_max<T>(v) * R.s >= least)) return;
+                float y[E];
+                unpack<T>(v, R.s, y);
+                unsigned hits = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (!(y[e] >= ylo && y[e] <= yhi && keep.ranked(y[e], sl.index(j, e)))) continue;
-                    const int b = bins.of(y[e]);
-                    unsigned v = 1;
-                    if (by_mass) v = (unsigned)(fminf(expf(y[e] - bins.top_of(b)), 1.f) * step);
-                    if (v) atomicAdd(&sm.hist[b], v);
-                }
+                for (int e = 0; e < E; ++e) hits |= y[e] >= least ? 1u << e : 0u;
+                n += __popc(hits);
+                append(sm, hits, y, sl.index(j, 0), [&](float x) { mass += (double)expf(x - m); });
             });
-            __syncthreads();
-            double part = (double)row_bin(sm, cluster);
-            if (by_mass) part *= exp((double)bins.top_of(threadIdx.x) - (double)m) / (double)step;
-            const double upto = above + block_scan(part, sm.wsum);
-            if (!by_mass && __syncthreads_or(threadIdx.x == NB - 1 && upto < target)) {
-                break;  // fewer elements than top-k asks for: all stay
-            }
-            int b = first_thread(sm, upto >= target);
-            // the bin's exact limits; a neighbour's if the rounded masses misled
-            for (int tries = 0; tries < 2 * NB; ++tries) {
-                Mass over, in;
-                unsigned n_over = 0, n_in = 0;
-                float lo = INFINITY, hi = -INFINITY;
-                R.each([&](int j, float (&y)[E]) {
-                    float wo[E], wi[E];
+            const Joined t = exchange<A | N, WARPS>(sm, R.phase, cluster, rank, mass, 0.0, n, 0.f, 0.f);
+            if (t.n <= (unsigned)kListCap &&
+                (top_k ? t.n >= want || least == floor : t.a >= (double)top_p * S)) {
+                join_lists(sm, rank, t.n_before);
+                if (!leader) return;
+                const int count = (int)t.n;
+                uint64_t e[PER], word[PER];
+                float w[PER];
+                uint64_t part = 0;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        wo[e] = wi[e] = 0.f;
-                        if (!(y[e] >= ylo && y[e] <= yhi && keep.ranked(y[e], sl.index(j, e)))) continue;
-                        const int q = bins.of(y[e]);
-                        if (q > b) continue;
-                        const float w = by_mass ? expf(y[e] - m) : 0.f;
-                        if (q < b) {
-                            wo[e] = w;
-                            ++n_over;
-                        } else {
-                            wi[e] = w;
-                            ++n_in;
-                            lo = fminf(lo, y[e]);
-                            hi = fmaxf(hi, y[e]);
-                        }
-                    }
-                    if (by_mass) {
-                        over.add(wo);
-                        in.add(wi);
-                    }
-                });
-                exchange(sm, R.phase, cluster, rank, by_mass ? over.total() : (double)n_over,
-                         by_mass ? in.total() : (double)n_in, n_in, lo, hi);
-                if (sm.all.a > 0.0 && above + sm.all.a >= target && b > 0)
-                    --b;
-                else if ((sm.all.n == 0 || above + sm.all.a + sm.all.b < target) && b < NB - 1)
-                    ++b;
-                else
-                    break;
-            }
-            const Xch x = sm.all;
-            above += x.a;
-            ylo = x.lo;
-            yhi = x.hi;
-            const unsigned n_in = x.n;
-            if (n_in == 0) break;  // not reached: the interval holds the crossing element
-            if (n_in <= (unsigned)kListCap) {
-                // the rest in the list: the crossing element by rank
-                if (leader && threadIdx.x == 0) sm.list_n = 0;
-                ring::cluster_sync();
-                R.each([&](int j, float (&y)[E]) {
+                for (int r = 0; r < PER; ++r) {
+                    const int i = r * THREADS + threadIdx.x;
+                    e[r] = i < count ? sm.list[i] : 0;
+                    w[r] = i < count ? expf(entry_value(e[r]) - m) : 0.f;
+                    word[r] = i < count ? weight_word(w[r]) : 0;
+                    part += word[r];
+                }
+                const uint64_t top = entry(m, 0), bottom = entry(least, 0xffffffffll);
+                uint64_t cut = bottom;  // the last entry kept
+                if (top_k && top_k < count) {
+                    uint64_t one[PER];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const int64_t i = sl.index(j, e);
-                        if (y[e] >= ylo && y[e] <= yhi && keep.ranked(y[e], i))
-                            append(sm, y[e], i);
-                    }
-                });
-                ring::cluster_sync();
-                if (leader) {
-                    sort_list(sm.list, (int)n_in);
-                    scan_list(sm, (int)n_in, [&](int i) {
-                        return by_mass ? (double)expf(value_of((uint32_t)(sm.list[i] >> 32)) - m) : 1.0;
-                    });
-                    const int at = first_in_list(sm, (int)n_in, [&](int i) { return above + sm.scan[i] >= target; });
-                    if (threadIdx.x == 0) {
-                        sm.tau = value_of((uint32_t)(sm.list[at] >> 32));
-                        sm.ilim = (int64_t)(uint32_t)~(uint32_t)sm.list[at];
+                    for (int r = 0; r < PER; ++r) one[r] = word[r] ? ((uint64_t)1 << kCountBits) | 1u : 0;
+                    cut = select_entry(sm, e, one, bottom, top, (uint64_t)top_k);
+                    part = 0;
+#pragma unroll
+                    for (int r = 0; r < PER; ++r) {
+                        if (e[r] < cut) word[r] = 0;
+                        part += word[r];
                     }
                 }
-                ring::cluster_sync();
-                uint32_t tb;
-                uint64_t ib;
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(tb) : "r"(ring::mapa(ring::saddr(&sm.tau), 0)) : "memory");
-                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(ib) : "r"(ring::mapa(ring::saddr(&sm.ilim), 0)) : "memory");
-                keep.tau = __uint_as_float(tb);
-                keep.ilim = (int64_t)ib;
-                ring::cluster_sync();
-                break;
+                if (use_p) {
+                    // of the whole mass without top-k: the list holds that share, up to the
+                    // words' rounding
+                    const uint64_t all = word_weight(block_sum64(sm, part));
+                    const double Z = top_k ? (double)all : S * (double)kUnit;
+                    cut = select_entry(sm, e, word, cut, top,
+                                       min(all, (uint64_t)fmax(ceil((double)top_p * Z), 1.0)));
+                }
+                part = 0;
+#pragma unroll
+                for (int r = 0; r < PER; ++r) {
+                    if (e[r] < cut || w[r] < min_p) word[r] = 0;
+                    part += word[r];
+                }
+                // the draw: the same over the kept indices, the lowest first
+                const uint64_t C = word_weight(block_sum64(sm, part));
+                uint64_t id[PER];
+#pragma unroll
+                for (int r = 0; r < PER; ++r) id[r] = e[r] & 0xffffffffu;
+                const uint64_t at = select_entry(sm, id, word, (uint64_t)(uint32_t)~(uint32_t)(p.vocab - 1),
+                                                 0xffffffffu, min(C, (uint64_t)(u * (double)C) + 1));
+#pragma unroll
+                for (int r = 0; r < PER; ++r)
+                    if (word[r] && id[r] == at) {
+                        const double d = (double)(entry_value(e[r]) - m);
+                        p.token[row] = entry_index(e[r]);
+                        p.logprob[row] = (float)(d - log(S));
+                        p.kept_logprob[row] = (float)(d - log((double)C / (double)kUnit));
+                    }
+                return;
             }
-            if (ylo == yhi) {
-                // all equal: the q-th of them in index order
-                const double each_one = by_mass ? (double)expf(ylo - m) : 1.0;
-                double q = ceil((target - above) / each_one);
-                q = fmin(fmax(q, 1.0), (double)n_in);
-                const int64_t nth = (int64_t)q;
-                unsigned n = 0;
-                R.each([&](int j, float (&y)[E]) {
+        }
+
+        // ---- selection over all elements: top-k, then top-p ----
+        double Z = S;
+        for (int what = 0; what < 2; ++what) {
+            const bool by_mass = what == 1;
+            if (!(by_mass ? use_p : top_k > 0)) continue;
+            const double target = by_mass ? (double)top_p * Z : (double)top_k;
+            // the crossing element (the last one kept) lies in y of [ylo, yhi]; `above` is
+            // what is placed before that interval
+            float ylo = fmaxf(floor, keep.tau), yhi = m;
+            if (by_mass) {
+                // elements whose weight is below (1 - p) Z / V have less than (1 - p) Z
+                // together, so the crossing lies above them (half a unit of y to spare)
+                ylo = fmaxf(ylo, m + logf((float)((1.0 - (double)top_p) * Z / (double)p.vocab)) - 0.5f);
+                bins = Bins::linear(m, ylo);
+            }
+            double above = 0.0;
+            for (;;) {
+                // histogram of the interval: counts, or weights relative to one of the bin's
+                // in steps of 2^-12 (larger ones for vocabularies above 2^18, so that a bin
+                // that holds every element fits 32 bits: a bin of equal width spans less than
+                // 0.21 units of y, so no weight is above 1.12 of its middle's)
+                const float step = by_mass ? fminf(4096.f, 1073741824.f / (float)p.vocab) : 1.f;
+                sm.hist[threadIdx.x] = 0;
+                if (threadIdx.x == 0) sm.list_n = 0;
+                __syncthreads();
+                const bool tied = keep.tau > -INFINITY;  // some of the equals at tau are out
+                if (bins.shift < 0) {
+                    // Adding 1.5 2^23 rounds to a whole number and leaves it in the low bits.
+                    // The fast exponential has a guide's precision.
+                    constexpr float kWhole = 12582912.f;
+                    const float to_log2 = kLog2e / bins.per_unit;
+                    R.each([&](int j, float (&y)[E]) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (y[e] == ylo && keep.ranked(y[e], sl.index(j, e))) ++n;
-                });
-                exchange(sm, R.phase, cluster, rank, 0.0, 0.0, n, 0.f, 0.f);
-                // per warp counts are in sm.wn (exchange's own scratch), in index order
-                int64_t run = sm.n_before;
-                for (int i = 0; i < warp; ++i) run += sm.wn[i];
-                const int64_t have = sm.wn[warp];
-                if (leader && threadIdx.x == 0) sm.ilim = -1;
-                ring::cluster_sync();
-                if (run < nth && nth <= run + have) {
-                    for (int j0 = sl.w0; j0 < sl.w1; j0 += 32) {
-                        const int j = j0 + lane;
-                        unsigned k = 0;
-                        float y[E];
-                        if (j < sl.w1) {
-                            unpack<T>(sl.vec(j), R.s, y);
+                        for (int e = 0; e < E; ++e) {
+                            if (!(y[e] >= ylo && y[e] <= yhi)) continue;
+                            if (tied && !keep.allows(y[e], sl, j, e)) continue;
+                            const float at = bins.place(y[e]), whole = at + kWhole;
+                            const unsigned b = __float_as_uint(whole) & (NB - 1);
+                            unsigned v = 1;
+                            if (by_mass)
+                                v = __float_as_uint(fmaf(ex2(((whole - kWhole) - at) * to_log2), step, 8388608.f)) &
+                                    0x7fffffu;
+                            atomicAdd(&sm.hist[b], v);
+                        }
+                    });
+                } else {
+                    R.each([&](int j, float (&y)[E]) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            if (!(y[e] >= ylo && y[e] <= yhi)) continue;
+                            if (tied && !keep.allows(y[e], sl, j, e)) continue;
+                            const int b = bins.of(y[e]);
+                            atomicAdd(&sm.hist[b], by_mass ? (unsigned)(__expf(y[e] - bins.base_of(b)) * step) : 1u);
+                        }
+                    });
+                }
+                double part = (double)row_bin(sm, cluster);
+                if (by_mass) part *= exp((double)bins.base_of(threadIdx.x) - (double)m) / (double)step;
+                const double upto = above + block_scan(part, sm.wscan);
+                if (!by_mass && __syncthreads_or(threadIdx.x == NB - 1 && upto < target))
+                    break;  // fewer elements than top-k asks for: all stay
+                int b = first_of(sm, upto >= target, threadIdx.x, NB - 1);
+                // the bin's exact limits, its elements into the list; a neighbour's if the
+                // rounded masses misled
+                Joined t;
+                for (int tries = 0; tries < 2 * NB; ++tries) {
+                    Mass over;
+                    double in = 0.0;
+                    unsigned n_over = 0, n_in = 0;
+                    float lo = INFINITY, hi = -INFINITY;
+                    const float fb = (float)b;
+                    R.each_vector([&](int j, uint4 x) {
+                        float y[E], w[E];
+                        unpack<T>(x, R.s, y);
+                        unsigned inside = 0;  // the vector's elements in the bin
+                        if (bins.shift < 0) {
+                            constexpr float kWhole = 12582912.f;
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                const float whole = bins.place(y[e]) + kWhole - kWhole;
+                                // past yhi or ylo: no bin (the interval is the first one)
+                                const bool here = y[e] >= ylo;
+                                inside |= here && whole == fb ? 1u << e : 0u;
+                                w[e] = here && whole < fb ? y[e] : -INFINITY;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                const bool here = y[e] >= ylo && y[e] <= yhi;
+                                const int q = here ? bins.of(y[e]) : NB;
+                                inside |= q == b ? 1u << e : 0u;
+                                w[e] = q < b ? y[e] : -INFINITY;
+                            }
+                        }
+                        if (tied) {
 #pragma unroll
                             for (int e = 0; e < E; ++e)
-                                if (y[e] == ylo && keep.ranked(y[e], sl.index(j, e))) ++k;
-                        }
-                        unsigned incl = k;
-#pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const unsigned t = __shfl_up_sync(0xffffffffu, incl, o);
-                            if (lane >= o) incl += t;
-                        }
-                        int64_t at = run + incl - k;
-                        if (k > 0 && at < nth && nth <= at + k) {
-                            for (int e = 0; e < E; ++e)
-                                if (y[e] == ylo && keep.ranked(y[e], sl.index(j, e)) && ++at == nth) {
-                                    const int64_t idx = sl.index(j, e);
-                                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(
-                                                     ring::mapa(ring::saddr(&sm.ilim), 0)),
-                                                 "l"(idx)
-                                                 : "memory");
+                                if (!keep.allows(y[e], sl, j, e)) {
+                                    w[e] = -INFINITY;
+                                    inside &= ~(1u << e);
                                 }
                         }
-                        run += __shfl_sync(0xffffffffu, incl, 31);
-                    }
+                        if (by_mass) {
+#pragma unroll
+                            for (int e = 0; e < E; e += 2) {
+                                const float2 d = add2(make_float2(w[e], w[e + 1]), splat(-m));
+                                w[e] = expf(d.x);
+                                w[e + 1] = expf(d.y);
+                            }
+                            over.add(w);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) n_over += w[e] > -INFINITY;
+                        }
+                        n_in += __popc(inside);
+                        append(sm, inside, y, sl.index(j, 0), [&](float v) {
+                            lo = fminf(lo, v);
+                            hi = fmaxf(hi, v);
+                            if (by_mass) in += (double)expf(v - m);
+                        });
+                    });
+                    t = exchange<A | B | N | RANGE, WARPS>(sm, R.phase, cluster, rank,
+                                                    by_mass ? over.total() : (double)n_over,
+                                                    by_mass ? in : (double)n_in, n_in, lo, hi);
+                    const int b0 = b;
+                    if (t.a > 0.0 && above + t.a >= target && b > 0)
+                        --b;
+                    else if ((t.n == 0 || above + t.a + t.b < target) && b < NB - 1)
+                        ++b;
+                    if (b == b0) break;
+                    if (threadIdx.x == 0) sm.list_n = 0;
+                    __syncthreads();
                 }
-                ring::cluster_sync();
-                uint64_t ib;
-                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(ib) : "r"(ring::mapa(ring::saddr(&sm.ilim), 0)) : "memory");
-                keep.tau = ylo;
-                keep.ilim = (int64_t)ib;
-                ring::cluster_sync();
-                break;
+                if (t.n == 0) break;  // not reached: the interval holds the crossing element
+                above += t.a;
+                ylo = t.lo;
+                yhi = t.hi;
+                if (t.n <= (unsigned)kListCap) {
+                    // the crossing element by rank in the list
+                    join_lists(sm, rank, t.n_before);
+                    if (leader) {
+                        const int count = (int)t.n;
+                        uint64_t e[PER], word[PER];
+#pragma unroll
+                        for (int r = 0; r < PER; ++r) {
+                            const int i = r * THREADS + threadIdx.x;
+                            e[r] = i < count ? sm.list[i] : 0;
+                            word[r] = i >= count ? 0
+                                      : by_mass  ? weight_word(expf(entry_value(e[r]) - m))
+                                                 : ((uint64_t)1 << kCountBits) | 1u;
+                        }
+                        const uint64_t all = word_weight(block_sum64(sm, word[0] + word[1] + word[2] + word[3]));
+                        const double rest = ceil((target - above) * (by_mass ? (double)kUnit : 1.0));
+                        const uint64_t at = select_entry(sm, e, word, entry(ylo, 0xffffffffll), entry(yhi, 0),
+                                                         min(all, (uint64_t)fmax(rest, 1.0)));
+                        if (threadIdx.x == 0) tell(sm, cluster, entry_value(at), entry_index(at));
+                    }
+                    ring::cluster_sync();
+                    break;
+                }
+                if (ylo == yhi) {
+                    // all equal: the nth of them in index order
+                    const double each_one = by_mass ? (double)expf(ylo - m) : 1.0;
+                    const int64_t nth =
+                        (int64_t)fmin(fmax(ceil((target - above) / each_one), 1.0), (double)t.n);
+                    unsigned n = 0;
+                    R.each([&](int j, float (&y)[E]) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (y[e] == ylo && keep.allows(y[e], sl, j, e)) ++n;
+                    });
+                    const Joined o = exchange<N, WARPS>(sm, R.phase, cluster, rank, 0.0, 0.0, n, 0.f, 0.f);
+                    int64_t run = o.n_before;
+                    for (int i = 0; i < warp; ++i) run += sm.wn[i];
+                    if (run < nth && nth <= run + (int64_t)sm.wn[warp]) {
+                        for (int j0 = sl.w0; j0 < sl.w1; j0 += 32) {
+                            const int j = j0 + lane;
+                            unsigned k = 0;
+                            float y[E];
+                            if (j < sl.w1) {
+                                unpack<T>(sl.vec(j), R.s, y);
+#pragma unroll
+                                for (int e = 0; e < E; ++e)
+                                    if (y[e] == ylo && keep.allows(y[e], sl, j, e)) ++k;
+                            }
+                            unsigned incl = k;
+#pragma unroll
+                            for (int o2 = 1; o2 < 32; o2 <<= 1) {
+                                const unsigned x = __shfl_up_sync(0xffffffffu, incl, o2);
+                                if (lane >= o2) incl += x;
+                            }
+                            int64_t at = run + incl - k;
+                            if (k > 0 && at < nth && nth <= at + k) {
+#pragma unroll
+                                for (int e = 0; e < E; ++e)
+                                    if (y[e] == ylo && keep.allows(y[e], sl, j, e) && ++at == nth)
+                                        tell(sm, cluster, ylo, sl.index(j, e));
+                            }
+                            run += __shfl_sync(0xffffffffu, incl, 31);
+                        }
+                    }
+                    ring::cluster_sync();
+                    break;
+                }
+                bins = Bins::keys(yhi, ylo);
             }
-            bins = Bins::keys(yhi, ylo);
+            if (sm.told) {
+                keep.tau = sm.tau;
+                keep.ilim = sm.ilim;
+            }
+            if (!by_mass && use_p) Z = R.template kept_mass<false>(sm, keep).a;
         }
-        if (!by_mass && use_p) {
-            Z = R.kept_mass(keep, false);
-            bins = Bins::linear(m, fmaxf(keep.tau, floor));
-        }
+        keep.min_p = min_p > 0.f ? min_p : 0.f;
+        const Joined C = R.template kept_mass<false>(sm, keep);
+        R.template draw<false>(sm, keep, C, u * C.a, S, p, row);
     }
-    keep.min_p = min_p > 0.f ? min_p : 0.f;
-    const double C = R.kept_mass(keep, false);
-    R.draw(keep, false, u * C, C, S, p, row);
-    ring::cluster_sync();
 }
 
 }  // namespace sample
