@@ -101,6 +101,7 @@ struct Smem {
     double wsum_b[kMaxWarps];
     unsigned wn[kMaxWarps];
     float wlo[kMaxWarps], whi[kMaxWarps];
+    double logs[2];            // of the whole and the kept mass
 };
 struct FilterSmem : Smem {
     uint64_t list[kListCap];
@@ -205,16 +206,35 @@ __device__ __forceinline__ void unpack(uint4 v, float s, float (&y)[DT<T>::kEPV]
     }
 }
 
-// Largest element of a vector (NaN if it holds one).
+// Largest element of a set of vectors (NaN if it holds one), in the elements' type: two
+// 16-bit elements per instruction.
+template <typename T>
+struct Peak {
+    uint32_t v = sizeof(T) == 4                  ? 0xff800000u
+                 : std::is_same_v<T, __half>     ? 0xfc00fc00u
+                                                 : 0xff80ff80u;
+    __device__ __forceinline__ void add(uint4 x) {
+        if constexpr (sizeof(T) == 4)
+            v = __float_as_uint(fmax_nan(
+                __uint_as_float(v), fmax_nan(fmax_nan(__uint_as_float(x.x), __uint_as_float(x.y)),
+                                             fmax_nan(__uint_as_float(x.z), __uint_as_float(x.w)))));
+        else
+            v = DT<T>::max2(v, DT<T>::max2(DT<T>::max2(x.x, x.y), DT<T>::max2(x.z, x.w)));
+    }
+    __device__ __forceinline__ float value() const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(v);
+        } else {
+            const float2 f = DT<T>::to_f2(v);
+            return fmax_nan(f.x, f.y);
+        }
+    }
+};
 template <typename T>
 __device__ __forceinline__ float vec_max(uint4 v) {
-    if constexpr (sizeof(T) == 4) {
-        return fmax_nan(fmax_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
-                        fmax_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
-    } else {
-        const float2 f = DT<T>::to_f2(DT<T>::max2(DT<T>::max2(v.x, v.y), DT<T>::max2(v.z, v.w)));
-        return fmax_nan(f.x, f.y);
-    }
+    Peak<T> p;
+    p.add(v);
+    return p.value();
 }
 
 // Exact running sum of weights in [0, 1]: multiples of 2^-13 add exactly in fp32 (up to 2^11
@@ -658,15 +678,17 @@ struct Row {
         const double end = rank + 1 < cluster ? c.before + sm.slot[phase ^ 1][rank].a : c.a;
         const double blk = sm.slot[phase ^ 1][rank].a;
         if (!(blk > 0.0) || target < c.before || !(target < end || !(end < c.a))) return;
+        // the logarithms while the others look for the element
+        if (lane == 0 && warp < 2) sm.logs[warp] = log(warp == 0 ? sum : c.a);
         int part = 0;
         double base = c.before, run = c.before;
+#pragma unroll
         for (int i = 0; i < WARPS; ++i) {
             const double w = sm.wsum[i];
-            if (w > 0.0) {
+            if (w > 0.0 && !(run > target)) {
                 part = i;
                 base = run;
                 run += w;
-                if (run > target) break;
             }
         }
         const int per = (sl.nvec + WARPS - 1) / WARPS;
@@ -692,10 +714,12 @@ struct Row {
             __syncthreads();
             double before = base, all = base;
             int last = 0;  // the last warp with any mass
+#pragma unroll
             for (int i = 0; i < WARPS; ++i) {
+                const double w = sm.wsum_b[i];
                 if (i == warp) before = all;
-                if (sm.wsum_b[i] > 0.0) last = i;
-                all += sm.wsum_b[i];
+                if (w > 0.0) last = i;
+                all += w;
             }
             const bool crossed = all > target;
             // one warp holds it: the first whose end exceeds the target; until one does, the
@@ -717,8 +741,8 @@ struct Row {
                             d = y[e] - m;
                         }
                     p.token[row] = token;
-                    p.logprob[row] = (float)((double)d - log(sum));
-                    p.kept_logprob[row] = (float)((double)d - log(c.a));
+                    p.logprob[row] = (float)((double)d - sm.logs[0]);
+                    p.kept_logprob[row] = (float)((double)d - sm.logs[1]);
                 }
             }
             if (crossed) return;
@@ -759,9 +783,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
     sl.w1 = min(sl.nvec, sl.w0 + per_warp);
 
     // ---- load; the maxima of this thread's NG groups of vectors ----
-    float g[NG];
-#pragma unroll
-    for (int q = 0; q < NG; ++q) g[q] = -INFINITY;
+    Peak<T> peak[NG];
     if constexpr (FILTER) {
         sm.hist[threadIdx.x] = 0;
         if (threadIdx.x == 0) {
@@ -770,32 +792,38 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
             sm.told = 0;
         }
     }
-    int j = sl.w0 + lane;
-    for (; j + 32 * (NG - 1) < sl.w1; j += 32 * NG) {
-        uint4 v[NG];
+    auto load = [&](auto get) {
+        int j = sl.w0 + lane;
+        for (; j + 32 * (NG - 1) < sl.w1; j += 32 * NG) {
+            uint4 v[NG];
 #pragma unroll
-        for (int q = 0; q < NG; ++q) v[q] = sl.load_global(j + 32 * q);
+            for (int q = 0; q < NG; ++q) v[q] = get(j + 32 * q);
 #pragma unroll
-        for (int q = 0; q < NG; ++q) {
-            if constexpr (RES) sl.buf[j + 32 * q] = v[q];
-            g[q] = fmax_nan(g[q], vec_max<T>(v[q]));
+            for (int q = 0; q < NG; ++q) {
+                if constexpr (RES) sl.buf[j + 32 * q] = v[q];
+                peak[q].add(v[q]);
+            }
         }
-    }
 #pragma unroll
-    for (int q = 0; q < NG; ++q)
-        if (j + 32 * q < sl.w1) {
-            const uint4 v = sl.load_global(j + 32 * q);
-            if constexpr (RES) sl.buf[j + 32 * q] = v;
-            g[q] = fmax_nan(g[q], vec_max<T>(v));
-        }
+        for (int q = 0; q < NG; ++q)
+            if (j + 32 * q < sl.w1) {
+                const uint4 v = get(j + 32 * q);
+                if constexpr (RES) sl.buf[j + 32 * q] = v;
+                peak[q].add(v);
+            }
+    };
+    if (sl.w0 >= sl.whole0 && sl.w1 <= sl.whole1)  // the warp's part lies inside the row
+        load([&](int j) { return ldg_stream(sl.base + j); });
+    else
+        load([&](int j) { return sl.load_global(j); });
     // the row's temperature
     const float temp = p.temperature ? p.temperature[row] : 1.f;
     const bool greedy = p.temperature ? temp == 0.f : p.greedy0;
     R.s = !p.temperature ? p.scale0 : greedy ? 1.f : (float)(1.0 / (double)temp);
-    float hi = -INFINITY, lo = INFINITY;
+    float g[NG], hi = -INFINITY, lo = INFINITY;
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
-        g[q] *= R.s;
+        g[q] = peak[q].value() * R.s;
         hi = fmax_nan(hi, g[q]);
         if (FILTER && g[q] > -INFINITY) lo = fminf(lo, g[q]);
     }
