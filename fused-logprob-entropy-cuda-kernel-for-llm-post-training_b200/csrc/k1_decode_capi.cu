@@ -238,7 +238,8 @@ int make_tmap8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
     return K1_OK;
 }
 
-// Largest inner dimension: the few-token kernel keeps its scales (64 tokens) in shared memory.
+// Largest inner dimension: the few-token kernel keeps its scales (up to 64 tokens) in shared
+// memory beside the ring.
 constexpr int64_t kMaxInner = 32768;
 
 template <int TN, typename OutT>
@@ -257,25 +258,54 @@ int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
     const size_t smem = S::smem((p.kb_total + split - 1) / split);
     rc = allow_smem(kern, dev, smem);
     if (rc) return rc;
-    const dim3 grid((unsigned)(tiles * split), (unsigned)tok);
+    const dim3 grid((unsigned)(tiles * tok * split));
     return launched(fn, launch_cluster(kern, grid, S::THREADS, smem, split, st, tx, tw, p, split));
+}
+
+// Pairs of the many-token kernel that can be resident at once; its persistent grid must not
+// exceed them.  Cached per device.
+template <typename Kernel>
+int wide_pairs(Kernel kern, int dev, int* out) {
+    static std::atomic<int> cache[kMaxDevices];
+    int v = cache[dev].load(std::memory_order_relaxed);
+    if (v == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2);
+        cfg.blockDim = dim3(k1::fp8::Wide::THREADS);
+        cfg.dynamicSmemBytes = k1::fp8::Wide::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cudaError_t e = cudaOccupancyMaxActiveClusters(&v, kern, &cfg);
+        if (e != cudaSuccess || v < 1)
+            return fail(K1_ERR_CUDA, "cudaOccupancyMaxActiveClusters: %s (%d)", cudaGetErrorString(e), v);
+        cache[dev].store(v, std::memory_order_relaxed);
+    }
+    *out = v;
+    return K1_OK;
 }
 
 template <typename OutT>
 int wide(const char* fn, k1::fp8::Params p, const void* x, int64_t ldx, const void* w, int64_t ldw,
-         int64_t inner, int sms, int dev, cudaStream_t st) {
+         int64_t inner, int dev, cudaStream_t st) {
     using S = k1::fp8::Wide;
     CUtensorMap tx, tw;
     int rc = make_tmap8(&tx, x, p.m, inner, ldx, k1::fp8::BM, "x");
-    if (!rc) rc = make_tmap8(&tw, w, p.n, inner, ldw, S::BN, "weight");
+    if (!rc) rc = make_tmap8(&tw, w, p.n, inner, ldw, S::LOAD_N, "weight");
     if (rc) return rc;
-    p.m_blocks = (int)((p.m + 127) / 128);
+    p.m_tiles = (int)((p.m + S::TM - 1) / S::TM);
     p.n_tiles = (int)((p.n + S::BN - 1) / S::BN);
     auto kern = k1::fp8::k1_fp8_wide_kernel<OutT>;
+    int pairs = 0;
     rc = allow_smem(kern, dev, S::SMEM);
+    if (!rc) rc = wide_pairs(kern, dev, &pairs);
     if (rc) return rc;
-    const int64_t grid = std::min<int64_t>(sms, (int64_t)p.m_blocks * p.n_tiles);
-    return launched(fn, launch(kern, grid, S::THREADS, (size_t)S::SMEM, st, tx, tw, p));
+    const dim3 grid((unsigned)(2 * std::min<int64_t>(pairs, (int64_t)p.m_tiles * p.n_tiles)));
+    return launched(fn, launch_cluster(kern, grid, S::THREADS, (size_t)S::SMEM, 2, st, tx, tw, p));
 }
 
 template <typename OutT>
@@ -283,10 +313,10 @@ int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
            int64_t inner, int sms, int dev, cudaStream_t st) {
     if (p.m <= 16) return skinny<16, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
     if (p.m <= 32) return skinny<32, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-    const int64_t wide_tiles = (p.m + 127) / 128 * ((p.n + 255) / 256);
-    if (p.m <= 64 || wide_tiles < sms / 2)
+    const int64_t wide_tiles = (p.m + 255) / 256 * ((p.n + 255) / 256);
+    if (p.m <= 128 || wide_tiles < sms / 4)
         return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-    return wide<OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+    return wide<OutT>(fn, p, x, ldx, w, ldw, inner, dev, st);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -465,7 +495,7 @@ int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const 
     if (inner < 16 || inner % 16 != 0 || inner > kMaxInner)
         return fail(K1_ERR_INVALID_ARGUMENT, "%s: inner must be a multiple of 16 in [16, %lld], got %lld", fn,
                     (long long)kMaxInner, (long long)inner);
-    if (tokens > (int64_t)65535 * 64 || outer > (int64_t)1 << 27)
+    if (tokens > (int64_t)1 << 24 || outer > (int64_t)1 << 27 || (tokens + 63) / 64 * ((outer + 127) / 128) > (int64_t)1 << 28)
         return fail(K1_ERR_INVALID_ARGUMENT, "%s: tokens or outer too large", fn);
     if (tokens == 0 || outer == 0) return K1_OK;
     if (!x || !x_scales || !weight || !weight_scales || !y)

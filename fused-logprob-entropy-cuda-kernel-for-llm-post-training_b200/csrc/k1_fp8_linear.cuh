@@ -16,9 +16,10 @@
 // a cluster of up to 8 when the weight has too few rows to fill the SMs, and the parts are
 // added through distributed shared memory in rank order (no atomics).
 //
-// Many tokens (k1_fp8_wide_kernel): 128 tokens x 256 rows of the weight per tile, one
-// persistent block per SM.  A thread owns one token and 128 columns (one block of weight
-// rows, so its scale is one product per block), 128 accumulators in registers.
+// Many tokens (k1_fp8_wide_kernel): 256 tokens x 256 rows of the weight per tile and pair of
+// CTAs, persistent.  A thread owns one token and 128 columns (one block of weight rows, so its
+// scale is one product per block), 128 accumulators in registers; it loads the next 32
+// columns from TMEM while it adds the last.
 //
 // Every mbarrier wait is bounded; one that runs out sets bit 4 of the wait status word, and
 // the outputs that could not be finished are NaN.
@@ -64,15 +65,28 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem) {
                  : "memory");
 }
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+// Bounded wait on the barrier at a shared-memory address.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort) {
     for (int i = 0; i < ring::kMaxTries; ++i) {
-        if (ring::try_wait(bar, parity)) return true;
+        if (ring::try_wait_at(bar, parity)) return true;
         if (*abort) return false;
     }
     atomicOr(&k1_ring_error, (unsigned)kAbortBit);
     *abort = 1;
     return false;
 }
+
+// A place in a ring of N slots and the parity of its current round.
+template <int N>
+struct Place {
+    uint32_t slot = 0, parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == N) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+};
 
 // 16 consecutive fp32 columns of this thread's TMEM lane (warp-collective).
 template <int OFF, int N>
@@ -88,13 +102,34 @@ __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[N]
         : "r"(taddr));
 }
 
+// Wait for this thread's TMEM loads; tied to the registers of one, so that nothing that reads
+// them is moved ahead of the wait.
+__device__ __forceinline__ void tmem_wait_on(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                   "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                   "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_on(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
 struct Params {
     const float* xs;  // [m, kb_total]
     const float* ws;  // [ceil(n / 128), kb_total]
     void* y;          // [m] rows of ldy elements
     int64_t m, n, ldy;
     int kb_total;     // ceil(k / 128)
-    int m_blocks, n_tiles;
+    int m_tiles, n_tiles;  // many tokens: tiles of 256 x 256
 };
 
 // ------------------------------------------------------------------------------------
@@ -105,7 +140,10 @@ struct Skinny {
     static constexpr int W_BYTES = BM * BK;           // 16 KB
     static constexpr int X_BYTES = TN * BK;
     static constexpr int STAGE = W_BYTES + X_BYTES;
-    static constexpr int STAGES = 4;
+#ifndef K1_SK_STAGES
+#define K1_SK_STAGES 4
+#endif
+    static constexpr int STAGES = K1_SK_STAGES;
     static constexpr int NBUF = TN <= 32 ? 4 : 2;     // TMEM buffers
     static constexpr int COLS = NBUF * TN;            // 64, 128, 128
     static constexpr int THREADS = 192;
@@ -114,8 +152,11 @@ struct Skinny {
     static constexpr size_t smem(int kb) { return 1024 + RING + 256 + (size_t)kb * TN * 4; }
 };
 
+#ifndef K1_SK_MINB
+#define K1_SK_MINB 2
+#endif
 template <int TN, typename OutT>
-__global__ void __launch_bounds__(192)
+__global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
     k1_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x,
                          const __grid_constant__ CUtensorMap tmap_w, Params p, int split) {
     using S = Skinny<TN>;
@@ -133,8 +174,11 @@ __global__ void __launch_bounds__(192)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = split > 1 ? (int)ring::cluster_rank() : 0;
-    const int tile = blockIdx.x / split;  // 128 rows of the weight
-    const int tok0 = blockIdx.y * TN;
+    // token blocks of one tile (128 rows of the weight) run side by side: the weight comes from
+    // HBM once and from L2 for the others
+    const int tok_blocks = (int)((p.m + TN - 1) / TN);
+    const int tile = (int)(blockIdx.x / split) / tok_blocks;
+    const int tok0 = ((int)(blockIdx.x / split) - tile * tok_blocks) * TN;
     const int kb0 = (int)((int64_t)rank * p.kb_total / split);
     const int kb1 = (int)((int64_t)(rank + 1) * p.kb_total / split);
     if (threadIdx.x == 0) {
@@ -144,7 +188,7 @@ __global__ void __launch_bounds__(192)
         }
         for (int a = 0; a < S::NBUF; ++a) {
             ring::bar_init(&tfull[a], 1);
-            ring::bar_init(&tempty[a], 128);
+            ring::bar_init(&tempty[a], 4);  // one arrival per epilogue warp
         }
         ring::bar_init(drain, 1);
         *abort = 0;
@@ -161,52 +205,66 @@ __global__ void __launch_bounds__(192)
     pdl_wait();
     pdl_trigger();
 
+    // shared-memory addresses
+    const uint32_t a_ring = ring::saddr(smem), a_full = ring::saddr(full), a_empty = ring::saddr(empty),
+                   a_tfull = ring::saddr(tfull), a_tempty = ring::saddr(tempty);
+    // The producer's and the issuer's warp walk their loops whole; one elected lane issues.
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            int issued = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-                const int s = issued % S::STAGES;
-                if (!wait(&empty[s], ((issued / S::STAGES) & 1) ^ 1u, abort)) {
-                    ok = false;
-                    break;
-                }
-#ifdef K1_WAIT_TEST
-                if (blockIdx.x == 0 && blockIdx.y == 0 && (long long)issued == k1_test_withhold) {
-                    ok = false;  // test only: block 0 issues nothing more
-                    break;
-                }
-#endif
-                unsigned char* st = smem + s * S::STAGE;
-                ring::arrive_expect(&full[s], S::STAGE);
-                tma_load_2d(st, &tmap_w, kb * BK, tile * BM, &full[s]);
-                tma_load_2d(st + S::W_BYTES, &tmap_x, kb * BK, tok0, &full[s]);
+        Place<S::STAGES> at;
+        bool ok = true;
+        int issued = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++issued, at.next()) {
+            if (!wait(a_empty + at.slot * 8, at.parity ^ 1u, abort)) {
+                ok = false;
+                break;
             }
-            if (!ok)  // stopping early: wait (bounded) for the copies in flight
-                for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
-                    ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+#ifdef K1_WAIT_TEST
+            if (blockIdx.x == 0 && (long long)issued == k1_test_withhold) {
+                ok = false;  // test only: block 0 issues nothing more
+                break;
+            }
+#endif
+            const uint32_t st = a_ring + at.slot * S::STAGE, bar = a_full + at.slot * 8;
+            if (ring::elect_one()) {
+                ring::arrive_expect(&full[at.slot], S::STAGE);
+                tma_load_2d_at(st, &tmap_w, kb * BK, tile * BM, bar);
+                tma_load_2d_at(st + S::W_BYTES, &tmap_x, kb * BK, tok0, bar);
+            }
+            __syncwarp();
         }
+        if (!ok)  // stopping early: wait (bounded) for the copies in flight
+            for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
+                ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         __syncwarp();
         if (split > 1) asm volatile("bar.arrive 2, 160;" ::: "memory");  // no copy is in flight
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t base = ring::saddr(smem);
-            for (int i = 0; i < kb1 - kb0; ++i) {
-                const int s = i % S::STAGES, a = i % S::NBUF;
-                if (!wait(&tempty[a], ((i / S::NBUF) & 1) ^ 1u, abort)) break;
-                if (!wait(&full[s], (i / S::STAGES) & 1, abort)) break;
-                tc_fence_after();
-                const uint64_t dw = smem_desc(base + s * S::STAGE);
-                const uint64_t dx = smem_desc(base + s * S::STAGE + S::W_BYTES);
+        Place<S::STAGES> at;
+        Place<S::NBUF> acc;
+        const uint64_t dw0 = smem_desc(a_ring), dx0 = smem_desc(a_ring + S::W_BYTES);
+        // both barriers of the next block are tested together, while this one's MMAs run
+        bool freed = true, there = false;
+        for (int i = 0; i < kb1 - kb0; ++i) {
+            if (!freed && !wait(a_tempty + acc.slot * 8, acc.parity ^ 1u, abort)) break;
+            if (!there && !wait(a_full + at.slot * 8, at.parity, abort)) break;
+            tc_fence_after();
+            const uint64_t dw = dw0 + at.slot * (S::STAGE >> 4), dx = dx0 + at.slot * (S::STAGE >> 4);
+            const uint32_t d = tmem + acc.slot * TN;
+            if (ring::elect_one()) {
 #pragma unroll
                 for (int k = 0; k < BK / UK; ++k)  // +32 bytes per K slice: +2 in >> 4 units
-                    umma8<TN>(tmem + (uint32_t)(a * TN), dw + 2 * k, dx + 2 * k, k > 0 ? 1u : 0u);
-                umma_commit(&empty[s]);
-                umma_commit(&tfull[a]);
+                    umma8<TN>(d, dw + 2 * k, dx + 2 * k, k > 0 ? 1u : 0u);
+                umma_commit_at(a_empty + at.slot * 8);
+                umma_commit_at(a_tfull + acc.slot * 8);
             }
-            umma_commit(drain);  // every MMA issued has completed before the TMEM is freed
-            ring::wait(drain, 0);
+            __syncwarp();
+            at.next();
+            acc.next();
+            there = ring::test_at(a_full + at.slot * 8, at.parity);
+            freed = ring::test_at(a_tempty + acc.slot * 8, acc.parity ^ 1u);
         }
+        if (ring::elect_one()) umma_commit(drain);  // every MMA issued has completed before
+        __syncwarp();                               // the TMEM is freed
+        ring::wait(drain, 0);
     } else {
         // each thread owns one row of the weight (a TMEM lane) and all TN tokens
         const int t = threadIdx.x - 64;
@@ -215,43 +273,58 @@ __global__ void __launch_bounds__(192)
         const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16);
         const int nkb = kb1 - kb0;
         const float* ws = p.ws + (int64_t)tile * p.kb_total + kb0;
-        for (int i = t; i < nkb * TN; i += 128) {
-            const int tok = i / nkb, kb = i - tok * nkb;
-            const int64_t m = tok0 + tok;
-            scales[kb * TN + tok] =
-                m < p.m ? __ldg(p.xs + m * p.kb_total + kb0 + kb) * __ldg(ws + kb) : 0.f;
+        {
+            // a thread's token is fixed (TN divides 128); eight loads in flight
+            const int64_t m = tok0 + t % TN;
+            const float* xs = p.xs + (m < p.m ? m : 0) * p.kb_total + kb0;
+            constexpr int STEP = 128 / TN;
+            for (int kb = t / TN; kb < nkb; kb += 8 * STEP) {
+                float f[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    f[q] = kb + q * STEP < nkb ? __ldg(xs + kb + q * STEP) * __ldg(ws + kb + q * STEP) : 0.f;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (kb + q * STEP < nkb) scales[(kb + q * STEP) * TN + t % TN] = m < p.m ? f[q] : 0.f;
+            }
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
         float acc[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[j] = 0.f;
-        for (int i = 0; i < nkb; ++i) {
-            const int a = i % S::NBUF;
+        Place<S::NBUF> buf;
+        for (int i = 0; i < nkb; ++i, buf.next()) {
+            const uint32_t a = buf.slot;
             // warp-uniform: the TMEM loads below are warp-collective
-            if (!__all_sync(0xffffffffu, wait(&tfull[a], (i / S::NBUF) & 1, abort))) {
+            if (!__all_sync(0xffffffffu, wait(a_tfull + a * 8, buf.parity, abort))) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[j] = __int_as_float(0x7fc00000);
                 break;
             }
             tc_fence_after();
-            uint32_t r[TN];
-            tmem_ld16_async<0>(tlane + (uint32_t)(a * TN), r);
-            if constexpr (TN >= 32) tmem_ld16_async<16 % TN>(tlane + (uint32_t)(a * TN + 16), r);
-            if constexpr (TN >= 64) {
-                tmem_ld16_async<32 % TN>(tlane + (uint32_t)(a * TN + 32), r);
-                tmem_ld16_async<48 % TN>(tlane + (uint32_t)(a * TN + 48), r);
-            }
-            tmem_wait();
-            tc_fence_before();
-            ring::arrive(&tempty[a]);
+            constexpr int CW = TN < 32 ? TN : 32;  // columns per TMEM wait
             const float4* sc = reinterpret_cast<const float4*>(scales + i * TN);
 #pragma unroll
-            for (int j = 0; j < TN; j += 4) {
-                const float4 f = sc[j / 4];
-                acc[j] = fmaf(__uint_as_float(r[j]), f.x, acc[j]);
-                acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), f.y, acc[j + 1]);
-                acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), f.z, acc[j + 2]);
-                acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), f.w, acc[j + 3]);
+            for (int c = 0; c < TN; c += CW) {
+                uint32_t r[CW];
+                if constexpr (CW == 32)
+                    tmem_ld32_async<0>(tlane + (uint32_t)(a * TN + c), r);
+                else
+                    tmem_ld16_async<0>(tlane + (uint32_t)(a * TN + c), r);
+                tmem_wait_on(r);
+                if (c + CW == TN) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ring::arrive_at(a_tempty + a * 8);
+                }
+#pragma unroll
+                for (int j = 0; j < CW; j += 4) {
+                    const float4 f = sc[(c + j) / 4];
+                    acc[c + j] = fmaf(__uint_as_float(r[j]), f.x, acc[c + j]);
+                    acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]), f.y, acc[c + j + 1]);
+                    acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]), f.z, acc[c + j + 2]);
+                    acc[c + j + 3] = fmaf(__uint_as_float(r[j + 3]), f.w, acc[c + j + 3]);
+                }
             }
         }
         const int64_t col = (int64_t)tile * BM + row;
@@ -304,50 +377,76 @@ __global__ void __launch_bounds__(192)
 // ------------------------------------------------------------------------------------
 // Many tokens
 // ------------------------------------------------------------------------------------
+// A pair of CTAs (two SMs) computes 256 tokens x 256 weight rows with cta_group::2 MMAs: each
+// CTA stages its 128 tokens and its 128 of the weight rows and keeps the sums of its tokens.
+// One CTA alone with 128 x 256 moves 1.5 times the bytes through its shared memory (48 KB in
+// by TMA and 48 KB out to the tensor cores per 512 cycles of MMA, at 128 bytes per cycle).
 struct Wide {
     static constexpr int BN = 256;
-    static constexpr int X_BYTES = BM * BK;  // 16 KB
-    static constexpr int W_BYTES = BN * BK;  // 32 KB
+    static constexpr int TM = 2 * BM;              // tokens per tile
+    static constexpr int LOAD_N = BN / 2;          // weight rows per CTA
+    static constexpr int X_BYTES = BM * BK;        // 16 KB
+    static constexpr int W_BYTES = LOAD_N * BK;    // 16 KB
     static constexpr int STAGE = X_BYTES + W_BYTES;
-    static constexpr int STAGES = 4;
+    static constexpr int STAGES = 6;
     static constexpr int NBUF = 2;
-    static constexpr int COLS = NBUF * BN;   // 512: all of TMEM
+    static constexpr int COLS = NBUF * BN;         // 512: all of TMEM
     static constexpr int EPI_WARPS = 8;
-    static constexpr int THREADS = (2 + EPI_WARPS) * 32;
-    static constexpr int GROUP_M = 16;       // token blocks that share the weight tiles in L2
-    static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
+    static constexpr int CPT = BN * 4 / EPI_WARPS; // columns per thread: 128
+    static constexpr int THREADS = (4 + EPI_WARPS) * 32;
+    // Registers: 384 threads start with 168 each; the first warpgroup goes down to 40 and the
+    // other two up to 232 (128 x 40 + 256 x 232 = 384 x 168).
+    static constexpr int REGS_DOWN = 40, REGS_UP = 232;
+    static constexpr int SB = 32;                  // blocks of K per chunk of token scales
+    static constexpr int SROW = BM + 1;            // its row pitch: stores along K meet no bank twice
+    static constexpr int S_BYTES = SB * SROW * 4 + SB * 8;  // and the two weight blocks' scales
+    static constexpr int GROUP_M = 8;              // token tiles that share the weight tiles in L2
+    static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * S_BYTES + 256;
+    static constexpr uint32_t IDESC =
+        (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
 };
+static_assert(Wide::SMEM <= 227 * 1024, "shared memory of one block");
 
-// Tiles in groups of GROUP_M token blocks, token block fastest.
-__device__ __forceinline__ void wide_tile(const Params& p, int u, int& mb, int& nt) {
+// Tiles in groups of GROUP_M token tiles, token tile fastest.
+__device__ __forceinline__ void wide_tile(const Params& p, int u, int& mt, int& nt) {
     const int per_group = Wide::GROUP_M * p.n_tiles;
     const int g = u / per_group, r = u - g * per_group;
-    const int rows = min(Wide::GROUP_M, p.m_blocks - g * Wide::GROUP_M);
+    const int rows = min(Wide::GROUP_M, p.m_tiles - g * Wide::GROUP_M);
     nt = r / rows;
-    mb = g * Wide::GROUP_M + (r - nt * rows);
+    mt = g * Wide::GROUP_M + (r - nt * rows);
 }
 
-// 32 columns of one row, `valid` of them.
+// 32 columns of one row, `valid` of them; align: bytes that every row piece starts at.
 template <typename OutT>
-__device__ __forceinline__ void store_row32(OutT* dst, const float* v, int valid, bool vec) {
-    if (vec && valid >= 32) {
-        if constexpr (sizeof(OutT) == 4) {
+__device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int valid, int align) {
+    if (align >= 16 && valid >= 32) {
+        constexpr int E = 16 / sizeof(OutT);  // elements of a vector
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else {
+        for (int i = 0; i < 32; i += 2 * E) {
+            uint4 w[2];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-                *reinterpret_cast<uint4*>(dst + i) =
-                    make_uint4(DT<OutT>::from_f2(make_float2(v[i], v[i + 1])),
-                               DT<OutT>::from_f2(make_float2(v[i + 2], v[i + 3])),
-                               DT<OutT>::from_f2(make_float2(v[i + 4], v[i + 5])),
-                               DT<OutT>::from_f2(make_float2(v[i + 6], v[i + 7])));
+            for (int h = 0; h < 2; ++h) {
+                const float2* s = v + (i + h * E) / 2;
+                if constexpr (sizeof(OutT) == 4)
+                    w[h] = make_uint4(__float_as_uint(s[0].x), __float_as_uint(s[0].y), __float_as_uint(s[1].x),
+                                      __float_as_uint(s[1].y));
+                else
+                    w[h] = make_uint4(DT<OutT>::from_f2(s[0]), DT<OutT>::from_f2(s[1]),
+                                      DT<OutT>::from_f2(s[2 % (E / 2)]), DT<OutT>::from_f2(s[3 % (E / 2)]));
+            }
+            if (align >= 32) {
+                stg32(dst + i, w[0], w[1]);
+            } else {
+                stg_stream(dst + i, w[0]);
+                stg_stream(dst + i + E, w[1]);
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < valid) DT<OutT>::store1(dst + i, v[i]);
+        for (int i = 0; i < 16; ++i) {
+            if (2 * i < valid) DT<OutT>::store1(dst + 2 * i, v[i].x);
+            if (2 * i + 1 < valid) DT<OutT>::store1(dst + 2 * i + 1, v[i].y);
+        }
     }
 }
 
@@ -359,24 +458,34 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
     extern __shared__ __align__(16) unsigned char wd_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(wd_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE);
+    float* scales = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);  // two chunks
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE + 2 * S::S_BYTES);
     uint64_t* empty = full + S::STAGES;
     uint64_t* tfull = empty + S::STAGES;
     uint64_t* tempty = tfull + S::NBUF;
-    uint64_t* drain = tempty + S::NBUF;
+    uint64_t* sfull = tempty + S::NBUF;
+    uint64_t* sempty = sfull + 2;
+    uint64_t* drain = sempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = p.m_blocks * p.n_tiles;
+    const uint32_t rank = ring::cluster_rank();  // 0: issues the pair's MMAs
+    const bool leader = rank == 0;
+    const int units = p.m_tiles * p.n_tiles;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
-            ring::bar_init(&full[s], 1);
+            ring::bar_init(&full[s], 2);  // both producers arrive at the leader's
             ring::bar_init(&empty[s], 1);
         }
         for (int a = 0; a < S::NBUF; ++a) {
             ring::bar_init(&tfull[a], 1);
-            ring::bar_init(&tempty[a], S::EPI_WARPS * 32);
+            ring::bar_init(&tempty[a], 2 * S::EPI_WARPS);  // at the leader's, one per warp of both
+        }
+        for (int a = 0; a < 2; ++a) {
+            ring::bar_init(&sfull[a], 1);
+            ring::bar_init(&sempty[a], S::EPI_WARPS);
         }
         ring::bar_init(drain, 1);
         *abort = 0;
@@ -384,25 +493,41 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
         prefetch_tmap(&tmap_x);
         prefetch_tmap(&tmap_w);
     }
-    if (warp == 1) tmem_alloc<S::COLS>(tmem_slot);
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         ring::saddr(tmem_slot)),
+                     "r"(S::COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
     __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    ring::cluster_sync();  // both CTAs' barriers are initialised before any remote arrival
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_trigger();
 
-    if (warp == 0) {
-        if (lane == 0) {
+    // shared-memory addresses
+    const uint32_t a_ring = ring::saddr(smem), a_full = ring::saddr(full), a_empty = ring::saddr(empty),
+                   a_tfull = ring::saddr(tfull), a_tempty = ring::saddr(tempty), a_sfull = ring::saddr(sfull),
+                   a_sempty = ring::saddr(sempty);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::REGS_DOWN));
+        if (warp == 0) {
+            // ---------------- TMA producer (each CTA's own tiles) ----------------
+            Place<S::STAGES> at;
             bool ok = true;
             uint32_t issued = 0;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                int mb, nt;
-                wide_tile(p, u, mb, nt);
-                for (int kb = 0; kb < p.kb_total; ++kb, ++issued) {
-                    const int s = issued % S::STAGES;
-                    if (!wait(&empty[s], ((issued / S::STAGES) & 1) ^ 1u, abort)) {
+            const uint32_t cl_full = ring::mapa(a_full, 0);  // the leader's barriers
+            for (int u = first; ok && u < units; u += step) {
+                int mt, nt;
+                wide_tile(p, u, mt, nt);
+                const int row_x = mt * S::TM + (int)rank * BM;
+                const int row_w = nt * S::BN + (int)rank * S::LOAD_N;
+                for (int kb = 0; kb < p.kb_total; ++kb, ++issued, at.next()) {
+                    if (!wait(a_empty + at.slot * 8, at.parity ^ 1u, abort)) {
                         ok = false;
                         break;
                     }
@@ -412,99 +537,188 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                         break;
                     }
 #endif
-                    unsigned char* st = smem + s * S::STAGE;
-                    ring::arrive_expect(&full[s], S::STAGE);
-                    tma_load_2d(st, &tmap_x, kb * BK, mb * BM, &full[s]);
-                    tma_load_2d(st + S::X_BYTES, &tmap_w, kb * BK, nt * S::BN, &full[s]);
+                    const uint32_t st = a_ring + at.slot * S::STAGE, cl = cl_full + at.slot * 8;
+                    if (ring::elect_one()) {
+                        tma_load_2d_pair_at(st, &tmap_x, kb * BK, row_x, cl);
+                        tma_load_2d_pair_at(st + S::X_BYTES, &tmap_w, kb * BK, row_w, cl);
+                        if (leader)
+                            ring::arrive_expect(&full[at.slot], 2 * S::STAGE);
+                        else
+                            ring::arrive_remote(cl);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok)
+            if (!ok && leader)  // stopping early: wait (bounded) for the copies in flight
                 for (uint32_t i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
                     ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t base = ring::saddr(smem);
-            uint32_t i = 0;
+        } else if (warp == 1) {
+            // ---------------- MMA issuer (the leader, for both) ----------------
+            if (leader) {
+                Place<S::STAGES> at;
+                Place<S::NBUF> acc;
+                bool ok = true;
+                const uint64_t dx0 = smem_desc(a_ring), dw0 = smem_desc(a_ring + S::X_BYTES);
+                // both barriers of the next block are tested together, while this one's MMAs run
+                bool freed = true, there = false;
+                for (int u = first; ok && u < units; u += step) {
+                    for (int kb = 0; kb < p.kb_total; ++kb) {
+                        if ((!freed && !wait(a_tempty + acc.slot * 8, acc.parity ^ 1u, abort)) ||
+                            (!there && !wait(a_full + at.slot * 8, at.parity, abort))) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t dx = dx0 + at.slot * (S::STAGE >> 4), dw = dw0 + at.slot * (S::STAGE >> 4);
+                        const uint32_t d = tmem + acc.slot * S::BN;
+                        if (ring::elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < BK / UK; ++k)
+                                asm volatile(
+                                    "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                    "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                                    "l"(dx + 2 * k), "l"(dw + 2 * k), "r"(S::IDESC), "r"(k > 0 ? 1u : 0u));
+                            umma_commit_pair_at(a_empty + at.slot * 8);
+                            umma_commit_pair_at(a_tfull + acc.slot * 8);
+                        }
+                        __syncwarp();
+                        at.next();
+                        acc.next();
+                        there = ring::test_at(a_full + at.slot * 8, at.parity);
+                        freed = ring::test_at(a_tempty + acc.slot * 8, acc.parity ^ 1u);
+                    }
+                }
+                if (ring::elect_one()) umma_commit_pair(drain);  // every MMA issued has completed
+                __syncwarp();                                    // before the TMEM is freed
+                ring::wait(drain, 0);
+            }
+        } else if (warp == 2) {
+            // ---------------- scales: tokens transposed, [K block][token], and weight ----------------
+            // Straight from global memory the epilogue's 32 lanes (32 tokens) would read 32
+            // rows for one block of K: 32 wavefronts per load instead of one.
+            Place<2> at;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                for (int kb = 0; kb < p.kb_total; ++kb, ++i) {
-                    const int s = i % S::STAGES, a = i % S::NBUF;
-                    if (!wait(&tempty[a], ((i / S::NBUF) & 1) ^ 1u, abort) ||
-                        !wait(&full[s], (i / S::STAGES) & 1, abort)) {
+            for (int u = first; ok && u < units; u += step) {
+                int mt, nt;
+                wide_tile(p, u, mt, nt);
+                const int64_t m0 = (int64_t)mt * S::TM + (int64_t)rank * BM;
+                const int rows = (int)max((int64_t)0, min((int64_t)BM, p.m - m0));
+                const int64_t nb = (int64_t)nt * 2, nb_last = (p.n - 1) / 128;
+                for (int k0 = 0; k0 < p.kb_total; k0 += S::SB, at.next()) {
+                    if (!__all_sync(0xffffffffu, wait(a_sempty + at.slot * 8, at.parity ^ 1u, abort))) {
+                        ok = false;
+                        break;
+                    }
+                    const bool in = k0 + lane < p.kb_total;
+                    const float* src = p.xs + m0 * p.kb_total + k0 + lane;
+                    float* chunk = scales + at.slot * (S::S_BYTES / 4);
+                    float* dst = chunk + lane * S::SROW;
+                    for (int r0 = 0; r0 < BM; r0 += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            f[q] = in && r0 + q < rows ? __ldg(src + (int64_t)(r0 + q) * p.kb_total) : 0.f;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) dst[r0 + q] = f[q];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        chunk[S::SB * S::SROW + 2 * lane + h] =
+                            in ? __ldg(p.ws + min(nb + h, nb_last) * p.kb_total + k0 + lane) : 0.f;
+                    __syncwarp();
+                    if (lane == 0) ring::arrive_at(a_sfull + at.slot * 8);
+                }
+            }
+        }
+    } else {
+        // ---------------- epilogue (each CTA's own 128 tokens) ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::REGS_UP));
+        constexpr int CPT = S::CPT;
+        const int quarter = warp & 3;          // TMEM lanes 32 quarter ...: tokens
+        const int part = (warp - 4) >> 2;      // CPT columns: one block of weight rows
+        const int rloc = quarter * 32 + lane;
+        const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * CPT);
+        const uintptr_t yat = reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * sizeof(OutT));
+        const int align = yat % 32 == 0 ? 32 : yat % 16 == 0 ? 16 : 1;
+        const uint32_t cl_tempty = ring::mapa(a_tempty, 0);  // the leader's barriers
+        static_assert(CPT == 128 && S::NBUF == 2, "four loads of 32 columns per block of K");
+        uint32_t buf = 0, parity = 0;
+        Place<2> chunk;
+        bool ok = true;
+        for (int u = first; u < units; u += step) {
+            int mt, nt;
+            wide_tile(p, u, mt, nt);
+            const int64_t row = (int64_t)mt * S::TM + (int64_t)rank * BM + rloc;
+            const int64_t col0 = (int64_t)nt * S::BN + part * CPT;
+            float2 acc[CPT / 2];
+#pragma unroll
+            for (int j = 0; j < CPT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+            uint32_t ra[32], rb[32];
+            auto add = [&](int c0, const uint32_t (&r)[32], float2 g) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 2)
+                    acc[(c0 + j) / 2] =
+                        fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), g, acc[(c0 + j) / 2]);
+            };
+            for (int k0 = 0; ok && k0 < p.kb_total; k0 += S::SB, chunk.next()) {
+                // warp-uniform: the TMEM loads are warp-collective
+                ok = __all_sync(0xffffffffu, wait(a_sfull + chunk.slot * 8, chunk.parity, abort));
+                if (!ok) break;
+                const float* sx = scales + chunk.slot * (S::S_BYTES / 4) + rloc;
+                const float* sw = scales + chunk.slot * (S::S_BYTES / 4) + S::SB * S::SROW + part;
+                const int n = min(S::SB, p.kb_total - k0);
+                for (int kc = 0; kc < n; ++kc) {
+                    const float2 f = splat(sx[kc * S::SROW] * sw[2 * kc]);
+                    if (!__all_sync(0xffffffffu, wait(a_tfull + buf * 8, parity, abort))) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t dx = smem_desc(base + s * S::STAGE);
-                    const uint64_t dw = smem_desc(base + s * S::STAGE + S::X_BYTES);
-#pragma unroll
-                    for (int k = 0; k < BK / UK; ++k)
-                        umma8<S::BN>(tmem + (uint32_t)(a * S::BN), dx + 2 * k, dw + 2 * k,
-                                     k > 0 ? 1u : 0u);
-                    umma_commit(&empty[s]);
-                    umma_commit(&tfull[a]);
+                    // the next 32 columns are loaded while the last ones are added
+                    const uint32_t t = tlane + buf * S::BN;
+                    tmem_ld32_async<0>(t, ra);
+                    tmem_wait_on(ra);
+                    tmem_ld32_async<0>(t + 32, rb);
+                    add(0, ra, f);
+                    tmem_wait_on(rb);
+                    tmem_ld32_async<0>(t + 64, ra);
+                    add(32, rb, f);
+                    tmem_wait_on(ra);
+                    tmem_ld32_async<0>(t + 96, rb);
+                    add(64, ra, f);
+                    tmem_wait_on(rb);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ring::arrive_remote(cl_tempty + buf * 8);
+                    buf ^= 1u;
+                    parity ^= buf ^ 1u;
+                    add(96, rb, f);
                 }
+                __syncwarp();
+                if (lane == 0) ring::arrive_at(a_sempty + chunk.slot * 8);
             }
-            umma_commit(drain);
-            ring::wait(drain, 0);
-        }
-    } else {
-        const int quarter = warp & 3;          // TMEM lanes 32 quarter ...: tokens
-        const int half = (warp - 2) >> 2;      // 128 columns: one block of weight rows
-        const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
-        const bool vec = (p.ldy * sizeof(OutT)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
-        uint32_t i = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            int mb, nt;
-            wide_tile(p, u, mb, nt);
-            const int64_t row = (int64_t)mb * BM + quarter * 32 + lane;
-            const int64_t col0 = (int64_t)nt * S::BN + half * 128;
-            const bool live = row < p.m && col0 < p.n;
-            const float* xs = p.xs + (live ? row : 0) * p.kb_total;
-            const float* ws = p.ws + (live ? col0 / 128 : 0) * p.kb_total;
-            float acc[128];
+            if (!ok) {  // a wait ran out: this tile and the CTA's later ones are NaN
 #pragma unroll
-            for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-            for (int kb = 0; kb < p.kb_total; ++kb, ++i) {
-                const int a = i % S::NBUF;
-                const float f = __ldg(xs + kb) * __ldg(ws + kb);
-                if (ok && !__all_sync(0xffffffffu, wait(&tfull[a], (i / S::NBUF) & 1, abort)))
-                    ok = false;
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t r[32];
-                    tmem_ld32_async<0>(tlane + (uint32_t)(a * S::BN + c), r);
-                    tmem_wait();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        acc[c + j] = fmaf(__uint_as_float(r[j]), f, acc[c + j]);
-                }
-                tc_fence_before();
-                ring::arrive(&tempty[a]);
+                for (int j = 0; j < CPT / 2; ++j) acc[j] = splat(__int_as_float(0x7fc00000));
             }
-            if (!ok)  // a wait ran out: this tile and the block's later ones are NaN
-#pragma unroll
-                for (int j = 0; j < 128; ++j) acc[j] = __int_as_float(0x7fc00000);
-            if (live) {
+            if (row < p.m) {
                 OutT* y = reinterpret_cast<OutT*>(p.y) + row * p.ldy + col0;
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    const int64_t left = p.n - col0 - c;
-                    if (left > 0) store_row32<OutT>(y + c, acc + c, left < 32 ? (int)left : 32, vec);
+                for (int c0 = 0; c0 < CPT; c0 += 32) {
+                    const int64_t left = p.n - col0 - c0;
+                    if (left > 0) store_row32<OutT>(y + c0, acc + c0 / 2, left < 32 ? (int)left : 32, align);
                 }
             }
         }
     }
     __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    ring::cluster_sync();  // neither CTA leaves while the pair's MMAs or arrivals may touch it
     tc_fence_after();
     __syncwarp();
-    if (warp == 1) tmem_free<S::COLS>(tmem);
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS)
+                     : "memory");
 }
 
 }  // namespace fp8

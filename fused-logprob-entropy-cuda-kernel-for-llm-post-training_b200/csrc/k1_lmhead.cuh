@@ -233,13 +233,6 @@ __device__ __forceinline__ void set_chunk_elem(uint4 (&v)[NV], int k, float val)
 
 // Store the first `valid` bf16 columns of a packed chunk of one row (the ragged or
 // unaligned case element by element, every register named statically).
-// 32 bytes at a 32-byte aligned address in one store.
-__device__ __forceinline__ void stg32(void* p, uint4 a, uint4 b) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x),
-                 "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
-                 : "memory");
-}
-
 // vec: 16-byte aligned row pieces (16-byte stores); vec32: 32-byte aligned (32-byte stores,
 // half the store instructions, each touching the warp's 32 rows once).
 template <int NV>
@@ -299,17 +292,6 @@ struct Geo {
                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
 };
 
-// Tiled 2-D copy into this CTA's shared memory whose completion is counted on the pair
-// leader's mbarrier (cl_bar, a shared::cluster address).  Each CTA copies
-// only its own tile, from this GPU's memory.
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y,
-                                                 uint32_t cl_bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3}], [%4];" ::"r"(ring::saddr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(cl_bar)
-        : "memory");
-}
 template <bool PAIR>
 __device__ __forceinline__ void umma_t(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t acc) {
     if constexpr (PAIR) {
@@ -326,12 +308,7 @@ __device__ __forceinline__ void umma_t(uint32_t tmem_d, uint64_t da, uint64_t db
 template <bool PAIR>
 __device__ __forceinline__ void commit_t(uint64_t* bar) {
     if constexpr (PAIR) {
-        const uint16_t both = 0x3;
-        asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-            "[%0], %1;" ::"r"(ring::saddr(bar)),
-            "h"(both)
-            : "memory");
+        umma_commit_pair(bar);
     } else {
         umma_commit(bar);
     }

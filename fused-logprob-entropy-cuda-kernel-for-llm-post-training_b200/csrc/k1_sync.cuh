@@ -67,12 +67,53 @@ __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity) {
     atomicOr(&k1_ring_error, 1u);
     return false;
 }
+// The same on the barrier's shared-memory address, for loops that keep addresses rather than
+// pointers (a pointer into shared memory is converted at every use).
+__device__ __forceinline__ void arrive_at(uint32_t b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
+}
+__device__ __forceinline__ bool try_wait_at(uint32_t b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(b), "r"(parity), "r"(kSuspendHintNs)
+        : "memory");
+    return ok != 0;
+}
+// Whether the phase has completed, without waiting for it.
+__device__ __forceinline__ bool test_at(uint32_t b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(b), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
             "r"(saddr(dst)),
         "l"(src), "r"(bytes), "r"(saddr(bar))
         : "memory");
+}
+
+// One lane of a converged warp (the same one at every call).  The compiler knows a branch on
+// it to be taken by one thread, so what it guards can use uniform registers; after a branch
+// on the lane's number, tcgen05 and TMA instructions cost several times the issue cycles.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one)
+        :
+        : "memory");
+    return one != 0;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
