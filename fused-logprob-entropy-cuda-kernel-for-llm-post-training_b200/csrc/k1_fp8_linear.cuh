@@ -123,6 +123,12 @@ __device__ __forceinline__ void tmem_wait_on(uint32_t (&r)[16]) {
                  : "memory");
 }
 
+// Asynchronous copy of 4 bytes into shared memory (zeros where not live).
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0)
+                 : "memory");
+}
+
 struct Params {
     const float* xs;  // [m, kb_total]
     const float* ws;  // [ceil(n / 128), kb_total]
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
     // shared-memory addresses
     const uint32_t a_ring = ring::saddr(smem), a_full = ring::saddr(full), a_empty = ring::saddr(empty),
                    a_tfull = ring::saddr(tfull), a_tempty = ring::saddr(tempty), a_sfull = ring::saddr(sfull),
-                   a_sempty = ring::saddr(sempty);
+                   a_sempty = ring::saddr(sempty), a_scales = ring::saddr(scales);
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::REGS_DOWN));
@@ -609,22 +615,21 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                         ok = false;
                         break;
                     }
+                    // asynchronous copies: all of a chunk in flight at once
                     const bool in = k0 + lane < p.kb_total;
-                    const float* src = p.xs + m0 * p.kb_total + k0 + lane;
-                    float* chunk = scales + at.slot * (S::S_BYTES / 4);
-                    float* dst = chunk + lane * S::SROW;
-                    for (int r0 = 0; r0 < BM; r0 += 8) {
-                        float f[8];
-#pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            f[q] = in && r0 + q < rows ? __ldg(src + (int64_t)(r0 + q) * p.kb_total) : 0.f;
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) dst[r0 + q] = f[q];
+                    const float* src = p.xs + (in ? m0 * p.kb_total + k0 + lane : 0);
+                    const uint32_t chunk = a_scales + at.slot * S::S_BYTES;
+                    const uint32_t dst = chunk + lane * (S::SROW * 4);
+#pragma unroll 8
+                    for (int r = 0; r < BM; ++r) {
+                        const bool live = in && r < rows;
+                        copy4(dst + r * 4, live ? src + (int64_t)r * p.kb_total : p.xs, live);
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        chunk[S::SB * S::SROW + 2 * lane + h] =
-                            in ? __ldg(p.ws + min(nb + h, nb_last) * p.kb_total + k0 + lane) : 0.f;
+                        copy4(chunk + (S::SB * S::SROW + 2 * lane + h) * 4,
+                              p.ws + (in ? min(nb + h, nb_last) * p.kb_total + k0 + lane : 0), in);
+                    asm volatile("cp.async.wait_all;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) ring::arrive_at(a_sfull + at.slot * 8);
                 }
