@@ -146,23 +146,25 @@ struct Skinny {
     static constexpr int W_BYTES = BM * BK;           // 16 KB
     static constexpr int X_BYTES = TN * BK;
     static constexpr int STAGE = W_BYTES + X_BYTES;
-#ifndef K1_SK_STAGES
-#define K1_SK_STAGES 4
-#endif
-    static constexpr int STAGES = K1_SK_STAGES;
+    static constexpr int STAGES = 4;
     static constexpr int NBUF = TN <= 32 ? 4 : 2;     // TMEM buffers
     static constexpr int COLS = NBUF * TN;            // 64, 128, 128
-    static constexpr int THREADS = 192;
+    static constexpr int GROUPS = TN <= 32 ? 1 : TN / 32;  // epilogue groups of 4 warps
+    static constexpr int CW = TN / GROUPS;                 // tokens per group: 16 or 32
+    static constexpr int THREADS = 64 + GROUPS * 128;
     static constexpr int RING = STAGES * STAGE;
     // ring (1024-byte aligned), barriers, scales [blocks of this CTA][TN]
     static constexpr size_t smem(int kb) { return 1024 + RING + 256 + (size_t)kb * TN * 4; }
 };
 
-#ifndef K1_SK_MINB
-#define K1_SK_MINB 2
-#endif
+// Two consecutive 16-bit elements in one store.
+template <typename OutT>
+__device__ __forceinline__ void store_pair(OutT* dst, float a, float b) {
+    if constexpr (sizeof(OutT) == 2) *reinterpret_cast<uint32_t*>(dst) = DT<OutT>::from_f2(make_float2(a, b));
+}
+
 template <int TN, typename OutT>
-__global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
+__global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
     k1_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x,
                          const __grid_constant__ CUtensorMap tmap_w, Params p, int split) {
     using S = Skinny<TN>;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
         }
         for (int a = 0; a < S::NBUF; ++a) {
             ring::bar_init(&tfull[a], 1);
-            ring::bar_init(&tempty[a], 4);  // one arrival per epilogue warp
+            ring::bar_init(&tempty[a], 4 * S::GROUPS);  // one arrival per epilogue warp
         }
         ring::bar_init(drain, 1);
         *abort = 0;
@@ -242,7 +244,8 @@ __global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
             for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
                 ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         __syncwarp();
-        if (split > 1) asm volatile("bar.arrive 2, 160;" ::: "memory");  // no copy is in flight
+        if (split > 1)  // no copy is in flight
+            asm volatile("bar.arrive 2, %0;" ::"n"(S::GROUPS * 128 + 32) : "memory");
     } else if (warp == 1) {
         Place<S::STAGES> at;
         Place<S::NBUF> acc;
@@ -272,18 +275,20 @@ __global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
         __syncwarp();                               // the TMEM is freed
         ring::wait(drain, 0);
     } else {
-        // each thread owns one row of the weight (a TMEM lane) and all TN tokens
+        // each thread owns one row of the weight (a TMEM lane) and its group's tokens
+        constexpr int CW = S::CW, EPI = S::GROUPS * 128;
         const int t = threadIdx.x - 64;
         const int quarter = warp & 3;
         const int row = quarter * 32 + lane;
-        const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16);
+        const int j0 = (t >> 7) * CW;  // the group's first token in the block
+        const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)j0;
         const int nkb = kb1 - kb0;
         const float* ws = p.ws + (int64_t)tile * p.kb_total + kb0;
         {
-            // a thread's token is fixed (TN divides 128); eight loads in flight
+            // a thread's token is fixed (TN divides the threads); eight loads in flight
             const int64_t m = tok0 + t % TN;
             const float* xs = p.xs + (m < p.m ? m : 0) * p.kb_total + kb0;
-            constexpr int STEP = 128 / TN;
+            constexpr int STEP = EPI / TN;
             for (int kb = t / TN; kb < nkb; kb += 8 * STEP) {
                 float f[8];
 #pragma unroll
@@ -294,59 +299,68 @@ __global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
                     if (kb + q * STEP < nkb) scales[(kb + q * STEP) * TN + t % TN] = m < p.m ? f[q] : 0.f;
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        float acc[TN];
+        asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
+        float acc[CW];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[j] = 0.f;
+        for (int j = 0; j < CW; ++j) acc[j] = 0.f;
         Place<S::NBUF> buf;
         for (int i = 0; i < nkb; ++i, buf.next()) {
             const uint32_t a = buf.slot;
             // warp-uniform: the TMEM loads below are warp-collective
             if (!__all_sync(0xffffffffu, wait(a_tfull + a * 8, buf.parity, abort))) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[j] = __int_as_float(0x7fc00000);
+                for (int j = 0; j < CW; ++j) acc[j] = __int_as_float(0x7fc00000);
                 break;
             }
             tc_fence_after();
-            constexpr int CW = TN < 32 ? TN : 32;  // columns per TMEM wait
-            const float4* sc = reinterpret_cast<const float4*>(scales + i * TN);
+            const float4* sc = reinterpret_cast<const float4*>(scales + i * TN + j0);
+            uint32_t r[CW];
+            if constexpr (CW == 32)
+                tmem_ld32_async<0>(tlane + a * TN, r);
+            else
+                tmem_ld16_async<0>(tlane + a * TN, r);
+            tmem_wait_on(r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ring::arrive_at(a_tempty + a * 8);
 #pragma unroll
-            for (int c = 0; c < TN; c += CW) {
-                uint32_t r[CW];
-                if constexpr (CW == 32)
-                    tmem_ld32_async<0>(tlane + (uint32_t)(a * TN + c), r);
-                else
-                    tmem_ld16_async<0>(tlane + (uint32_t)(a * TN + c), r);
-                tmem_wait_on(r);
-                if (c + CW == TN) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ring::arrive_at(a_tempty + a * 8);
-                }
-#pragma unroll
-                for (int j = 0; j < CW; j += 4) {
-                    const float4 f = sc[(c + j) / 4];
-                    acc[c + j] = fmaf(__uint_as_float(r[j]), f.x, acc[c + j]);
-                    acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]), f.y, acc[c + j + 1]);
-                    acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]), f.z, acc[c + j + 2]);
-                    acc[c + j + 3] = fmaf(__uint_as_float(r[j + 3]), f.w, acc[c + j + 3]);
-                }
+            for (int j = 0; j < CW; j += 4) {
+                const float4 f = sc[j / 4];
+                acc[j] = fmaf(__uint_as_float(r[j]), f.x, acc[j]);
+                acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), f.y, acc[j + 1]);
+                acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), f.z, acc[j + 2]);
+                acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), f.w, acc[j + 3]);
             }
         }
         const int64_t col = (int64_t)tile * BM + row;
+        const int tok = tok0 + j0;
         OutT* y = reinterpret_cast<OutT*>(p.y);
         if (split == 1) {
-            if (col < p.n)
+            // 16-bit outputs: two lanes trade, so that each stores two columns of one of two
+            // tokens in one word
+            const bool paired = sizeof(OutT) == 2 && (p.ldy & 1) == 0 &&
+                                (reinterpret_cast<uintptr_t>(y) & 3) == 0 && ((p.n & 1) == 0);
+            if (paired) {
+                const bool odd = lane & 1;
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    if (tok0 + j < p.m) DT<OutT>::store1(y + (tok0 + j) * p.ldy + col, acc[j]);
+                for (int j = 0; j < CW; j += 2) {
+                    const float got = __shfl_xor_sync(0xffffffffu, odd ? acc[j] : acc[j + 1], 1);
+                    const int tj = tok + j + odd;
+                    if (col < p.n && tj < p.m)
+                        store_pair(y + (int64_t)tj * p.ldy + (col - odd), odd ? got : acc[j], odd ? acc[j + 1] : got);
+                }
+            } else if (col < p.n) {
+#pragma unroll
+                for (int j = 0; j < CW; ++j)
+                    if (tok + j < p.m) DT<OutT>::store1(y + (int64_t)(tok + j) * p.ldy + col, acc[j]);
+            }
         } else {
             // the ring is done with: every stage was consumed before the last block's sums (or,
             // after a wait that ran out, the producer has waited for its copies)
-            asm volatile("bar.sync 2, 160;" ::: "memory");
+            asm volatile("bar.sync 2, %0;" ::"n"(EPI + 32) : "memory");
             float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) part[j * BM + row] = acc[j];
+            for (int j = 0; j < CW; ++j) part[(j0 + j) * BM + row] = acc[j];
         }
     }
     __syncwarp();
@@ -354,11 +368,12 @@ __global__ void __launch_bounds__(192, TN <= 32 ? 3 : K1_SK_MINB)
     if (split > 1) {
         ring::cluster_sync();  // every rank's part is in its shared memory
         if (warp >= 2) {
-            // rank r finishes tokens r, r + split, ...: the parts added in rank order
+            // rank r finishes tokens r, r + split, ... (dealt to its groups): the parts added in
+            // rank order
             const int row = (warp & 3) * 32 + lane;
             const int64_t col = (int64_t)tile * BM + row;
             const uint32_t mine = ring::saddr(smem) + (uint32_t)row * 4;
-            for (int j = rank; j < TN; j += split) {
+            for (int j = rank + split * ((warp - 2) >> 2); j < TN; j += split * S::GROUPS) {
                 float v = 0.f;
                 for (int r = 0; r < split; ++r) {
                     float f;
