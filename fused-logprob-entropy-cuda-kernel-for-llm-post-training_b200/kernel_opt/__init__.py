@@ -6,7 +6,8 @@ the same public functions, the same `_C` binding names, and the lazily imported
 `KernelOptGRPOTrainer` (needs `trl`).  Multi-GPU helpers live in `kernel_opt.parallel`,
 the GRPO completion-window node in `kernel_opt.grpo`, the LM head fused with K1 in
 `kernel_opt.lm_head`.  The operators of a decoding step's tail, which produce the tokens that
-K1 scores, are in `kernel_opt.norm`, `kernel_opt.fp8` and `kernel_opt.sampling`.
+K1 scores, are in `kernel_opt.norm`, `kernel_opt.fp8` and `kernel_opt.sampling`, and run together
+in `kernel_opt.rollout`.
 """
 import torch  # noqa: F401  (loads libc10 / libtorch before the extension)
 
@@ -27,6 +28,7 @@ from .lm_head import fused_linear_logprob_entropy  # noqa: F401
 from .norm import fused_residual_rmsnorm, fused_residual_rmsnorm_fp8  # noqa: F401
 from .fp8 import fp8_linear, quantize_fp8_blocks, quantize_fp8_rows  # noqa: F401
 from .sampling import sample_tokens  # noqa: F401
+from .rollout import RolloutHead  # noqa: F401
 
 
 def set_check_waits(on: bool = True) -> None:
