@@ -80,7 +80,7 @@ int launched(const char* fn, cudaError_t e) {
 // Residual RMS norm
 // ---------------------------------------------------------------------------------------
 // Threads and pieces per thread of a row of `hidden` elements; nv is one of the kernel's
-// instances (vectors: 1, 2, 4 or 8; single elements: 4 or 32).
+// instances (vectors: 1, 2, 4 or 8; single elements: 4, 8 or 32).
 struct NormShape {
     bool vec;
     int nv, threads;
@@ -94,7 +94,7 @@ NormShape norm_shape(int hidden, int es, bool vec) {
         s.nv = 1;
         while (s.nv < 8 && pieces > 256 * s.nv && (s.nv < 2 || pieces > 512 * s.nv)) s.nv *= 2;
     } else {
-        s.nv = pieces <= 4 * k1::norm::kMaxThreads ? 4 : 32;
+        s.nv = pieces <= 4 * k1::norm::kMaxThreads ? 4 : pieces <= 8 * k1::norm::kMaxThreads ? 8 : 32;
     }
     // whole groups of 128 threads, so that single elements' blocks of 128 are whole warps
     const int unit = vec ? 32 : 128;
@@ -114,8 +114,9 @@ template <typename T, int OUT>
 cudaError_t norm_launch(const k1::norm::FwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
     using namespace k1::norm;
     if (!s.vec)
-        return s.nv == 4 ? launch(k1_rmsnorm_kernel<T, false, 4, OUT>, grid, s.threads, 0, st, p)
-                         : launch(k1_rmsnorm_kernel<T, false, 32, OUT>, grid, s.threads, 0, st, p);
+        return s.nv == 4   ? launch(k1_rmsnorm_kernel<T, false, 4, OUT>, grid, s.threads, 0, st, p)
+               : s.nv == 8 ? launch(k1_rmsnorm_kernel<T, false, 8, OUT>, grid, s.threads, 0, st, p)
+                           : launch(k1_rmsnorm_kernel<T, false, 32, OUT>, grid, s.threads, 0, st, p);
     switch (s.nv) {
         case 1: return launch(k1_rmsnorm_kernel<T, true, 1, OUT>, grid, s.threads, 0, st, p);
         case 2: return launch(k1_rmsnorm_kernel<T, true, 2, OUT>, grid, s.threads, 0, st, p);
@@ -131,8 +132,9 @@ template <typename T>
 cudaError_t norm_bwd_launch(const k1::norm::BwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
     using namespace k1::norm;
     if (!s.vec)
-        return s.nv == 4 ? launch(k1_rmsnorm_bwd_kernel<T, false, 4>, grid, s.threads, 0, st, p)
-                         : launch(k1_rmsnorm_bwd_kernel<T, false, 32>, grid, s.threads, 0, st, p);
+        return s.nv == 4   ? launch(k1_rmsnorm_bwd_kernel<T, false, 4>, grid, s.threads, 0, st, p)
+               : s.nv == 8 ? launch(k1_rmsnorm_bwd_kernel<T, false, 8>, grid, s.threads, 0, st, p)
+                           : launch(k1_rmsnorm_bwd_kernel<T, false, 32>, grid, s.threads, 0, st, p);
     switch (s.nv) {
         case 1: return launch(k1_rmsnorm_bwd_kernel<T, true, 1>, grid, s.threads, 0, st, p);
         case 2: return launch(k1_rmsnorm_bwd_kernel<T, true, 2>, grid, s.threads, 0, st, p);
@@ -161,11 +163,14 @@ bool rows_vec(const void* p, int64_t stride, int64_t n, int es) {
     return !p || (aligned(p, 16) && (n <= 1 || (stride * es) % 16 == 0));
 }
 
-// What the backward's grid takes of the SM: three streams of vectors in flight per thread
-// and as few partial rows of dw as keep the loads going.
+// The backward's grid: every block writes a partial row of dw, so no more blocks than keep the
+// loads going, and at least four rows each once every SM has a block.  Measured (bf16, us a
+// training step of 16384 x 3584 with 3, 4, 6 blocks per SM): 189, 172, 184.
 constexpr int kBwdBlocksPerSm = 4;
 
-int64_t norm_bwd_grid(int64_t n, int threads, int sms) { return norm_grid(n, threads, sms, kBwdBlocksPerSm); }
+int64_t norm_bwd_grid(int64_t n, int threads, int sms) {
+    return std::min(norm_grid(n, threads, sms, kBwdBlocksPerSm), std::max<int64_t>(sms, n / 4));
+}
 
 int norm_forward(const char* fn, int out, const void* x, int64_t x_stride, const void* r, int64_t r_stride,
                  const void* w, int weight_dtype, int dtype, int64_t n, int64_t hidden, float eps, void* s,

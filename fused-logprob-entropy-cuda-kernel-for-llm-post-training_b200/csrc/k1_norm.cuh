@@ -393,8 +393,10 @@ __global__ void __launch_bounds__(512) k1_rmsnorm_dw_kernel(const float* part, i
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + lane;
     float v = 0.f;
-    if (col < h)
+    if (col < h) {
+#pragma unroll 8
         for (int i = warp; i < parts; i += 16) v += part[(int64_t)i * h + col];
+    }
     sums[warp][lane] = v;
     __syncthreads();
     if (warp == 0 && col < h) {
