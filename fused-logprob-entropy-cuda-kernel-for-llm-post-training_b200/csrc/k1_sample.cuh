@@ -440,16 +440,9 @@ __device__ __forceinline__ V block_scan(V v, V* warp_sums) {
     return base + v;
 }
 
-// The smallest value of `v` among the block's threads that hit, `none` without one.
-__device__ __forceinline__ int first_of(FilterSmem& sm, bool hit, int v, int none) {
-    if (threadIdx.x == 0) sm.pick = none;
-    __syncthreads();
-    if (hit) atomicMin(&sm.pick, v);
-    __syncthreads();
-    v = sm.pick;
-    __syncthreads();
-    return v;
-}
+// The first bin whose prefix (thread b's, growing with b) reaches what is asked for; the last
+// one if none does.
+__device__ __forceinline__ int first_bin(bool reached) { return min(__syncthreads_count(!reached), NB - 1); }
 
 // ------------------------------------------------------------------------------------
 // The list: entries of the row (key of y, ~index), in the row's first block
@@ -839,9 +832,9 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
         return;
     }
     const double u = (double)p.u[row];
-    Keep keep = {-INFINITY, 0, 0.f};
 
     if constexpr (!FILTER) {
+        const Keep keep = {-INFINITY, 0, 0.f};
         const Joined S = R.template kept_mass<true>(sm, keep);
         R.template draw<true>(sm, keep, S, u * S.a, S.a, p, row);
     } else {
@@ -852,16 +845,52 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
         const float min_p = greedy ? 0.f : fminf(p.min_p ? p.min_p[row] : p.min_p0, 1.f);
         const float floor = m - kFloor;
 
-        // ---- the whole mass ----
+        // ---- a bound for a short list ----
+        // What at least `want` elements reach (about; whether so many do is seen from their
+        // number): the bin of the groups' maxima in which their count gets that far.  Twice
+        // the groups' range, so that the elements below the lowest of them spread too.
         const bool try_list = top_k ? top_k <= min(kListK, cluster * THREADS) : use_p;
-        // twice the groups' range: the elements below the lowest group maximum spread too
+        const unsigned want = top_k ? top_k : kNucleusK;
         Bins bins = Bins::linear(m, fmaxf(m - 2.f * (m - range.lo), floor));
+        float least = INFINITY;
         if (try_list) {
 #pragma unroll
             for (int q = 0; q < NG; ++q)
                 if (g[q] >= floor) atomicAdd(&sm.hist[bins.of(g[q])], 1u);
+            const unsigned upto = block_scan(row_bin(sm, cluster), sm.wn);
+            const int b = first_bin(upto >= want);
+            least = b == NB - 1 ? floor : fmaxf(floor, m - ((float)b + 0.5f) / bins.per_unit);
         }
-        const Joined whole = R.template kept_mass<true>(sm, keep);
+
+        // ---- the whole mass, and the list ----
+        Keep keep = {-INFINITY, 0, 0.f};
+        Joined whole;
+        if (try_list) {
+            Mass mass;
+            double listed = 0.0;
+            unsigned n = 0;
+            R.each_vector([&](int j, uint4 v) {
+                float y[E], w[E];
+                unpack<T>(v, R.s, y);
+                R.template weights<true>(keep, j, y, w);
+                mass.add(w);
+                float top = y[0];
+#pragma unroll
+                for (int e = 1; e < E; ++e) top = fmaxf(top, y[e]);
+                if (!__any_sync(0xffffffffu, top >= least)) return;
+                unsigned hits = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    hits |= y[e] >= least ? 1u << e : 0u;
+                    listed += y[e] >= least ? (double)w[e] : 0.0;
+                }
+                n += __popc(hits);
+                append(sm, hits, y, sl.index(j, 0), [](float) {});
+            });
+            whole = exchange<A | B | N, WARPS>(sm, R.phase, cluster, rank, mass.total(), listed, n, 0.f, 0.f);
+        } else {
+            whole = R.template kept_mass<true>(sm, keep);
+        }
         const double S = whole.a;
 
         if (!top_k && !use_p && !(min_p > 0.f)) {
@@ -871,30 +900,11 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
 
         // ---- a short list ----
         if (try_list) {
-            const unsigned want = top_k ? top_k : kNucleusK;
-            const unsigned upto = block_scan(row_bin(sm, cluster), sm.wn);
-            const int b = first_of(sm, upto >= want, threadIdx.x, NB - 1);
-            // about the lower edge of bin b; whether at least `want` elements reach it is
-            // seen from their number
-            const float least = b == NB - 1 ? floor : fmaxf(floor, m - ((float)b + 0.5f) / bins.per_unit);
-            double mass = 0.0;
-            unsigned n = 0;
-            R.each_vector([&](int j, uint4 v) {
-                if (!__any_sync(0xffffffffu, vec_max<T>(v) * R.s >= least)) return;
-                float y[E];
-                unpack<T>(v, R.s, y);
-                unsigned hits = 0;
-#pragma unroll
-                for (int e = 0; e < E; ++e) hits |= y[e] >= least ? 1u << e : 0u;
-                n += __popc(hits);
-                append(sm, hits, y, sl.index(j, 0), [&](float x) { mass += (double)expf(x - m); });
-            });
-            const Joined t = exchange<A | N, WARPS>(sm, R.phase, cluster, rank, mass, 0.0, n, 0.f, 0.f);
-            if (t.n <= (unsigned)kListCap &&
-                (top_k ? t.n >= want || least == floor : t.a >= (double)top_p * S)) {
-                join_lists(sm, rank, t.n_before);
+            if (whole.n <= (unsigned)kListCap &&
+                (top_k ? whole.n >= want || least == floor : whole.b >= (double)top_p * S)) {
+                join_lists(sm, rank, whole.n_before);
                 if (!leader) return;
-                const int count = (int)t.n;
+                const int count = (int)whole.n;
                 uint64_t e[PER], word[PER];
                 float w[PER];
                 uint64_t part = 0;
@@ -1014,7 +1024,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                 const double upto = above + block_scan(part, sm.wscan);
                 if (!by_mass && __syncthreads_or(threadIdx.x == NB - 1 && upto < target))
                     break;  // fewer elements than top-k asks for: all stay
-                int b = first_of(sm, upto >= target, threadIdx.x, NB - 1);
+                int b = first_bin(upto >= target);
                 // the bin's exact limits, its elements into the list; a neighbour's if the
                 // rounded masses misled
                 Joined t;
