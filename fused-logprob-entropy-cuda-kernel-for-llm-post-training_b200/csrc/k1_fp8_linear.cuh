@@ -437,6 +437,25 @@ __device__ __forceinline__ void wide_tile(const Params& p, int u, int& mt, int& 
     mt = g * Wide::GROUP_M + (r - nt * rows);
 }
 
+// Transposes 32 x 32 values across a warp: lane l's v[i] becomes lane i's v[l].
+__device__ __forceinline__ void warp_transpose(float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const bool up = lane & d;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if (i & d) continue;
+            // the half of each pair that belongs to the other lane
+            const float other = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + d], d);
+            if (up)
+                v[i] = other;
+            else
+                v[i + d] = other;
+        }
+    }
+}
+
 // 32 columns of one row, `valid` of them; align: bytes that every row piece starts at.
 template <typename OutT>
 __device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int valid, int align) {
@@ -721,12 +740,37 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < CPT / 2; ++j) acc[j] = splat(__int_as_float(0x7fc00000));
             }
-            if (row < p.m) {
-                OutT* y = reinterpret_cast<OutT*>(p.y) + row * p.ldy + col0;
+            if (align >= 16) {
+                if (row < p.m) {
+                    OutT* y = reinterpret_cast<OutT*>(p.y) + row * p.ldy + col0;
+#pragma unroll
+                    for (int c0 = 0; c0 < CPT; c0 += 32) {
+                        const int64_t left = p.n - col0 - c0;
+                        if (left > 0) store_row32<OutT>(y + c0, acc + c0 / 2, left < 32 ? (int)left : 32, align);
+                    }
+                }
+            } else {
+                // rows that start anywhere: turned across the warp, so that its lanes store
+                // consecutive columns of one row (element by element of its own row, a warp's
+                // store would touch 32 rows)
+                const int64_t row0 = row - lane;
+                const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
 #pragma unroll
                 for (int c0 = 0; c0 < CPT; c0 += 32) {
-                    const int64_t left = p.n - col0 - c0;
-                    if (left > 0) store_row32<OutT>(y + c0, acc + c0 / 2, left < 32 ? (int)left : 32, align);
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        v[i] = acc[(c0 + i) / 2].x;
+                        v[i + 1] = acc[(c0 + i) / 2].y;
+                    }
+                    warp_transpose(v);
+                    const int64_t col = col0 + c0 + lane;
+                    OutT* y = reinterpret_cast<OutT*>(p.y) + row0 * p.ldy + col;
+                    if (col < p.n) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < rows) DT<OutT>::store1(y + (int64_t)i * p.ldy, v[i]);
+                    }
                 }
             }
         }
