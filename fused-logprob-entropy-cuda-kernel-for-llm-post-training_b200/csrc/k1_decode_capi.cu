@@ -256,9 +256,13 @@ int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
     if (!rc) rc = make_tmap8(&tw, w, p.n, inner, ldw, k1::fp8::BM, "weight");
     if (rc) return rc;
     const int64_t tiles = (p.n + 127) / 128, tok = (p.m + TN - 1) / TN;
-    // split K while the blocks do not fill the SMs twice and every part keeps two blocks of K
+    // K is split over a cluster where a third of the SMs or more would stay without a block,
+    // until all have one and while every part keeps two blocks of K.  Measured (us, bf16 out):
+    // 100 x 3584 x 4096 in 64 / 128 / 256 parts - / 14.0 / 12.0; 200 x 3584 x 3584 in 112 / 224
+    // 15.1 / 18.7; 936 x 800 x 1978 in 240 / 480 8.7 / 22.9.
     int split = 1;
-    while (split < 8 && tiles * tok * split < 2 * sms && p.kb_total >= 4 * split) split *= 2;
+    if (tiles * tok * 3 < 2 * sms)
+        while (split < 8 && tiles * tok * split < sms && p.kb_total >= 4 * split) split *= 2;
     auto kern = k1::fp8::k1_fp8_skinny_kernel<TN, OutT>;
     const size_t smem = S::smem((p.kb_total + split - 1) / split);
     rc = allow_smem(kern, dev, smem);
@@ -304,7 +308,8 @@ int wide(const char* fn, k1::fp8::Params p, const void* x, int64_t ldx, const vo
     if (rc) return rc;
     p.m_tiles = (int)((p.m + S::TM - 1) / S::TM);
     p.n_tiles = (int)((p.n + S::BN - 1) / S::BN);
-    auto kern = k1::fp8::k1_fp8_wide_kernel<OutT>;
+    const bool aligned16 = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * sizeof(OutT))) & 15) == 0;
+    auto kern = aligned16 ? k1::fp8::k1_fp8_wide_kernel<OutT, true> : k1::fp8::k1_fp8_wide_kernel<OutT, false>;
     int pairs = 0;
     rc = allow_smem(kern, dev, S::SMEM);
     if (!rc) rc = wide_pairs(kern, dev, &pairs);
@@ -318,9 +323,15 @@ int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
            int64_t inner, int sms, int dev, cudaStream_t st) {
     if (p.m <= 16) return skinny<16, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
     if (p.m <= 32) return skinny<32, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-    const int64_t wide_tiles = (p.m + 255) / 256 * ((p.n + 255) / 256);
-    if (p.m <= 128 || wide_tiles < sms / 4)
-        return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+    // The few-token kernel in blocks of 64 tokens (two blocks of threads per SM) or the
+    // many-token kernel (a tile per two SMs), by their rounds times what a round takes: about
+    // 4 + 0.65 us per block of K, and 10 + 0.6.  Measured (us, few / many): 936 x 800 x 1978
+    // 8.7 / 17.2; 162 x 1328 x 12141 12.9 / 20.3; 142 x 4352 x 14269 41 / 33; 300 x 3584 x 8192
+    // 34 / 26; 128 x 3584 x 32768 43 / 44; 2180 x 6160 x 3492 127 / 71.
+    const int64_t few = (p.m + 63) / 64 * ((p.n + 127) / 128), many = (p.m + 255) / 256 * ((p.n + 255) / 256);
+    const double few_us = (double)((few + 2 * sms - 1) / (2 * sms)) * (4.0 + 0.65 * p.kb_total);
+    const double many_us = (double)((many + sms / 2 - 1) / (sms / 2)) * (10.0 + 0.6 * p.kb_total);
+    if (p.m <= 64 || few_us <= many_us) return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
     return wide<OutT>(fn, p, x, ldx, w, ldw, inner, dev, st);
 }
 

@@ -456,10 +456,11 @@ __device__ __forceinline__ void warp_transpose(float (&v)[32]) {
     }
 }
 
-// 32 columns of one row, `valid` of them; align: bytes that every row piece starts at.
+// 32 columns of one row that starts at a multiple of 16 bytes (32 with align32), `valid` of
+// them.
 template <typename OutT>
-__device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int valid, int align) {
-    if (align >= 16 && valid >= 32) {
+__device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int valid, bool align32) {
+    if (valid >= 32) {
         constexpr int E = 16 / sizeof(OutT);  // elements of a vector
 #pragma unroll
         for (int i = 0; i < 32; i += 2 * E) {
@@ -474,7 +475,7 @@ __device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int vali
                     w[h] = make_uint4(DT<OutT>::from_f2(s[0]), DT<OutT>::from_f2(s[1]),
                                       DT<OutT>::from_f2(s[2 % (E / 2)]), DT<OutT>::from_f2(s[3 % (E / 2)]));
             }
-            if (align >= 32) {
+            if (align32) {
                 stg32(dst + i, w[0], w[1]);
             } else {
                 stg_stream(dst + i, w[0]);
@@ -490,7 +491,8 @@ __device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int vali
     }
 }
 
-template <typename OutT>
+// ALIGNED: the output's rows start at multiples of 16 bytes.
+template <typename OutT, bool ALIGNED>
 __global__ void __launch_bounds__(Wide::THREADS, 1)
     k1_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x,
                        const __grid_constant__ CUtensorMap tmap_w, Params p) {
@@ -677,8 +679,8 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
         const int part = (warp - 4) >> 2;      // CPT columns: one block of weight rows
         const int rloc = quarter * 32 + lane;
         const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * CPT);
-        const uintptr_t yat = reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * sizeof(OutT));
-        const int align = yat % 32 == 0 ? 32 : yat % 16 == 0 ? 16 : 1;
+        const bool align32 =
+            ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * sizeof(OutT))) & 31) == 0;
         const uint32_t cl_tempty = ring::mapa(a_tempty, 0);  // the leader's barriers
         static_assert(CPT == 128 && S::NBUF == 2, "four loads of 32 columns per block of K");
         uint32_t buf = 0, parity = 0;
@@ -740,13 +742,13 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < CPT / 2; ++j) acc[j] = splat(__int_as_float(0x7fc00000));
             }
-            if (align >= 16) {
+            if constexpr (ALIGNED) {
                 if (row < p.m) {
                     OutT* y = reinterpret_cast<OutT*>(p.y) + row * p.ldy + col0;
 #pragma unroll
                     for (int c0 = 0; c0 < CPT; c0 += 32) {
                         const int64_t left = p.n - col0 - c0;
-                        if (left > 0) store_row32<OutT>(y + c0, acc + c0 / 2, left < 32 ? (int)left : 32, align);
+                        if (left > 0) store_row32<OutT>(y + c0, acc + c0 / 2, left < 32 ? (int)left : 32, align32);
                     }
                 }
             } else {
