@@ -79,24 +79,24 @@ int launched(const char* fn, cudaError_t e) {
 // ---------------------------------------------------------------------------------------
 // Residual RMS norm
 // ---------------------------------------------------------------------------------------
-// Threads and pieces per thread of a row of `hidden` elements; nv is one of the kernel's
-// instances (vectors: 1, 2, 4 or 8; single elements: 4, 8 or 32).
+// Elements per piece (a 16-byte vector, 2 or 1), pieces per thread and threads of a row of
+// `hidden` elements; nv is one of the kernel's instances (vectors: 1, 2, 4 or 8; others: 2, 4,
+// 8 or 16).
 struct NormShape {
-    bool vec;
-    int nv, threads;
+    int e, nv, threads;
 };
 
-NormShape norm_shape(int hidden, int es, bool vec) {
-    const int pieces = vec ? hidden * es / 16 : hidden;
+NormShape norm_shape(int hidden, int es, int e) {
     NormShape s;
-    s.vec = vec;
-    if (vec) {
-        s.nv = 1;
+    s.e = e;
+    const int pieces = hidden / e;
+    const bool vec = e * es == 16;
+    s.nv = vec ? 1 : 2;
+    if (vec)
         while (s.nv < 8 && pieces > 256 * s.nv && (s.nv < 2 || pieces > 512 * s.nv)) s.nv *= 2;
-    } else {
-        s.nv = pieces <= 4 * k1::norm::kMaxThreads ? 4 : pieces <= 8 * k1::norm::kMaxThreads ? 8 : 32;
-    }
-    // whole groups of 128 threads, so that single elements' blocks of 128 are whole warps
+    else
+        while (pieces > s.nv * k1::norm::kMaxSmall) s.nv *= 2;
+    // whole groups of 128 threads, so that the columns of a scale are whole warps
     const int unit = vec ? 32 : 128;
     s.threads = std::max(unit, (pieces + s.nv - 1) / s.nv);
     s.threads = (s.threads + unit - 1) / unit * unit;
@@ -110,40 +110,54 @@ int64_t norm_grid(int64_t n, int threads, int sms, int most_per_sm) {
     return std::min<int64_t>(n, (int64_t)sms * per_sm);
 }
 
+template <typename T, int OUT, int E, int NV>
+cudaError_t norm_launch1(const k1::norm::FwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
+    return launch(k1::norm::k1_rmsnorm_kernel<T, E, NV, OUT>, grid, s.threads, 0, st, p);
+}
+
 template <typename T, int OUT>
 cudaError_t norm_launch(const k1::norm::FwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
-    using namespace k1::norm;
-    if (!s.vec)
-        return s.nv == 4   ? launch(k1_rmsnorm_kernel<T, false, 4, OUT>, grid, s.threads, 0, st, p)
-               : s.nv == 8 ? launch(k1_rmsnorm_kernel<T, false, 8, OUT>, grid, s.threads, 0, st, p)
-                           : launch(k1_rmsnorm_kernel<T, false, 32, OUT>, grid, s.threads, 0, st, p);
-    switch (s.nv) {
-        case 1: return launch(k1_rmsnorm_kernel<T, true, 1, OUT>, grid, s.threads, 0, st, p);
-        case 2: return launch(k1_rmsnorm_kernel<T, true, 2, OUT>, grid, s.threads, 0, st, p);
-        case 4: return launch(k1_rmsnorm_kernel<T, true, 4, OUT>, grid, s.threads, 0, st, p);
-        default:
-            if constexpr (sizeof(T) == 4)
-                return launch(k1_rmsnorm_kernel<T, true, 8, OUT>, grid, s.threads, 0, st, p);
-            return cudaErrorInvalidValue;
+    constexpr int V = k1::DT<T>::kEPV;
+    switch (s.e * 100 + s.nv) {
+        case 102: return norm_launch1<T, OUT, 1, 2>(p, s, grid, st);
+        case 104: return norm_launch1<T, OUT, 1, 4>(p, s, grid, st);
+        case 108: return norm_launch1<T, OUT, 1, 8>(p, s, grid, st);
+        case 116: return norm_launch1<T, OUT, 1, 16>(p, s, grid, st);
+        case 202: return norm_launch1<T, OUT, 2, 2>(p, s, grid, st);
+        case 204: return norm_launch1<T, OUT, 2, 4>(p, s, grid, st);
+        case 208: return norm_launch1<T, OUT, 2, 8>(p, s, grid, st);
+        case V * 100 + 1: return norm_launch1<T, OUT, V, 1>(p, s, grid, st);
+        case V * 100 + 2: return norm_launch1<T, OUT, V, 2>(p, s, grid, st);
+        case V * 100 + 4: return norm_launch1<T, OUT, V, 4>(p, s, grid, st);
+        case 408:
+            if constexpr (V == 4) return norm_launch1<T, OUT, 4, 8>(p, s, grid, st);
     }
+    return cudaErrorInvalidValue;
+}
+
+template <typename T, int E, int NV>
+cudaError_t norm_bwd_launch1(const k1::norm::BwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
+    return launch(k1::norm::k1_rmsnorm_bwd_kernel<T, E, NV>, grid, s.threads, 0, st, p);
 }
 
 template <typename T>
 cudaError_t norm_bwd_launch(const k1::norm::BwdParams& p, const NormShape& s, int64_t grid, cudaStream_t st) {
-    using namespace k1::norm;
-    if (!s.vec)
-        return s.nv == 4   ? launch(k1_rmsnorm_bwd_kernel<T, false, 4>, grid, s.threads, 0, st, p)
-               : s.nv == 8 ? launch(k1_rmsnorm_bwd_kernel<T, false, 8>, grid, s.threads, 0, st, p)
-                           : launch(k1_rmsnorm_bwd_kernel<T, false, 32>, grid, s.threads, 0, st, p);
-    switch (s.nv) {
-        case 1: return launch(k1_rmsnorm_bwd_kernel<T, true, 1>, grid, s.threads, 0, st, p);
-        case 2: return launch(k1_rmsnorm_bwd_kernel<T, true, 2>, grid, s.threads, 0, st, p);
-        case 4: return launch(k1_rmsnorm_bwd_kernel<T, true, 4>, grid, s.threads, 0, st, p);
-        default:
-            if constexpr (sizeof(T) == 4)
-                return launch(k1_rmsnorm_bwd_kernel<T, true, 8>, grid, s.threads, 0, st, p);
-            return cudaErrorInvalidValue;
+    constexpr int V = k1::DT<T>::kEPV;
+    switch (s.e * 100 + s.nv) {
+        case 102: return norm_bwd_launch1<T, 1, 2>(p, s, grid, st);
+        case 104: return norm_bwd_launch1<T, 1, 4>(p, s, grid, st);
+        case 108: return norm_bwd_launch1<T, 1, 8>(p, s, grid, st);
+        case 116: return norm_bwd_launch1<T, 1, 16>(p, s, grid, st);
+        case 202: return norm_bwd_launch1<T, 2, 2>(p, s, grid, st);
+        case 204: return norm_bwd_launch1<T, 2, 4>(p, s, grid, st);
+        case 208: return norm_bwd_launch1<T, 2, 8>(p, s, grid, st);
+        case V * 100 + 1: return norm_bwd_launch1<T, V, 1>(p, s, grid, st);
+        case V * 100 + 2: return norm_bwd_launch1<T, V, 2>(p, s, grid, st);
+        case V * 100 + 4: return norm_bwd_launch1<T, V, 4>(p, s, grid, st);
+        case 408:
+            if constexpr (V == 4) return norm_bwd_launch1<T, 4, 8>(p, s, grid, st);
     }
+    return cudaErrorInvalidValue;
 }
 
 int norm_check(const char* fn, int dtype, int weight_dtype, int64_t n_rows, int64_t hidden) {
@@ -158,9 +172,18 @@ int norm_check(const char* fn, int dtype, int weight_dtype, int64_t n_rows, int6
     return K1_OK;
 }
 
-// Whether the rows of a matrix are whole 16-byte vectors at 16-byte addresses.
-bool rows_vec(const void* p, int64_t stride, int64_t n, int es) {
-    return !p || (aligned(p, 16) && (n <= 1 || (stride * es) % 16 == 0));
+// The most of `bytes` at which every row of a matrix starts (NULL: no limit).
+int rows_align(const void* p, int64_t stride, int64_t n, int es, int bytes) {
+    if (!p) return bytes;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p) | (n > 1 ? (uintptr_t)(stride * es) : 0);
+    while (bytes > es && at % bytes != 0) bytes /= 2;
+    return bytes;
+}
+
+// Elements per piece: a 16-byte vector, a pair, or one, by the width and every address.
+int norm_piece(int64_t hidden, int es, int align) {
+    if ((hidden * es) % 16 == 0 && align >= 16) return 16 / es;
+    return hidden % 2 == 0 && align >= 2 * es ? 2 : 1;
 }
 
 // The backward's grid: every block writes a partial row of dw, so no more blocks than keep the
@@ -193,9 +216,14 @@ int norm_forward(const char* fn, int out, const void* x, int64_t x_stride, const
     rc = current_device(&dev);
     if (!rc) rc = sm_count(dev, &sms);
     if (rc) return rc;
-    const bool vec = (hidden * es) % 16 == 0 && rows_vec(x, x_stride, n, es) && rows_vec(r, r_stride, n, es) &&
-                     aligned(w, 16) && aligned(s, 16) && aligned(y, 16);
-    const NormShape sh = norm_shape((int)hidden, es, vec);
+    // outputs are contiguous; a vector of the weight in fp32 is two or more
+    int align = rows_align(x, x_stride, n, es, 16);
+    align = rows_align(r, r_stride, n, es, align);
+    align = rows_align(s, hidden, n, es, align);
+    if (out == k1::norm::SAME) align = rows_align(y, hidden, n, es, align);
+    const int e = std::min(norm_piece(hidden, es, align), !w || aligned(w, 16) ? 8 : aligned(w, 2 * es) ? 2 : 1);
+    const NormShape sh = norm_shape((int)hidden, es,
+                                    out != k1::norm::SAME && !aligned(y, e) ? 1 : e);
     k1::norm::FwdParams p = {};
     p.x = x;
     p.r = r;
@@ -463,10 +491,12 @@ int k1_residual_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
     rc = current_device(&dev);
     if (!rc) rc = sm_count(dev, &sms);
     if (rc) return rc;
-    const bool vec = (hidden * es) % 16 == 0 && rows_vec(g_y, g_y_stride, n_rows, es) &&
-                     rows_vec(g_stream, g_stream_stride, n_rows, es) &&
-                     rows_vec(stream_in, stream_stride, n_rows, es) && aligned(weight, 16) && aligned(d_x, 16);
-    const NormShape sh = norm_shape((int)hidden, es, vec);
+    int align = rows_align(g_y, g_y_stride, n_rows, es, 16);
+    align = rows_align(g_stream, g_stream_stride, n_rows, es, align);
+    align = rows_align(stream_in, stream_stride, n_rows, es, align);
+    align = rows_align(d_x, hidden, n_rows, es, align);
+    const NormShape sh = norm_shape(
+        (int)hidden, es, std::min(norm_piece(hidden, es, align), aligned(weight, 16) ? 8 : aligned(weight, 2 * es) ? 2 : 1));
     const int64_t grid = norm_bwd_grid(n_rows, sh.threads, sms);
     if (d_weight && (!workspace || !aligned(workspace, 16) ||
                      workspace_bytes < (size_t)grid * hidden * sizeof(float)))

@@ -20,12 +20,19 @@
 // not depend on timing).
 #pragma once
 
+#include <type_traits>
+
 #include "k1_common.cuh"
 
 namespace k1 {
 namespace norm {
 
+// Threads of a block: rows of vectors need at most 512; rows of smaller pieces get more
+// threads rather than more registers.
 constexpr int kMaxThreads = 512;
+constexpr int kMaxSmall = 1024;
+template <int E>
+constexpr int kThreads = E >= 4 ? kMaxThreads : kMaxSmall;
 constexpr int kMaxHidden = 16384;
 constexpr int kFp8Block = 128;       // columns that share a scale
 constexpr float kFp8Max = 448.f;     // largest finite e4m3
@@ -38,16 +45,18 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
     return r;
 }
 
-// A thread's piece of a row: E consecutive elements, one 16-byte vector (VEC) or one
-// element, kept as loaded; converted to fp32 where it is used.
-template <typename T, bool VEC>
+// A thread's piece of a row: E consecutive elements, kept as loaded and converted to fp32
+// where they are used: a 16-byte vector, two elements (rows of an even width that no vector
+// divides) or one.
+template <typename T, int E>
 struct Piece;
 
 template <typename T>
-struct Piece<T, true> {
+struct Piece<T, DT<T>::kEPV> {
     static constexpr int E = DT<T>::kEPV;
     uint4 v;
     __device__ __forceinline__ void load(const T* p) { v = ldg_stream(p); }
+    __device__ __forceinline__ void load_cached(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
     __device__ __forceinline__ void store(T* p) const { stg_stream(p, v); }
     __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&f)[E]) const {
@@ -78,10 +87,35 @@ struct Piece<T, true> {
 };
 
 template <typename T>
-struct Piece<T, false> {
-    static constexpr int E = 1;
+struct Piece<T, 2> {
+    using V = std::conditional_t<sizeof(T) == 4, float2, uint32_t>;
+    V v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
+    __device__ __forceinline__ void load_cached(const T* p) { v = *reinterpret_cast<const V*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<V*>(p) = v; }
+    __device__ __forceinline__ void zero() { v = V{}; }
+    __device__ __forceinline__ void get(float (&f)[2]) const {
+        float2 t;
+        if constexpr (sizeof(T) == 4)
+            t = v;
+        else
+            t = DT<T>::to_f2(v);
+        f[0] = t.x;
+        f[1] = t.y;
+    }
+    __device__ __forceinline__ void set(const float (&f)[2]) {
+        if constexpr (sizeof(T) == 4)
+            v = make_float2(f[0], f[1]);
+        else
+            v = DT<T>::from_f2(make_float2(f[0], f[1]));
+    }
+};
+
+template <typename T>
+struct Piece<T, 1> {
     T v;
     __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void load_cached(const T* p) { v = *p; }
     __device__ __forceinline__ void store(T* p) const { *p = v; }
     __device__ __forceinline__ void zero() { DT<T>::store1(&v, 0.f); }
     __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = DT<T>::load1(&v); }
@@ -90,13 +124,11 @@ struct Piece<T, false> {
 
 // The weight's columns, fp32 or T (w32 is uniform over the launch).  Read through L1: a
 // block reads the same columns for every row.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight(const void* w, bool w32, int col,
-                                            float (&f)[Piece<T, VEC>::E]) {
-    constexpr int E = Piece<T, VEC>::E;
+template <typename T, int E>
+__device__ __forceinline__ void load_weight(const void* w, bool w32, int col, float (&f)[E]) {
     if (w32) {
         const float* p = reinterpret_cast<const float*>(w) + col;
-        if constexpr (VEC) {
+        if constexpr (E >= 4) {
 #pragma unroll
             for (int i = 0; i < E; i += 4) {
                 const float4 t = __ldg(reinterpret_cast<const float4*>(p + i));
@@ -106,17 +138,21 @@ __device__ __forceinline__ void load_weight(const void* w, bool w32, int col,
                 f[i + 3] = t.w;
             }
         } else {
-            f[0] = __ldg(p);
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = __ldg(p + i);
         }
     } else {
-        const T* p = reinterpret_cast<const T*>(w) + col;
-        Piece<T, VEC> t;
-        if constexpr (VEC)
-            t.v = __ldg(reinterpret_cast<const uint4*>(p));
-        else
-            t.v = *p;
+        Piece<T, E> t;
+        t.load_cached(reinterpret_cast<const T*>(w) + col);
         t.get(f);
     }
+}
+
+// 1 / x to one unit in the last place (x: a scale, never subnormal).
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Sum over the block, the same value (and order) in every thread.  scratch: 32 floats, not
@@ -148,12 +184,12 @@ struct FwdParams {
 };
 
 // NV pieces per thread: piece j of thread t starts at column (j * threads + t) * E.
-template <typename T, bool VEC, int NV, int OUT>
-__global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_kernel(FwdParams p) {
-    using P = Piece<T, VEC>;
-    constexpr int E = P::E;
+template <typename T, int E, int NV, int OUT>
+__global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
+    using P = Piece<T, E>;
+    constexpr bool VEC = E >= 4;
     __shared__ float scratch[2][32];
-    __shared__ float wmax[(!VEC && OUT != SAME) ? NV : 1][kMaxThreads / 32];
+    __shared__ float wmax[(!VEC && OUT != SAME) ? NV : 1][kMaxSmall / 32];
     pdl_wait();
     pdl_trigger();
     const int threads = blockDim.x, tid = threadIdx.x;
@@ -216,7 +252,7 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_kernel(FwdParams p) {
                 if (col >= p.h) break;
                 float a[E], w[E];
                 s[j].get(a);
-                load_weight<T, VEC>(p.w, p.w32, col, w);
+                load_weight<T, E>(p.w, p.w32, col, w);
 #pragma unroll
                 for (int i = 0; i < E; ++i) a[i] = a[i] * rstd * w[i];
                 P o;
@@ -225,7 +261,7 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_kernel(FwdParams p) {
             }
         } else {
             // 128 columns are 128 / E consecutive threads' pieces: 16 lanes (16-bit types),
-            // a warp (fp32), or four warps (single elements)
+            // a warp (fp32), or two or four warps (pairs, single elements)
             uint8_t* y = reinterpret_cast<uint8_t*>(p.y) + row * (int64_t)p.h;
             float a[NV][E];
             if constexpr (!VEC) __syncthreads();  // wmax of the previous row has been read
@@ -237,7 +273,7 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_kernel(FwdParams p) {
                 if (col < p.h) {
                     if constexpr (OUT == FP8) {
                         float w[E];
-                        load_weight<T, VEC>(p.w, p.w32, col, w);
+                        load_weight<T, E>(p.w, p.w32, col, w);
 #pragma unroll
                         for (int i = 0; i < E; ++i) a[j][i] = a[j][i] * rstd * w[i];
                     }
@@ -251,14 +287,14 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_kernel(FwdParams p) {
                 if constexpr (VEC) {
                     const float scale = fmax_nan(m, kAmaxFloor) / kFp8Max;
                     if (col < p.h) {
-                        const float inv = 1.f / scale;
-                        uint32_t q[E / 4];
+                        const float inv = reciprocal(scale);
+                        uint32_t q[(E + 3) / 4];
 #pragma unroll
                         for (int i = 0; i < E; i += 4)
                             q[i / 4] = e4m3x2(a[j][i] * inv, a[j][i + 1] * inv) |
                                        (e4m3x2(a[j][i + 2] * inv, a[j][i + 3] * inv) << 16);
                         if constexpr (E == 8)
-                            *reinterpret_cast<uint2*>(y + col) = make_uint2(q[0], q[E / 4 - 1]);
+                            *reinterpret_cast<uint2*>(y + col) = make_uint2(q[0], q[(E + 3) / 4 - 1]);
                         else
                             *reinterpret_cast<uint32_t*>(y + col) = q[0];
                         if ((tid & (LANES - 1)) == 0)
@@ -272,14 +308,21 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_kernel(FwdParams p) {
                 __syncthreads();
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    const int col = j * threads + tid;
+                    const int col = (j * threads + tid) * E;
                     if (col >= p.h) break;
-                    const float* g = wmax[j] + ((tid >> 5) & ~3);
-                    const float m = fmax_nan(fmax_nan(g[0], g[1]), fmax_nan(g[2], g[3]));
+                    constexpr int W = kFp8Block / E / 32;  // warps that share a scale
+                    const float* g = wmax[j] + ((tid >> 5) & ~(W - 1));
+                    float m = g[0];
+#pragma unroll
+                    for (int i = 1; i < W; ++i) m = fmax_nan(m, g[i]);
                     const float scale = fmax_nan(m, kAmaxFloor) / kFp8Max;
-                    y[col] = (uint8_t)e4m3x2(a[j][0] * (1.f / scale), 0.f);
-                    if ((tid & (kFp8Block - 1)) == 0)
-                        p.scales[row * n_blocks + col / kFp8Block] = scale;
+                    const float inv = reciprocal(scale);
+                    const uint32_t q = e4m3x2(a[j][0] * inv, a[j][E - 1] * inv);
+                    if constexpr (E == 2)
+                        *reinterpret_cast<uint16_t*>(y + col) = (uint16_t)q;
+                    else
+                        y[col] = (uint8_t)q;
+                    if (col % kFp8Block == 0) p.scales[row * n_blocks + col / kFp8Block] = scale;
                 }
             }
         }
@@ -298,10 +341,9 @@ struct BwdParams {
     int h, w32;
 };
 
-template <typename T, bool VEC, int NV>
-__global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_bwd_kernel(BwdParams p) {
-    using P = Piece<T, VEC>;
-    constexpr int E = P::E;
+template <typename T, int E, int NV>
+__global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_bwd_kernel(BwdParams p) {
+    using P = Piece<T, E>;
     __shared__ float scratch[2][32];
     pdl_wait();
     pdl_trigger();
@@ -342,7 +384,7 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_bwd_kernel(BwdParams p
             float a[E], b[E], w[E];
             g[j].get(a);
             s[j].get(b);
-            load_weight<T, VEC>(p.w, p.w32, col, w);
+            load_weight<T, E>(p.w, p.w32, col, w);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const float n = b[i] * rstd;
@@ -361,7 +403,7 @@ __global__ void __launch_bounds__(kMaxThreads) k1_rmsnorm_bwd_kernel(BwdParams p
                 g[j].get(a);
                 s[j].get(b);
                 u[j].get(t);
-                load_weight<T, VEC>(p.w, p.w32, col, w);
+                load_weight<T, E>(p.w, p.w32, col, w);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     t[i] = fmaf(rstd, fmaf(-(b[i] * rstd), c, a[i] * w[i]), t[i]);
@@ -436,7 +478,7 @@ __global__ void __launch_bounds__(256) k1_quantize_blocks_kernel(const T* w, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmax_nan(m, wmax[i]);
     const float scale = fmax_nan(m, kAmaxFloor) / kFp8Max;
-    const float inv = 1.f / scale;
+    const float inv = reciprocal(scale);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t r = r0 + warp + 8 * i;

@@ -75,7 +75,7 @@ def train(x, r, w, gy, gs, eps=EPS):
 
 
 SHAPES = [(1, 1), (3, 2), (5, 7), (2, 8), (9, 100), (4, 129), (1, 3584), (700, 3584), (333, 2051), (6, 8192),
-          (3, 16384), (3, 16383), (2, 4104), (1300, 64)]
+          (3, 16384), (3, 16383), (2, 4104), (1300, 64), (3, 16382), (5, 5002), (2, 8198)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
