@@ -370,10 +370,11 @@ template <typename T, bool FILTER>
 int sample_launch(const char* fn, k1::sample::Params p, int sms, int dev, cudaStream_t st) {
     using namespace k1::sample;
     constexpr int E = k1::DT<T>::kEPV;
-    // Bytes of a row's part in one block: what lets two blocks with lists, or three without,
-    // share an SM; a lone block takes up to kLone; a row that is longer still stays in global
-    // memory.
-    constexpr int64_t kShared = (FILTER ? 92 : K1_SP_KB) * 1024, kLone = 184 * 1024, kLeast = 8 * 1024;
+    // Bytes of a row's part in one block: what lets two blocks with lists, or five without,
+    // share an SM (with lists, 512 rows of 152064 bf16, top-k 50: 159 us in four parts of 76 KB,
+    // 239 in eight of 38); a lone block takes up to kLone; a row that is longer still stays in
+    // global memory.
+    constexpr int64_t kShared = (FILTER ? 92 : 48) * 1024, kLone = 184 * 1024, kLeast = 8 * 1024;
     const int64_t row_bytes = ((p.vocab + E - 1) / E + 1) * 16;  // one more for the shift
     int cluster = 1;
     while (cluster < kMaxCluster && row_bytes > cluster * kShared) cluster *= 2;

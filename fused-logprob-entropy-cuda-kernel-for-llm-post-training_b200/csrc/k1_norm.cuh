@@ -24,6 +24,10 @@
 
 #include "k1_common.cuh"
 
+//
+// Measured on B200: 16384 x 3584 bf16 training step 173 us (940 MB, 5.4 TB/s), 8192 x 3584 bf16 with
+// 8-bit output 43 us, one row 2.8 us of device time; rows of odd width move single elements and
+// take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 61 us, bytes 18).
 namespace k1 {
 namespace norm {
 
