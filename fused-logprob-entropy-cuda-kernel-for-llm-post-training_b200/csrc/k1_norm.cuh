@@ -3,13 +3,14 @@
 //
 //   s = T(x + r)                         the residual stream, as stored (T: the tensors' type)
 //   R = 1 / sqrt(mean(s^2) + eps)        one per row, fp32
-//   y = T(s R w)                         or, in 8 bits, q = e4m3(s R w / a), a = amax / 448
+//   y = T(s R w)                         or, in 8 bits, q = e4m3(y / a), a = max |y| / 448
 //   ds = R (t - s R c) + gs,  t = gy w,  c = mean(t s R);      dx = dr = T(ds)
 //   dw = sum over rows of gy s R
 //
 // The norm reads the stream as it is stored, so the forward, the backward (which keeps only
 // s and R) and the next layer all see the same numbers.  Sums, R and dw are fp32; y (and ds)
-// is rounded once.  The 8-bit output is rounded once too, from the fp32 value.
+// is rounded once.  The 8-bit output is rounded once too, from fp32 (in bf16 from the exact
+// quotient: R cancels in y / a, and s w has 16 bits).
 //
 // One block of threads owns a row at a time and keeps it in registers between the sum of
 // squares and the output, so every tensor crosses HBM once: 4 N H elements forward (x, r, s,
@@ -27,7 +28,8 @@
 //
 // Measured on B200: 16384 x 3584 bf16 training step 173 us (940 MB, 5.4 TB/s), 8192 x 3584 bf16 with
 // 8-bit output 43 us, one row 2.8 us of device time; rows of odd width move single elements and
-// take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 61 us, bytes 18).
+// take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 55 us, with 8-bit output 74; its bytes
+// 18).
 namespace k1 {
 namespace norm {
 
@@ -152,13 +154,27 @@ __device__ __forceinline__ void load_weight(const void* w, bool w32, int col, fl
     }
 }
 
-// y / scale from inv = 1 / scale, with one Newton step on the residual: the bare product's
-// rounding would move values that lie midway between two of e4m3's, and a division for each
+// The 8-bit values of a block whose largest magnitude is m: 448 y / m, as n / step with
+// n = 7/8 y and step = m / 512 = 7/8 m / 448.  7/8 y takes three more bits than y and the step
+// none, so for products of two bf16 numbers nothing is rounded before the quotient, and a value
+// that lies midway between two of e4m3's (1e-4 of them do) is seen as that; y / (m / 448), with
+// m / 448 rounded, moves some of them.
+//
+// The quotient of many values by one step: a product with the reciprocal and one Newton step on
+// its residual.  The bare product would move the midway values again, and a division for each
 // element costs 7 us of 42 at 8192 x 3584.
-__device__ __forceinline__ float quotient(float y, float scale, float inv) {
-    const float q = y * inv;
-    return fmaf(fmaf(-q, scale, y), inv, q);
-}
+struct Quotient {
+    float inv, step;
+    __device__ __forceinline__ explicit Quotient(float d) : Quotient(d, 1.f / d) {}
+    __device__ __forceinline__ Quotient(float d, float one_over_d) {
+        inv = one_over_d;
+        step = inv == 0.f ? 0.f : d;  // infinite: finite values give 0, not 0 x inf
+    }
+    __device__ __forceinline__ float operator()(float n) const {
+        const float q = n * inv;
+        return fmaf(fmaf(-q, step, n), inv, q);
+    }
+};
 
 // Sum over the block, the same value (and order) in every thread.  scratch: 32 floats, not
 // reused before the next __syncthreads of the caller's loop (two alternate buffers).
@@ -188,9 +204,11 @@ struct FwdParams {
     float eps;
 };
 
-// NV pieces per thread: piece j of thread t starts at column (j * threads + t) * E.
+// NV pieces per thread: piece j of thread t starts at column (j * threads + t) * E.  Rows of few
+// small pieces per thread keep to 32 registers, so that two blocks of 1024 threads share an SM
+// (4096 x 3585 bf16, us: forward 62 -> 55, with 8-bit output 93 -> 74).
 template <typename T, int E, int NV, int OUT>
-__global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
+__global__ void __launch_bounds__(kThreads<E>, E < 4 && E * NV <= 4 ? 2 : 1) k1_rmsnorm_kernel(FwdParams p) {
     using P = Piece<T, E>;
     constexpr bool VEC = E >= 4;
     __shared__ float scratch[2][32];
@@ -236,6 +254,9 @@ __global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
             }
         }
         float rstd = 1.f;
+        // 8 bits: the quotients' numerators are 7/8 y / 2^k, 2^k <= R < 2^(k + 1), so that no bits
+        // are lost to R (it cancels in y / amax) and the range is still y's
+        float unit = 0.875f, rest = 1.f, least = kAmaxFloor;
         if constexpr (OUT != FP8_ONLY) {
             float sum = 0.f;
 #pragma unroll
@@ -248,6 +269,12 @@ __global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
             sum = block_sum(sum, scratch[flip]);
             rstd = rsqrtf(sum / (float)p.h + p.eps);
             if (p.rstd && tid == 0) p.rstd[row] = rstd;
+            if constexpr (OUT == FP8) {
+                const uint32_t bits = __float_as_uint(rstd);
+                unit *= rstd == rstd ? __uint_as_float(bits & 0x7f800000u) : rstd;
+                rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) * (8.f / 7.f);
+                least = kAmaxFloor / rest;
+            }
         }
         if constexpr (OUT == SAME) {
             T* y = reinterpret_cast<T*>(p.y) + row * p.h;
@@ -269,6 +296,10 @@ __global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
             // a warp (fp32), or two or four warps (pairs, single elements)
             uint8_t* y = reinterpret_cast<uint8_t*>(p.y) + row * (int64_t)p.h;
             float a[NV][E];
+            auto step_of = [&](float& m) {  // m: the largest numerator (FP8) or value
+                m = fmax_nan(m, least);
+                return OUT == FP8 ? m / kFp8Max : m * (1.f / 512.f);
+            };
             if constexpr (!VEC) __syncthreads();  // wmax of the previous row has been read
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -280,20 +311,24 @@ __global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
                         float w[E];
                         load_weight<T, E>(p.w, p.w32, col, w);
 #pragma unroll
-                        for (int i = 0; i < E; ++i) a[j][i] = a[j][i] * rstd * w[i];
+                        for (int i = 0; i < E; ++i) a[j][i] = a[j][i] * unit * w[i];
                     }
 #pragma unroll
                     for (int i = 0; i < E; ++i) m = fmax_nan(m, fabsf(a[j][i]));
+                    if constexpr (OUT == FP8_ONLY) {
+#pragma unroll
+                        for (int i = 0; i < E; ++i) a[j][i] *= unit;
+                    }
                 }
                 constexpr int LANES = kFp8Block / E < 32 ? kFp8Block / E : 32;
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1)
                     m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                 if constexpr (VEC) {
-                    const float scale = fmax_nan(m, kAmaxFloor) / kFp8Max;
                     if (col < p.h) {
-                        const float inv = 1.f / scale;
-                        auto quo = [&](int i) { return quotient(a[j][i], scale, inv); };
+                        const float step = step_of(m);
+                        const Quotient to(step);
+                        auto quo = [&](int i) { return to(a[j][i]); };
                         uint32_t q[(E + 3) / 4];
 #pragma unroll
                         for (int i = 0; i < E; i += 4)
@@ -303,30 +338,40 @@ __global__ void __launch_bounds__(kThreads<E>) k1_rmsnorm_kernel(FwdParams p) {
                         else
                             *reinterpret_cast<uint32_t*>(y + col) = q[0];
                         if ((tid & (LANES - 1)) == 0)
-                            p.scales[row * n_blocks + col / kFp8Block] = scale;
+                            p.scales[row * n_blocks + col / kFp8Block] = OUT == FP8 ? step * rest : m / kFp8Max;
                     }
                 } else {
                     if ((tid & 31) == 0) wmax[j][tid >> 5] = m;
                 }
             }
             if constexpr (!VEC) {
+                // a thread for each scale: its step and the step's reciprocal go where its
+                // warps' maxima were
+                constexpr int W = kFp8Block / E / 32;  // warps that share a scale
+                const int per = threads * E / kFp8Block;
+                __syncthreads();
+                if (tid < NV * per && tid < n_blocks) {
+                    float* g = &wmax[tid / per][tid % per * W];
+                    float m = g[0];
+#pragma unroll
+                    for (int i = 1; i < W; ++i) m = fmax_nan(m, g[i]);
+                    const float step = step_of(m);
+                    g[0] = step;
+                    g[1] = 1.f / step;
+                    p.scales[row * n_blocks + tid] = OUT == FP8 ? step * rest : m / kFp8Max;
+                }
                 __syncthreads();
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
                     const int col = (j * threads + tid) * E;
                     if (col >= p.h) break;
-                    constexpr int W = kFp8Block / E / 32;  // warps that share a scale
                     const float* g = wmax[j] + ((tid >> 5) & ~(W - 1));
-                    float m = g[0];
-#pragma unroll
-                    for (int i = 1; i < W; ++i) m = fmax_nan(m, g[i]);
-                    const float scale = fmax_nan(m, kAmaxFloor) / kFp8Max;
-                    const uint32_t q = e4m3x2(a[j][0] / scale, a[j][E - 1] / scale);
+                    const Quotient to(g[0], g[1]);
+                    const uint32_t q = e4m3x2(to(a[j][0]), to(a[j][E - 1]));
                     if constexpr (E == 2)
                         *reinterpret_cast<uint16_t*>(y + col) = (uint16_t)q;
                     else
                         y[col] = (uint8_t)q;
-                    if (col % kFp8Block == 0) p.scales[row * n_blocks + col / kFp8Block] = scale;
                 }
             }
         }
@@ -481,17 +526,18 @@ __global__ void __launch_bounds__(256) k1_quantize_blocks_kernel(const T* w, int
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmax_nan(m, wmax[i]);
-    const float scale = fmax_nan(m, kAmaxFloor) / kFp8Max;
+    m = fmax_nan(m, kAmaxFloor);
+    const Quotient to(m * (1.f / 512.f));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t r = r0 + warp + 8 * i;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int64_t c = c0 + lane + 32 * k;
-            if (r < rows && c < cols) q[r * cols + c] = (uint8_t)e4m3x2(v[i][k] / scale, 0.f);
+            if (r < rows && c < cols) q[r * cols + c] = (uint8_t)e4m3x2(to(0.875f * v[i][k]), 0.f);
         }
     }
-    if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = scale;
+    if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = m / kFp8Max;
 }
 
 }  // namespace norm

@@ -298,3 +298,51 @@ def test_refusals():
         f(torch.zeros(1, 16385, device="cuda"), None, torch.zeros(16385, device="cuda"))
     with pytest.raises(ValueError, match="CUDA"):
         f(x.cpu(), r.cpu(), w.cpu())
+
+
+def exact_q(y, of_block):
+    """The e4m3 number nearest to 448 y / amax, from 64 bits."""
+    return (448 * y / of_block).to(torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("n,h", [(40, 3584), (33, 1026), (50, 1003), (5, 1024), (300, 128)])
+def test_8_bit_values_of_bf16_are_exact(n, h):
+    """A product of two bf16 numbers has 16 bits, so the quotient by the largest of 128 lies at
+    least 2^-22 (relative) away from a midpoint of e4m3 unless it is one: computed without a
+    rounding before the quotient, every value is the nearest, and midpoints go to even."""
+    x, r, w, _, _ = inputs(n, h, torch.bfloat16)
+    per_row = lambda a: torch.nn.functional.pad(a.double().abs(), (0, -h % 128)).view(n, -1, 128).amax(
+        2).repeat_interleave(128, 1)[:, :h]
+    q, _, s = kernel_opt.fused_residual_rmsnorm_fp8(x, r, w, EPS)
+    y = s.double() * w.double()
+    assert torch.equal(q.float(), exact_q(y, per_row(y)).float())
+    q, _ = kernel_opt.quantize_fp8_rows(x)
+    assert torch.equal(q.float(), exact_q(x.double(), per_row(x)).float())
+    q, scale = kernel_opt.quantize_fp8_blocks(x)
+    ob, hb = scale.shape
+    top = torch.nn.functional.pad(x.double().abs(), (0, -h % 128, 0, -n % 128)).view(ob, 128, hb, 128).amax((1, 3))
+    top = top.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :h]
+    assert torch.equal(q.float(), exact_q(x.double(), top).float())
+
+
+@pytest.mark.parametrize("h", [256, 258, 259])
+def test_8_bit_values_beside_an_infinity(h):
+    x = torch.randn(3, h, device="cuda")
+    x[1, 5] = float("-inf")
+    for q, scale in (kernel_opt.quantize_fp8_rows(x), kernel_opt.quantize_fp8_blocks(x)):
+        f = q.float()
+        assert torch.isnan(f[1, 5]) and scale[(1, 0) if scale.shape[0] == 3 else (0, 0)] == float("inf")
+        f[1, 5] = 0
+        assert torch.equal(f[1, :128], torch.zeros(128, device="cuda"))
+        assert not torch.isnan(f).any()
+
+
+@pytest.mark.parametrize("scale", [1e-34, 1e-30, 2.0 ** -60, 1e15])
+@pytest.mark.parametrize("h", [256, 258, 259])
+def test_8_bit_values_of_extreme_streams(h, scale):
+    """Values far from 1: eps rules the small ones (R = 1000), and squares up to 1e30 sum."""
+    x = torch.randn(4, h, device="cuda") * scale
+    w = 1 + 0.1 * torch.randn(h, device="cuda")
+    q, s, stream = kernel_opt.fused_residual_rmsnorm_fp8(x, None, w, EPS)
+    want, _ = reference(stream, w)
+    check_q(q, s, want, 44 * E)
