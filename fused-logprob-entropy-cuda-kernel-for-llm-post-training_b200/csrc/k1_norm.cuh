@@ -19,17 +19,17 @@
 // lets the backward add up its columns of dw in registers and write one partial row per
 // block; a second kernel adds the blocks' partials in block order (no atomics, so dw does
 // not depend on timing).
+//
+// Measured on B200: 16384 x 3584 bf16 training step 173 us (940 MB, 5.4 TB/s), 8192 x 3584 bf16 with
+// 8-bit output 43 us, one row 2.8 us of device time; rows of odd width move single elements and
+// take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 55 us, with 8-bit output 74; its bytes
+// 18).
 #pragma once
 
 #include <type_traits>
 
 #include "k1_common.cuh"
 
-//
-// Measured on B200: 16384 x 3584 bf16 training step 173 us (940 MB, 5.4 TB/s), 8192 x 3584 bf16 with
-// 8-bit output 43 us, one row 2.8 us of device time; rows of odd width move single elements and
-// take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 55 us, with 8-bit output 74; its bytes
-// 18).
 namespace k1 {
 namespace norm {
 

@@ -31,12 +31,21 @@ class RolloutHead:
                              f"{tuple(norm_weight.shape)} and {tuple(lm_head_weight.shape)}")
         self.eps = eps
         self.logits_dtype = logits_dtype
+        self.norm_weight = self.weight = self.weight_scales = None
         self.update(norm_weight, lm_head_weight)
 
     def update(self, norm_weight: torch.Tensor, lm_head_weight: torch.Tensor) -> None:
-        """Take (and quantise) new weights."""
-        self.norm_weight = norm_weight.detach()
-        self.weight, self.weight_scales = quantize_fp8_blocks(lm_head_weight.detach())
+        """Take (and quantise) new weights.  Both are copies: a step sees the weights of the last
+        update.  They are written where the old ones of the same shape and type lie, so captured
+        steps see them too."""
+        new = (norm_weight.detach(), *quantize_fp8_blocks(lm_head_weight.detach()))
+        old = (self.norm_weight, self.weight, self.weight_scales)
+        if old[0] is not None and all(a.shape == b.shape and a.dtype == b.dtype and a.device == b.device
+                                      for a, b in zip(old, new)):
+            for a, b in zip(old, new):
+                a.copy_(b)
+        else:
+            self.norm_weight, self.weight, self.weight_scales = new[0].clone(), new[1], new[2]
 
     def logits(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """[..., V] logits of the last layer's output x [..., H] and the residual stream."""

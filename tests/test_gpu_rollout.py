@@ -65,6 +65,22 @@ def test_update_takes_new_weights():
     assert torch.equal(head.logits(x), kernel_opt.RolloutHead(nw2, w2).logits(x))
 
 
+def test_update_reaches_captured_steps():
+    nw, w = weights(1000, 256)
+    nw2, w2 = weights(1000, 256, seed=1)
+    head = kernel_opt.RolloutHead(nw, w)
+    x = torch.randn(3, 256, device="cuda").bfloat16()
+    want = head.logits(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = head.logits(x)
+    nw.copy_(nw2)  # as an optimizer writes it: the head keeps both weights until it is told
+    assert torch.equal(head.logits(x), want)
+    head.update(nw2, w2)
+    g.replay()
+    assert torch.equal(out, kernel_opt.RolloutHead(nw2, w2).logits(x))
+
+
 def test_refusals():
     nw, w = weights(100, 64)
     with pytest.raises(ValueError, match="norm_weight"):
