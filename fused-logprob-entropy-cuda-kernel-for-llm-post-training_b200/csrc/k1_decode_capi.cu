@@ -370,14 +370,21 @@ template <typename T, bool FILTER>
 int sample_launch(const char* fn, k1::sample::Params p, int sms, int dev, cudaStream_t st) {
     using namespace k1::sample;
     constexpr int E = k1::DT<T>::kEPV;
-    // Bytes of a row's part in one block: what lets two blocks with lists, or five without,
-    // share an SM (with lists, 512 rows of 152064 bf16, top-k 50: 159 us in four parts of 76 KB,
-    // 239 in eight of 38); a lone block takes up to kLone; a row that is longer still stays in
-    // global memory.
-    constexpr int64_t kShared = (FILTER ? 92 : 48) * 1024, kLone = 184 * 1024, kLeast = 8 * 1024;
+    // Bytes of a row's part in one block: what lets two blocks with lists (113 KB each, 300 x
+    // 70000 fp32, top-k 50: 75 us, 100 with one), or five without, share an SM (with lists, 512
+    // rows of 152064 bf16, top-k 50: 157 us in four parts of 76 KB, 239 in eight of 38); a lone
+    // block takes up to kLone; a row that is longer still stays in global memory.
+    constexpr int64_t kShared = FILTER ? 113 * 1024 - (int64_t)smem_header<true>() : 48 * 1024;
+    constexpr int64_t kLone = 184 * 1024, kLeast = 8 * 1024;
     const int64_t row_bytes = ((p.vocab + E - 1) / E + 1) * 16;  // one more for the shift
+    // As few parts as fit where the rows fill the device 2.5 times or more, else a power of two
+    // of them, whose shorter parts end a partial round sooner.  Measured (us, filters, 128256
+    // wide, fewest / power of two): fp32 in 6 / 8, 567 rows 232 / 262, 150 rows 68 / 74, 64 rows
+    // 88 / 84; bf16 in 3 / 4, 512 rows 131 / 138, 200 rows 218 / 214, 64 rows 97 / 82.
+    const int fewest = (int)std::min<int64_t>((row_bytes + kShared - 1) / kShared, kMaxCluster);
     int cluster = 1;
-    while (cluster < kMaxCluster && row_bytes > cluster * kShared) cluster *= 2;
+    while (cluster < fewest) cluster *= 2;
+    if (FILTER && p.n_rows * fewest >= 5 * sms) cluster = fewest;
     // few rows: more blocks per row, so that the SMs share the load
     while (cluster < kMaxCluster && p.n_rows * cluster < sms && row_bytes > 2 * cluster * kLeast) cluster *= 2;
     const int64_t vecs = (row_bytes / 16 + cluster - 1) / cluster;

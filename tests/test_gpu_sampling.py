@@ -294,3 +294,19 @@ def test_refusals():
         f(x[:, :0], u)
     with pytest.raises(ValueError, match="CUDA"):
         f(x.cpu(), u.cpu())
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=50), dict(top_p=0.9), dict(top_k=3000, min_p=0.001)], ids=str)
+def test_many_rows_cut_into_any_number_of_parts(kw):
+    """Rows in 3, 5, 6 or 7 parts (taken where there are many rows) give what the same rows give
+    alone, in the power of two of parts that few rows take."""
+    for v, dtype in ((128256, torch.bfloat16), (100001, torch.float32), (128256, torch.float32),
+                     (152063, torch.float32)):
+        base = (torch.randn(8, v, device="cuda") * 3).to(dtype)
+        u = torch.rand(320, device="cuda")
+        rows = base.repeat(40, 1)
+        tok, lp, kp = kernel_opt.sample_tokens(rows, u, **kw)
+        for at in (0, 7, 163, 319):
+            t, l, k = kernel_opt.sample_tokens(rows[at:at + 1], u[at:at + 1], **kw)
+            assert t == tok[at]
+            assert (l - lp[at]).abs() <= 2 ** -22 * l.abs() and (k - kp[at]).abs() <= 2 ** -22 * k.abs() + 2 ** -24
