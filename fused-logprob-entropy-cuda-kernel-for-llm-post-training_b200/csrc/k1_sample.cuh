@@ -760,6 +760,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
     const int rank = blockIdx.x % cluster;
     const int64_t row = blockIdx.x / cluster;
     const bool leader = rank == 0;
+    ring::cluster_arrive();  // this block has started: the others may write its shared memory
     pdl_wait();
     pdl_trigger();
 
@@ -820,6 +821,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
         hi = fmax_nan(hi, g[q]);
         if (FILTER && g[q] > -INFINITY) lo = fminf(lo, g[q]);
     }
+    ring::cluster_wait();  // every block of the row has started; the loads lay between
     const Joined range = exchange<RANGE, WARPS>(sm, R.phase, cluster, rank, 0.0, 0.0, 0, lo, hi);
     const float m = range.hi;
     R.m = m;

@@ -131,6 +131,13 @@ __device__ __forceinline__ uint32_t mapa(uint32_t saddr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// Its two halves, for work that lies between them.
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
 // Arrive on an mbarrier of another CTA of the cluster (address from mapa).  The default
 // (CTA-scope) semantics: a release at cluster scope here would make the arriving thread
 // wait for its own bulk copies in flight, which serialises the producer.
