@@ -24,6 +24,18 @@ cudaError_t k1_decode_wait_status(unsigned* bits) {
 cudaError_t k1_decode_set_withhold(long long withhold) {
     return cudaMemcpyToSymbol(k1::k1_test_withhold, &withhold, sizeof withhold);
 }
+
+// Host-side tests of the sampling kernel's arithmetic (the wait-timeout test library alone has
+// them).  The words of a list of n weights, and the target at which `share` of its mass is reached.
+extern "C" void k1_test_list(const float* w, int n, double share, uint64_t* words, uint64_t* target) {
+    using namespace k1::sample;
+    double mass = 0.0;
+    for (int i = 0; i < n; ++i) mass += (double)w[i];
+    const double unit = list_unit(mass);
+    uint64_t all = 0;
+    for (int i = 0; i < n; ++i) all += words[i] = weight_word(w[i], unit);
+    *target = list_target(share * mass * unit, word_weight(all));
+}
 #endif
 
 namespace {

@@ -45,6 +45,7 @@
 #pragma once
 
 #include "k1_common.cuh"
+#include "k1_sample_math.cuh"
 #include "k1_sync.cuh"
 
 #include <type_traits>
@@ -109,7 +110,7 @@ struct FilterSmem : Smem {
     unsigned hist[NB];    // histogram of the block's elements
     double wscan[kMaxWarps];
     uint64_t wsum64[kMaxWarps];
-    uint64_t few_key[32], few_word[32];
+    uint64_t few_key[32], few_word[32];  // kFew
     unsigned few_n;
     uint64_t entry;       // block-wide values
     uint64_t above;
@@ -500,15 +501,6 @@ __device__ __forceinline__ void tell(FilterSmem& sm, int cluster, float tau, int
     }
 }
 
-// A weight (or a count of one) and the number of entries in one word: 2^-40 units of weight
-// above 12 bits of count, so sums over a list fit 63 bits and do not depend on their order.
-constexpr int kCountBits = 12;
-constexpr float kUnit = 1099511627776.f;  // 2^40
-__device__ __forceinline__ uint64_t weight_word(float w) {
-    return ((uint64_t)__float2ull_rn(w * kUnit) << kCountBits) | 1u;
-}
-__device__ __forceinline__ uint64_t word_weight(uint64_t v) { return v >> kCountBits; }
-
 __device__ __forceinline__ uint64_t block_sum64(FilterSmem& sm, uint64_t v) {
     v = warp_add(v);
     __syncthreads();
@@ -520,17 +512,25 @@ __device__ __forceinline__ uint64_t block_sum64(FilterSmem& sm, uint64_t v) {
 }
 
 // Of the block's entries (PER to a thread, distinct keys, a word of 0 for none), largest key
-// first: the key at which the weight added up so far first reaches `target` (> 0); the entries'
-// keys lie in [lo, hi], and their whole weight is at least `target`.  Each round adds the
-// words up in 512 bins of the remaining key range and keeps the crossing bin, until that
-// holds few entries: one round for spread keys, 64 / 9 at most.
+// first: the key at which the weight added up so far first reaches `target`; the entries' keys
+// lie in [lo, hi].  `lo`, which keeps them all, where none does (a target of 0 or more than their
+// whole weight).  Each round adds the words up in 512 bins of the remaining key range and keeps
+// the crossing bin, until that holds few entries: one round for spread keys; kRounds leave one key
+// to a bin.
+constexpr int kFew = 32;           // one to a lane
+constexpr int kRounds = (64 + 8) / 9;
 __device__ __forceinline__ uint64_t select_entry(FilterSmem& sm, const uint64_t (&key)[PER],
                                                  const uint64_t (&word)[PER], uint64_t lo, uint64_t hi,
                                                  uint64_t target) {
     uint64_t above = 0;
-    for (;;) {
+    const uint64_t none = lo;
+    for (int round = 0; round < kRounds; ++round) {
         const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
         sm.sums[threadIdx.x] = 0;
+        if (threadIdx.x == 0) {
+            sm.found = 0;
+            sm.entry = none;
+        }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < PER; ++r)
@@ -548,12 +548,13 @@ __device__ __forceinline__ uint64_t select_entry(FilterSmem& sm, const uint64_t 
             sm.found = (unsigned)(mine & ((1u << kCountBits) - 1));
         }
         __syncthreads();
+        if (sm.found == 0) break;  // none crosses
         const uint64_t top = hi - ((uint64_t)sm.pick << shift);
         const uint64_t bottom = top - (((uint64_t)1 << shift) - 1);
         lo = bottom > top || bottom < lo ? lo : bottom;
         hi = top;
         above = sm.above;
-        if (sm.found <= 32) break;
+        if (sm.found <= kFew) break;
         __syncthreads();
     }
     // the bin's entries, one to a lane, against one another
@@ -561,12 +562,14 @@ __device__ __forceinline__ uint64_t select_entry(FilterSmem& sm, const uint64_t 
     for (int r = 0; r < PER; ++r)
         if (word[r] && key[r] >= lo && key[r] <= hi) {
             const unsigned i = atomicAdd(&sm.few_n, 1u);
-            sm.few_key[i] = key[r];
-            sm.few_word[i] = word_weight(word[r]);
+            if (i < kFew) {
+                sm.few_key[i] = key[r];
+                sm.few_word[i] = word_weight(word[r]);
+            }
         }
     __syncthreads();
     if (threadIdx.x < 32) {
-        const unsigned n = sm.found, lane = threadIdx.x;
+        const unsigned n = min(sm.found, (unsigned)kFew), lane = threadIdx.x;
         const uint64_t k = lane < n ? sm.few_key[lane] : 0, w = lane < n ? sm.few_word[lane] : 0;
         uint64_t before = above;
         for (unsigned i = 0; i < n; ++i) before += sm.few_key[i] > k ? sm.few_word[i] : 0;
@@ -907,6 +910,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                 join_lists(sm, rank, whole.n_before);
                 if (!leader) return;
                 const int count = (int)whole.n;
+                const double unit = list_unit(whole.b);
                 uint64_t e[PER], word[PER];
                 float w[PER];
                 uint64_t part = 0;
@@ -915,7 +919,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                     const int i = r * THREADS + threadIdx.x;
                     e[r] = i < count ? sm.list[i] : 0;
                     w[r] = i < count ? expf(entry_value(e[r]) - m) : 0.f;
-                    word[r] = i < count ? weight_word(w[r]) : 0;
+                    word[r] = i < count ? weight_word(w[r], unit) : 0;
                     part += word[r];
                 }
                 const uint64_t top = entry(m, 0), bottom = entry(least, 0xffffffffll);
@@ -923,7 +927,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                 if (top_k && top_k < count) {
                     uint64_t one[PER];
 #pragma unroll
-                    for (int r = 0; r < PER; ++r) one[r] = word[r] ? ((uint64_t)1 << kCountBits) | 1u : 0;
+                    for (int r = 0; r < PER; ++r) one[r] = word[r] ? count_word() : 0;
                     cut = select_entry(sm, e, one, bottom, top, (uint64_t)top_k);
                     part = 0;
 #pragma unroll
@@ -936,9 +940,8 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                     // of the whole mass without top-k: the list holds that share, up to the
                     // words' rounding
                     const uint64_t all = word_weight(block_sum64(sm, part));
-                    const double Z = top_k ? (double)all : S * (double)kUnit;
-                    cut = select_entry(sm, e, word, cut, top,
-                                       min(all, (uint64_t)fmax(ceil((double)top_p * Z), 1.0)));
+                    const double Z = top_k ? (double)all : S * unit;
+                    cut = select_entry(sm, e, word, cut, top, list_target((double)top_p * Z, all));
                 }
                 part = 0;
 #pragma unroll
@@ -959,7 +962,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                         const double d = (double)(entry_value(e[r]) - m);
                         p.token[row] = entry_index(e[r]);
                         p.logprob[row] = (float)(d - log(S));
-                        p.kept_logprob[row] = (float)(d - log((double)C / (double)kUnit));
+                        p.kept_logprob[row] = (float)(d - log((double)C / unit));
                     }
                 return;
             }
@@ -1107,19 +1110,19 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
                     join_lists(sm, rank, t.n_before);
                     if (leader) {
                         const int count = (int)t.n;
+                        const double unit = by_mass ? list_unit(t.b) : 1.0;
                         uint64_t e[PER], word[PER];
 #pragma unroll
                         for (int r = 0; r < PER; ++r) {
                             const int i = r * THREADS + threadIdx.x;
                             e[r] = i < count ? sm.list[i] : 0;
                             word[r] = i >= count ? 0
-                                      : by_mass  ? weight_word(expf(entry_value(e[r]) - m))
-                                                 : ((uint64_t)1 << kCountBits) | 1u;
+                                      : by_mass  ? weight_word(expf(entry_value(e[r]) - m), unit)
+                                                 : count_word();
                         }
                         const uint64_t all = word_weight(block_sum64(sm, word[0] + word[1] + word[2] + word[3]));
-                        const double rest = ceil((target - above) * (by_mass ? (double)kUnit : 1.0));
                         const uint64_t at = select_entry(sm, e, word, entry(ylo, 0xffffffffll), entry(yhi, 0),
-                                                         min(all, (uint64_t)fmax(rest, 1.0)));
+                                                         list_target((target - above) * unit, all));
                         if (threadIdx.x == 0) tell(sm, cluster, entry_value(at), entry_index(at));
                     }
                     ring::cluster_sync();
