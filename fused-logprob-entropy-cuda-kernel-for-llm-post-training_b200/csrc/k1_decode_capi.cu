@@ -36,6 +36,13 @@ extern "C" void k1_test_list(const float* w, int n, double share, uint64_t* word
     for (int i = 0; i < n; ++i) all += words[i] = weight_word(w[i], unit);
     *target = list_target(share * mass * unit, word_weight(all));
 }
+
+// The element that a lane with these eight weights draws.
+extern "C" int k1_test_pick(const float* w, double cum, double target) {
+    float v[8];
+    for (int i = 0; i < 8; ++i) v[i] = w[i];
+    return k1::sample::pick_element(v, cum, target);
+}
 #endif
 
 namespace {

@@ -726,17 +726,11 @@ struct Row {
                 const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0);
                 const int at = over ? __ffs(over) - 1 : 31 - __clz(some);
                 if (lane == at) {
-                    double cum = before + incl - mass;
-                    int64_t token = -1;
+                    const int el = pick_element(w, before + incl - mass, over ? target : INFINITY);
                     float d = 0.f;
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (w[e] > 0.f && !(over && cum > target)) {
-                            cum += (double)w[e];
-                            token = sl.index(j, e);
-                            d = y[e] - m;
-                        }
-                    p.token[row] = token;
+                    for (int e = 0; e < E; ++e) d = e == el ? y[e] - m : d;
+                    p.token[row] = sl.index(j, el);
                     p.logprob[row] = (float)((double)d - sm.logs[0]);
                     p.kept_logprob[row] = (float)((double)d - sm.logs[1]);
                 }

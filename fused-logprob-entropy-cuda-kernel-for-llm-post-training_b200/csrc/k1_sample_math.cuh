@@ -46,5 +46,21 @@ K1_HD uint64_t list_target(double mass, uint64_t all) {
     return t < (double)all ? (uint64_t)t : all;
 }
 
+// The element of a lane's vector at which the mass, `cum` in front of the vector, first exceeds
+// `target`, or the last one with a weight; -1 if none has any.  The first one with a weight is taken
+// even where `cum` is above the target already: `cum` is the lane's prefix sum less its own mass,
+// which in floating point may come out above the prefix of the lane before, the one that was compared.
+template <int E>
+K1_HD int pick_element(const float (&w)[E], double cum, double target) {
+    int at = -1;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (w[e] > 0.f && (at < 0 || !(cum > target))) {
+            cum += (double)w[e];
+            at = e;
+        }
+    return at;
+}
+
 }  // namespace sample
 }  // namespace k1

@@ -56,3 +56,27 @@ def test_a_nucleus_that_ends_among_the_lightest(v, dtype, lo, hi, below_one):
     u = torch.linspace(0, 1.2 * light, n, device="cuda")
     for kw in (dict(top_p=1 - below_one), dict(top_p=1 - below_one, top_k=v // 2), dict(top_p=1 - 2 * below_one)):
         check(x, u, 1e-9, **kw)
+
+
+# Rows (id: logit, the others masked) of two equal elements and a few whose weights are about half of
+# 2^-52: u = 1/2 falls on a prefix that two orders of adding round to either side of it.
+TIES = [{2: 0.0, 33: -36.75, 37: -36.75, 42: -38.375, 47: -36.75, 900: 0.0},
+        {5: -38.5, 12: 0.0, 33: -38.5, 43: -36.875, 900: 0.0},
+        {10: -38.0, 14: 0.0, 16: -36.375, 34: -35.75, 37: -35.25, 41: -38.25, 900: 0.0},
+        {4: -38.75, 6: -38.375, 18: 0.0, 41: -37.0, 45: -37.0, 900: 0.0},
+        {10: 0.0, 32: -38.5, 36: -37.75, 44: -37.0, 900: 0.0}]
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(min_p=1e-18)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_a_prefix_that_rounds_to_either_side_of_the_target(dtype, kw):
+    x = torch.full((len(TIES), 1024), float("-inf"))
+    for r, row in enumerate(TIES):
+        for i, y in row.items():
+            x[r, i] = y
+    x = x.to(dtype).cuda()
+    tok, lp, kp = kernel_opt.sample_tokens(x, torch.full((len(TIES),), 0.5, device="cuda"), **kw)
+    for r, row in enumerate(TIES):
+        # any element between the two heavy ones (their ends included): the masses there differ by 2^-51
+        assert int(tok[r]) in row, (r, int(tok[r]))
+        assert abs(float(lp[r]) - (row[int(tok[r])] - 0.6931472)) < 1e-5 and abs(float(kp[r] - lp[r])) < 1e-6

@@ -1,5 +1,5 @@
 """The sampling kernel's arithmetic on the host (csrc/k1_sample_math.cuh, through the test-only
-library): a list's weights as whole numbers, whatever their size."""
+library): a list's weights as whole numbers, whatever their size, and the element that a lane draws."""
 import ctypes
 import math
 
@@ -18,6 +18,8 @@ def lib():
     lib = ctypes.CDLL(WAIT_TEST_LIB)
     lib.k1_test_list.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p]
     lib.k1_test_list.restype = None
+    lib.k1_test_pick.argtypes = [ctypes.c_void_p, ctypes.c_double, ctypes.c_double]
+    lib.k1_test_pick.restype = ctypes.c_int
     return lib
 
 
@@ -66,3 +68,34 @@ def test_a_list_keeps_its_mass(lib, name, w, share):
 def test_a_list_without_mass_asks_for_nothing(lib):
     out, target = words(lib, [0.0, 0.0], 0.9)
     assert out == [1, 1] and target == 0
+
+
+def pick(lib, w, cum, target):
+    w = np.array(list(w) + [0] * (8 - len(w)), np.float32)
+    return lib.k1_test_pick(w.ctypes.data, cum, target)
+
+
+def test_the_element_whose_prefix_exceeds_the_target(lib):
+    assert pick(lib, [0.25, 0, 0.25, 0.5], 1.0, 1.0) == 0
+    assert pick(lib, [0.25, 0, 0.25, 0.5], 1.0, 1.25) == 2
+    assert pick(lib, [0.25, 0, 0.25, 0.5], 1.0, 1.49) == 2
+    assert pick(lib, [0.25, 0, 0.25, 0.5], 1.0, 1.5) == 3
+    assert pick(lib, [0.25, 0, 0.25, 0.5], 1.0, math.inf) == 3   # none exceeds: the last with a weight
+    assert pick(lib, [0, 0, 0, 0.5], 0.0, 0.0) == 3
+    assert pick(lib, [0] * 8, 0.0, 0.0) == -1
+
+
+def test_a_lane_with_mass_always_draws(lib):
+    """The prefix sums of a warp's lanes are rounded in another order than a lane's prefix less its
+    own mass: here the third lane's prefix exceeds the target, which the second's does not, and its
+    start (1 + 2^-52) does too."""
+    t = 0.4 * 2.0 ** -52
+    lane = [np.float32(t)]
+    incl = 1.0 + (t + t)                 # a tree adds the two small ones first
+    assert 1.0 + t == 1.0 and incl == 1.0 + 2.0 ** -52 and incl - t > 1.0
+    assert pick(lib, lane, incl - float(np.float32(t)), 1.0) == 0
+    rng = np.random.default_rng(2)
+    for _ in range(2000):
+        w = rng.random(8).astype(np.float32) * (rng.random(8) < 0.5)
+        got = pick(lib, w, rng.random() * 2, rng.random() * 2)
+        assert (got >= 0) == bool((w > 0).any()) and (got < 0 or w[got] > 0)
