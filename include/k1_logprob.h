@@ -406,8 +406,9 @@ typedef struct k1_sampling {
  *     token = the first kept index at which the kept mass up to it (in index order) exceeds
  *     u * (kept mass), u in [0, 1)
  *     logprob = log(w_token / sum of all w), kept_logprob = log(w_token / kept mass)
- * (at temperature 0: logprob at temperature 1, kept_logprob 0).  Sums are accurate to about
- * 1e-11, so a token does not depend on how the work is split.  A row with a NaN or +inf, with
+ * (at temperature 0: logprob at temperature 1, kept_logprob 0).  Sums are right to about 1e-12 of
+ * the mass, so a token depends on how the work is split (a row's address, the number of rows) only
+ * where u or top_p lies that close to a boundary.  A row with a NaN or +inf, with
  * nothing above -inf, or with a temperature that is negative or not finite gives token -1
  * and NaN log-probabilities.  logits: n_rows rows of `vocab` elements, row_stride apart.
  */

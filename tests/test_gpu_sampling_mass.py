@@ -80,3 +80,76 @@ def test_a_prefix_that_rounds_to_either_side_of_the_target(dtype, kw):
         # any element between the two heavy ones (their ends included): the masses there differ by 2^-51
         assert int(tok[r]) in row, (r, int(tok[r]))
         assert abs(float(lp[r]) - (row[int(tok[r])] - 0.6931472)) < 1e-5 and abs(float(kp[r] - lp[r])) < 1e-6
+
+
+# Sums are right to a few 1e-13 of the mass (a list's to 2^-40), so a u whose share lies NEAR[0] or
+# more from every prefix draws what sums in 64 bits draw; those tried lie within NEAR[1] of one.
+NEAR = (4e-12, 4e-11)
+
+
+def near_boundaries(w):
+    """fp32 numbers u in [1/4, 1) whose distance from a prefix of the weights w (as a share of their
+    sum) is in NEAR, and the tokens that they draw."""
+    c = w.double().cumsum(-1)
+    c = c / c[-1]
+    c = c[(c >= 0.25) & (c < 1 - 1e-6)]
+    u = c.float()
+    d = (u.double() - c).abs()
+    u = u[(d > NEAR[0]) & (d < NEAR[1])]
+    full = w.double().cumsum(-1)
+    share = u.double() * full[-1]
+    at = torch.searchsorted(full, share, right=True)
+    gap = torch.minimum((full[at] - share).abs(), (share - full[at - 1]).abs()) / full[-1]
+    return u[gap > NEAR[0]], at[gap > NEAR[0]]
+
+
+@pytest.mark.parametrize("v,dtype,peak,sigma", [
+    (152063, torch.float32, 12.0, 0.5), (152063, torch.bfloat16, 12.0, 0.5), (128256, torch.float16, 10.0, 1.0),
+    (152064, torch.float32, 0.0, 3.0), (400003, torch.float32, 14.0, 0.5)])
+def test_shares_are_right_at_any_address_and_in_any_batch(v, dtype, peak, sigma):
+    """One heavy element over a heavy tail of light ones, at addresses that are not all alike to a
+    16-byte vector, in batches that cut rows into 8, 4 or 2 parts or none."""
+    g = torch.Generator(device="cuda").manual_seed(v)
+    row = torch.randn(v, generator=g, device="cuda").mul_(sigma)
+    if peak:
+        row[v // 7] = peak
+    row = row.to(dtype)
+    y = row.float()
+    u, want = near_boundaries(torch.exp(y - y.max()))
+    assert len(u) >= 20, len(u)
+    buf = torch.empty(v + 8, dtype=dtype, device="cuda")
+    for shift in (0, 1, 3):
+        buf[shift:shift + v] = row
+        x = buf[shift:shift + v]
+        for n in (1, 20, 300):
+            for at in range(0, min(len(u), 4 * n), n):
+                k = len(u[at:at + n])
+                tok = kernel_opt.sample_tokens(x.expand(n, v)[:k], u[at:at + n])[0]
+                assert torch.equal(tok, want[at:at + n]), (shift, n, int((tok != want[at:at + n]).sum()))
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=1000), dict(top_k=1000, top_p=0.95), dict(top_k=5000), dict(top_p=0.9)], ids=str)
+@pytest.mark.parametrize("sigma", [1.0, 3.0])
+def test_shares_of_what_is_kept_are_right_in_any_batch(sigma, kw):
+    """The same behind filters, whose threshold comes from a list or from the whole row."""
+    n, v = 200, 50257
+    g = torch.Generator(device="cuda").manual_seed(int(sigma))
+    x = torch.randn(n, v, generator=g, device="cuda").mul_(sigma)
+    u, want = torch.full((n,), 0.5, device="cuda"), torch.full((n,), -1, device="cuda")
+    for r in range(n):
+        w = torch.exp(x[r] - x[r].max())
+        ws, order = torch.sort(w.double(), descending=True, stable=True)
+        kept = kw.get("top_k", v)
+        if "top_p" in kw:
+            cum = ws[:kept].cumsum(0)
+            kept = max(1, int((cum - ws[:kept] < float(torch.tensor(kw["top_p"])) * cum[-1]).sum()))
+        ids = torch.sort(order[:kept]).values
+        some, at = near_boundaries(w[ids])
+        if len(some):
+            u[r], want[r] = some[0], ids[at[0]]
+    hit = want >= 0
+    assert int(hit.sum()) >= 10
+    tok = kernel_opt.sample_tokens(x, u, **kw)[0]
+    assert torch.equal(tok[hit], want[hit]), int((tok != want)[hit].sum())
+    for r in torch.nonzero(hit)[:20, 0].tolist():
+        assert int(kernel_opt.sample_tokens(x[r:r + 1], u[r:r + 1], **kw)[0]) == int(want[r])
