@@ -43,7 +43,9 @@
 // cannot hide all of it.
 //
 // A row that holds a NaN or +inf, or nothing above -inf, has no distribution: token -1 and
-// NaN log-probabilities.
+// NaN log-probabilities.  So does one whose own settings mean nothing (a temperature that is negative
+// or not finite, a negative top-p, a min-p outside [0, 1], a NaN); as numbers for all rows they are
+// refused.
 #pragma once
 
 #include "k1_common.cuh"
@@ -843,8 +845,13 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
     const Joined range = exchange<RANGE, WARPS>(sm, R.phase, cluster, rank, 0.0, 0.0, 0, lo, hi);
     const float m = range.hi;
     R.m = m;
-    // NaN, +inf, or nothing above -inf; or a temperature that is negative or no number
-    if (!(m > -INFINITY && m < INFINITY) || !(temp >= 0.f && R.s > 0.f)) {
+    // NaN, +inf, or nothing above -inf; or a setting of the row's own that means nothing
+    bool none = !(m > -INFINITY && m < INFINITY) || !(temp >= 0.f && R.s > 0.f);
+    if constexpr (FILTER) {
+        if (p.top_p) none |= !(p.top_p[row] >= 0.f);
+        if (p.min_p) none |= !(p.min_p[row] >= 0.f && p.min_p[row] <= 1.f);
+    }
+    if (none) {
         if (leader && threadIdx.x == 0) {
             p.token[row] = -1;
             p.logprob[row] = p.kept_logprob[row] = __int_as_float(0x7fc00000);
@@ -862,7 +869,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
         if (top_k <= 0 || top_k >= p.vocab) top_k = 0;
         const float top_p = greedy ? 1.f : p.top_p ? p.top_p[row] : p.top_p0;
         const bool use_p = top_p < 1.f;
-        const float min_p = greedy ? 0.f : fminf(p.min_p ? p.min_p[row] : p.min_p0, 1.f);
+        const float min_p = greedy ? 0.f : p.min_p ? p.min_p[row] : p.min_p0;
         const float floor = m - kFloor;
 
         // ---- a bound for a short list ----
@@ -1195,7 +1202,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
             }
             if (!by_mass && use_p) Z = R.template kept_mass<false>(sm, keep).a;
         }
-        keep.min_p = min_p > 0.f ? min_p : 0.f;
+        keep.min_p = min_p;
         const Joined C = R.template kept_mass<false>(sm, keep);
         R.template draw<false>(sm, keep, C, u * C.a, S, p, row);
     }

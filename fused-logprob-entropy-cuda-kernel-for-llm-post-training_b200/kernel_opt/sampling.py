@@ -30,7 +30,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     are off; temperature 0 takes the first largest logit.
 
     logprobs: of the token in the whole distribution at this temperature (at 0: at 1);
-    kept_logprobs: in the filtered, renormalised one.  A row with a NaN or +inf, or nothing
-    above -inf (or, per row, a temperature that is negative or not finite), gives token -1 and
-    NaN."""
+    kept_logprobs: in the filtered, renormalised one.  No gradient flows.  A row with a NaN or
+    +inf (after the division too), or nothing above -inf, gives token -1 and NaN; so does one whose
+    own setting means nothing (a temperature that is negative or not finite, a negative top_p, a
+    min_p outside [0, 1], a NaN), which as a number for all rows is refused."""
     return _C.sample_tokens(logits, u, temperature, top_k, top_p, min_p)

@@ -409,8 +409,9 @@ typedef struct k1_sampling {
  * (at temperature 0: logprob at temperature 1, kept_logprob 0).  Sums are right to about 1e-12 of
  * the mass, so a token depends on how the work is split (a row's address, the number of rows) only
  * where u or top_p lies that close to a boundary.  A row with a NaN or +inf, with
- * nothing above -inf, or with a temperature that is negative or not finite gives token -1
- * and NaN log-probabilities.  logits: n_rows rows of `vocab` elements, row_stride apart.
+ * nothing above -inf, or with a setting of its own that means nothing (a temperature that is
+ * negative or not finite, a negative top_p, a min_p outside [0, 1], a NaN: refused as numbers)
+ * gives token -1 and NaN log-probabilities.  logits: n_rows rows of `vocab` elements, row_stride apart.
  */
 int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
                      int64_t row_stride, const float* u, const k1_sampling* settings,
