@@ -743,7 +743,9 @@ const V* setting(const pybind11::object& v, at::ScalarType type, const at::Tenso
     const at::Tensor& t = THPVariable_Unpack(v.ptr());
     TORCH_CHECK_VALUE(t.dim() == 0 || t.sizes() == u.sizes(), what,
                       " must be a number or a tensor shaped like the rows ", u.sizes(), ", got ", t.sizes());
-    rows = t.to(u.device(), type).expand(u.sizes()).contiguous();
+    // 64-bit whole numbers are cut to 32 bits as numbers are, not to their low halves
+    const bool wide = type == at::kInt && t.scalar_type() == at::kLong;
+    rows = (wide ? t.clamp(0, INT32_MAX) : t).to(u.device(), type).expand(u.sizes()).contiguous();
     return rows.const_data_ptr<V>();
 }
 
@@ -769,6 +771,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sample_tokens(const at::Tensor& l
     s.top_k_rows = setting<int>(top_k, at::kInt, u, "top_k", &k, k_rows);
     s.top_p_rows = setting<float>(top_p, at::kFloat, u, "top_p", &p, p_rows);
     s.min_p_rows = setting<float>(min_p, at::kFloat, u, "min_p", &q, q_rows);
+    TORCH_CHECK_VALUE(k == k, "top_k must be a whole number, got nan");
     s.top_k = (int)std::min(std::max(k, 0.0), (double)INT32_MAX);
     s.top_p = (float)p;
     s.min_p = (float)q;

@@ -35,3 +35,21 @@ def test_a_greedy_row_with_a_bad_filter():
     u = torch.rand(2, device="cuda")
     tok, lp, _ = kernel_opt.sample_tokens(x, u, temperature=0.0, min_p=torch.tensor([NAN, 0.0], device="cuda"))
     assert int(tok[0]) == -1 and torch.isnan(lp[0]) and int(tok[1]) == int(x[1].argmax())
+
+
+def test_top_k_beyond_32_bits():
+    """A 64-bit top_k above the vocabulary is off, not what its low 32 bits say."""
+    x = torch.randn(4, 3000, device="cuda")
+    u = torch.full((4,), 0.999, device="cuda")
+    want = kernel_opt.sample_tokens(x, u)
+    k = torch.tensor([2 ** 32 + 1, 2 ** 31, 2 ** 62, -2 ** 40 + 1], device="cuda")
+    got = kernel_opt.sample_tokens(x, u, top_k=k)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], got[1])
+    got = kernel_opt.sample_tokens(x, u, top_k=2 ** 32 + 1)
+    assert torch.equal(got[0], want[0])
+
+
+def test_a_top_k_that_is_no_number():
+    x, u = torch.randn(1, 100, device="cuda"), torch.rand(1, device="cuda")
+    with pytest.raises(ValueError, match="top_k must be"):
+        kernel_opt.sample_tokens(x, u, top_k=NAN)
