@@ -61,7 +61,8 @@ template <typename T>
 struct Piece<T, DT<T>::kEPV> {
     static constexpr int E = DT<T>::kEPV;
     uint4 v;
-    __device__ __forceinline__ void load(const T* p) { v = ldg_stream(p); }
+    // not .nc: the stream may be written over x or the residual
+    __device__ __forceinline__ void load(const T* p) { v = ld_stream(p); }
     __device__ __forceinline__ void load_cached(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
     __device__ __forceinline__ void store(T* p) const { stg_stream(p, v); }
     __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
