@@ -83,6 +83,13 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
     return false;
 }
 
+// The same for a converged warp, true where all lanes saw the phase complete: lanes whose limit ran
+// out and lanes whose poll came after the completion must not part before the warp's next elect or
+// TMEM load.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, wait(bar, parity, abort));
+}
+
 // A place in a ring of N slots and the parity of its current round.
 template <int N>
 struct Place {
@@ -223,64 +230,63 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
     // shared-memory addresses
     const uint32_t a_ring = ring::saddr(smem), a_full = ring::saddr(full), a_empty = ring::saddr(empty),
                    a_tfull = ring::saddr(tfull), a_tempty = ring::saddr(tempty);
-    // The producer's and the issuer's warp walk their loops whole; one elected lane issues.
+    // One elected lane walks the producer's loop, and one the issuer's: it waits and issues.  (A whole
+    // warp that elects a lane at every block of K would have to vote on each bounded wait, so that
+    // its lanes stop together: 64 x 3584 x 128256 102.5 us with one lane, 104.6 with votes.)
     if (warp == 0) {
-        Place<S::STAGES> at;
-        bool ok = true;
-        int issued = 0;
-        for (int kb = kb0; kb < kb1; ++kb, ++issued, at.next()) {
-            if (!wait(a_empty + at.slot * 8, at.parity ^ 1u, abort)) {
-                ok = false;
-                break;
-            }
+        if (ring::elect_one()) {
+            Place<S::STAGES> at;
+            bool ok = true;
+            int issued = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++issued, at.next()) {
+                if (!wait(a_empty + at.slot * 8, at.parity ^ 1u, abort)) {
+                    ok = false;
+                    break;
+                }
 #ifdef K1_WAIT_TEST
-            if (blockIdx.x == 0 && (long long)issued == k1_test_withhold) {
-                ok = false;  // test only: block 0 issues nothing more
-                break;
-            }
+                if (blockIdx.x == 0 && (long long)issued == k1_test_withhold) {
+                    ok = false;  // test only: block 0 issues nothing more
+                    break;
+                }
 #endif
-            const uint32_t st = a_ring + at.slot * S::STAGE, bar = a_full + at.slot * 8;
-            if (ring::elect_one()) {
+                const uint32_t st = a_ring + at.slot * S::STAGE, bar = a_full + at.slot * 8;
                 ring::arrive_expect(&full[at.slot], S::STAGE);
                 tma_load_2d_at(st, &tmap_w, kb * BK, tile * BM, bar);
                 tma_load_2d_at(st + S::W_BYTES, &tmap_x, kb * BK, tok0, bar);
             }
-            __syncwarp();
+            if (!ok)  // stopping early: wait (bounded) for the copies in flight
+                for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
+                    ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         }
-        if (!ok)  // stopping early: wait (bounded) for the copies in flight
-            for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
-                ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         __syncwarp();
         if (split > 1)  // no copy is in flight
             asm volatile("bar.arrive 2, %0;" ::"n"(S::GROUPS * 128 + 32) : "memory");
     } else if (warp == 1) {
-        Place<S::STAGES> at;
-        Place<S::NBUF> acc;
-        const uint64_t dw0 = smem_desc(a_ring), dx0 = smem_desc(a_ring + S::W_BYTES);
-        // both barriers of the next block are tested together, while this one's MMAs run
-        bool freed = true, there = false;
-        for (int i = 0; i < kb1 - kb0; ++i) {
-            if (!freed && !wait(a_tempty + acc.slot * 8, acc.parity ^ 1u, abort)) break;
-            if (!there && !wait(a_full + at.slot * 8, at.parity, abort)) break;
-            tc_fence_after();
-            const uint64_t dw = dw0 + at.slot * (S::STAGE >> 4), dx = dx0 + at.slot * (S::STAGE >> 4);
-            const uint32_t d = tmem + acc.slot * TN;
-            if (ring::elect_one()) {
+        if (ring::elect_one()) {
+            Place<S::STAGES> at;
+            Place<S::NBUF> acc;
+            const uint64_t dw0 = smem_desc(a_ring), dx0 = smem_desc(a_ring + S::W_BYTES);
+            // both barriers of the next block are tested together, while this one's MMAs run
+            bool freed = true, there = false;
+            for (int i = 0; i < kb1 - kb0; ++i) {
+                if (!freed && !wait(a_tempty + acc.slot * 8, acc.parity ^ 1u, abort)) break;
+                if (!there && !wait(a_full + at.slot * 8, at.parity, abort)) break;
+                tc_fence_after();
+                const uint64_t dw = dw0 + at.slot * (S::STAGE >> 4), dx = dx0 + at.slot * (S::STAGE >> 4);
+                const uint32_t d = tmem + acc.slot * TN;
 #pragma unroll
                 for (int k = 0; k < BK / UK; ++k)  // +32 bytes per K slice: +2 in >> 4 units
                     umma8<TN>(d, dw + 2 * k, dx + 2 * k, k > 0 ? 1u : 0u);
                 umma_commit_at(a_empty + at.slot * 8);
                 umma_commit_at(a_tfull + acc.slot * 8);
+                at.next();
+                acc.next();
+                there = ring::test_at(a_full + at.slot * 8, at.parity);
+                freed = ring::test_at(a_tempty + acc.slot * 8, acc.parity ^ 1u);
             }
-            __syncwarp();
-            at.next();
-            acc.next();
-            there = ring::test_at(a_full + at.slot * 8, at.parity);
-            freed = ring::test_at(a_tempty + acc.slot * 8, acc.parity ^ 1u);
+            umma_commit(drain);  // every MMA issued has completed before the TMEM is freed
+            ring::wait(drain, 0);
         }
-        if (ring::elect_one()) umma_commit(drain);  // every MMA issued has completed before
-        __syncwarp();                               // the TMEM is freed
-        ring::wait(drain, 0);
     } else {
         // each thread owns one row of the weight (a TMEM lane) and its group's tokens
         constexpr int CW = S::CW, EPI = S::GROUPS * 128;
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
         for (int i = 0; i < nkb; ++i, buf.next()) {
             const uint32_t a = buf.slot;
             // warp-uniform: the TMEM loads below are warp-collective
-            if (!__all_sync(0xffffffffu, wait(a_tfull + a * 8, buf.parity, abort))) {
+            if (!warp_wait(a_tfull + a * 8, buf.parity, abort)) {
 #pragma unroll
                 for (int j = 0; j < CW; ++j) acc[j] = __int_as_float(0x7fc00000);
                 break;
@@ -570,24 +576,24 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
             bool ok = true;
             uint32_t issued = 0;
             const uint32_t cl_full = ring::mapa(a_full, 0);  // the leader's barriers
-            for (int u = first; ok && u < units; u += step) {
-                int mt, nt;
-                wide_tile(p, u, mt, nt);
-                const int row_x = mt * S::TM + (int)rank * BM;
-                const int row_w = nt * S::BN + (int)rank * S::LOAD_N;
-                for (int kb = 0; kb < p.kb_total; ++kb, ++issued, at.next()) {
-                    if (!wait(a_empty + at.slot * 8, at.parity ^ 1u, abort)) {
-                        ok = false;
-                        break;
-                    }
+            if (ring::elect_one()) {
+                for (int u = first; ok && u < units; u += step) {
+                    int mt, nt;
+                    wide_tile(p, u, mt, nt);
+                    const int row_x = mt * S::TM + (int)rank * BM;
+                    const int row_w = nt * S::BN + (int)rank * S::LOAD_N;
+                    for (int kb = 0; kb < p.kb_total; ++kb, ++issued, at.next()) {
+                        if (!wait(a_empty + at.slot * 8, at.parity ^ 1u, abort)) {
+                            ok = false;
+                            break;
+                        }
 #ifdef K1_WAIT_TEST
-                    if (blockIdx.x == 0 && (long long)issued == k1_test_withhold) {
-                        ok = false;  // test only: block 0 issues nothing more
-                        break;
-                    }
+                        if (blockIdx.x == 0 && (long long)issued == k1_test_withhold) {
+                            ok = false;  // test only: block 0 issues nothing more
+                            break;
+                        }
 #endif
-                    const uint32_t st = a_ring + at.slot * S::STAGE, cl = cl_full + at.slot * 8;
-                    if (ring::elect_one()) {
+                        const uint32_t st = a_ring + at.slot * S::STAGE, cl = cl_full + at.slot * 8;
                         tma_load_2d_pair_at(st, &tmap_x, kb * BK, row_x, cl);
                         tma_load_2d_pair_at(st + S::X_BYTES, &tmap_w, kb * BK, row_w, cl);
                         if (leader)
@@ -595,15 +601,14 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                         else
                             ring::arrive_remote(cl);
                     }
-                    __syncwarp();
                 }
+                if (!ok && leader)  // stopping early: wait (bounded) for the copies in flight
+                    for (uint32_t i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
+                        ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
             }
-            if (!ok && leader)  // stopping early: wait (bounded) for the copies in flight
-                for (uint32_t i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
-                    ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
         } else if (warp == 1) {
             // ---------------- MMA issuer (the leader, for both) ----------------
-            if (leader) {
+            if (leader && ring::elect_one()) {
                 Place<S::STAGES> at;
                 Place<S::NBUF> acc;
                 bool ok = true;
@@ -620,25 +625,21 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                         tc_fence_after();
                         const uint64_t dx = dx0 + at.slot * (S::STAGE >> 4), dw = dw0 + at.slot * (S::STAGE >> 4);
                         const uint32_t d = tmem + acc.slot * S::BN;
-                        if (ring::elect_one()) {
 #pragma unroll
-                            for (int k = 0; k < BK / UK; ++k)
-                                asm volatile(
-                                    "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                                    "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                                    "l"(dx + 2 * k), "l"(dw + 2 * k), "r"(S::IDESC), "r"(k > 0 ? 1u : 0u));
-                            umma_commit_pair_at(a_empty + at.slot * 8);
-                            umma_commit_pair_at(a_tfull + acc.slot * 8);
-                        }
-                        __syncwarp();
+                        for (int k = 0; k < BK / UK; ++k)
+                            asm volatile(
+                                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                                "l"(dx + 2 * k), "l"(dw + 2 * k), "r"(S::IDESC), "r"(k > 0 ? 1u : 0u));
+                        umma_commit_pair_at(a_empty + at.slot * 8);
+                        umma_commit_pair_at(a_tfull + acc.slot * 8);
                         at.next();
                         acc.next();
                         there = ring::test_at(a_full + at.slot * 8, at.parity);
                         freed = ring::test_at(a_tempty + acc.slot * 8, acc.parity ^ 1u);
                     }
                 }
-                if (ring::elect_one()) umma_commit_pair(drain);  // every MMA issued has completed
-                __syncwarp();                                    // before the TMEM is freed
+                umma_commit_pair(drain);  // every MMA issued has completed before the TMEM is freed
                 ring::wait(drain, 0);
             }
         } else if (warp == 2) {
@@ -654,7 +655,7 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                 const int rows = (int)max((int64_t)0, min((int64_t)BM, p.m - m0));
                 const int64_t nb = (int64_t)nt * 2, nb_last = (p.n - 1) / 128;
                 for (int k0 = 0; k0 < p.kb_total; k0 += S::SB, at.next()) {
-                    if (!__all_sync(0xffffffffu, wait(a_sempty + at.slot * 8, at.parity ^ 1u, abort))) {
+                    if (!warp_wait(a_sempty + at.slot * 8, at.parity ^ 1u, abort)) {
                         ok = false;
                         break;
                     }
@@ -710,14 +711,14 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
             };
             for (int k0 = 0; ok && k0 < p.kb_total; k0 += S::SB, chunk.next()) {
                 // warp-uniform: the TMEM loads are warp-collective
-                ok = __all_sync(0xffffffffu, wait(a_sfull + chunk.slot * 8, chunk.parity, abort));
+                ok = warp_wait(a_sfull + chunk.slot * 8, chunk.parity, abort);
                 if (!ok) break;
                 const float* sx = scales + chunk.slot * (S::S_BYTES / 4) + rloc;
                 const float* sw = scales + chunk.slot * (S::S_BYTES / 4) + S::SB * S::SROW + part;
                 const int n = min(S::SB, p.kb_total - k0);
                 for (int kc = 0; kc < n; ++kc) {
                     const float2 f = splat(sx[kc * S::SROW] * sw[2 * kc]);
-                    if (!__all_sync(0xffffffffu, wait(a_tfull + buf * 8, parity, abort))) {
+                    if (!warp_wait(a_tfull + buf * 8, parity, abort)) {
                         ok = false;
                         break;
                     }
