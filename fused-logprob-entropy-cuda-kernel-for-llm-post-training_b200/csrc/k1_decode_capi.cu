@@ -365,21 +365,31 @@ int wide(const char* fn, k1::fp8::Params p, const void* x, int64_t ldx, const vo
     return launched(fn, launch_cluster(kern, grid, S::THREADS, (size_t)S::SMEM, 2, st, tx, tw, p));
 }
 
-template <typename OutT>
-int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
-           int64_t inner, int sms, int dev, cudaStream_t st) {
-    if (p.m <= 16) return skinny<16, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-    if (p.m <= 32) return skinny<32, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+// The kernel of a product: the tokens per block of the few-token kernel, or 0 for the many-token
+// kernel.
+int linear_kernel(int64_t m, int64_t n, int kb_total, int sms) {
+    if (m <= 16) return 16;
+    if (m <= 32) return 32;
     // The few-token kernel in blocks of 64 tokens (two blocks of threads per SM) or the
     // many-token kernel (a tile per two SMs), by their rounds times what a round takes: about
     // 4 + 0.65 us per block of K, and 10 + 0.6.  Measured (us, few / many): 936 x 800 x 1978
     // 8.7 / 17.2; 162 x 1328 x 12141 12.9 / 20.3; 142 x 4352 x 14269 41 / 33; 300 x 3584 x 8192
     // 34 / 26; 128 x 3584 x 32768 43 / 44; 2180 x 6160 x 3492 127 / 71.
-    const int64_t few = (p.m + 63) / 64 * ((p.n + 127) / 128), many = (p.m + 255) / 256 * ((p.n + 255) / 256);
-    const double few_us = (double)((few + 2 * sms - 1) / (2 * sms)) * (4.0 + 0.65 * p.kb_total);
-    const double many_us = (double)((many + sms / 2 - 1) / (sms / 2)) * (10.0 + 0.6 * p.kb_total);
-    if (p.m <= 64 || few_us <= many_us) return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-    return wide<OutT>(fn, p, x, ldx, w, ldw, inner, dev, st);
+    const int64_t few = (m + 63) / 64 * ((n + 127) / 128), many = (m + 255) / 256 * ((n + 255) / 256);
+    const double few_us = (double)((few + 2 * sms - 1) / (2 * sms)) * (4.0 + 0.65 * kb_total);
+    const double many_us = (double)((many + sms / 2 - 1) / (sms / 2)) * (10.0 + 0.6 * kb_total);
+    return m <= 64 || few_us <= many_us ? 64 : 0;
+}
+
+template <typename OutT>
+int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
+           int64_t inner, int sms, int dev, cudaStream_t st) {
+    switch (linear_kernel(p.m, p.n, p.kb_total, sms)) {
+        case 16: return skinny<16, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+        case 32: return skinny<32, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+        case 64: return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+        default: return wide<OutT>(fn, p, x, ldx, w, ldw, inner, dev, st);
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -430,6 +440,13 @@ int sample(const char* fn, const k1::sample::Params& p, int sms, int dev, cudaSt
 }  // namespace
 
 extern "C" {
+
+#ifdef K1_WAIT_TEST
+// Which kernel a product takes on a device of `sms` SMs, so that a test knows which one it tests.
+int k1_test_linear_kernel(int64_t tokens, int64_t inner, int64_t outer, int sms) {
+    return linear_kernel(tokens, outer, (int)((inner + 127) / 128), sms);
+}
+#endif
 
 int k1_residual_rmsnorm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                         const void* weight, int weight_dtype, int dtype, int64_t n_rows, int64_t hidden,
