@@ -602,9 +602,14 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                             ring::arrive_remote(cl);
                     }
                 }
-                if (!ok && leader)  // stopping early: wait (bounded) for the copies in flight
+                // Stopping early: wait (bounded) for the copies in flight.  They are counted on the
+                // leader's barriers, which the other CTA cannot wait on: it stays about a millisecond,
+                // a hundred times what a tile takes, before it lets its shared memory go.
+                if (!ok && leader)
                     for (uint32_t i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
                         ring::wait(&full[i % S::STAGES], (i / S::STAGES) & 1);
+                else if (!ok)
+                    for (long long i = 0, t = clock64(); i < 1000 && clock64() - t < 2000000; ++i) __nanosleep(2000);
             }
         } else if (warp == 1) {
             // ---------------- MMA issuer (the leader, for both) ----------------

@@ -2,11 +2,12 @@
 the rule between them cannot move the tests away from what they test."""
 import pytest
 
+import test_gpu_decode_waits_pair as waits
 import test_gpu_fp8_many_tokens as many
 from _linear import MANY, kernel_of
 
 
-@pytest.mark.parametrize("m,k,n", many.SHAPES + [many.LAYOUT])
+@pytest.mark.parametrize("m,k,n", many.SHAPES + waits.SHAPES + [many.LAYOUT])
 def test_many_tokens(m, k, n):
     assert kernel_of(m, k, n) == MANY
 

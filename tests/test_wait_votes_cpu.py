@@ -29,3 +29,13 @@ def test_waits_are_one_lanes_or_voted_on(name):
         assert not any(a <= m.start() < b for a, b in elected)
     for a, b in elected:  # nothing that a whole warp must reach
         assert "sync" not in body[a:b] and "bar." not in body[a:b]
+
+
+def test_both_ctas_of_a_pair_stay_for_their_copies():
+    """A producer that stops early keeps its shared memory until its copies have landed: the pair's
+    leader, whose barriers count them, and the other CTA, which has none to wait on."""
+    body = kernel_body("k1_fp8_linear.cuh", "k1_fp8_wide_kernel")
+    at = body.index("if (!ok && leader)")
+    stay = re.match(r"if \(!ok && leader\)\s*for \([^{}]*ring::wait\([^;]*;\s*else if \(!ok\)\s*for \([^{}]*__nanosleep",
+                    body[at:])
+    assert stay
