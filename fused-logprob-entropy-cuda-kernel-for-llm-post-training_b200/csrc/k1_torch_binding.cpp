@@ -640,6 +640,10 @@ struct ResidualRmsnorm : public torch::autograd::Function<ResidualRmsnorm> {
 std::tuple<at::Tensor, at::Tensor> residual_rmsnorm(const at::Tensor& x, const c10::optional<at::Tensor>& residual_,
                                                     const at::Tensor& weight, double eps) {
     const at::Tensor residual = residual_.has_value() ? *residual_ : at::Tensor();
+    // a tangent would be lost where the node is not entered
+    for (const at::Tensor* t : {&x, &residual, &weight})
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                    "the residual RMS norm does not support forward AD: it has no jvp");
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || weight.requires_grad() || (residual.defined() && residual.requires_grad()))) {
         norm_inputs(x, residual, weight, eps);

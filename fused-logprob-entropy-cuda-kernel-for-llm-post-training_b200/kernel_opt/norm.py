@@ -21,7 +21,7 @@ def fused_residual_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weigh
 
     x, residual: [..., H] bf16 / fp16 / fp32 of one shape and dtype (H at most 16384; rows may
     be strided); weight: [H] of the same dtype or fp32.  `residual=None`: stream is x itself.
-    Differentiable in x, residual and weight, through y and through the stream."""
+    Differentiable (once, backwards) in x, residual and weight, through y and through the stream."""
     return _C.residual_rmsnorm(x, residual, weight, eps)
 
 
