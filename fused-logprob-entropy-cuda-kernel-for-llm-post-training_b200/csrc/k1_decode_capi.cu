@@ -122,8 +122,8 @@ NormShape norm_shape(int hidden, int es, int e) {
     return s;
 }
 
-// Blocks that fill the device: as many as are resident at 2048 threads per SM, or the
-// rows if there are fewer.
+// Blocks of a launch: as many as 2048 threads per SM make (registers, which may let fewer reside,
+// are not counted), or the rows if there are fewer.
 int64_t norm_grid(int64_t n, int threads, int sms, int most_per_sm) {
     const int per_sm = std::max(1, std::min(most_per_sm, 2048 / threads));
     return std::min<int64_t>(n, (int64_t)sms * per_sm);

@@ -21,8 +21,8 @@
 // scale is one product per block), 128 accumulators in registers; it loads the next 32
 // columns from TMEM while it adds the last.
 //
-// Measured on B200: 1 x 3584 x 152064 82 us (the weight's bytes at 6.6 TB/s, the measured copy
-// rate), 64 x 3584 x 128256 101 us (4.7 TB/s: the last round of blocks and the 64-column epilogue
+// Measured on B200: 1 x 3584 x 152064 83 us (the weight's bytes at 6.6 TB/s, the measured copy
+// rate), 64 x 3584 x 128256 101 to 103 us (4.6 to 4.7 TB/s: the last round of blocks and the 64-column epilogue
 // between loads), 2048 x 3584 x 32768 285 to 295 us (1.63 to 1.69 PFLOP/s: adding the blocks in
 // fp32 takes about 40 us of it that the tensor cores do not hide, and a block of K's
 // handshakes, tile copies and operand reads fill what the MMAs leave of shared memory's

@@ -9,21 +9,23 @@
 //
 // The norm reads the stream as it is stored, so the forward, the backward (which keeps only
 // s and R) and the next layer all see the same numbers.  Sums, R and dw are fp32; y (and ds)
-// is rounded once.  The 8-bit output is rounded once too, from fp32 (in bf16 from the exact
-// quotient: R cancels in y / a, and s w has 16 bits).
+// is rounded once.  The 8-bit output is rounded once too, from fp32: in bf16 (values and weight)
+// from the exact quotient, since R cancels in y / a and s w has 16 bits; in fp16 and fp32 the product
+// is rounded to 24 bits first, so a value that lies that close to a midpoint may land one step off.
 //
 // One block of threads owns a row at a time and keeps it in registers between the sum of
 // squares and the output, so every tensor crosses HBM once: 4 N H elements forward (x, r, s,
 // y), 4 N H backward (gy, gs, s, ds).  Both are bound by that traffic.  Blocks are
-// persistent (grid = resident blocks): a thread keeps the same columns for every row, which
-// lets the backward add up its columns of dw in registers and write one partial row per
-// block; a second kernel adds the blocks' partials in block order (no atomics, so dw does
-// not depend on timing).
+// persistent, as many as 2048 threads per SM make (four per SM at most in the backward).  Registers
+// may let fewer reside at a time: with 8-bit output 8192 x 3584 bf16 runs its 8 blocks per SM in two
+// rounds of 4.  A thread keeps the same columns for every row, which lets the backward add up its
+// columns of dw in registers and write one partial row per block; a second kernel adds the blocks'
+// partials in block order (no atomics, so dw does not depend on timing).
 //
-// Measured on B200: 16384 x 3584 bf16 training step 173 us (940 MB, 5.4 TB/s), 8192 x 3584 bf16 with
-// 8-bit output 43 us, one row 2.8 us of device time; rows of odd width move single elements and
-// take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 55 us, with 8-bit output 74; its bytes
-// 18).
+// Measured on B200: 16384 x 3584 bf16 training step 168 to 174 us (940 MB, 5.4 to 5.6 TB/s), 8192 x
+// 3584 bf16 with 8-bit output 43 us, one row 2.8 us of device time; rows of odd width move single
+// elements and take 2 to 4 times their bytes' time (4096 x 3585 bf16 forward 55 us, with 8-bit output
+// 74; its bytes 18).
 #pragma once
 
 #include <type_traits>

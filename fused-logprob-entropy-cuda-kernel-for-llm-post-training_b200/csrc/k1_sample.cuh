@@ -35,12 +35,12 @@
 //                           list, and again inside the bin while it has too many.
 //
 // Measured on B200 (us; bf16, N(0, 3^2) with half of the rows peaked, unless noted): no
-// filter, 512 x 152064 76 (2.04 TB/s; its bytes alone 24) and 1 x 151936 7.3; 512 x 152064 top-k 50
-// 157, top-k 1000 227, top-p 0.9 526; 567 x 128256 fp32 top-k 40 top-p 0.82 232; 64 x 128256
-// fp32 with mixed settings 60; 128 x 50257 fp16 top-p 0.95 57.  Without a filter the time goes to the weights (about 15 instructions per
-// element: expf, the exact split, conversions) and the exchanges; loading alone takes 30 us of the 76.
-// With filters the chain of short phases in each block is the limit: two blocks per SM
-// cannot hide all of it.
+// filter, 512 x 152064 81 (1.92 TB/s; its bytes alone 24) and 1 x 151936 7.5; 512 x 152064 top-k 50
+// 164, top-k 1000 233, top-p 0.9 553; 567 x 128256 fp32 top-k 40 top-p 0.82 235; 64 x 128256
+// fp32 with mixed settings 61; 128 x 50257 fp16 top-p 0.95 59.  Without a filter the time goes to
+// instructions, about 24 per element by the counters, most of them for the weights (expf, the exact
+// split, conversions), and to the exchanges; loading alone takes 30 us of the 81.  With filters the
+// chain of short phases in each block is the limit: two blocks per SM cannot hide all of it.
 //
 // A row that holds a NaN or +inf, or nothing above -inf, has no distribution: token -1 and
 // NaN log-probabilities.  So does one whose own settings mean nothing (a temperature that is negative

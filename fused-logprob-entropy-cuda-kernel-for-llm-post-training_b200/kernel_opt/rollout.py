@@ -6,8 +6,13 @@
 
 Three kernels a step; the logits are written once and read once.  The weight is quantised
 when the head is built (and by `update` after an optimizer step), not in a step.  A step
-allocates only its outputs and is safe to capture in a CUDA graph.  No counterpart in the
-reference, which scores tokens that another library generated.
+allocates only its outputs and is safe to capture in a CUDA graph.
+
+The log-probabilities are the 8-bit head's, which drew the token.  The bf16 training head gives the
+same token another value: for a random head (H = 3584, V = 151936) the two are 0.09 apart on average
+and 0.4 at most over 1024 tokens.  A ratio whose old policy should be the training head's takes the old
+values from `fused_linear_logprob_entropy` on the rollout's states, or corrects for the difference.
+No counterpart in the reference, which scores tokens that another library generated.
 """
 from __future__ import annotations
 

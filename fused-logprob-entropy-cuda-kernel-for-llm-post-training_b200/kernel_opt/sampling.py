@@ -3,10 +3,11 @@
 One kernel over the rows of [..., V] logits (csrc/k1_sample.cuh), which reads them once.  The
 random numbers are inputs, and the sums that decide a token are right to about 1e-12 of the mass,
 so the same logits and numbers give the same token whatever batch the row is in, unless a number
-lies that close to the boundary between two tokens.  The returned
-`logprob` is K1's log-probability of the drawn token (at the sampling temperature, over the
-whole vocabulary): the old-policy value that GRPO's ratio needs.  No counterpart in the
-reference, whose generation runs in another library.
+lies that close to the boundary between two tokens.  The returned `logprob` is K1's log-probability
+of the drawn token under the logits given (at the sampling temperature, over the whole vocabulary).
+It is the old-policy value of GRPO's ratio where those are the training head's logits; an 8-bit
+head's are another policy's (see `kernel_opt.rollout`).  No counterpart in the reference, whose
+generation runs in another library.
 """
 from __future__ import annotations
 
