@@ -35,11 +35,11 @@
 //                           list, and again inside the bin while it has too many.
 //
 // Measured on B200 (us; bf16, N(0, 3^2) with half of the rows peaked, unless noted): no
-// filter, 512 x 152064 81 (1.92 TB/s; its bytes alone 24) and 1 x 151936 7.5; 512 x 152064 top-k 50
+// filter, 512 x 152064 82 (1.89 TB/s; its bytes alone 24) and 1 x 151936 7.5; 512 x 152064 top-k 50
 // 164, top-k 1000 233, top-p 0.9 553; 567 x 128256 fp32 top-k 40 top-p 0.82 235; 64 x 128256
 // fp32 with mixed settings 61; 128 x 50257 fp16 top-p 0.95 59.  Without a filter the time goes to
 // instructions, about 24 per element by the counters, most of them for the weights (expf, the exact
-// split, conversions), and to the exchanges; loading alone takes 30 us of the 81.  With filters the
+// split, conversions), and to the exchanges; loading alone takes 30 us of the 82.  With filters the
 // chain of short phases in each block is the limit: two blocks per SM cannot hide all of it.
 //
 // A row that holds a NaN or +inf, or nothing above -inf, has no distribution: token -1 and
@@ -190,21 +190,26 @@ struct Slice {
     __device__ __forceinline__ int64_t index(int j, int e) const { return i0 + (int64_t)j * E + e; }
 };
 
+// y = x * s, rounded.  A packed product (mul2) whose use is a sum or a difference is carried out
+// together with it, y never being rounded: the largest element's y - m is then that rounding's error
+// instead of 0, and equal y fall into different bins.  An fma whose addend is -0 (which the compiler
+// does not know: s is a number it has not seen) is the rounded product and joins nothing.  (Single
+// products, __fmul_rn, do as well: 512 x 152064 bf16 83.8 us, 82.3 so.)
 template <typename T>
 __device__ __forceinline__ void unpack(uint4 v, float s, float (&y)[DT<T>::kEPV]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const float2 zero = splat(__fmul_rn(s, -0.f));
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-            const float2 f =
-                mul2(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), splat(s));
+            const float2 f = fma2(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), splat(s), zero);
             y[i] = f.x;
             y[i + 1] = f.y;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = mul2(DT<T>::to_f2(w[i]), splat(s));
+            const float2 f = fma2(DT<T>::to_f2(w[i]), splat(s), zero);
             y[2 * i] = f.x;
             y[2 * i + 1] = f.y;
         }
@@ -837,7 +842,7 @@ __global__ void __launch_bounds__(FILTER ? kFilterThreads : kPlainThreads, FILTE
     float g[NG], hi = -INFINITY, lo = INFINITY;
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
-        g[q] = peak[q].value() * R.s;
+        g[q] = __fmul_rn(peak[q].value(), R.s);
         hi = fmax_nan(hi, g[q]);
         if (FILTER && g[q] > -INFINITY) lo = fminf(lo, g[q]);
     }

@@ -10,17 +10,18 @@ import kernel_opt
 pytestmark = pytest.mark.gpu
 
 
-def check(x, u, slack, scale=1.0, top_k=0, top_p=1.0, tokens=None):
+def check(x, u, slack, top_k=0, top_p=1.0):
     """Every token is one that sums within `slack` (a share of the mass) of the exact ones allow:
     kept, where the nucleus may end anywhere within `slack` of its share, and at u in the order
     of ids."""
-    tok = kernel_opt.sample_tokens(x, u, 1.0, top_k, top_p)[0] if tokens is None else tokens
+    tok = kernel_opt.sample_tokens(x, u, 1.0, top_k, top_p)[0]
     n, v = x.shape
     p = float(torch.tensor(top_p).float())
     for r in range(n):
         y = x[r].float()
         w = torch.exp(y - y.max()).double()
-        ws, order = torch.sort(w, descending=True, stable=True)
+        order = torch.sort(y, descending=True, stable=True).indices  # by y: weights may be equal where y is not
+        ws = w[order]
         kept = min(top_k, v) if top_k > 0 else v
         cum = ws[:kept].cumsum(0)
         if p < 1:
@@ -138,7 +139,8 @@ def test_shares_of_what_is_kept_are_right_in_any_batch(sigma, kw):
     u, want = torch.full((n,), 0.5, device="cuda"), torch.full((n,), -1, device="cuda")
     for r in range(n):
         w = torch.exp(x[r] - x[r].max())
-        ws, order = torch.sort(w.double(), descending=True, stable=True)
+        order = torch.sort(x[r], descending=True, stable=True).indices
+        ws = w[order].double()
         kept = kw.get("top_k", v)
         if "top_p" in kw:
             cum = ws[:kept].cumsum(0)
@@ -153,3 +155,39 @@ def test_shares_of_what_is_kept_are_right_in_any_batch(sigma, kw):
     assert torch.equal(tok[hit], want[hit]), int((tok != want)[hit].sum())
     for r in torch.nonzero(hit)[:20, 0].tolist():
         assert int(kernel_opt.sample_tokens(x[r:r + 1], u[r:r + 1], **kw)[0]) == int(want[r])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.01, 0.3, 0.7, 1.3, 5.0])
+def test_log_probabilities_are_of_the_rounded_quotients(dtype, temperature):
+    """y = x * fp32(1 / T) is rounded before the maximum is taken from it: a token that is certain has
+    the log-probability 0 however large y is, and every other one's is right to fp32's rounding
+    (2^-24 of it, one more for the sum's logarithm) and the weights' 2^-21."""
+    s = torch.tensor(1.0 / temperature).float()
+    x = torch.rand(64, 1, device="cuda").mul_(100).to(dtype)
+    u = torch.rand(64, device="cuda")
+    for kw in (dict(), dict(top_k=5, min_p=1e-3), dict(min_p=1e-3)):
+        _, lp, kp = kernel_opt.sample_tokens(x, u, temperature, **kw)
+        assert not lp.any() and not kp.any()
+    x = torch.randn(64, 5003, device="cuda").mul_(4).add_(60).to(dtype)
+    for kw in (dict(), dict(min_p=1e-6), dict(top_k=3000), dict(top_p=0.99)):
+        tok, lp, _ = kernel_opt.sample_tokens(x, u, temperature, **kw)
+        y = x.float() * s.cuda()
+        d = (y - y.amax(1, keepdim=True)).double()
+        want = torch.log_softmax(d, 1).gather(1, tok[:, None])[:, 0]
+        assert ((lp.double() - want).abs() <= 2.0 ** -23 * want.abs() + 2.0 ** -21).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.37, 0.7, 1.3])
+def test_shares_at_a_temperature(dtype, temperature):
+    """The weights are those of the rounded y: with y rounded or not, shares differ by 1e-7 of them."""
+    v = 152064
+    g = torch.Generator(device="cuda").manual_seed(int(100 * temperature))
+    x = torch.randn(1, v, generator=g, device="cuda").mul_(2).to(dtype)
+    y = x[0].float() * torch.tensor(1.0 / temperature).float().cuda()
+    u, want = near_boundaries(torch.exp(y - y.max()))
+    assert len(u) >= 20
+    for kw in (dict(), dict(min_p=1e-30)):
+        tok = kernel_opt.sample_tokens(x.expand(len(u), v), u, temperature, **kw)[0]
+        assert torch.equal(tok, want), int((tok != want).sum())
