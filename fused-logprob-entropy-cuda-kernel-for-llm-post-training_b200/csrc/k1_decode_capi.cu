@@ -3,10 +3,8 @@
 // validation, kernel choice, launches.
 #include <algorithm>
 #include <cmath>
-#include <map>
 #include <mutex>
 #include <tuple>
-#include <utility>
 
 #include "k1_fp8_linear.cuh"
 #include "k1_host.cuh"
@@ -46,54 +44,6 @@ extern "C" int k1_test_pick(const float* w, double cum, double target) {
 #endif
 
 namespace {
-
-bool known_dtype(int d) { return d == K1_DTYPE_F32 || d == K1_DTYPE_F16 || d == K1_DTYPE_BF16; }
-
-bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-
-// Opt in to `smem` bytes of dynamic shared memory, once per device and kernel (the largest
-// asked for so far).
-template <typename Kernel>
-int allow_smem(Kernel kernel, int dev, size_t smem) {
-    static std::mutex mu;
-    static std::map<std::pair<int, const void*>, size_t> cache;
-    std::lock_guard<std::mutex> lock(mu);
-    size_t& have = cache[std::make_pair(dev, reinterpret_cast<const void*>(kernel))];
-    if (smem <= have) return K1_OK;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return fail(K1_ERR_CUDA, "cudaFuncSetAttribute(smem): %s", cudaGetErrorString(e));
-    have = smem;
-    return K1_OK;
-}
-
-// `launch` with a cluster of `cluster` blocks along x.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, int cluster,
-                           cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = K1_PDL ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-int launched(const char* fn, cudaError_t e) {
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return fail(K1_ERR_CUDA, "%s: kernel launch failed: %s", fn, cudaGetErrorString(e));
-    }
-    return K1_OK;
-}
 
 // ---------------------------------------------------------------------------------------
 // Residual RMS norm

@@ -1,0 +1,783 @@
+// k1_score.cuh -- log-probabilities of given tokens and of the k most likely ones, with entropy
+// and log-sum-exp, in one pass over the logits, and their gradient.
+//
+//   y_i = s x_i (s = 1/T in fp32; y is not rounded),  l = log sum exp y_i,  log p_i = y_i - l
+//   H = -sum p_i log p_i
+//   the k most likely: larger x first, the lowest index first among equals
+//   dL/dx_i = s ( G_i + p_i (g_l - sum of all g_j - g_H (log p_i + H)) ),  G_i: the sum of the
+//   upstream gradients of the entries of row's lists that name token i
+//
+// A row is read once as 16-byte vectors from its own 16-byte boundary (the first and last vector
+// may be partly outside the row: those are put together from single elements).  A block of
+// threads owns a row, or a part of one where there are few rows; the parts' blocks are a cluster
+// and meet in the first one's shared memory.  Sums run as in k1_common.cuh (the maximum's own
+// terms counted apart, so that a near-one-hot row's entropy keeps its precision), on x itself
+// with the factor s log2 e in the exponent, so a temperature costs no instruction.
+//
+// The k most likely cost almost nothing while streaming: each thread stores the maximum of every
+// group of its vectors (one chunk's 8 usually), which the sums need anyway.  Then
+//   T0, the k-th largest of the threads' maxima cut to 16 bits, is a bound that at least k
+//   elements reach, and usually few more;
+//   the groups that reach T0 are read again (from L2, some k x 128 bytes) and their elements that
+//   do go to a list of 64-bit keys (value, then lowest index), each key's rank in the list is its
+//   place.
+// Where that overflows (many equal values, masks that leave fewer than k, rows whose large values
+// lie in few threads' columns) the block finds the k-th largest value by histograms of 8 bits a
+// pass and takes the equal ones in index order.  Either way the result is exact.
+#pragma once
+
+#include <type_traits>
+
+#include "k1_common.cuh"
+#include "k1_sync.cuh"
+
+namespace k1 {
+namespace score {
+
+constexpr int U = 8;             // vectors per thread and chunk
+constexpr int kMaxGroups = 32;   // maxima per thread
+constexpr int kCand = 1024;      // entries of the list
+constexpr int kMaxTop = 128;     // largest k
+constexpr int kMaxIds = 1024;    // given tokens per row
+constexpr int kMaxCluster = 8;
+static_assert(kMaxCluster * kMaxTop <= kCand, "the parts' lists meet in one");
+
+// Values at or below this count as masked (p = 0); 16-bit types: as the type rounds it.  pad: what
+// stands for elements outside the row.
+template <typename T>
+struct Floor;
+template <>
+struct Floor<__nv_bfloat16> {
+    static constexpr uint32_t pad = 0xFE96FE96u;  // -9.97e37, both halves
+    static constexpr float value = -9.969209968386869e37f;
+};
+template <>
+struct Floor<__half> {
+    static constexpr uint32_t pad = 0xFC00FC00u;  // -inf, both halves
+    static constexpr float value = -1.0e38f;      // fp16's own values lie above
+};
+template <>
+struct Floor<float> {
+    static constexpr uint32_t pad = 0xFE967699u;  // -1e38
+    static constexpr float value = -1.0e38f;
+};
+
+struct FwdParams {
+    const void* logits;
+    RowLayout lay;
+    int64_t vocab;
+    float scale;
+    const int64_t* ids;  // [n, n_ids]
+    int n_ids;
+    float* logprobs;     // [n, n_ids]
+    int k;
+    int64_t* top_ids;    // [n, k]
+    float* top_logprobs; // [n, k]
+    float* entropy;
+    float* lse;
+    int cluster;         // blocks per row
+    int slice;           // vectors per block
+    int groups;          // groups per thread
+    int group_chunks;    // chunks per group
+};
+
+// One thread's sums, relative to its maximum m (k1_common.cuh's FwdState with the exponent's
+// factor c = s log2 e as a variable; t is a sum of e d in x, not y).
+struct State {
+    float m, np;
+    float2 zs, ms, t;
+    __device__ __forceinline__ void init() {
+        m = -3.402823466e38f;
+        np = 0.f;
+        zs = ms = t = splat(0.f);
+    }
+    __device__ __forceinline__ float2 at_max() const { return make_float2(np - ms.x, np - ms.y); }
+    __device__ __forceinline__ void rescale(float mc, float c) {
+        const float mn = fmax_nan(m, mc);
+        const float dl = m - mn;
+        const bool moved = !(dl == 0.f);
+        const float s = moved ? ex2(dl * c) : 1.f;
+        const float2 z = add2(zs, at_max());
+        t = fma2(splat(dl * s), z, mul2(t, splat(s)));
+        if (moved) {
+            zs = mul2(z, splat(s));
+            ms = splat(0.f);
+            np = 0.f;
+        }
+        m = mn;
+    }
+    __device__ __forceinline__ void accum(float2 d, float2 c2) {
+        const float2 a = mul2(d, c2);
+        const float2 e = make_float2(ex2(a.x), ex2(a.y));
+        const float2 nz = make_float2(not_zero(d.x), not_zero(d.y));
+        zs = fma2(e, nz, zs);
+        ms = add2(ms, nz);
+        t = fma2(e, d, t);
+    }
+    __device__ __forceinline__ double z64() const {
+        const float2 c = at_max();
+        return ((double)c.x + (double)c.y) + ((double)zs.x + (double)zs.y);
+    }
+    __device__ __forceinline__ double t64() const { return (double)t.x + (double)t.y; }
+};
+
+// Adds a chunk of N vectors to the state; returns their maximum (of the values as clamped).
+template <typename T, int N>
+__device__ __forceinline__ float add_chunk(const uint4 (&v)[N], State& st, float c) {
+    const float2 c2 = splat(c);
+    uint32_t w[4 * N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        w[4 * u] = v[u].x;
+        w[4 * u + 1] = v[u].y;
+        w[4 * u + 2] = v[u].z;
+        w[4 * u + 3] = v[u].w;
+    }
+    float mc;
+    if constexpr (sizeof(T) == 2) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+            for (int i = 0; i < 4 * N; ++i) w[i] = DT<T>::max2(w[i], Floor<T>::pad);
+        }
+        uint32_t mx[4 * N];
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) mx[i] = w[i];
+#pragma unroll
+        for (int s = 2 * N; s >= 1; s >>= 1)
+#pragma unroll
+            for (int i = 0; i < s; ++i) mx[i] = DT<T>::max2(mx[i], mx[i + s]);
+        const float2 mf = DT<T>::to_f2(mx[0]);
+        mc = fmax_nan(mf.x, mf.y);
+        st.rescale(mc, c);
+        const float nm = -st.m;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                st.accum(bf16x2_minus(w[i], nm), c2);
+            } else {  // -inf stays outside fp16's range, so that -65504 is a value like others
+                const float2 d = f16x2_minus(w[i], nm);
+                st.accum(make_float2(fmax_nan(d.x, Floor<T>::value), fmax_nan(d.y, Floor<T>::value)), c2);
+            }
+        }
+        st.np += (float)(4 * N);
+    } else {
+        float f[4 * N], mx[4 * N];
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) mx[i] = f[i] = fmax_nan(__uint_as_float(w[i]), Floor<T>::value);
+#pragma unroll
+        for (int s = 2 * N; s >= 1; s >>= 1)
+#pragma unroll
+            for (int i = 0; i < s; ++i) mx[i] = fmax_nan(mx[i], mx[i + s]);
+        mc = mx[0];
+        st.rescale(mc, c);
+        const float2 nm = splat(-st.m);
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) st.accum(add2(make_float2(f[2 * i], f[2 * i + 1]), nm), c2);
+        st.np += (float)(2 * N);
+    }
+    return mc;
+}
+
+// A row as vectors from the 16-byte boundary at or before its first element: vector j holds
+// elements j E - shift ... ; whole vectors are [lo, hi), all that touch the row [0, n).
+template <typename T>
+struct Row {
+    static constexpr int E = DT<T>::kEPV;
+    const T* p;
+    const uint4* base;
+    int shift, lo, hi, n;
+    int64_t vocab;
+    __device__ __forceinline__ Row(const T* row, int64_t v) {
+        p = row;
+        vocab = v;
+        shift = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+        base = reinterpret_cast<const uint4*>(row - shift);
+        lo = shift ? 1 : 0;
+        hi = (int)((shift + v) / E);
+        n = (int)((shift + v + E - 1) / E);
+    }
+    // element i of vector j
+    __device__ __forceinline__ int64_t at(int j, int i) const { return (int64_t)j * E + i - shift; }
+    __device__ __forceinline__ bool inside(int64_t e) const { return (uint64_t)e < (uint64_t)vocab; }
+    // a vector that is partly outside the row, put together from its elements (rare)
+    __device__ __noinline__ uint4 partial(int j) const {
+        uint32_t w[4];
+        const uint32_t pad = Floor<T>::pad;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pad;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int64_t e = at(j, i);
+            if (inside(e)) {
+                if constexpr (sizeof(T) == 2) {
+                    const uint32_t b = *reinterpret_cast<const uint16_t*>(p + e);
+                    w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (b << 16) : (w[i / 2] & 0xffff0000u) | b;
+                } else {
+                    w[i] = *reinterpret_cast<const uint32_t*>(p + e);
+                }
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // vectors j, j + step, ... below `end`; what lies beyond reads as padding
+    template <int N>
+    __device__ __forceinline__ void load(uint4 (&v)[N], int j, int step, int end) const {
+        const uint32_t pad = Floor<T>::pad;
+        const int to = min(end, hi);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int a = j + u * step;
+            v[u] = a >= lo && a < to ? ldg_stream(base + a) : make_uint4(pad, pad, pad, pad);
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int a = j + u * step;
+            if (a < end && (a < lo || a >= hi)) v[u] = partial(a);
+        }
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(uint4 v, float (&f)[DT<T>::kEPV]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = __uint_as_float(w[i]);
+        } else {
+            const float2 t = DT<T>::to_f2(w[i]);
+            f[2 * i] = t.x;
+            f[2 * i + 1] = t.y;
+        }
+    }
+}
+
+// Keys in the values' order (-0 as 0), and back.
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// Larger is earlier in the list: the larger value, then the lower index.
+__device__ __forceinline__ uint64_t entry_of(float x, int64_t e) {
+    return ((uint64_t)key_of(x) << 32) | (uint32_t)~(uint32_t)e;
+}
+
+template <int TH>
+struct FwdSmem {
+    static constexpr int W = TH / 32;
+    float wmax[W];
+    double wz[W], wt[W];
+    RowPartial part;          // this block's, read by the cluster's first block
+    int n_list, n_cand, n_sorted;
+    unsigned bound;           // T0's key, its upper 16 bits
+    unsigned prefix, need, above, scan[W];
+    uint64_t sorted[kMaxTop];
+    uint16_t keys[TH];
+    uint16_t list[kCand];
+    unsigned hist[256];
+    uint64_t cand[kCand];
+    float gmax[1];            // [groups][TH]
+};
+
+// The block's list by exact selection: the kk-th largest key by histograms, what lies above it,
+// and the first ones in index order among what equals it.
+template <typename T, int TH>
+__device__ __noinline__ void select_exact(const Row<T>& row, int j0, int j1, int kk, FwdSmem<TH>& sm) {
+    constexpr int E = DT<T>::kEPV;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto each = [&](int j, auto&& f) {
+        uint4 v[1];
+        row.template load<1>(v, j, 0, j1);
+        float x[E];
+        unpack<T>(v[0], x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int64_t e = row.at(j, i);
+            if (j < j1 && row.inside(e)) f(x[i], e);
+        }
+    };
+    unsigned prefix = 0, mask = 0, need = (unsigned)kk;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += TH) sm.hist[i] = 0;
+        __syncthreads();
+        unsigned bin = 0, run = 0;  // equal values in a row are counted together
+        for (int j = j0 + tid; j < j1; j += TH)
+            each(j, [&](float x, int64_t) {
+                const unsigned k = key_of(x);
+                if ((k & mask) != prefix) return;
+                const unsigned b = (k >> shift) & 255u;
+                if (b != bin) {
+                    if (run) atomicAdd(&sm.hist[bin], run);
+                    bin = b;
+                    run = 0;
+                }
+                ++run;
+            });
+        if (run) atomicAdd(&sm.hist[bin], run);
+        __syncthreads();
+        if (tid == 0) {
+            unsigned sum = 0;
+            int b = 255;
+            while (b > 0 && sum + sm.hist[b] < need) sum += sm.hist[b--];
+            sm.prefix = prefix | ((unsigned)b << shift);
+            sm.need = need - sum;
+        }
+        __syncthreads();
+        prefix = sm.prefix;
+        need = sm.need;
+        mask |= 255u << shift;
+    }
+    const int above = kk - (int)need;
+    if (tid == 0) sm.n_cand = 0;
+    __syncthreads();
+    for (int j = j0 + tid; j < j1; j += TH)
+        each(j, [&](float x, int64_t e) {
+            if (key_of(x) > prefix) sm.cand[atomicAdd(&sm.n_cand, 1)] = entry_of(x, e);
+        });
+    unsigned found = 0;
+    for (int jb = j0; jb < j1 && found < need; jb += TH) {
+        const int j = jb + tid;
+        unsigned n = 0;
+        each(j, [&](float x, int64_t) { n += key_of(x) == prefix; });
+        unsigned upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned a = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += a;
+        }
+        __syncthreads();
+        if (lane == 31) sm.scan[warp] = upto;
+        __syncthreads();
+        unsigned at = found + upto - n;
+        for (int w = 0; w < TH / 32; ++w) {
+            if (w < warp) at += sm.scan[w];
+            found += sm.scan[w];
+        }
+        if (n && at < need)
+            each(j, [&](float x, int64_t e) {
+                if (key_of(x) == prefix && at < need) sm.cand[above + at++] = entry_of(x, e);
+            });
+    }
+    __syncthreads();
+    if (tid == 0) sm.n_cand = kk;
+    __syncthreads();
+}
+
+// The block's part of the list, sorted: sm.sorted[0, sm.n_sorted).
+template <typename T, int TH>
+__device__ __forceinline__ void select(const Row<T>& row, int j0, int j1, float thread_max, const FwdParams& p,
+                                       FwdSmem<TH>& sm) {
+    constexpr int E = DT<T>::kEPV;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // elements of the part
+    const int64_t first = max((int64_t)0, row.at(j0, 0)), last = min(row.vocab, row.at(j1, 0));
+    const int kk = (int)min((int64_t)p.k, max((int64_t)0, last - first));
+    sm.keys[tid] = thread_max > Floor<T>::value ? (uint16_t)(key_of(thread_max) >> 16) : (uint16_t)0;
+    if (tid == 0) sm.n_list = sm.n_cand = 0;
+    __syncthreads();
+    if (warp == 0) {
+        unsigned mine[TH / 32];
+#pragma unroll
+        for (int i = 0; i < TH / 32; ++i) mine[i] = sm.keys[lane + 32 * i];
+        unsigned t = 0;
+#pragma unroll
+        for (int b = 15; b >= 0; --b) {
+            const unsigned cand = t | (1u << b);
+            unsigned n = 0;
+#pragma unroll
+            for (int i = 0; i < TH / 32; ++i) n += mine[i] >= cand;
+            if (__reduce_add_sync(0xffffffffu, n) >= (unsigned)kk) t = cand;
+        }
+        if (lane == 0) sm.bound = t;
+    }
+    __syncthreads();
+    const unsigned bound = sm.bound;
+    const float t0 = value_of(bound << 16);
+    for (int g = 0; g < p.groups; ++g) {
+        if (bound == 0 || sm.gmax[g * TH + tid] >= t0) {
+            const int at = atomicAdd(&sm.n_list, 1);
+            if (at < kCand) sm.list[at] = (uint16_t)(g * TH + tid);
+        }
+    }
+    __syncthreads();
+    const int n_list = sm.n_list, per = p.group_chunks * U;
+    if (n_list <= kCand) {
+        for (int i = tid; i < n_list * per; i += TH) {
+            const int entry = sm.list[i / per], u = i % per;
+            const int j = j0 + (entry / TH * per + u) * TH + entry % TH;
+            if (j >= j1) continue;
+            uint4 v[1];
+            row.template load<1>(v, j, 0, j1);
+            float x[E];
+            unpack<T>(v[0], x);
+#pragma unroll
+            for (int q = 0; q < E; ++q) {
+                const int64_t e = row.at(j, q);
+                if ((bound == 0 || x[q] >= t0) && row.inside(e)) {
+                    const int at = atomicAdd(&sm.n_cand, 1);
+                    if (at < kCand) sm.cand[at] = entry_of(x[q], e);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (n_list > kCand || sm.n_cand > kCand) {  // uniform
+        __syncthreads();
+        select_exact<T, TH>(row, j0, j1, kk, sm);
+    }
+    const int n = sm.n_cand;
+    for (int i = tid; i < n; i += TH) {
+        const uint64_t key = sm.cand[i];
+        int rank = 0;
+        for (int q = 0; q < n; ++q) rank += sm.cand[q] > key;
+        if (rank < kk) sm.sorted[rank] = key;
+    }
+    if (tid == 0) sm.n_sorted = kk;
+    __syncthreads();
+}
+
+// 32 or 64 bits of another block's shared memory.
+__device__ __forceinline__ uint64_t ld_cluster64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+
+template <typename T, int TH, bool TOP>
+__global__ void __launch_bounds__(TH, 768 / TH) k1_score_kernel(FwdParams p) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    FwdSmem<TH>& sm = *reinterpret_cast<FwdSmem<TH>*>(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = p.cluster > 1 ? (int)ring::cluster_rank() : 0;
+    const int64_t r = p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
+    pdl_wait();
+    pdl_trigger();
+    const Row<T> row(reinterpret_cast<const T*>(p.logits) + p.lay.offset(r), p.vocab);
+    const int j0 = min(row.n, rank * p.slice), j1 = min(row.n, j0 + p.slice);
+    const float c = p.scale * kLog2e;
+
+    // the given tokens' logits, in flight with the first chunk
+    int64_t id = -1;
+    float xid = 0.f;
+    if (rank == 0 && tid < p.n_ids) {
+        id = p.ids[r * p.n_ids + tid];
+        if (row.inside(id)) xid = DT<T>::load1(row.p + id);
+    }
+
+    State st;
+    st.init();
+    {
+        int g = 0, left = p.group_chunks;
+        float gm = -INFINITY;
+        for (int j = j0; j < j1; j += U * TH) {
+            uint4 v[U];
+            if (j >= row.lo && j + U * TH <= min(j1, row.hi)) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = ldg_stream(row.base + j + tid + u * TH);
+            } else {
+                row.template load<U>(v, j + tid, TH, j1);
+            }
+            const float mc = add_chunk<T, U>(v, st, c);
+            if constexpr (TOP) {
+                gm = fmax_nan(gm, mc);
+                if (--left == 0 || j + U * TH >= j1) {
+                    sm.gmax[g * TH + tid] = gm;
+                    ++g;
+                    left = p.group_chunks;
+                    gm = -INFINITY;
+                }
+            }
+        }
+        if constexpr (TOP)
+            for (; g < p.groups; ++g) sm.gmax[g * TH + tid] = -INFINITY;
+    }
+
+    // the block's sums, relative to its maximum
+    const bool empty = st.m <= Floor<T>::value;
+    const float wm = warp_max_nan(empty ? -INFINITY : st.m);
+    if (lane == 0) sm.wmax[warp] = wm;
+    __syncthreads();
+    RowPartial part;
+    part.m = sm.wmax[0];
+#pragma unroll
+    for (int i = 1; i < TH / 32; ++i) part.m = fmax_nan(part.m, sm.wmax[i]);
+    {
+        double z = 0.0, t = 0.0;
+        if (!empty) {
+            const float dm = st.m - part.m;
+            const double f = dm == 0.f ? 1.f : ex2(dm * c);
+            z = f * st.z64();
+            t = f * st.t64() + f * (double)dm * st.z64();
+        }
+        z = warp_sum(z);
+        t = warp_sum(t);
+        if (lane == 0) {
+            sm.wz[warp] = z;
+            sm.wt[warp] = t;
+        }
+    }
+    __syncthreads();
+    part.z = part.t = 0.0;
+#pragma unroll
+    for (int i = 0; i < TH / 32; ++i) {
+        part.z += sm.wz[i];
+        part.t += sm.wt[i];
+    }
+    part.pad = 0.f;
+    // NaN somewhere: no list either (a part's list must not hold what cannot be ordered)
+    const bool sound = part.m < INFINITY;
+    if constexpr (TOP) {
+        if (sound)
+            select<T, TH>(row, j0, j1, st.m, p, sm);
+        else if (tid == 0)
+            sm.n_sorted = 0;
+    }
+
+    if (p.cluster > 1) {
+        if (tid == 0) sm.part = part;
+        ring::cluster_sync();
+        if (rank == 0) {
+            float M = part.m;
+            for (int q = 1; q < p.cluster; ++q)
+                M = fmax_nan(M, __uint_as_float(ld_cluster32(ring::mapa(ring::saddr(&sm.part.m), q))));
+            double z = 0.0, t = 0.0;
+            for (int q = 0; q < p.cluster; ++q) {
+                const float m = __uint_as_float(ld_cluster32(ring::mapa(ring::saddr(&sm.part.m), q)));
+                const double zq = __longlong_as_double((long long)ld_cluster64(ring::mapa(ring::saddr(&sm.part.z), q)));
+                const double tq = __longlong_as_double((long long)ld_cluster64(ring::mapa(ring::saddr(&sm.part.t), q)));
+                if (m != -INFINITY) {
+                    const float dm = m - M;
+                    const double f = dm == 0.f ? 1.f : ex2(dm * c);
+                    z += f * zq;
+                    t += f * tq + f * (double)dm * zq;
+                }
+            }
+            part.m = M;
+            part.z = z;
+            part.t = t;
+            if constexpr (TOP) {
+                // the parts' lists side by side, then every entry's place in all of them
+                int total = 0;
+                for (int q = 0; q < p.cluster; ++q) {
+                    const int n = (int)ld_cluster32(ring::mapa(ring::saddr(&sm.n_sorted), q));
+                    for (int i = tid; i < n; i += TH)
+                        sm.cand[q * kMaxTop + i] = ld_cluster64(ring::mapa(ring::saddr(&sm.sorted[i]), q));
+                    if (tid == 0) sm.hist[q] = (unsigned)n;
+                    total += n;
+                }
+                __syncthreads();
+                for (int i = tid; i < p.cluster * kMaxTop; i += TH) {
+                    const int q = i / kMaxTop, at = i % kMaxTop;
+                    if (at >= (int)sm.hist[q]) continue;
+                    const uint64_t key = sm.cand[i];
+                    int place = at;
+                    for (int o = 0; o < p.cluster && place < p.k; ++o) {
+                        if (o == q) continue;
+                        int lo = 0, hi = (int)sm.hist[o];  // entries of list o before this one
+                        while (lo < hi) {
+                            const int mid = (lo + hi) >> 1;
+                            if (sm.cand[o * kMaxTop + mid] > key)
+                                lo = mid + 1;
+                            else
+                                hi = mid;
+                        }
+                        place += lo;
+                    }
+                    if (place < p.k) sm.sorted[place] = key;
+                }
+                __syncthreads();
+            }
+        }
+        ring::cluster_sync();  // no block leaves while its shared memory may be read
+        if (rank != 0) return;
+    }
+
+    // the row's values
+    const double s = (double)p.scale;
+    const bool none = part.m == -INFINITY;  // nothing above the floor
+    double l, h;
+    if (none) {
+        l = -INFINITY;
+        h = NAN;
+    } else {
+        const double lz = log(part.z);
+        l = s * (double)part.m + lz;
+        h = lz - s * part.t / part.z;
+    }
+    const bool fine = !none && part.m < INFINITY && l - l == 0.0;
+    if (tid == 0) {
+        p.lse[r] = fine || none ? (float)l : NAN;
+        p.entropy[r] = fine ? (float)h : NAN;
+    }
+    if (tid < p.n_ids) p.logprobs[r * p.n_ids + tid] = fine ? (float)(s * (double)xid - l) : NAN;
+    for (int i = tid + TH; i < p.n_ids; i += TH) {
+        const int64_t e = p.ids[r * p.n_ids + i];
+        const float x = row.inside(e) ? DT<T>::load1(row.p + e) : 0.f;
+        p.logprobs[r * p.n_ids + i] = fine ? (float)(s * (double)x - l) : NAN;
+    }
+    if constexpr (TOP) {
+        for (int i = tid; i < p.k; i += TH) {
+            const uint64_t key = fine ? sm.sorted[i] : 0;
+            p.top_ids[r * p.k + i] = fine ? (int64_t)(uint32_t)~(uint32_t)key : -1;
+            p.top_logprobs[r * p.k + i] = fine ? (float)(s * (double)value_of((uint32_t)(key >> 32)) - l) : NAN;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------
+// Backward
+// ------------------------------------------------------------------------------------
+struct BwdParams {
+    const void* logits;
+    RowLayout lay;
+    int64_t vocab;
+    float scale;
+    const int64_t* ids;      // [n, n_ids]
+    const float* g_ids;      // [n, n_ids], NULL: none
+    const int64_t* top_ids;  // [n, k]
+    const float* g_top;      // [n, k], NULL: none
+    int n_ids, k;            // 0 without gradient
+    const float* lse;
+    const float* entropy;
+    const float* g_entropy;  // NULL: none
+    const float* g_lse;      // NULL: none
+    void* d;                 // rows d_stride elements apart
+    int64_t d_stride;
+    int parts;               // blocks per row
+    int slice;               // vectors per block
+};
+
+constexpr int kBwdThreads = 256;
+constexpr int UB = 4;
+
+// dL/dx of a vector of logits that no list names.
+struct BwdRow {
+    float s, nl, c0, ge;  // s, -lse, s (g_lse - sum g - g_H H), s g_H
+};
+template <typename T>
+__device__ __forceinline__ uint4 grad_vector(uint4 v, const BwdRow& q) {
+    constexpr int E = DT<T>::kEPV;
+    float x[E];
+    unpack<T>(v, x);
+    float2 g[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+        float2 d = fma2(make_float2(x[2 * i], x[2 * i + 1]), splat(q.s), splat(q.nl));
+        d = make_float2(fmax_nan(d.x, -1e30f), fmax_nan(d.y, -1e30f));
+        const float2 a = mul2(d, splat(kLog2e));
+        g[i] = mul2(make_float2(ex2(a.x), ex2(a.y)), fma2(d, splat(-q.ge), splat(q.c0)));
+    }
+    if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(g[0].x), __float_as_uint(g[0].y), __float_as_uint(g[1].x),
+                          __float_as_uint(g[1].y));
+    else
+        return make_uint4(DT<T>::from_f2(g[0]), DT<T>::from_f2(g[1]), DT<T>::from_f2(g[2 % (E / 2)]),
+                          DT<T>::from_f2(g[3 % (E / 2)]));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads, 4) k1_score_bwd_kernel(BwdParams p) {
+    constexpr int E = DT<T>::kEPV, TH = kBwdThreads;
+    __shared__ double wsum[TH / 32];
+    extern __shared__ __align__(16) unsigned char raw[];
+    int64_t* ids = reinterpret_cast<int64_t*>(raw);
+    float* gs = reinterpret_cast<float*>(ids + p.n_ids + p.k);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t r = blockIdx.x / p.parts;
+    const int rank = (int)(blockIdx.x - r * p.parts);
+    pdl_wait();
+    pdl_trigger();
+    const Row<T> row(reinterpret_cast<const T*>(p.logits) + p.lay.offset(r), p.vocab);
+    T* out = reinterpret_cast<T*>(p.d) + r * p.d_stride;
+    const int j0 = min(row.n, rank * p.slice), j1 = min(row.n, j0 + p.slice);
+    const int n = p.n_ids + p.k;
+    const float ge = p.g_entropy ? p.g_entropy[r] : 0.f, gl = p.g_lse ? p.g_lse[r] : 0.f;
+    double sum = 0.0;
+    bool any = ge != 0.f || gl != 0.f;  // true for a NaN
+    for (int i = tid; i < n; i += TH) {
+        const bool given = i < p.n_ids;
+        ids[i] = given ? p.ids[r * p.n_ids + i] : p.top_ids[r * p.k + i - p.n_ids];
+        const float g = given ? p.g_ids[r * p.n_ids + i] : p.g_top[r * p.k + i - p.n_ids];
+        gs[i] = g;
+        sum += (double)g;
+        any |= g != 0.f;
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) wsum[warp] = sum;
+    any = __syncthreads_or(any);
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < TH / 32; ++i) sum += wsum[i];
+    const float lse = p.lse[r], h = p.entropy[r];
+    BwdRow q;
+    q.s = p.scale;
+    q.nl = lse - lse == 0.f ? -lse : NAN;  // a row without a distribution
+    q.ge = p.scale * ge;
+    // entropy: only where it has a gradient, so that a row without one needs no finite entropy
+    const double c0 = (double)gl - sum - (ge != 0.f ? (double)ge * (double)h : 0.0);
+    q.c0 = (float)((double)p.scale * c0);
+    const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.p)) & 15u) == 0;
+    uint4* ov = reinterpret_cast<uint4*>(out - row.shift);
+    auto store = [&](int j, uint4 v) {
+        if (same && j >= row.lo && j < row.hi) {
+            stg_stream(ov + j, v);
+        } else {
+            float x[E];
+            unpack<T>(v, x);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int64_t e = row.at(j, i);
+                if (row.inside(e)) DT<T>::store1(out + e, x[i]);
+            }
+        }
+    };
+    if (!any) {  // nothing asked of this row (a padded position): zeros whatever it holds
+        for (int j = j0 + tid; j < j1; j += TH) store(j, make_uint4(0, 0, 0, 0));
+        return;
+    }
+    for (int j = j0; j < j1; j += UB * TH) {
+        uint4 v[UB];
+        if (same && j >= row.lo && j + UB * TH <= min(j1, row.hi)) {
+#pragma unroll
+            for (int u = 0; u < UB; ++u) v[u] = ldg_stream(row.base + j + tid + u * TH);
+#pragma unroll
+            for (int u = 0; u < UB; ++u) stg_stream(ov + j + tid + u * TH, grad_vector<T>(v[u], q));
+        } else {
+            row.template load<UB>(v, j + tid, TH, j1);
+#pragma unroll
+            for (int u = 0; u < UB; ++u)
+                if (j + tid + u * TH < j1) store(j + tid + u * TH, grad_vector<T>(v[u], q));
+        }
+    }
+    __syncthreads();  // the named tokens' own gradients replace what the block wrote there
+    const int64_t e0 = row.at(j0, 0), e1 = row.at(j1, 0);
+    for (int i = tid; i < n; i += TH) {
+        const int64_t e = ids[i];
+        if (!row.inside(e) || e < e0 || e >= e1) continue;
+        // a token named more than once is written by its first entry, with all entries' gradients
+        double mine = 0.0, others = 0.0;
+        bool first = true;
+        for (int o = 0; o < n; ++o) {
+            const bool eq = ids[o] == e;
+            if (eq && o < i) first = false;
+            (eq ? mine : others) += (double)gs[o];
+        }
+        if (!first) continue;
+        const double lp = (double)p.scale * (double)DT<T>::load1(row.p + e) - (double)lse;
+        const double pr = exp(lp);
+        double g = mine * -expm1(lp) + pr * ((double)gl - others);
+        if (ge != 0.f && pr > 0.0) g -= (double)ge * pr * (lp + (double)h);
+        DT<T>::store1(out + e, (float)((double)p.scale * g));
+    }
+}
+
+}  // namespace score
+}  // namespace k1

@@ -788,6 +788,127 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sample_tokens(const at::Tensor& l
     return {token, logprob, kept};
 }
 
+// ---------------------------------------------------------------------------------------
+// Log-probabilities of given tokens and of the most likely ones
+// ---------------------------------------------------------------------------------------
+struct ScoreOut {
+    at::Tensor logprobs, entropy, lse, top_ids, top;
+};
+
+// The rows of logits; without any, a grouping that the C ABI takes.
+Rows score_rows(const at::Tensor& logits) {
+    Rows L = logits_rows(logits);
+    if (L.n_rows == 0) L.inner_rows = 1;
+    return L;
+}
+
+// ids: [..., K] (K = 1 for a target), undefined: none.
+ScoreOut score_run(const at::Tensor& logits, const at::Tensor& ids, int64_t k, double temperature) {
+    const Rows L = score_rows(logits);
+    c10::cuda::CUDAGuard guard(logits.device());
+    const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+    const auto f32 = logits.options().dtype(at::kFloat);
+    ScoreOut o;
+    o.entropy = at::empty(lead, f32);
+    o.lse = at::empty(lead, f32);
+    std::vector<int64_t> wide(lead.begin(), lead.end());
+    wide.push_back(k);
+    const int64_t n_ids = ids.defined() ? ids.size(-1) : 0;
+    if (ids.defined()) o.logprobs = at::empty(ids.sizes(), f32);
+    o.top_ids = at::empty(wide, logits.options().dtype(at::kLong));
+    o.top = at::empty(wide, f32);
+    const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+    check_launch(k1_token_logprobs(
+        logits.data_ptr(), dtype_code(logits), L.n_rows, L.vocab, L.inner_rows, L.inner_stride, L.outer_stride,
+        temperature, ids.defined() ? ids.data_ptr<int64_t>() : nullptr, n_ids, ptr(o.logprobs), k,
+        o.top_ids.data_ptr<int64_t>(), o.top.data_ptr<float>(), o.entropy.data_ptr<float>(), o.lse.data_ptr<float>(),
+        at::cuda::getCurrentCUDAStream().stream()));
+    return o;
+}
+
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits,
+                                                  const c10::optional<at::Tensor>& ids_, int64_t k,
+                                                  double temperature) {
+        const at::Tensor ids = ids_.has_value() ? *ids_ : at::Tensor();
+        ScoreOut o = score_run(logits, ids, k, temperature);
+        ctx->save_for_backward({logits, ids, o.entropy, o.lse, o.top_ids});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({o.top_ids});
+        if (ids.defined()) return {o.entropy, o.lse, o.top_ids, o.top, o.logprobs};
+        return {o.entropy, o.lse, o.top_ids, o.top};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "the log-probabilities have no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &ids = saved[1], &entropy = saved[2], &lse = saved[3], &top_ids = saved[4];
+        const at::Tensor none;
+        const Rows L = score_rows(logits);
+        c10::cuda::CUDAGuard guard(logits.device());
+        const auto ready = [](const at::Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; };
+        const at::Tensor g_ent = ready(grads[0]), g_lse = ready(grads[1]), g_top = ready(grads[3]),
+                         g_ids = grads.size() > 4 ? ready(grads[4]) : none;
+        if (!g_ent.defined() && !g_lse.defined() && !g_top.defined() && !g_ids.defined()) return {none, none, none, none};
+        const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+        at::Tensor d = at::empty(logits.sizes(), logits.options());
+        check_launch(k1_token_logprobs_backward(
+            logits.data_ptr(), dtype_code(logits), L.n_rows, L.vocab, L.inner_rows, L.inner_stride, L.outer_stride,
+            ctx->saved_data["temperature"].toDouble(), ids.defined() ? ids.data_ptr<int64_t>() : nullptr,
+            ids.defined() ? ids.size(-1) : 0, ptr(g_ids), top_ids.data_ptr<int64_t>(), top_ids.size(-1), ptr(g_top),
+            lse.data_ptr<float>(), entropy.data_ptr<float>(), ptr(g_ent), ptr(g_lse), d.data_ptr(), L.vocab,
+            at::cuda::getCurrentCUDAStream().stream()));
+        return {d, none, none, none};
+    }
+};
+
+ScoreOut score(const at::Tensor& logits, const at::Tensor& ids_, int64_t k, double temperature) {
+    TORCH_CHECK(!logits._fw_grad(/*level=*/0).defined(),
+                "the log-probabilities do not support forward AD: they have no jvp");
+    const at::Tensor ids = ids_.defined() ? ids_.contiguous() : ids_;
+    if (!at::GradMode::is_enabled() || !logits.requires_grad()) return score_run(logits, ids, k, temperature);
+    auto out = TokenLogprobs::apply(logits, ids.defined() ? c10::optional<at::Tensor>(ids) : c10::nullopt, k, temperature);
+    return {ids.defined() ? out[4] : at::Tensor(), out[0], out[1], out[2], out[3]};
+}
+
+void score_tokens(const at::Tensor& ids, const at::Tensor& logits, const char* what) {
+    TORCH_CHECK_VALUE(ids.device() == logits.device(), what, " must be on the logits' device");
+    TORCH_CHECK(ids.scalar_type() == at::kLong, what, " must be int64");
+}
+
+// (logprob or None, entropy, lse, top_ids, top_logprobs)
+std::tuple<c10::optional<at::Tensor>, at::Tensor, at::Tensor, at::Tensor, at::Tensor> top_logprobs(
+    const at::Tensor& logits, const c10::optional<at::Tensor>& targets, int64_t k, double temperature) {
+    float_dtype(logits, "logits");
+    TORCH_CHECK_VALUE(logits.dim() >= 1, "logits must have a vocab dimension");
+    TORCH_CHECK_VALUE(k >= 1, "k must be at least 1, got ", k);
+    at::Tensor ids;
+    if (targets.has_value()) {
+        TORCH_CHECK_VALUE(targets->sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                          "targets must be shaped like the rows of logits ", logits.sizes(), ", got ", targets->sizes());
+        score_tokens(*targets, logits, "targets");
+        ids = targets->unsqueeze(-1);
+    }
+    ScoreOut o = score(logits, ids, k, temperature);
+    return {ids.defined() ? c10::optional<at::Tensor>(o.logprobs.squeeze(-1)) : c10::nullopt, o.entropy, o.lse, o.top_ids,
+            o.top};
+}
+
+// (logprobs, entropy, lse)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& ids,
+                                                              double temperature) {
+    float_dtype(logits, "logits");
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && ids.dim() == logits.dim() &&
+                          ids.sizes().slice(0, ids.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+                      "token_ids must be [..., K] with the leading dimensions of logits ", logits.sizes(), ", got ",
+                      ids.sizes());
+    score_tokens(ids, logits, "token_ids");
+    ScoreOut o = score(logits, ids, 0, temperature);
+    return {o.logprobs, o.entropy, o.lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -861,6 +982,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "One token per row from given uniform numbers: (token, logprob, kept_logprob).",
           pybind11::arg("logits"), pybind11::arg("u"), pybind11::arg("temperature"), pybind11::arg("top_k"),
           pybind11::arg("top_p"), pybind11::arg("min_p"));
+    m.def("top_logprobs", &top_logprobs,
+          "The k most likely tokens with their log-probabilities, the target's, entropy and lse; differentiable.",
+          pybind11::arg("logits"), pybind11::arg("targets"), pybind11::arg("k"), pybind11::arg("temperature"));
+    m.def("token_logprobs", &token_logprobs,
+          "Log-probabilities of K given tokens per row, entropy and lse; differentiable.", pybind11::arg("logits"),
+          pybind11::arg("token_ids"), pybind11::arg("temperature"));
     m.def("abi_version", &k1_abi_version, "C ABI version of the loaded libk1_b200.so.");
     m.def(
         "ring_status",

@@ -7,7 +7,7 @@ the same public functions, the same `_C` binding names, and the lazily imported
 the GRPO completion-window node in `kernel_opt.grpo`, the LM head fused with K1 in
 `kernel_opt.lm_head`.  The operators of a decoding step's tail, which produce the tokens that
 K1 scores, are in `kernel_opt.norm`, `kernel_opt.fp8` and `kernel_opt.sampling`, and run together
-in `kernel_opt.rollout`.
+in `kernel_opt.rollout`.  `kernel_opt.score` has the log-probabilities of lists of tokens.
 """
 import torch  # noqa: F401  (loads libc10 / libtorch before the extension)
 
@@ -28,6 +28,7 @@ from .lm_head import fused_linear_logprob_entropy  # noqa: F401
 from .norm import fused_residual_rmsnorm, fused_residual_rmsnorm_fp8  # noqa: F401
 from .fp8 import fp8_linear, quantize_fp8_blocks, quantize_fp8_rows  # noqa: F401
 from .sampling import sample_tokens  # noqa: F401
+from .score import fused_token_logprobs, fused_top_logprobs  # noqa: F401
 from .rollout import RolloutHead  # noqa: F401
 
 
