@@ -31,7 +31,10 @@ CAPI_UNITS = {
     "k1_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_tc.cuh", "k1_kernels.cuh",
                    "k1_ring.cuh", "k1_fwd_sm.cuh", "k1_lmhead.cuh"],
     "k1_decode_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_tc.cuh",
-                          "k1_norm.cuh", "k1_fp8_linear.cuh", "k1_sample.cuh", "k1_sample_math.cuh"],
+                          "k1_norm.cuh", "k1_norm_host.cuh", "k1_fp8_linear.cuh", "k1_sample.cuh",
+                          "k1_sample_math.cuh"],
+    "k1_sandwich_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_norm.cuh", "k1_norm_host.cuh",
+                            "k1_sandwich.cuh"],
     "k1_score_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_score.cuh"],
 }
 OBJDIR = os.path.join(HERE, "build")

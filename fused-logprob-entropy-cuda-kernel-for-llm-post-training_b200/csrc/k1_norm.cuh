@@ -205,16 +205,45 @@ struct FwdParams {
     int64_t n, x_stride, r_stride;
     int h, w32;
     float eps;
+    // POST: the norm after the block, its gate and the scales of both terms
+    const void* wp;
+    const void* gate;
+    int64_t gate_stride;
+    int gate_kind;
+    float branch_scale, residual_scale;
+    float* rstd_post;  // may be NULL
 };
+
+// The gate of the branch: none, one per column (the weights' type), one per row, or one per
+// element (the tensors' type).
+enum Gate : int { GATE_NONE = 0, GATE_COLUMN = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
+
+// The gate's values for a piece; `token` is the row's.
+template <typename T, int E>
+__device__ __forceinline__ void load_gate(const void* gate, int kind, int64_t row_at, float token, bool w32, int col,
+                                          float (&f)[E]) {
+    if (kind == GATE_COLUMN) {
+        load_weight<T, E>(gate, w32, col, f);
+    } else if (kind == GATE_FULL) {
+        Piece<T, E> t;
+        t.load(reinterpret_cast<const T*>(gate) + row_at + col);
+        t.get(f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = token;
+    }
+}
 
 // NV pieces per thread: piece j of thread t starts at column (j * threads + t) * E.  Rows of few
 // small pieces per thread keep to 32 registers, so that two blocks of 1024 threads share an SM
 // (4096 x 3585 bf16, us: forward 62 -> 55, with 8-bit output 93 -> 74).
-template <typename T, int E, int NV, int OUT>
+//
+// POST: x goes through a norm of its own first, s = T(residual_scale r + branch_scale gate (x R1 wp)).
+template <typename T, int E, int NV, int OUT, bool POST = false>
 __global__ void __launch_bounds__(kThreads<E>, E < 4 && E * NV <= 4 ? 2 : 1) k1_rmsnorm_kernel(FwdParams p) {
     using P = Piece<T, E>;
     constexpr bool VEC = E >= 4;
-    __shared__ float scratch[2][32];
+    __shared__ float scratch[POST ? 4 : 2][32];
     __shared__ float wmax[(!VEC && OUT != SAME) ? NV : 1][kMaxSmall / 32];
     pdl_wait();
     pdl_trigger();
@@ -243,6 +272,23 @@ __global__ void __launch_bounds__(kThreads<E>, E < 4 && E * NV <= 4 ? 2 : 1) k1_
                 else
                     q[j].zero();
             }
+            float scale = 1.f, token = 1.f;
+            int64_t gate_row = 0;
+            if constexpr (POST) {
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    float a[E];
+                    s[j].get(a);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) sum = fmaf(a[i], a[i], sum);
+                }
+                gate_row = row * p.gate_stride;
+                if (p.gate_kind == GATE_TOKEN) token = DT<T>::load1(reinterpret_cast<const T*>(p.gate) + gate_row);
+                sum = block_sum(sum, scratch[2 + flip]);
+                scale = rsqrtf(sum / (float)p.h + p.eps);
+                if (p.rstd_post && tid == 0) p.rstd_post[row] = scale;
+            }
             T* so = reinterpret_cast<T*>(p.s) + row * p.h;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -250,6 +296,18 @@ __global__ void __launch_bounds__(kThreads<E>, E < 4 && E * NV <= 4 ? 2 : 1) k1_
                 float a[E], b[E];
                 s[j].get(a);
                 q[j].get(b);
+                if constexpr (POST) {
+                    if (col < p.h) {
+                        float wp[E], gate[E];
+                        load_weight<T, E>(p.wp, p.w32, col, wp);
+                        load_gate<T, E>(p.gate, p.gate_kind, gate_row, token, p.w32, col, gate);
+#pragma unroll
+                        for (int i = 0; i < E; ++i) {
+                            a[i] = a[i] * scale * wp[i] * (gate[i] * p.branch_scale);
+                            b[i] *= p.residual_scale;
+                        }
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < E; ++i) a[i] += b[i];
                 s[j].set(a);

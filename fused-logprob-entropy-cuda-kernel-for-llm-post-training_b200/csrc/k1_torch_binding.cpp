@@ -789,6 +789,178 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sample_tokens(const at::Tensor& l
 }
 
 // ---------------------------------------------------------------------------------------
+// The norms around a block's end
+// ---------------------------------------------------------------------------------------
+// The arguments as rows (those of the gate where it has rows) and what kind of gate it is.
+struct Sandwich {
+    at::Tensor x, residual, post_weight, weight, gate;
+    int kind = K1_GATE_NONE;
+    int64_t gate_stride = 0;
+    int dt = 0;
+    const void* gate_ptr() const { return kind == K1_GATE_NONE ? nullptr : gate.data_ptr(); }
+};
+
+Sandwich sandwich_inputs(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& post_weight,
+                         const at::Tensor& weight, const at::Tensor& gate, double eps) {
+    Sandwich a;
+    TORCH_CHECK_VALUE(residual.defined(), "a residual is expected");
+    a.dt = norm_inputs(x, residual, weight, eps);
+    TORCH_CHECK_VALUE(post_weight.sizes() == weight.sizes() && post_weight.scalar_type() == weight.scalar_type() &&
+                          post_weight.device() == x.device(),
+                      "post_weight must match weight in shape, dtype and device, got ", post_weight.sizes(), " ",
+                      post_weight.scalar_type(), " for ", weight.sizes(), " ", weight.scalar_type());
+    if (gate.defined()) {
+        TORCH_CHECK_VALUE(gate.device() == x.device(), "gate must be on x's device");
+        const int64_t H = x.size(-1);
+        const bool rows = gate.dim() == x.dim() && gate.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
+        if (gate.dim() == 1 && gate.size(0) == H) {
+            a.kind = K1_GATE_COLUMN;
+            TORCH_CHECK(gate.scalar_type() == weight.scalar_type(), "a gate per column must have the weights' dtype");
+        } else {
+            TORCH_CHECK_VALUE(rows && (gate.size(-1) == H || gate.size(-1) == 1),
+                              "gate must be [H], or shaped like x with H or 1 columns, got ", gate.sizes(), " for ",
+                              x.sizes());
+            a.kind = gate.size(-1) == H ? K1_GATE_FULL : K1_GATE_TOKEN;
+            TORCH_CHECK(gate.scalar_type() == x.scalar_type(), "a gate with rows must have x's dtype");
+        }
+    }
+    return a;
+}
+
+// Rows of the arguments; on x's device.
+void sandwich_rows(Sandwich& a, const at::Tensor& x, const at::Tensor& residual, const at::Tensor& post_weight,
+                   const at::Tensor& weight, const at::Tensor& gate) {
+    a.x = rows2d(x);
+    if (residual.defined()) a.residual = rows2d(residual);
+    a.post_weight = post_weight.contiguous();
+    a.weight = weight.contiguous();
+    if (a.kind == K1_GATE_COLUMN) {
+        a.gate = gate.contiguous();
+    } else if (a.kind != K1_GATE_NONE) {
+        a.gate = rows2d(gate);
+        a.gate_stride = a.gate.stride(0);
+    }
+}
+
+struct SandwichRmsnorm : public torch::autograd::Function<SandwichRmsnorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                  const at::Tensor& residual, const at::Tensor& post_weight,
+                                                  const at::Tensor& weight, const c10::optional<at::Tensor>& gate_,
+                                                  double branch_scale, double residual_scale, double eps, bool want) {
+        const at::Tensor gate = gate_.has_value() ? *gate_ : at::Tensor();
+        c10::cuda::CUDAGuard guard(x.device());
+        Sandwich a = sandwich_inputs(x, residual, post_weight, weight, gate, eps);
+        sandwich_rows(a, x, residual, post_weight, weight, gate);
+        const int64_t N = a.x.size(0), H = a.x.size(1);
+        at::Tensor y = at::empty({N, H}, x.options()), stream = at::empty({N, H}, x.options()), r1, r2;
+        if (want) {
+            r1 = at::empty({N}, x.options().dtype(at::kFloat));
+            r2 = at::empty({N}, x.options().dtype(at::kFloat));
+        }
+        check_launch(k1_sandwich_rmsnorm(a.x.data_ptr(), a.x.stride(0), a.residual.data_ptr(), a.residual.stride(0),
+                                         a.post_weight.data_ptr(), a.gate_ptr(), a.kind, a.gate_stride,
+                                         a.weight.data_ptr(), dtype_code(weight), a.dt, N, H, (float)branch_scale,
+                                         (float)residual_scale, (float)eps, stream.data_ptr(), y.data_ptr(),
+                                         want ? r1.data_ptr<float>() : nullptr, want ? r2.data_ptr<float>() : nullptr,
+                                         at::cuda::getCurrentCUDAStream().stream()));
+        y = shaped(y, x.sizes());
+        stream = shaped(stream, x.sizes());
+        if (want) {
+            ctx->save_for_backward({stream, x, r1, r2, post_weight, weight, gate});
+            ctx->set_materialize_grads(false);
+            ctx->saved_data["kind"] = (int64_t)a.kind;
+            ctx->saved_data["branch_scale"] = branch_scale;
+            ctx->saved_data["residual_scale"] = residual_scale;
+        }
+        return {y, stream};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "the sandwich RMS norm has no second derivative");
+        const at::Tensor none;
+        const at::Tensor &g_y = grads[0], &g_s = grads[1];
+        torch::autograd::variable_list out(9);
+        if (!g_y.defined() && !g_s.defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &stream = saved[0], &x = saved[1], &r1 = saved[2], &r2 = saved[3], &post_weight = saved[4],
+                         &weight = saved[5], &gate = saved[6];
+        c10::cuda::CUDAGuard guard(stream.device());
+        Sandwich a;
+        a.kind = (int)ctx->saved_data["kind"].toInt();
+        sandwich_rows(a, x, none, post_weight, weight, gate);
+        const at::Tensor s2 = rows2d(stream), gy2 = g_y.defined() ? rows2d(g_y) : none,
+                         gs2 = g_s.defined() ? rows2d(g_s) : none;
+        const int64_t N = s2.size(0), H = s2.size(1);
+        // counted over the tensors that were given
+        if (ctx->needs_input_grad(0)) out[0] = at::empty({N, H}, stream.options());
+        if (ctx->needs_input_grad(1)) out[1] = at::empty({N, H}, stream.options());
+        if (ctx->needs_input_grad(2)) out[2] = at::empty(post_weight.sizes(), post_weight.options());
+        if (ctx->needs_input_grad(3)) out[3] = at::empty(weight.sizes(), weight.options());
+        if (gate.defined() && ctx->needs_input_grad(4)) out[4] = at::empty(gate.sizes(), gate.options());
+        size_t ws_bytes = 0;
+        at::Tensor ws;
+        if (out[2].defined() || out[3].defined() || (out[4].defined() && a.kind == K1_GATE_COLUMN)) {
+            ws_bytes = k1_sandwich_rmsnorm_workspace_bytes(N, H, stream.get_device());
+            ws = at::empty({(int64_t)ws_bytes}, stream.options().dtype(at::kByte));
+        }
+        const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+        const auto step = [](const at::Tensor& t) { return t.defined() ? t.stride(0) : 0; };
+        check_launch(k1_sandwich_rmsnorm_backward(
+            ptr(gy2), step(gy2), ptr(gs2), step(gs2), s2.data_ptr(), s2.stride(0), a.x.data_ptr(), a.x.stride(0),
+            a.post_weight.data_ptr(), a.gate_ptr(), a.kind, a.gate_stride, a.weight.data_ptr(), dtype_code(weight),
+            dtype_code(stream), r1.data_ptr<float>(), r2.data_ptr<float>(), N, H,
+            (float)ctx->saved_data["branch_scale"].toDouble(), (float)ctx->saved_data["residual_scale"].toDouble(),
+            ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[4]), ptr(out[3]), ptr(ws), ws_bytes,
+            at::cuda::getCurrentCUDAStream().stream()));
+        for (int i : {0, 1})
+            if (out[i].defined()) out[i] = shaped(out[i], stream.sizes());
+        return out;
+    }
+};
+
+// (y, stream); differentiable in x, residual, both weights and the gate.
+std::tuple<at::Tensor, at::Tensor> sandwich_rmsnorm(const at::Tensor& x, const at::Tensor& residual,
+                                                    const at::Tensor& post_weight, const at::Tensor& weight,
+                                                    const c10::optional<at::Tensor>& gate_, double branch_scale,
+                                                    double residual_scale, double eps) {
+    const at::Tensor gate = gate_.has_value() ? *gate_ : at::Tensor();
+    sandwich_inputs(x, residual, post_weight, weight, gate, eps);
+    bool want = false;
+    for (const at::Tensor* t : {&x, &residual, &post_weight, &weight, &gate}) {
+        if (!t->defined()) continue;
+        TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(),
+                    "the sandwich RMS norm does not support forward AD: it has no jvp");
+        want |= t->requires_grad();
+    }
+    want &= at::GradMode::is_enabled();
+    auto out = SandwichRmsnorm::apply(x, residual, post_weight, weight, gate_, branch_scale, residual_scale, eps, want);
+    return {out[0], out[1]};
+}
+
+// (q, scales, stream)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> sandwich_rmsnorm_fp8(const at::Tensor& x, const at::Tensor& residual,
+                                                                    const at::Tensor& post_weight,
+                                                                    const at::Tensor& weight,
+                                                                    const c10::optional<at::Tensor>& gate_,
+                                                                    double branch_scale, double residual_scale,
+                                                                    double eps) {
+    const at::Tensor gate = gate_.has_value() ? *gate_ : at::Tensor();
+    Sandwich a = sandwich_inputs(x, residual, post_weight, weight, gate, eps);
+    c10::cuda::CUDAGuard guard(x.device());
+    sandwich_rows(a, x, residual, post_weight, weight, gate);
+    const int64_t N = a.x.size(0), H = a.x.size(1);
+    at::Tensor q = at::empty({N, H}, x.options().dtype(at::kFloat8_e4m3fn)), stream = at::empty({N, H}, x.options());
+    at::Tensor scales = at::empty({N, (H + 127) / 128}, x.options().dtype(at::kFloat));
+    check_launch(k1_sandwich_rmsnorm_fp8(a.x.data_ptr(), a.x.stride(0), a.residual.data_ptr(), a.residual.stride(0),
+                                         a.post_weight.data_ptr(), a.gate_ptr(), a.kind, a.gate_stride,
+                                         a.weight.data_ptr(), dtype_code(weight), a.dt, N, H, (float)branch_scale,
+                                         (float)residual_scale, (float)eps, stream.data_ptr(), q.data_ptr(),
+                                         scales.data_ptr<float>(), at::cuda::getCurrentCUDAStream().stream()));
+    return {lead_shaped(q, x), lead_shaped(scales, x), lead_shaped(stream, x)};
+}
+
+// ---------------------------------------------------------------------------------------
 // Log-probabilities of given tokens and of the most likely ones
 // ---------------------------------------------------------------------------------------
 struct ScoreOut {
@@ -982,6 +1154,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "One token per row from given uniform numbers: (token, logprob, kept_logprob).",
           pybind11::arg("logits"), pybind11::arg("u"), pybind11::arg("temperature"), pybind11::arg("top_k"),
           pybind11::arg("top_p"), pybind11::arg("min_p"));
+    m.def("sandwich_rmsnorm", &sandwich_rmsnorm,
+          "stream = residual_scale residual + branch_scale gate norm(x) post_weight, y = its RMS norm times the "
+          "weight: (y, stream), differentiable.",
+          pybind11::arg("x"), pybind11::arg("residual"), pybind11::arg("post_weight"), pybind11::arg("weight"),
+          pybind11::arg("gate"), pybind11::arg("branch_scale"), pybind11::arg("residual_scale"), pybind11::arg("eps"));
+    m.def("sandwich_rmsnorm_fp8", &sandwich_rmsnorm_fp8,
+          "sandwich_rmsnorm with y in 8 bits, one scale per row and 128 columns: (q, scales, stream).",
+          pybind11::arg("x"), pybind11::arg("residual"), pybind11::arg("post_weight"), pybind11::arg("weight"),
+          pybind11::arg("gate"), pybind11::arg("branch_scale"), pybind11::arg("residual_scale"), pybind11::arg("eps"));
     m.def("top_logprobs", &top_logprobs,
           "The k most likely tokens with their log-probabilities, the target's, entropy and lse; differentiable.",
           pybind11::arg("logits"), pybind11::arg("targets"), pybind11::arg("k"), pybind11::arg("temperature"));

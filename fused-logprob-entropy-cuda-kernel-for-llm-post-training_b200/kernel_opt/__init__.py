@@ -25,7 +25,12 @@ from .ops import (  # noqa: F401
     fused_logprob_entropy_scaled,
 )
 from .lm_head import fused_linear_logprob_entropy  # noqa: F401
-from .norm import fused_residual_rmsnorm, fused_residual_rmsnorm_fp8  # noqa: F401
+from .norm import (  # noqa: F401
+    fused_residual_rmsnorm,
+    fused_residual_rmsnorm_fp8,
+    fused_sandwich_rmsnorm,
+    fused_sandwich_rmsnorm_fp8,
+)
 from .fp8 import fp8_linear, quantize_fp8_blocks, quantize_fp8_rows  # noqa: F401
 from .sampling import sample_tokens  # noqa: F401
 from .score import fused_token_logprobs, fused_top_logprobs  # noqa: F401

@@ -33,3 +33,27 @@ def fused_residual_rmsnorm_fp8(x: torch.Tensor, residual: torch.Tensor | None,
     (largest magnitude / 448), y = q * scale.  y is rounded once, from fp32.  Inference only:
     no gradient flows."""
     return _C.residual_rmsnorm_fp8(x, residual, weight, eps)
+
+
+def fused_sandwich_rmsnorm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
+                           weight: torch.Tensor, gate: torch.Tensor | None = None,
+                           branch_scale: float = 1.0, residual_scale: float = 1.0, eps: float = 1e-6):
+    """(y, stream): the norm after a block and the one before the next.
+
+        stream = residual_scale * residual + branch_scale * gate * (RMS norm of x times post_weight)
+        y      = RMS norm of the stream (as stored) times weight
+
+    x, residual: [..., H] as in `fused_residual_rmsnorm`; post_weight, weight: [H] of x's dtype or
+    both fp32.  gate: None, [H] of the weights' dtype, or x's leading dimensions with H or 1 columns in
+    x's dtype (other shapes: expand them).  branch_scale, residual_scale: finite numbers.
+    Differentiable (once, backwards) in x, residual, both weights and the gate, through y and the
+    stream."""
+    return _C.sandwich_rmsnorm(x, residual, post_weight, weight, gate, branch_scale, residual_scale, eps)
+
+
+def fused_sandwich_rmsnorm_fp8(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
+                               weight: torch.Tensor, gate: torch.Tensor | None = None,
+                               branch_scale: float = 1.0, residual_scale: float = 1.0, eps: float = 1e-6):
+    """(q, scales, stream): `fused_sandwich_rmsnorm` with y in 8 bits, for `fp8_linear` (q and
+    scales as in `fused_residual_rmsnorm_fp8`).  Inference only: no gradient flows."""
+    return _C.sandwich_rmsnorm_fp8(x, residual, post_weight, weight, gate, branch_scale, residual_scale, eps)

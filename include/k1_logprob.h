@@ -418,6 +418,59 @@ int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t voca
                      int64_t* token, float* logprob, float* kept_logprob, void* stream);
 
 /*
+ * The norms around a block's end: the norm after the block, its gate and the scales of both
+ * terms, the residual addition, and the norm in front of the next block.  Over matrices as in
+ * k1_residual_rmsnorm:
+ *     rstd_post  = 1 / sqrt(mean(x^2) + eps)
+ *     stream_out = dtype(residual_scale residual + branch_scale gate (x rstd_post post_weight))
+ *     rstd       = 1 / sqrt(mean(stream^2) + eps)
+ *     y          = dtype(stream rstd weight)
+ * gate: none (NULL); hidden values of weight_dtype (per column); one value of dtype per row, or
+ * hidden of them, rows gate_stride elements apart.  Both weights have weight_dtype (dtype or fp32).
+ * stream_out and y are contiguous (stream_out may be x or residual if that is contiguous); the
+ * scales are finite.  rstd_post and rstd may be NULL (no backward).
+ */
+#define K1_GATE_NONE 0
+#define K1_GATE_COLUMN 1
+#define K1_GATE_TOKEN 2
+#define K1_GATE_FULL 3
+int k1_sandwich_rmsnorm(const void* x, int64_t x_stride, const void* residual,
+                        int64_t residual_stride, const void* post_weight, const void* gate,
+                        int gate_kind, int64_t gate_stride, const void* weight, int weight_dtype,
+                        int dtype, int64_t n_rows, int64_t hidden, float branch_scale,
+                        float residual_scale, float eps, void* stream_out, void* y,
+                        float* rstd_post, float* rstd, void* stream);
+
+/* The same with the output in 8 bits (q and scales as in k1_residual_rmsnorm_fp8). */
+int k1_sandwich_rmsnorm_fp8(const void* x, int64_t x_stride, const void* residual,
+                            int64_t residual_stride, const void* post_weight, const void* gate,
+                            int gate_kind, int64_t gate_stride, const void* weight,
+                            int weight_dtype, int dtype, int64_t n_rows, int64_t hidden,
+                            float branch_scale, float residual_scale, float eps, void* stream_out,
+                            void* q, float* scales, void* stream);
+
+/* Workspace bytes of the backward's gradients per column; 0 for invalid arguments. */
+size_t k1_sandwich_rmsnorm_workspace_bytes(int64_t n_rows, int64_t hidden, int device);
+
+/*
+ * Backward of k1_sandwich_rmsnorm from g_y, g_stream (each may be NULL: none), the stored stream,
+ * x and both rstd.  Outputs, each NULL if not wanted: d_x, d_residual (contiguous, dtype),
+ * d_post_weight, d_weight (weight_dtype), d_gate (shaped and typed like the gate, contiguous); sums
+ * over rows and columns are fp32 in a fixed order.  The workspace is only needed for the
+ * gradients per column: d_post_weight, d_weight and a gate's per column.
+ */
+int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void* g_stream,
+                                 int64_t g_stream_stride, const void* stream_in,
+                                 int64_t stream_stride, const void* x, int64_t x_stride,
+                                 const void* post_weight, const void* gate, int gate_kind,
+                                 int64_t gate_stride, const void* weight, int weight_dtype,
+                                 int dtype, const float* rstd_post, const float* rstd,
+                                 int64_t n_rows, int64_t hidden, float branch_scale,
+                                 float residual_scale, void* d_x, void* d_residual,
+                                 void* d_post_weight, void* d_gate, void* d_weight,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Log-probabilities of given tokens and of the k most likely ones, with entropy and
  * log-sum-exp, in one pass over the logits.  With y = fp32(1 / temperature) x, not rounded to
  * the logits' type, and l = log sum exp y, per row:
