@@ -179,7 +179,7 @@ int make_tmap8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
 // memory beside the ring.
 constexpr int64_t kMaxInner = 32768;
 
-template <int TN, typename OutT>
+template <int TN, typename OutT, bool EPI>
 int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
            int64_t inner, int sms, int dev, cudaStream_t st) {
     using S = k1::fp8::Skinny<TN>;
@@ -195,7 +195,7 @@ int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
     int split = 1;
     if (tiles * tok * 3 < 2 * sms)
         while (split < 8 && tiles * tok * split < sms && p.kb_total >= 4 * split) split *= 2;
-    auto kern = k1::fp8::k1_fp8_skinny_kernel<TN, OutT>;
+    auto kern = k1::fp8::k1_fp8_skinny_kernel<TN, OutT, EPI>;
     const size_t smem = S::smem((p.kb_total + split - 1) / split);
     rc = allow_smem(kern, dev, smem);
     if (rc) return rc;
@@ -230,7 +230,7 @@ int wide_pairs(Kernel kern, int dev, int* out) {
     return K1_OK;
 }
 
-template <typename OutT>
+template <typename OutT, bool EPI>
 int wide(const char* fn, k1::fp8::Params p, const void* x, int64_t ldx, const void* w, int64_t ldw,
          int64_t inner, int dev, cudaStream_t st) {
     using S = k1::fp8::Wide;
@@ -241,7 +241,7 @@ int wide(const char* fn, k1::fp8::Params p, const void* x, int64_t ldx, const vo
     p.m_tiles = (int)((p.m + S::TM - 1) / S::TM);
     p.n_tiles = (int)((p.n + S::BN - 1) / S::BN);
     const bool aligned16 = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * sizeof(OutT))) & 15) == 0;
-    auto kern = aligned16 ? k1::fp8::k1_fp8_wide_kernel<OutT, true> : k1::fp8::k1_fp8_wide_kernel<OutT, false>;
+    auto kern = aligned16 ? k1::fp8::k1_fp8_wide_kernel<OutT, true, EPI> : k1::fp8::k1_fp8_wide_kernel<OutT, false, EPI>;
     int pairs = 0;
     rc = allow_smem(kern, dev, S::SMEM);
     if (!rc) rc = wide_pairs(kern, dev, &pairs);
@@ -266,14 +266,14 @@ int linear_kernel(int64_t m, int64_t n, int kb_total, int sms) {
     return m <= 64 || few_us <= many_us ? 64 : 0;
 }
 
-template <typename OutT>
+template <typename OutT, bool EPI>
 int linear(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
            int64_t inner, int sms, int dev, cudaStream_t st) {
     switch (linear_kernel(p.m, p.n, p.kb_total, sms)) {
-        case 16: return skinny<16, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-        case 32: return skinny<32, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-        case 64: return skinny<64, OutT>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
-        default: return wide<OutT>(fn, p, x, ldx, w, ldw, inner, dev, st);
+        case 16: return skinny<16, OutT, EPI>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+        case 32: return skinny<32, OutT, EPI>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+        case 64: return skinny<64, OutT, EPI>(fn, p, x, ldx, w, ldw, inner, sms, dev, st);
+        default: return wide<OutT, EPI>(fn, p, x, ldx, w, ldw, inner, dev, st);
     }
 }
 
@@ -460,12 +460,15 @@ int k1_residual_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
                                                        : sum(float{}));
 }
 
-int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const void* weight,
-                  int64_t weight_stride, const float* weight_scales, int64_t tokens, int64_t inner,
-                  int64_t outer, void* y, int64_t y_stride, int out_dtype, void* stream) {
+int k1_fp8_linear_epilogue(const void* x, int64_t x_stride, const float* x_scales, const void* weight,
+                           int64_t weight_stride, const float* weight_scales, int64_t tokens, int64_t inner,
+                           int64_t outer, const void* bias, int bias_dtype, int activation, const void* residual,
+                           int64_t residual_stride, void* y, int64_t y_stride, int out_dtype, void* stream) {
     static const char* fn = "k1_fp8_linear";
     if (!known_dtype(out_dtype))
         return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: the output's dtype must be bf16, fp16, or fp32", fn);
+    if (activation < K1_ACT_NONE || activation > K1_ACT_GELU_TANH)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: activation must be one of K1_ACT_*, got %d", fn, activation);
     if (tokens < 0 || outer < 0) return fail(K1_ERR_INVALID_ARGUMENT, "%s: tokens and outer must be >= 0", fn);
     if (inner < 16 || inner % 16 != 0 || inner > kMaxInner)
         return fail(K1_ERR_INVALID_ARGUMENT, "%s: inner must be a multiple of 16 in [16, %lld], got %lld", fn,
@@ -482,6 +485,12 @@ int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const 
     if (y_stride < outer) return fail(K1_ERR_INVALID_ARGUMENT, "%s: y_stride must be >= outer", fn);
     if (!aligned(y, elem_size(out_dtype)) || !aligned(x_scales, 4) || !aligned(weight_scales, 4))
         return fail(K1_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element size", fn);
+    if (bias && bias_dtype != out_dtype && bias_dtype != K1_DTYPE_F32)
+        return fail(K1_ERR_UNSUPPORTED_DTYPE, "%s: the bias must have the output's dtype or fp32", fn);
+    if (residual && residual_stride < outer)
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: residual_stride must be >= outer", fn);
+    if (!aligned(residual, elem_size(out_dtype)) || (bias && !aligned(bias, elem_size(bias_dtype))))
+        return fail(K1_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element size", fn);
     int dev = 0, sms = 0;
     int rc = current_device(&dev);
     if (!rc) rc = sm_count(dev, &sms);
@@ -494,15 +503,28 @@ int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const 
     p.n = outer;
     p.ldy = y_stride;
     p.kb_total = (int)((inner + 127) / 128);
+    p.bias = bias;
+    p.bias32 = bias_dtype == K1_DTYPE_F32;
+    p.act = activation;
+    p.residual = residual;
+    p.ldr = residual_stride;
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    switch (out_dtype) {
-        case K1_DTYPE_BF16:
-            return linear<__nv_bfloat16>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
-        case K1_DTYPE_F16:
-            return linear<__half>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
-        default:
-            return linear<float>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
-    }
+    const bool epilogue = bias || residual || activation != K1_ACT_NONE;
+    auto go = [&](auto tag) {
+        using OutT = decltype(tag);
+        return epilogue ? linear<OutT, true>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st)
+                        : linear<OutT, false>(fn, p, x, x_stride, weight, weight_stride, inner, sms, dev, st);
+    };
+    return out_dtype == K1_DTYPE_BF16  ? go(__nv_bfloat16{})
+           : out_dtype == K1_DTYPE_F16 ? go(__half{})
+                                       : go(float{});
+}
+
+int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const void* weight,
+                  int64_t weight_stride, const float* weight_scales, int64_t tokens, int64_t inner,
+                  int64_t outer, void* y, int64_t y_stride, int out_dtype, void* stream) {
+    return k1_fp8_linear_epilogue(x, x_stride, x_scales, weight, weight_stride, weight_scales, tokens, inner, outer,
+                                  nullptr, out_dtype, K1_ACT_NONE, nullptr, 0, y, y_stride, out_dtype, stream);
 }
 
 int k1_sample_tokens(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,

@@ -32,6 +32,8 @@
 // the outputs that could not be finished are NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "k1_common.cuh"
 #include "k1_tc.cuh"
 
@@ -150,7 +152,58 @@ struct Params {
     int64_t m, n, ldy;
     int kb_total;     // ceil(k / 128)
     int m_tiles, n_tiles;  // many tokens: tiles of 256 x 256
+    // the epilogue: y = OutT(act(product + bias) + residual)
+    const void* bias;      // [n], fp32 or OutT; NULL: none
+    const void* residual;  // [m] rows of ldr elements of OutT (may be y itself); NULL: none
+    int64_t ldr;
+    int bias32, act;
 };
+
+enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
+
+// The activation in fp32, in forms that keep relative accuracy in the tails that go to 0.  What is
+// rounded to 16 bits takes the fast exponential and quotient (both right to about 2^-21 there).
+template <int ACT, bool FAST>
+__device__ __forceinline__ float activate(float v) {
+    if constexpr (ACT == ACT_RELU) {
+        return v < 0.f ? 0.f : v;  // NaN stays
+    } else if constexpr (ACT == ACT_GELU) {
+        return 0.5f * v * erfcf(-0.70710678f * v);
+    } else if constexpr (ACT == ACT_SILU || ACT == ACT_GELU_TANH) {
+        // v / (1 + exp(-u)); with u = 2 sqrt(2 / pi) (v + 0.044715 v^3) that is v/2 (1 + tanh(u / 2))
+        const float u = ACT == ACT_SILU ? v : 1.5957691f * fmaf(0.044715f * v * v, v, v);
+        if constexpr (FAST) return __fdividef(v, 1.f + __expf(-u));
+        return v / (1.f + expf(-u));
+    }
+    return v;
+}
+
+// f(activation as a compile-time constant)
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+    switch (act) {
+        case ACT_RELU: f(std::integral_constant<int, ACT_RELU>{}); break;
+        case ACT_SILU: f(std::integral_constant<int, ACT_SILU>{}); break;
+        case ACT_GELU: f(std::integral_constant<int, ACT_GELU>{}); break;
+        case ACT_GELU_TANH: f(std::integral_constant<int, ACT_GELU_TANH>{}); break;
+        default: f(std::integral_constant<int, ACT_NONE>{});
+    }
+}
+
+// The bias of column `col` (0 beyond the last one).
+template <typename OutT>
+__device__ __forceinline__ float bias_of(const Params& p, int64_t col) {
+    if (!p.bias || col >= p.n) return 0.f;
+    return p.bias32 ? __ldg(reinterpret_cast<const float*>(p.bias) + col)
+                    : DT<OutT>::load1(reinterpret_cast<const OutT*>(p.bias) + col);
+}
+
+// The residual of one element (it may be the output's own memory: the thread that writes an element
+// reads it first, and no other thread does).
+template <typename OutT>
+__device__ __forceinline__ float residual_of(const Params& p, int64_t row, int64_t col) {
+    return DT<OutT>::load1(reinterpret_cast<const OutT*>(p.residual) + row * p.ldr + col);
+}
 
 // ------------------------------------------------------------------------------------
 // Few tokens
@@ -177,7 +230,7 @@ __device__ __forceinline__ void store_pair(OutT* dst, float a, float b) {
     if constexpr (sizeof(OutT) == 2) *reinterpret_cast<uint32_t*>(dst) = DT<OutT>::from_f2(make_float2(a, b));
 }
 
-template <int TN, typename OutT>
+template <int TN, typename OutT, bool EPI = false>
 __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
     k1_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmap_x,
                          const __grid_constant__ CUtensorMap tmap_w, Params p, int split) {
@@ -289,7 +342,7 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
         }
     } else {
         // each thread owns one row of the weight (a TMEM lane) and its group's tokens
-        constexpr int CW = S::CW, EPI = S::GROUPS * 128;
+        constexpr int CW = S::CW, EPI_THREADS = S::GROUPS * 128;
         const int t = threadIdx.x - 64;
         const int quarter = warp & 3;
         const int row = quarter * 32 + lane;
@@ -301,7 +354,7 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
             // a thread's token is fixed (TN divides the threads); eight loads in flight
             const int64_t m = tok0 + t % TN;
             const float* xs = p.xs + (m < p.m ? m : 0) * p.kb_total + kb0;
-            constexpr int STEP = EPI / TN;
+            constexpr int STEP = EPI_THREADS / TN;
             for (int kb = t / TN; kb < nkb; kb += 8 * STEP) {
                 float f[8];
 #pragma unroll
@@ -312,7 +365,7 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
                     if (kb + q * STEP < nkb) scales[(kb + q * STEP) * TN + t % TN] = m < p.m ? f[q] : 0.f;
             }
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");
         float acc[CW];
 #pragma unroll
         for (int j = 0; j < CW; ++j) acc[j] = 0.f;
@@ -348,6 +401,14 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
         const int64_t col = (int64_t)tile * BM + row;
         const int tok = tok0 + j0;
         OutT* y = reinterpret_cast<OutT*>(p.y);
+        if (EPI && split == 1) {
+            // bias and activation here, the residual by the lane that stores
+            const float bias = bias_of<OutT>(p, col);
+            with_act(p.act, [&](auto act) {
+#pragma unroll
+                for (int j = 0; j < CW; ++j) acc[j] = activate<act, sizeof(OutT) == 2>(acc[j] + bias);
+            });
+        }
         if (split == 1) {
             // 16-bit outputs: two lanes trade, so that each stores two columns of one of two
             // tokens in one word
@@ -359,18 +420,31 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
                 for (int j = 0; j < CW; j += 2) {
                     const float got = __shfl_xor_sync(0xffffffffu, odd ? acc[j] : acc[j + 1], 1);
                     const int tj = tok + j + odd;
-                    if (col < p.n && tj < p.m)
-                        store_pair(y + (int64_t)tj * p.ldy + (col - odd), odd ? got : acc[j], odd ? acc[j + 1] : got);
+                    float a = odd ? got : acc[j], b = odd ? acc[j + 1] : got;
+                    if (col < p.n && tj < p.m) {
+                        if constexpr (EPI) {
+                            if (p.residual) {
+                                a += residual_of<OutT>(p, tj, col - odd);
+                                b += residual_of<OutT>(p, tj, col - odd + 1);
+                            }
+                        }
+                        store_pair(y + (int64_t)tj * p.ldy + (col - odd), a, b);
+                    }
                 }
             } else if (col < p.n) {
 #pragma unroll
-                for (int j = 0; j < CW; ++j)
-                    if (tok + j < p.m) DT<OutT>::store1(y + (int64_t)(tok + j) * p.ldy + col, acc[j]);
+                for (int j = 0; j < CW; ++j) {
+                    if (tok + j >= p.m) continue;
+                    if constexpr (EPI) {
+                        if (p.residual) acc[j] += residual_of<OutT>(p, tok + j, col);
+                    }
+                    DT<OutT>::store1(y + (int64_t)(tok + j) * p.ldy + col, acc[j]);
+                }
             }
         } else {
             // the ring is done with: every stage was consumed before the last block's sums (or,
             // after a wait that ran out, the producer has waited for its copies)
-            asm volatile("bar.sync 2, %0;" ::"n"(EPI + 32) : "memory");
+            asm volatile("bar.sync 2, %0;" ::"n"(EPI_THREADS + 32) : "memory");
             float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
             for (int j = 0; j < CW; ++j) part[(j0 + j) * BM + row] = acc[j];
@@ -395,8 +469,14 @@ __global__ void __launch_bounds__(Skinny<TN>::THREADS, TN <= 32 ? 3 : 2)
                                  : "r"(ring::mapa(mine + (uint32_t)j * BM * 4, r)));
                     v += f;
                 }
-                if (col < p.n && tok0 + j < p.m)
+                if (col < p.n && tok0 + j < p.m) {
+                    if constexpr (EPI) {
+                        v += bias_of<OutT>(p, col);
+                        with_act(p.act, [&](auto act) { v = activate<act, sizeof(OutT) == 2>(v); });
+                        if (p.residual) v += residual_of<OutT>(p, tok0 + j, col);
+                    }
                     DT<OutT>::store1(reinterpret_cast<OutT*>(p.y) + (tok0 + j) * p.ldy + col, v);
+                }
             }
         }
         ring::cluster_sync();  // no rank leaves while its part may be read
@@ -504,8 +584,35 @@ __device__ __forceinline__ void store_row32(OutT* dst, const float2* v, int vali
     }
 }
 
+// Adds 32 columns of a residual's row to v, `valid` of them; aligned: 16-byte loads.
+template <typename OutT>
+__device__ __forceinline__ void add_row32(const OutT* src, float2* v, int valid, bool aligned) {
+    constexpr int E = 16 / sizeof(OutT);
+    if (aligned && valid >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += E) {
+            const uint4 w = ld_stream(src + i);
+            if constexpr (sizeof(OutT) == 4) {
+                v[i / 2] = add2(v[i / 2], make_float2(__uint_as_float(w.x), __uint_as_float(w.y)));
+                v[i / 2 + 1] = add2(v[i / 2 + 1], make_float2(__uint_as_float(w.z), __uint_as_float(w.w)));
+            } else {
+                v[i / 2] = add2(v[i / 2], DT<OutT>::to_f2(w.x));
+                v[i / 2 + 1] = add2(v[i / 2 + 1], DT<OutT>::to_f2(w.y));
+                v[(i / 2 + 2) % 16] = add2(v[(i / 2 + 2) % 16], DT<OutT>::to_f2(w.z));
+                v[(i / 2 + 3) % 16] = add2(v[(i / 2 + 3) % 16], DT<OutT>::to_f2(w.w));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (2 * i < valid) v[i].x += DT<OutT>::load1(src + 2 * i);
+            if (2 * i + 1 < valid) v[i].y += DT<OutT>::load1(src + 2 * i + 1);
+        }
+    }
+}
+
 // ALIGNED: the output's rows start at multiples of 16 bytes.
-template <typename OutT, bool ALIGNED>
+template <typename OutT, bool ALIGNED, bool EPI = false>
 __global__ void __launch_bounds__(Wide::THREADS, 1)
     k1_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x,
                        const __grid_constant__ CUtensorMap tmap_w, Params p) {
@@ -755,9 +862,37 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < CPT / 2; ++j) acc[j] = splat(__int_as_float(0x7fc00000));
             }
+            if constexpr (EPI) {
+                // a warp's lanes have the same columns: one broadcast load for each
+                if (p.bias) {
+#pragma unroll
+                    for (int j = 0; j < CPT / 2; ++j) {
+                        acc[j].x += bias_of<OutT>(p, col0 + 2 * j);
+                        acc[j].y += bias_of<OutT>(p, col0 + 2 * j + 1);
+                    }
+                }
+                with_act(p.act, [&](auto act) {
+#pragma unroll
+                    for (int j = 0; j < CPT / 2; ++j) {
+                        acc[j].x = activate<act, sizeof(OutT) == 2>(acc[j].x);
+                        acc[j].y = activate<act, sizeof(OutT) == 2>(acc[j].y);
+                    }
+                });
+            }
             if constexpr (ALIGNED) {
                 if (row < p.m) {
                     OutT* y = reinterpret_cast<OutT*>(p.y) + row * p.ldy + col0;
+                    if constexpr (EPI) {
+                        if (p.residual) {
+                            const OutT* res = reinterpret_cast<const OutT*>(p.residual) + row * p.ldr + col0;
+                            const bool vec = (reinterpret_cast<uintptr_t>(res) & 15) == 0;
+#pragma unroll
+                            for (int c0 = 0; c0 < CPT; c0 += 32) {
+                                const int64_t left = p.n - col0 - c0;
+                                if (left > 0) add_row32<OutT>(res + c0, acc + c0 / 2, left < 32 ? (int)left : 32, vec);
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int c0 = 0; c0 < CPT; c0 += 32) {
                         const int64_t left = p.n - col0 - c0;
@@ -783,8 +918,13 @@ __global__ void __launch_bounds__(Wide::THREADS, 1)
                     OutT* y = reinterpret_cast<OutT*>(p.y) + row0 * p.ldy + col;
                     if (col < p.n) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i < rows) DT<OutT>::store1(y + (int64_t)i * p.ldy, v[i]);
+                        for (int i = 0; i < 32; ++i) {
+                            if (i >= rows) continue;
+                            if constexpr (EPI) {
+                                if (p.residual) v[i] += residual_of<OutT>(p, row0 + i, col);
+                            }
+                            DT<OutT>::store1(y + (int64_t)i * p.ldy, v[i]);
+                        }
                     }
                 }
             }

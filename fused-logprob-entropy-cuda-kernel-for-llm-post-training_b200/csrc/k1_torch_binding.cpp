@@ -699,7 +699,9 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8_blocks(const at::Tensor& w) {
 }
 
 at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
-                      const at::Tensor& weight_scales, at::ScalarType out_dtype, const c10::optional<at::Tensor>& out) {
+                      const at::Tensor& weight_scales, at::ScalarType out_dtype, const c10::optional<at::Tensor>& out,
+                      const c10::optional<at::Tensor>& bias_, const c10::optional<std::string>& activation,
+                      const c10::optional<at::Tensor>& residual_) {
     TORCH_CHECK_VALUE(x.is_cuda() && weight.is_cuda(), "x and weight must be CUDA tensors");
     TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && weight.scalar_type() == at::kFloat8_e4m3fn,
                 "x and weight must be float8_e4m3fn");
@@ -730,9 +732,47 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scales, const at:
                           "out_dtype must be bf16, fp16, or fp32, got ", out_dtype);
         y = at::empty({M, N}, x.options().dtype(out_dtype));
     }
-    check_launch(k1_fp8_linear(x2.data_ptr(), M > 1 ? x2.stride(0) : K, xs.data_ptr<float>(), w2.data_ptr(),
-                               N > 1 ? w2.stride(0) : K, ws.data_ptr<float>(), M, K, N, y.data_ptr(),
-                               M > 1 ? y.stride(0) : N, dtype_code(y), at::cuda::getCurrentCUDAStream().stream()));
+    int act = K1_ACT_NONE;
+    if (activation.has_value()) {
+        static const char* const names[] = {"none", "relu", "silu", "gelu", "gelu_tanh"};
+        for (act = K1_ACT_GELU_TANH; act > K1_ACT_NONE && *activation != names[act]; --act) {}
+        TORCH_CHECK_VALUE(act != K1_ACT_NONE, "activation must be None, 'relu', 'silu', 'gelu' or 'gelu_tanh', got '",
+                          *activation, "'");
+    }
+    at::Tensor bias, residual;
+    if (bias_.has_value()) {
+        TORCH_CHECK_VALUE(bias_->dim() == 1 && bias_->size(0) == N && bias_->device() == x.device(),
+                          "bias must be [O] on x's device, got ", bias_->sizes());
+        TORCH_CHECK(bias_->scalar_type() == y.scalar_type() || bias_->scalar_type() == at::kFloat,
+                    "bias must have the output's dtype or fp32");
+        bias = bias_->contiguous();
+    }
+    if (residual_.has_value()) {
+        TORCH_CHECK_VALUE(residual_->dim() == x.dim() && residual_->size(-1) == N &&
+                              residual_->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1) &&
+                              residual_->device() == x.device(),
+                          "residual must be shaped like the product, on x's device, got ", residual_->sizes());
+        TORCH_CHECK(residual_->scalar_type() == y.scalar_type(), "residual must have the output's dtype");
+        residual = rows2d(*residual_);
+        // broadcast rows (and what torch lets overlap) are laid out
+        if (M > 1 && residual.stride(0) < N) residual = residual.contiguous();
+        if (out.has_value() && M > 0 && N > 0) {
+            const auto range = [&](const at::Tensor& t) {
+                const char* at = (const char*)t.data_ptr();
+                return std::make_pair(at, at + ((M - 1) * (M > 1 ? t.stride(0) : 0) + N) * t.element_size());
+            };
+            const auto a = range(y), b = range(residual);
+            const bool same = a.first == b.first && (M == 1 || y.stride(0) == residual.stride(0));
+            TORCH_CHECK_VALUE(same || a.second <= b.first || b.second <= a.first,
+                              "residual must be the output itself or lie apart from it");
+        }
+    }
+    check_launch(k1_fp8_linear_epilogue(
+        x2.data_ptr(), M > 1 ? x2.stride(0) : K, xs.data_ptr<float>(), w2.data_ptr(), N > 1 ? w2.stride(0) : K,
+        ws.data_ptr<float>(), M, K, N, bias.defined() ? bias.data_ptr() : nullptr,
+        bias.defined() ? dtype_code(bias) : K1_DTYPE_F32, act, residual.defined() ? residual.data_ptr() : nullptr,
+        residual.defined() && M > 1 ? residual.stride(0) : N, y.data_ptr(), M > 1 ? y.stride(0) : N, dtype_code(y),
+        at::cuda::getCurrentCUDAStream().stream()));
     return out.has_value() ? y : lead_shaped(y, x);
 }
 
@@ -1147,9 +1187,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           pybind11::arg("x"));
     m.def("quantize_fp8_blocks", &quantize_fp8_blocks,
           "A weight in 8 bits: (q, scales [ceil(O / 128), ceil(H / 128)]).", pybind11::arg("weight"));
-    m.def("fp8_linear", &fp8_linear, "y = x weight^T of 8-bit operands with a scale per block of 128.",
+    m.def("fp8_linear", &fp8_linear,
+          "y = act(x weight^T + bias) + residual of 8-bit operands with a scale per block of 128.",
           pybind11::arg("x"), pybind11::arg("x_scales"), pybind11::arg("weight"),
-          pybind11::arg("weight_scales"), pybind11::arg("out_dtype"), pybind11::arg("out"));
+          pybind11::arg("weight_scales"), pybind11::arg("out_dtype"), pybind11::arg("out"),
+          pybind11::arg("bias") = pybind11::none(), pybind11::arg("activation") = pybind11::none(),
+          pybind11::arg("residual") = pybind11::none());
     m.def("sample_tokens", &sample_tokens,
           "One token per row from given uniform numbers: (token, logprob, kept_logprob).",
           pybind11::arg("logits"), pybind11::arg("u"), pybind11::arg("temperature"), pybind11::arg("top_k"),

@@ -27,10 +27,17 @@ def quantize_fp8_blocks(weight: torch.Tensor):
 
 def fp8_linear(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor,
                weight_scales: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
-               out: torch.Tensor | None = None) -> torch.Tensor:
-    """(x * x_scales) @ (weight * weight_scales).T: [..., O] in `out_dtype` (bf16 / fp16 / fp32).
+               out: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               activation: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act((x * x_scales) @ (weight * weight_scales).T + bias) + residual: [..., O] in `out_dtype`
+    (bf16 / fp16 / fp32), in fp32 up to one rounding.
 
     x: float8_e4m3fn [..., H]; x_scales: fp32 [..., ceil(H / 128)]; weight: float8_e4m3fn
     [O, H]; weight_scales: fp32 [ceil(O / 128), ceil(H / 128)].  H must be a multiple of 16, at
-    most 32768.  `out`: a tensor to write ([N, O], unit stride along O) instead of a new one."""
-    return _C.fp8_linear(x, x_scales, weight, weight_scales, out_dtype, out)
+    most 32768.  `out`: a tensor to write ([N, O], unit stride along O) instead of a new one, whose
+    dtype then counts.
+
+    bias: [O] of the output's dtype or fp32; activation: None, 'relu', 'silu', 'gelu' (the erf form) or
+    'gelu_tanh'; residual: [..., O] of the output's dtype.  A residual may be `out` itself (its rows, as
+    [N, O]), which is then updated in place, but not overlap it otherwise."""
+    return _C.fp8_linear(x, x_scales, weight, weight_scales, out_dtype, out, bias, activation, residual)

@@ -383,6 +383,25 @@ int k1_fp8_linear(const void* x, int64_t x_stride, const float* x_scales, const 
                   int64_t outer, void* y, int64_t y_stride, int out_dtype, void* stream);
 
 /*
+ * The same product with its epilogue: y = out_dtype(act(product + bias) + residual), in fp32 up to
+ * the one rounding.  bias: `outer` values of out_dtype or fp32, or NULL.  residual: tokens x outer of
+ * out_dtype, rows residual_stride elements apart, or NULL; it may be y itself (same address and
+ * stride) but not overlap it otherwise.  gelu: x/2 (1 + erf(x / sqrt 2)); gelu_tanh: its tanh form;
+ * silu: x / (1 + exp(-x)).
+ */
+#define K1_ACT_NONE 0
+#define K1_ACT_RELU 1
+#define K1_ACT_SILU 2
+#define K1_ACT_GELU 3
+#define K1_ACT_GELU_TANH 4
+int k1_fp8_linear_epilogue(const void* x, int64_t x_stride, const float* x_scales,
+                           const void* weight, int64_t weight_stride, const float* weight_scales,
+                           int64_t tokens, int64_t inner, int64_t outer, const void* bias,
+                           int bias_dtype, int activation, const void* residual,
+                           int64_t residual_stride, void* y, int64_t y_stride, int out_dtype,
+                           void* stream);
+
+/*
  * One token per row of logits.  A *_rows pointer (n_rows values on the device) takes the
  * place of the single value; temperature 0 takes the first largest logit, top_k <= 0, top_p
  * >= 1 and min_p = 0 are off.
