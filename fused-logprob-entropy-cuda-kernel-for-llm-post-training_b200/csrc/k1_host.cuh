@@ -11,6 +11,7 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <utility>
 
 #include "k1_logprob.h"
@@ -128,6 +129,25 @@ int allow_smem(Kernel kernel, int dev, size_t smem) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(K1_ERR_CUDA, "cudaFuncSetAttribute(smem): %s", cudaGetErrorString(e));
     have = smem;
+    return K1_OK;
+}
+
+// Blocks of `threads` threads and `smem` bytes of dynamic shared memory that an SM holds at once.
+// Cached per device and launch shape.
+template <typename Kernel>
+int resident_blocks(Kernel kernel, int dev, int threads, size_t smem, int* out) {
+    static std::mutex mu;
+    static std::map<std::tuple<int, const void*, int, size_t>, int> cache;
+    std::lock_guard<std::mutex> lock(mu);
+    int& have = cache[std::make_tuple(dev, reinterpret_cast<const void*>(kernel), threads, smem)];
+    if (have == 0) {
+        cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&have, kernel, threads, smem);
+        if (e != cudaSuccess || have < 1) {
+            have = 0;
+            return fail(K1_ERR_CUDA, "cudaOccupancyMaxActiveBlocksPerMultiprocessor: %s", cudaGetErrorString(e));
+        }
+    }
+    *out = have;
     return K1_OK;
 }
 

@@ -111,23 +111,21 @@ int sandwich_forward(const char* fn, int out, const void* x, int64_t x_stride, c
     p.branch_scale = branch_scale;
     p.residual_scale = residual_scale;
     p.rstd_post = rstd_post;
-    const int64_t grid = norm_grid(n, sh.threads, sms, 8);
+    // as many blocks as reside at once (or rows): a row costs the same everywhere, so a second round
+    // of blocks would leave SMs idle
     auto go = [&](auto tag) {
         using T = decltype(tag);
         return with_shape<T>(sh, [&](auto E, auto NV) {
-            if (same) return launch(k1::norm::k1_rmsnorm_kernel<T, E, NV, k1::norm::SAME, true>, grid, sh.threads, 0, st, p);
-            return launch(k1::norm::k1_rmsnorm_kernel<T, E, NV, k1::norm::FP8, true>, grid, sh.threads, 0, st, p);
+            auto kern = same ? k1::norm::k1_rmsnorm_kernel<T, E, NV, k1::norm::SAME, true>
+                             : k1::norm::k1_rmsnorm_kernel<T, E, NV, k1::norm::FP8, true>;
+            int per_sm = 0;
+            if (resident_blocks(kern, dev, sh.threads, 0, &per_sm) != K1_OK) return cudaErrorInvalidValue;
+            return launch(kern, std::min<int64_t>(n, (int64_t)sms * per_sm), sh.threads, 0, st, p);
         });
     };
     return launched(fn, dtype == K1_DTYPE_BF16  ? go(__nv_bfloat16{})
                         : dtype == K1_DTYPE_F16 ? go(__half{})
                                                 : go(float{}));
-}
-
-// The backward's blocks: as the norm's own, but no more than their shared sums let reside.
-int64_t sandwich_bwd_grid(int64_t n, int threads, int64_t hidden, int sms) {
-    const int64_t fit = std::max<int64_t>(1, (220 * 1024) / (hidden * 12 + 1024));
-    return std::min(norm_bwd_grid(n, threads, sms), std::max<int64_t>(sms, fit * sms));
 }
 
 }  // namespace
@@ -213,9 +211,9 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
     align = gate_align(d_gate, gate_kind, hidden, n_rows, es, align);
     const NormShape sh = norm_shape((int)hidden, es, std::min(norm_piece(hidden, es, align),
                                                               weights_piece(es, {weight, post_weight, column})));
-    const int64_t grid = sandwich_bwd_grid(n_rows, sh.threads, hidden, sms);
     const int want = (d_weight ? 1 : 0) | (d_post_weight ? 2 : 0) | (d_column ? 4 : 0);
-    if (want && (!workspace || !aligned(workspace, 16) || workspace_bytes < (size_t)grid * hidden * 3 * sizeof(float)))
+    if (want && (!workspace || !aligned(workspace, 16) ||
+                 workspace_bytes < k1_sandwich_rmsnorm_workspace_bytes(n_rows, hidden, dev)))
         return fail(K1_ERR_WORKSPACE, "%s: the weights' gradients need %zu bytes of 16-byte aligned workspace", fn,
                     k1_sandwich_rmsnorm_workspace_bytes(n_rows, hidden, dev));
     k1::norm::SandwichBwdParams p = {};
@@ -245,11 +243,16 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
     p.branch_scale = branch_scale;
     p.residual_scale = residual_scale;
     const size_t smem = (size_t)hidden * 12;
+    int64_t grid = 0;  // resident blocks, as in the forward
     auto go = [&](auto tag) {
         using T = decltype(tag);
         return with_shape<T>(sh, [&](auto E, auto NV) {
             auto kern = k1::norm::k1_sandwich_bwd_kernel<T, E, NV>;
-            if (allow_smem(kern, dev, smem) != K1_OK) return cudaErrorInvalidValue;
+            int per_sm = 0;
+            if (allow_smem(kern, dev, smem) != K1_OK ||
+                resident_blocks(kern, dev, sh.threads, smem, &per_sm) != K1_OK)
+                return cudaErrorInvalidValue;
+            grid = std::min<int64_t>(n_rows, (int64_t)sms * std::min(per_sm, kBwdBlocksPerSm));
             return launch(kern, grid, sh.threads, smem, st, p);
         });
     };

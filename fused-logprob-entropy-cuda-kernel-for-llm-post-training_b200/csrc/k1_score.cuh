@@ -34,13 +34,12 @@
 namespace k1 {
 namespace score {
 
-constexpr int U = 8;             // vectors per thread and chunk
 constexpr int kMaxGroups = 32;   // maxima per thread
+constexpr int kKeys = 256;       // maxima that the bound is found among
 constexpr int kCand = 1024;      // entries of the list
 constexpr int kMaxTop = 128;     // largest k
 constexpr int kMaxIds = 1024;    // given tokens per row
 constexpr int kMaxCluster = 8;
-static_assert(kMaxCluster * kMaxTop <= kCand, "the parts' lists meet in one");
 
 // Values at or below this count as masked (p = 0); 16-bit types: as the type rounds it.  pad: what
 // stands for elements outside the row.
@@ -268,18 +267,20 @@ __device__ __forceinline__ uint64_t entry_of(float x, int64_t e) {
 template <int TH>
 struct FwdSmem {
     static constexpr int W = TH / 32;
-    float wmax[W];
+    unsigned wmax[W];         // keys of the warps' maxima
     double wz[W], wt[W];
-    RowPartial part;          // this block's, read by the cluster's first block
-    int n_list, n_cand, n_sorted;
+    int n_cand;
     unsigned bound;           // T0's key, its upper 16 bits
-    unsigned prefix, need, above, scan[W];
-    uint64_t sorted[kMaxTop];
-    uint16_t keys[TH];
-    uint16_t list[kCand];
+    unsigned prefix, need, scan[W];
+    uint16_t keys[kKeys];
     unsigned hist[256];
     uint64_t cand[kCand];
-    float gmax[1];            // [groups][TH]
+};
+// Of a cluster's first block, written by all: their sums and their lists.
+struct Meet {
+    RowPartial part[kMaxCluster];
+    int n[kMaxCluster];
+    uint64_t list[kMaxCluster][kMaxTop];
 };
 
 // The block's list by exact selection: the kk-th largest key by histograms, what lies above it,
@@ -366,114 +367,134 @@ __device__ __noinline__ void select_exact(const Row<T>& row, int j0, int j1, int
     __syncthreads();
 }
 
-// The block's part of the list, sorted: sm.sorted[0, sm.n_sorted).
-template <typename T, int TH>
-__device__ __forceinline__ void select(const Row<T>& row, int j0, int j1, float thread_max, const FwdParams& p,
-                                       FwdSmem<TH>& sm) {
-    constexpr int E = DT<T>::kEPV;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // elements of the part
-    const int64_t first = max((int64_t)0, row.at(j0, 0)), last = min(row.vocab, row.at(j1, 0));
-    const int kk = (int)min((int64_t)p.k, max((int64_t)0, last - first));
-    sm.keys[tid] = thread_max > Floor<T>::value ? (uint16_t)(key_of(thread_max) >> 16) : (uint16_t)0;
-    if (tid == 0) sm.n_list = sm.n_cand = 0;
-    __syncthreads();
-    if (warp == 0) {
-        unsigned mine[TH / 32];
+// T0: a bound that kk of the threads' maxima reach and, to 16 bits, no more than their equals do (one
+// warp).
+template <int TH>
+__device__ __forceinline__ void find_bound(int kk, FwdSmem<TH>& sm) {
+    const int lane = threadIdx.x & 31;
+    unsigned mine[kKeys / 32], top = 0, low = 0xffffu;
 #pragma unroll
-        for (int i = 0; i < TH / 32; ++i) mine[i] = sm.keys[lane + 32 * i];
-        unsigned t = 0;
-#pragma unroll
-        for (int b = 15; b >= 0; --b) {
-            const unsigned cand = t | (1u << b);
+    for (int i = 0; i < kKeys / 32; ++i) {
+        mine[i] = sm.keys[lane + 32 * i];
+        top = max(top, mine[i]);
+        low = min(low, mine[i]);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    // bit by bit below the common prefix of all keys
+    unsigned t = top;
+    if (top != low) {
+        int b = 31 - __clz((int)(top ^ low));
+        t = top & ~((2u << b) - 1u);
+        for (; b >= 0; --b) {
+            const unsigned next = t | (1u << b);
             unsigned n = 0;
 #pragma unroll
-            for (int i = 0; i < TH / 32; ++i) n += mine[i] >= cand;
-            if (__reduce_add_sync(0xffffffffu, n) >= (unsigned)kk) t = cand;
+            for (int i = 0; i < kKeys / 32; ++i) n += mine[i] >= next;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (n >= (unsigned)kk) t = next;
+            if (n == (unsigned)kk) break;
         }
-        if (lane == 0) sm.bound = t;
     }
-    __syncthreads();
-    const unsigned bound = sm.bound;
+    if (lane == 0) sm.bound = t;
+}
+
+// The elements of the part that reach T0 go to sm.cand: their groups are read again, U lanes to a
+// group.  Every warp sees to its own threads' groups.
+template <typename T, int TH, int U>
+__device__ __forceinline__ void gather(const Row<T>& row, int j0, int j1, float thread_max, const FwdParams& p,
+                                       const float* gmax, unsigned bound, FwdSmem<TH>& sm) {
+    constexpr int E = DT<T>::kEPV;
+    const int tid = threadIdx.x, lane = tid & 31;
     const float t0 = value_of(bound << 16);
-    for (int g = 0; g < p.groups; ++g) {
-        if (bound == 0 || sm.gmax[g * TH + tid] >= t0) {
-            const int at = atomicAdd(&sm.n_list, 1);
-            if (at < kCand) sm.list[at] = (uint16_t)(g * TH + tid);
-        }
+    unsigned mine = 0;  // this thread's groups
+    if (bound == 0) {
+        mine = p.groups < 32 ? (1u << p.groups) - 1u : ~0u;
+    } else if (thread_max >= t0) {
+#pragma unroll 4
+        for (int g = 0; g < p.groups; ++g) mine |= (gmax[g * TH + tid] >= t0 ? 1u : 0u) << g;
     }
-    __syncthreads();
-    const int n_list = sm.n_list, per = p.group_chunks * U;
-    if (n_list <= kCand) {
-        for (int i = tid; i < n_list * per; i += TH) {
-            const int entry = sm.list[i / per], u = i % per;
-            const int j = j0 + (entry / TH * per + u) * TH + entry % TH;
-            if (j >= j1) continue;
-            uint4 v[1];
-            row.template load<1>(v, j, 0, j1);
-            float x[E];
-            unpack<T>(v[0], x);
+    unsigned any = __ballot_sync(0xffffffffu, mine != 0);
+    while (any) {
+        int of = -1, group = 0;
 #pragma unroll
-            for (int q = 0; q < E; ++q) {
-                const int64_t e = row.at(j, q);
-                if ((bound == 0 || x[q] >= t0) && row.inside(e)) {
-                    const int at = atomicAdd(&sm.n_cand, 1);
-                    if (at < kCand) sm.cand[at] = entry_of(x[q], e);
+        for (int s = 0; s < 32 / U; ++s) {
+            if (!any) break;
+            const int l = __ffs((int)any) - 1;
+            const unsigned m = __shfl_sync(0xffffffffu, mine, l);
+            if (lane == l) mine &= mine - 1;
+            if ((m & (m - 1)) == 0) any &= any - 1;
+            if (lane / U == s) {
+                of = l;
+                group = __ffs((int)m) - 1;
+            }
+        }
+        if (of >= 0) {
+            int j = j0 + (group * p.group_chunks * U + lane % U) * TH + (tid - lane) + of;
+            for (int c = 0; c < p.group_chunks && j < j1; ++c, j += U * TH) {
+                uint4 v[1];
+                row.template load<1>(v, j, 0, j1);
+                float x[E];
+                unpack<T>(v[0], x);
+                unsigned hit = 0;
+#pragma unroll
+                for (int q = 0; q < E; ++q) hit |= (bound == 0 || x[q] >= t0 ? 1u : 0u) << q;
+                if (j < row.lo || j >= row.hi)
+#pragma unroll
+                    for (int q = 0; q < E; ++q)
+                        if (!row.inside(row.at(j, q))) hit &= ~(1u << q);
+                if (hit) {
+                    int at = atomicAdd(&sm.n_cand, __popc(hit));
+#pragma unroll
+                    for (int q = 0; q < E; ++q)
+                        if (hit >> q & 1) {
+                            if (at < kCand) sm.cand[at] = entry_of(x[q], row.at(j, q));
+                            ++at;
+                        }
                 }
             }
         }
+        __syncwarp();
     }
-    __syncthreads();
-    if (n_list > kCand || sm.n_cand > kCand) {  // uniform
-        __syncthreads();
-        select_exact<T, TH>(row, j0, j1, kk, sm);
-    }
-    const int n = sm.n_cand;
-    for (int i = tid; i < n; i += TH) {
-        const uint64_t key = sm.cand[i];
-        int rank = 0;
-        for (int q = 0; q < n; ++q) rank += sm.cand[q] > key;
-        if (rank < kk) sm.sorted[rank] = key;
-    }
-    if (tid == 0) sm.n_sorted = kk;
-    __syncthreads();
 }
 
-// 32 or 64 bits of another block's shared memory.
-__device__ __forceinline__ uint64_t ld_cluster64(uint32_t addr) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
+// How many of n keys are larger.
+__device__ __forceinline__ int rank_among(const uint64_t* keys, int n, uint64_t key) {
+    int rank = 0;
+#pragma unroll 8
+    for (int q = 0; q < n; ++q) rank += keys[q] > key;
+    return rank;
 }
 
-template <typename T, int TH, bool TOP>
-__global__ void __launch_bounds__(TH, 768 / TH) k1_score_kernel(FwdParams p) {
+// Stores into another block's shared memory.
+__device__ __forceinline__ void st_cluster64(uint32_t addr, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+template <typename T, int TH, int U, int MINB, bool TOP>
+__global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char raw[];
     FwdSmem<TH>& sm = *reinterpret_cast<FwdSmem<TH>*>(raw);
+    Meet& meet = *reinterpret_cast<Meet*>(raw + sizeof(FwdSmem<TH>));  // only in a cluster
+    float* gmax = reinterpret_cast<float*>(raw + sizeof(FwdSmem<TH>) + (p.cluster > 1 ? sizeof(Meet) : 0));  // [groups][TH]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = p.cluster > 1 ? (int)ring::cluster_rank() : 0;
     const int64_t r = p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
+    if (p.cluster > 1) ring::cluster_arrive();
     pdl_wait();
     pdl_trigger();
     const Row<T> row(reinterpret_cast<const T*>(p.logits) + p.lay.offset(r), p.vocab);
     const int j0 = min(row.n, rank * p.slice), j1 = min(row.n, j0 + p.slice);
     const float c = p.scale * kLog2e;
 
-    // the given tokens' logits, in flight with the first chunk
-    int64_t id = -1;
-    float xid = 0.f;
-    if (rank == 0 && tid < p.n_ids) {
-        id = p.ids[r * p.n_ids + tid];
-        if (row.inside(id)) xid = DT<T>::load1(row.p + id);
-    }
+    const int64_t id = rank == 0 && tid < p.n_ids ? p.ids[r * p.n_ids + tid] : -1;
 
     State st;
     st.init();
+    float odd = -INFINITY;  // the maximum of the groups of odd number, where threads give two keys
     {
         int g = 0, left = p.group_chunks;
         float gm = -INFINITY;
@@ -489,27 +510,43 @@ __global__ void __launch_bounds__(TH, 768 / TH) k1_score_kernel(FwdParams p) {
             if constexpr (TOP) {
                 gm = fmax_nan(gm, mc);
                 if (--left == 0 || j + U * TH >= j1) {
-                    sm.gmax[g * TH + tid] = gm;
+                    gmax[g * TH + tid] = gm;
+                    if (TH < kKeys && (g & 1)) odd = fmax_nan(odd, gm);
                     ++g;
                     left = p.group_chunks;
                     gm = -INFINITY;
                 }
             }
         }
-        if constexpr (TOP)
-            for (; g < p.groups; ++g) sm.gmax[g * TH + tid] = -INFINITY;
+        if constexpr (TOP) {
+            for (; g < p.groups; ++g) gmax[g * TH + tid] = -INFINITY;
+            auto key16 = [](float m) { return m > Floor<T>::value ? (uint16_t)(key_of(m) >> 16) : (uint16_t)0; };
+            if constexpr (TH < kKeys) {
+                float even = -INFINITY;
+                for (int q = 0; q < p.groups; q += 2) even = fmax_nan(even, gmax[q * TH + tid]);
+                sm.keys[tid] = key16(even);
+                sm.keys[TH + tid] = key16(odd);
+            } else {
+                sm.keys[tid] = key16(st.m);
+            }
+        }
     }
 
-    // the block's sums, relative to its maximum
+    // the given token's logit, in flight until the row's values are written
+    const float xid = row.inside(id) ? DT<T>::load1(row.p + id) : 0.f;
+
+    // the block's sums, relative to its maximum; one warp looks for the bound meanwhile
     const bool empty = st.m <= Floor<T>::value;
-    const float wm = warp_max_nan(empty ? -INFINITY : st.m);
+    const unsigned wm = __reduce_max_sync(0xffffffffu, key_of(empty ? -INFINITY : st.m));
     if (lane == 0) sm.wmax[warp] = wm;
+    if (TOP && tid == 0) sm.n_cand = 0;
     __syncthreads();
     RowPartial part;
-    part.m = sm.wmax[0];
-#pragma unroll
-    for (int i = 1; i < TH / 32; ++i) part.m = fmax_nan(part.m, sm.wmax[i]);
     {
+        unsigned m = sm.wmax[0];
+#pragma unroll
+        for (int i = 1; i < TH / 32; ++i) m = max(m, sm.wmax[i]);
+        part.m = value_of(m);
         double z = 0.0, t = 0.0;
         if (!empty) {
             const float dm = st.m - part.m;
@@ -524,6 +561,11 @@ __global__ void __launch_bounds__(TH, 768 / TH) k1_score_kernel(FwdParams p) {
             sm.wt[warp] = t;
         }
     }
+    // elements of the part, and the entries wanted of it
+    const int64_t elements = max((int64_t)0, min(row.vocab, row.at(j1, 0)) - max((int64_t)0, row.at(j0, 0)));
+    const int kk = (int)min((int64_t)p.k, elements);
+    if constexpr (TOP)
+        if (warp == 0) find_bound<TH>(kk, sm);
     __syncthreads();
     part.z = part.t = 0.0;
 #pragma unroll
@@ -532,90 +574,108 @@ __global__ void __launch_bounds__(TH, 768 / TH) k1_score_kernel(FwdParams p) {
         part.t += sm.wt[i];
     }
     part.pad = 0.f;
-    // NaN somewhere: no list either (a part's list must not hold what cannot be ordered)
+    // a NaN or +inf somewhere: no list either, what cannot be ordered must not reach one
     const bool sound = part.m < INFINITY;
+    const double s = (double)p.scale;
+    double l = s * (double)part.m + (p.cluster > 1 ? 0.0 : log(part.z));
+    int n = 0;
     if constexpr (TOP) {
-        if (sound)
-            select<T, TH>(row, j0, j1, st.m, p, sm);
-        else if (tid == 0)
-            sm.n_sorted = 0;
-    }
-
-    if (p.cluster > 1) {
-        if (tid == 0) sm.part = part;
-        ring::cluster_sync();
-        if (rank == 0) {
-            float M = part.m;
-            for (int q = 1; q < p.cluster; ++q)
-                M = fmax_nan(M, __uint_as_float(ld_cluster32(ring::mapa(ring::saddr(&sm.part.m), q))));
-            double z = 0.0, t = 0.0;
-            for (int q = 0; q < p.cluster; ++q) {
-                const float m = __uint_as_float(ld_cluster32(ring::mapa(ring::saddr(&sm.part.m), q)));
-                const double zq = __longlong_as_double((long long)ld_cluster64(ring::mapa(ring::saddr(&sm.part.z), q)));
-                const double tq = __longlong_as_double((long long)ld_cluster64(ring::mapa(ring::saddr(&sm.part.t), q)));
-                if (m != -INFINITY) {
-                    const float dm = m - M;
-                    const double f = dm == 0.f ? 1.f : ex2(dm * c);
-                    z += f * zq;
-                    t += f * tq + f * (double)dm * zq;
-                }
-            }
-            part.m = M;
-            part.z = z;
-            part.t = t;
-            if constexpr (TOP) {
-                // the parts' lists side by side, then every entry's place in all of them
-                int total = 0;
-                for (int q = 0; q < p.cluster; ++q) {
-                    const int n = (int)ld_cluster32(ring::mapa(ring::saddr(&sm.n_sorted), q));
-                    for (int i = tid; i < n; i += TH)
-                        sm.cand[q * kMaxTop + i] = ld_cluster64(ring::mapa(ring::saddr(&sm.sorted[i]), q));
-                    if (tid == 0) sm.hist[q] = (unsigned)n;
-                    total += n;
-                }
+        if (sound && kk > 0) {
+            const unsigned bound = sm.bound;
+            const bool all = bound == 0 && elements > kCand;
+            if (!all) gather<T, TH, U>(row, j0, j1, st.m, p, gmax, bound, sm);
+            __syncthreads();
+            n = sm.n_cand;
+            if (all || n > kCand) {  // uniform
                 __syncthreads();
-                for (int i = tid; i < p.cluster * kMaxTop; i += TH) {
-                    const int q = i / kMaxTop, at = i % kMaxTop;
-                    if (at >= (int)sm.hist[q]) continue;
-                    const uint64_t key = sm.cand[i];
-                    int place = at;
-                    for (int o = 0; o < p.cluster && place < p.k; ++o) {
-                        if (o == q) continue;
-                        int lo = 0, hi = (int)sm.hist[o];  // entries of list o before this one
-                        while (lo < hi) {
-                            const int mid = (lo + hi) >> 1;
-                            if (sm.cand[o * kMaxTop + mid] > key)
-                                lo = mid + 1;
-                            else
-                                hi = mid;
-                        }
-                        place += lo;
-                    }
-                    if (place < p.k) sm.sorted[place] = key;
-                }
-                __syncthreads();
+                select_exact<T, TH>(row, j0, j1, kk, sm);
+                n = kk;
             }
         }
-        ring::cluster_sync();  // no block leaves while its shared memory may be read
+    }
+
+    auto emit = [&](int place, uint64_t key) {
+        p.top_ids[r * p.k + place] = (int64_t)(uint32_t)~(uint32_t)key;
+        p.top_logprobs[r * p.k + place] = (float)(s * (double)value_of((uint32_t)(key >> 32)) - l);
+    };
+    if (p.cluster == 1) {
+        if constexpr (TOP)
+            for (int i = tid; i < n; i += TH) {
+                const uint64_t key = sm.cand[i];
+                const int place = rank_among(sm.cand, n, key);
+                if (place < kk) emit(place, key);
+            }
+    } else {
+        // every block writes its sums and its list, sorted, into the first one's shared memory
+        ring::cluster_wait();  // which runs by now
+        const uint32_t to = ring::mapa(ring::saddr(&meet), 0);
+        const uint32_t base = ring::saddr(&meet);
+        if constexpr (TOP)
+            for (int i = tid; i < n; i += TH) {
+                const uint64_t key = sm.cand[i];
+                const int place = rank_among(sm.cand, n, key);
+                if (place < kk) st_cluster64(to + (ring::saddr(&meet.list[rank][place]) - base), key);
+            }
+        if (tid == 0) {
+            st_cluster64(to + (ring::saddr(&meet.part[rank].z) - base), (uint64_t)__double_as_longlong(part.z));
+            st_cluster64(to + (ring::saddr(&meet.part[rank].t) - base), (uint64_t)__double_as_longlong(part.t));
+            st_cluster32(to + (ring::saddr(&meet.part[rank].m) - base), __float_as_uint(part.m));
+            st_cluster32(to + (ring::saddr(&meet.n[rank]) - base), sound ? (uint32_t)kk : 0u);
+        }
+        ring::cluster_sync();
         if (rank != 0) return;
+        float M = meet.part[0].m;
+        int total = meet.n[0];
+        for (int q = 1; q < p.cluster; ++q) {
+            M = fmax_nan(M, meet.part[q].m);
+            total += meet.n[q];
+        }
+        part.z = part.t = 0.0;
+        for (int q = 0; q < p.cluster; ++q) {
+            const float m = meet.part[q].m;
+            if (m != -INFINITY) {
+                const float dm = m - M;
+                const double f = dm == 0.f ? 1.f : ex2(dm * c);
+                part.z += f * meet.part[q].z;
+                part.t += f * meet.part[q].t + f * (double)dm * meet.part[q].z;
+            }
+        }
+        part.m = M;
+        l = s * (double)M + log(part.z);
+        if constexpr (TOP) {
+            if (M < INFINITY)
+                for (int i = tid; i < p.cluster * p.k; i += TH) {
+                    const int q = i / p.k, at = i - q * p.k;
+                    if (at >= meet.n[q]) continue;
+                    const uint64_t key = meet.list[q][at];
+                    int place = 0;
+                    for (int o = 0; o < p.cluster; ++o) {
+                        // entries of list o before this one: counted, or by bisection of long lists
+                        if (p.k <= 32) {
+                            place += rank_among(meet.list[o], meet.n[o], key);
+                        } else {
+                            int lo = 0, hi = meet.n[o];
+                            while (lo < hi) {
+                                const int mid = (lo + hi) >> 1;
+                                if (meet.list[o][mid] > key)
+                                    lo = mid + 1;
+                                else
+                                    hi = mid;
+                            }
+                            place += lo;
+                        }
+                    }
+                    if (place < p.k) emit(place, key);
+                }
+        }
     }
 
     // the row's values
-    const double s = (double)p.scale;
     const bool none = part.m == -INFINITY;  // nothing above the floor
-    double l, h;
-    if (none) {
-        l = -INFINITY;
-        h = NAN;
-    } else {
-        const double lz = log(part.z);
-        l = s * (double)part.m + lz;
-        h = lz - s * part.t / part.z;
-    }
     const bool fine = !none && part.m < INFINITY && l - l == 0.0;
     if (tid == 0) {
-        p.lse[r] = fine || none ? (float)l : NAN;
-        p.entropy[r] = fine ? (float)h : NAN;
+        p.lse[r] = fine ? (float)l : none ? -INFINITY : NAN;
+        p.entropy[r] = fine ? (float)(l - s * (double)part.m - s * part.t / part.z) : NAN;
     }
     if (tid < p.n_ids) p.logprobs[r * p.n_ids + tid] = fine ? (float)(s * (double)xid - l) : NAN;
     for (int i = tid + TH; i < p.n_ids; i += TH) {
@@ -624,10 +684,11 @@ __global__ void __launch_bounds__(TH, 768 / TH) k1_score_kernel(FwdParams p) {
         p.logprobs[r * p.n_ids + i] = fine ? (float)(s * (double)x - l) : NAN;
     }
     if constexpr (TOP) {
+        if (fine) return;
+        __syncthreads();  // in place of what the block may have written
         for (int i = tid; i < p.k; i += TH) {
-            const uint64_t key = fine ? sm.sorted[i] : 0;
-            p.top_ids[r * p.k + i] = fine ? (int64_t)(uint32_t)~(uint32_t)key : -1;
-            p.top_logprobs[r * p.k + i] = fine ? (float)(s * (double)value_of((uint32_t)(key >> 32)) - l) : NAN;
+            p.top_ids[r * p.k + i] = -1;
+            p.top_logprobs[r * p.k + i] = NAN;
         }
     }
 }

@@ -40,7 +40,7 @@ int score_check(const char* fn, const void* logits, int dtype, int64_t n_rows, i
     return K1_OK;
 }
 
-template <typename T, int TH, bool TOP>
+template <typename T, int TH, int U, int MINB, bool TOP>
 int score_launch(const char* fn, k1::score::FwdParams p, int64_t n_rows, int sms, int dev, cudaStream_t st) {
     using namespace k1::score;
     constexpr int E = k1::DT<T>::kEPV;
@@ -53,8 +53,8 @@ int score_launch(const char* fn, k1::score::FwdParams p, int64_t n_rows, int sms
     const int chunks = (p.slice + chunk - 1) / chunk;
     p.group_chunks = (chunks + kMaxGroups - 1) / kMaxGroups;
     p.groups = (chunks + p.group_chunks - 1) / p.group_chunks;
-    auto kern = k1_score_kernel<T, TH, TOP>;
-    const size_t smem = sizeof(FwdSmem<TH>) + (TOP ? (size_t)p.groups * TH * 4 : 0);
+    auto kern = k1_score_kernel<T, TH, U, MINB, TOP>;
+    const size_t smem = sizeof(FwdSmem<TH>) + (cluster > 1 ? sizeof(Meet) : 0) + (TOP ? (size_t)p.groups * TH * 4 : 0);
     int rc = allow_smem(kern, dev, smem);
     if (rc) return rc;
     return launched(fn, launch_cluster(kern, dim3((unsigned)(n_rows * cluster)), TH, smem, cluster, st, p));
@@ -62,8 +62,9 @@ int score_launch(const char* fn, k1::score::FwdParams p, int64_t n_rows, int sms
 
 template <typename T>
 int score_forward(const char* fn, const k1::score::FwdParams& p, int64_t n_rows, int sms, int dev, cudaStream_t st) {
-    return p.k > 0 ? score_launch<T, 256, true>(fn, p, n_rows, sms, dev, st)
-                   : score_launch<T, 256, false>(fn, p, n_rows, sms, dev, st);
+    if (p.k == 0) return score_launch<T, 256, 8, 3, false>(fn, p, n_rows, sms, dev, st);
+    return n_rows >= 6 * sms ? score_launch<T, 128, 4, 8, true>(fn, p, n_rows, sms, dev, st)
+                             : score_launch<T, 256, 4, 4, true>(fn, p, n_rows, sms, dev, st);
 }
 
 template <typename T>
