@@ -822,6 +822,8 @@ int k1_ring_status(unsigned* out) {
     unsigned more = 0;
     if (e == cudaSuccess) e = k1_decode_wait_status(&more);
     v |= more;
+    if (e == cudaSuccess) e = k1_sandwich_wait_status(&more);
+    v |= more;
     if (e != cudaSuccess) return fail(K1_ERR_CUDA, "k1_ring_status: %s", cudaGetErrorString(e));
     if (out) *out = v;
     return K1_OK;
@@ -1188,12 +1190,14 @@ int k1_lm_head_shard_backward(const void* hidden, const void* weight_shard, int6
 // Only in the wait-timeout test library (built with -DK1_WAIT_TEST and short wait limits;
 // not part of libk1_b200.so): sets the knobs that make one block's bounded waits run out
 // on the current device.  withhold: the backward ring's block 0, and the LM head's CTA 0,
-// issue no bulk copy from that copy number on; skip_grab: the one-block-per-SM forward's
+// issue no bulk copy from that copy number on (the sandwich norm's block 0 none for its groups' rows
+// from that number on); skip_grab: the one-block-per-SM forward's
 // block 0 drops that grab.  -1 turns a knob off.
 int k1_test_set_knobs(long long withhold, long long skip_grab) {
     cudaError_t e = cudaMemcpyToSymbol(k1::k1_test_withhold, &withhold, sizeof withhold);
     if (e == cudaSuccess) e = cudaMemcpyToSymbol(k1::k1_test_skip_grab, &skip_grab, sizeof skip_grab);
     if (e == cudaSuccess) e = k1_decode_set_withhold(withhold);
+    if (e == cudaSuccess) e = k1_sandwich_set_withhold(withhold);
     if (e != cudaSuccess) return fail(K1_ERR_CUDA, "k1_test_set_knobs: %s", cudaGetErrorString(e));
     return K1_OK;
 }

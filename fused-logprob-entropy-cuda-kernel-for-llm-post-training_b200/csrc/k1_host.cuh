@@ -19,10 +19,12 @@
 // Not part of the C ABI: one definition (k1_capi.cu) for all translation units.
 #define K1_INTERNAL __attribute__((visibility("hidden")))
 K1_INTERNAL int k1_host_fail(int code, const char* message);
-// The wait status word and test knobs of k1_decode_capi.cu's kernels.
+// The wait status word and test knobs of the other translation units' kernels.
 K1_INTERNAL cudaError_t k1_decode_wait_status(unsigned* bits);
+K1_INTERNAL cudaError_t k1_sandwich_wait_status(unsigned* bits);
 #ifdef K1_WAIT_TEST
 K1_INTERNAL cudaError_t k1_decode_set_withhold(long long withhold);
+K1_INTERNAL cudaError_t k1_sandwich_set_withhold(long long withhold);
 #endif
 
 namespace {

@@ -18,6 +18,7 @@
 #pragma once
 
 #include "k1_norm.cuh"
+#include "k1_sync.cuh"
 
 namespace k1 {
 namespace norm {
@@ -35,8 +36,8 @@ struct SandwichBwdParams {
     void* dx;        // outputs that are NULL are not wanted
     void* dr;
     void* dgate;     // per row or per element; per column it is a partial sum
-    float* sums;     // [3][gridDim.x][h]: dw, dwp, dgate per column; NULL: none is wanted
-    int want;        // bits: 1 dw, 2 dwp, 4 dgate per column
+    float* sums;     // [2][gridDim.x][h]: dw, and what dwp and a column gate's are multiples of
+    int want;        // bits: 1 dw, 2 dwp, 4 dgate per column; 0: sums is NULL
     int64_t n, gy_stride, gs_stride, s_stride, x_stride, gate_stride;
     int h, w32, gate_kind;
     float branch_scale, residual_scale;
@@ -86,11 +87,11 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
     constexpr bool EARLY = E * NV <= (E >= 4 ? 16 : 4);
     __shared__ float scratch[2][32];
     __shared__ float2 scratch2[2][32];
-    extern __shared__ __align__(16) float sums[];  // [3][h]
+    extern __shared__ __align__(16) float sums[];  // [2][h]
     pdl_wait();
     pdl_trigger();
     const int threads = blockDim.x, tid = threadIdx.x, h = p.h;
-    for (int i = tid; i < 3 * h; i += threads) sums[i] = 0.f;
+    for (int i = tid; i < 2 * h; i += threads) sums[i] = 0.f;
     __syncthreads();
     int flip = 0;
     for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x, flip ^= 1) {
@@ -183,14 +184,12 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
                 a[i] *= p.branch_scale;
                 b[i] *= r1;
                 e[i] = a[i] * b[i] * w[i];          // dgate
-                a[i] *= gate[i];
-                t[j][i] = a[i] * w[i];
-                a[i] *= b[i];                       // dwp
+                t[j][i] = a[i] * gate[i] * w[i];
+                a[i] *= p.gate_kind == GATE_COLUMN ? b[i] : gate[i] * b[i];
                 dots.x = fmaf(t[j][i], b[i], dots.x);
                 dots.y += e[i];
             }
-            if (p.want & 2) add_to<E>(sums + h + col, a);
-            if (p.want & 4) add_to<E>(sums + 2 * h + col, e);
+            if (p.want & 6) add_to<E>(sums + h + col, a);
             if (p.dgate && p.gate_kind == GATE_FULL) {
                 P o;
                 o.set(e);
@@ -220,23 +219,587 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
     }
     if (p.sums) {
         __syncthreads();
-        for (int k = 0; k < 3; ++k) {
-            if (!(p.want >> k & 1)) continue;
+        for (int k = 0; k < 2; ++k) {
+            if (!(p.want & (k == 0 ? 1 : 6))) continue;
             float* out = p.sums + ((int64_t)k * gridDim.x + blockIdx.x) * h;
             for (int i = tid; i < h; i += threads) out[i] = sums[k * h + i];
         }
     }
 }
 
-// The blocks' partial sums of dw, dwp and dgate (blockIdx.y), added in a fixed order as in
-// k1_rmsnorm_dw_kernel.
-template <typename W>
-__global__ void __launch_bounds__(512) k1_sandwich_dw_kernel(const float* part, int parts, int h, W* dw, W* dwp, W* dg) {
-    __shared__ float sums[16][33];
-    W* out = blockIdx.y == 0 ? dw : blockIdx.y == 1 ? dwp : dg;
+// ------------------------------------------------------------------------------------
+// Rows of vectors, many of them: loads by bulk copies
+// ------------------------------------------------------------------------------------
+// The kernels above and in k1_norm.cuh load a row, reduce it twice and store it, and nothing is in flight
+// meanwhile but other blocks' loads, of which registers allow two or three blocks per SM (75 us
+// forward and 128 backward at 8192 x 3584 bf16; the bytes alone take 36 and 55).  Here a block is a few
+// groups of threads, each with rows and a ring of stages of its own: a stage holds one row of every
+// input, a bulk copy each, counted on the stage's mbarrier.  When a group has read a stage (which the
+// row's second reduction, a barrier of the group, tells), one thread orders the group's next row
+// into it.  So 100 KB and more per SM are in flight whatever the groups wait for.  A thread has the
+// columns that it would have in the other kernels and sums in the same order, so results are the
+// same bits.  Sums over rows stay in registers and are added over the groups, in their order, at
+// the end.  Backward the weights are in shared memory too, as fp32, so that registers serve three
+// groups.
+//
+// Every wait is bounded; one that runs out sets bit 0 of the wait status word, the group's rows from
+// there on are NaN, and a block leaves only when the copies that it ordered have landed.
+struct Ring {
+    int groups, threads;  // groups per block, threads per group
+    int e, nv;            // elements of a vector, vectors per thread
+    int stages;           // per group
+    int slot;             // bytes of one input's row in a stage (a multiple of 128)
+    int inputs;           // of the stage
+};
+
+constexpr int kMaxRingGroups = 15;  // a named barrier each
+constexpr int kMaxRingStages = 4;
+// Threads of a block: what registers allow (a thread holds E NV columns, and backward 2 E NV sums).
+template <int E, int NV>
+constexpr int kRingFwd = E * NV >= 16 ? 512 : 960;
+template <int E, int NV>
+constexpr int kRingBwd = E * NV >= 16 ? 512 : 896;
+
+struct RingSmem {
+    uint64_t full[kMaxRingGroups * kMaxRingStages];
+    float scratch[kMaxRingGroups][2][16];
+};
+// weights: fp32 ones kept beside the rings.
+constexpr size_t ring_smem(const Ring& q, int weights) {
+    return sizeof(RingSmem) + 128 + (size_t)q.groups * q.stages * q.slot * q.inputs +
+           (size_t)weights * q.threads * q.nv * q.e * 4;
+}
+
+// 16 bytes of shared memory by address (addresses of 32 bits: generic pointers would cost these
+// kernels a fifth of their instructions).
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// One group's view of its ring (shared-memory addresses).
+struct RingGroup {
+    uint32_t rings;    // all groups' stages
+    uint32_t stages;   // this group's
+    uint32_t full;
+    uint32_t scratch;
+    int t, id, stage_bytes, slots;
+    int at;            // the current row's stage, and
+    uint32_t parity;   // the parity of its use
+    int failed;        // the row whose wait ran out
+    bool ok;
+    __device__ __forceinline__ void init(unsigned char* raw, const Ring& q) {
+        RingSmem* sm = reinterpret_cast<RingSmem*>(raw);
+        rings = (ring::saddr(raw) + (uint32_t)sizeof(RingSmem) + 127u) & ~127u;
+        id = threadIdx.x / q.threads;
+        t = threadIdx.x - id * q.threads;
+        slots = q.stages;
+        stage_bytes = q.slot * q.inputs;
+        stages = rings + id * slots * stage_bytes;
+        full = ring::saddr(sm->full + id * slots);
+        scratch = ring::saddr(sm->scratch[id][0]);
+        at = 0;
+        parity = 0;
+        failed = 0;
+        ok = true;
+        for (int i = threadIdx.x; i < kMaxRingGroups * 32; i += blockDim.x) sm->scratch[0][0][i] = 0.f;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < q.groups * slots; ++i) ring::bar_init(&sm->full[i], 1);
+            ring::fence_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ bool wait_for(int slot, uint32_t parity_) const {
+        for (int i = 0; i < ring::kMaxTries; ++i)
+            if (ring::try_wait_at(full + slot * 8, parity_)) return true;
+        atomicOr(&k1_ring_error, 1u);
+        return false;
+    }
+    // The current stage holds row i of the group (or the wait ran out, now or before).
+    __device__ __forceinline__ uint32_t wait(int i) {
+        if (ok && !(ok = wait_for(at, parity))) failed = i;
+        return stages + at * stage_bytes;
+    }
+    __device__ __forceinline__ void next() {
+        if (++at == slots) {
+            at = 0;
+            parity ^= 1u;
+        }
+    }
+    // The thread that orders, before it leaves: the copies that it has not seen land.
+    __device__ __forceinline__ void drain(int rows) const {
+        if (ok) return;
+        for (int i = failed; i < min(rows, failed + slots); ++i) wait_for(i % slots, (uint32_t)(i / slots) & 1u);
+    }
+    // The sum over the group (what lies behind the last warp is 0).  Two buffers: `second` is the
+    // caller's second sum of a row.
+    __device__ __forceinline__ float sum(float v, int threads, bool second) const {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        const uint32_t to = scratch + (second ? 64 : 0);
+        if ((t & 31) == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (t >> 5) * 4), "f"(v) : "memory");
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + id), "r"(threads) : "memory");
+        auto four = [&](uint32_t from) {
+            const uint4 a = lds16(from), b = lds16(from + 16);
+            return add2(add2(make_float2(__uint_as_float(a.x), __uint_as_float(a.y)),
+                             make_float2(__uint_as_float(a.z), __uint_as_float(a.w))),
+                        add2(make_float2(__uint_as_float(b.x), __uint_as_float(b.y)),
+                             make_float2(__uint_as_float(b.z), __uint_as_float(b.w))));
+        };
+        float2 s = four(to);
+        if (threads > 256) s = add2(s, four(to + 32));
+        return s.x + s.y;
+    }
+};
+
+// Orders row i of the group, of every input that is not NULL, into a stage.
+template <int N>
+__device__ __forceinline__ void order_row(const RingGroup& g, const Ring& q, int i, int stage,
+                                          const void* const (&rows)[N], int bytes) {
+#ifdef K1_WAIT_TEST
+    if (blockIdx.x == 0 && k1_test_withhold >= 0 && i >= k1_test_withhold) return;  // test only
+#endif
+    const uint32_t bar = g.full + stage * 8;
+    uint32_t to = g.stages + stage * g.stage_bytes;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(q.inputs * bytes) : "memory");
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (rows[k]) {
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                         "l"(rows[k]), "r"(bytes), "r"(bar)
+                         : "memory");
+            to += q.slot;
+        }
+}
+
+// Vectors as pairs of fp32 numbers: instructions per element are what these kernels run out of first.
+template <typename T>
+struct Vec {
+    static constexpr int E = DT<T>::kEPV, N = E / 2;
+    __device__ static __forceinline__ uint4 at(uint32_t p) { return lds16(p); }
+    __device__ static __forceinline__ void get(uint4 v, float2 (&f)[N]) {
+        if constexpr (sizeof(T) == 4) {
+            f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+            f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+        } else {
+            f[0] = DT<T>::to_f2(v.x);
+            f[1] = DT<T>::to_f2(v.y);
+            f[2 % N] = DT<T>::to_f2(v.z);
+            f[3 % N] = DT<T>::to_f2(v.w);
+        }
+    }
+    __device__ static __forceinline__ uint4 put(const float2 (&f)[N]) {
+        if constexpr (sizeof(T) == 4)
+            return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
+                              __float_as_uint(f[1].y));
+        else
+            return make_uint4(DT<T>::from_f2(f[0]), DT<T>::from_f2(f[1]), DT<T>::from_f2(f[2 % N]),
+                              DT<T>::from_f2(f[3 % N]));
+    }
+};
+
+// A thread's columns of a weight as fp32 pairs (0 beyond the last column).
+template <typename T, int NV, int N>
+__device__ __forceinline__ void hold_weight(const void* w, bool w32, int t, int threads, int h, float2 (&f)[NV][N]) {
+    constexpr int E = 2 * N;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (j * threads + t) * E;
+        float v[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = 0.f;
+        if (col < h) load_weight<T, E>(w, w32, col, v);
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[j][k] = make_float2(v[2 * k], v[2 * k + 1]);
+    }
+}
+
+template <typename T, int NV, int OUT>
+__global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring_kernel(FwdParams p, Ring q) {
+    using V = Vec<T>;
+    constexpr int E = V::E, N = V::N;
+    extern __shared__ __align__(16) unsigned char raw[];
+    RingGroup g;
+    g.init(raw, q);
     pdl_wait();
     pdl_trigger();
-    if (!out) return;
+    const int t = g.t, threads = q.threads, h = p.h, bytes = h * (int)sizeof(T);
+    const int64_t step = (int64_t)gridDim.x * q.groups, first = (int64_t)blockIdx.x * q.groups + g.id;
+    const int rows = first < p.n ? (int)((p.n - 1 - first) / step + 1) : 0;
+    const int n_blocks = (h + kFp8Block - 1) / kFp8Block;
+    const T* gates = p.gate_kind == GATE_FULL ? reinterpret_cast<const T*>(p.gate) : nullptr;
+    auto order = [&](int i, int stage) {
+        const int64_t row = first + i * step;
+        const void* from[3] = {reinterpret_cast<const T*>(p.x) + row * p.x_stride,
+                               reinterpret_cast<const T*>(p.r) + row * p.r_stride,
+                               gates ? gates + row * p.gate_stride : nullptr};
+        order_row(g, q, i, stage, from, bytes);
+    };
+    if (t == 0)
+        for (int i = 0; i < min(rows, q.stages); ++i) order(i, i);
+    // the thread's columns of the weight, and of post_weight times branch_scale and a gate per column
+    float2 w[NV][N], wg[NV][N];
+    hold_weight<T, NV, N>(p.w, p.w32, t, threads, h, w);
+    hold_weight<T, NV, N>(p.wp, p.w32, t, threads, h, wg);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < N; ++k) wg[j][k] = mul2(wg[j][k], splat(p.branch_scale));
+    if (p.gate_kind == GATE_COLUMN) {
+        float2 c[NV][N];
+        hold_weight<T, NV, N>(p.gate, p.w32, t, threads, h, c);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int k = 0; k < N; ++k) wg[j][k] = mul2(wg[j][k], c[j][k]);
+    }
+    const float2 rs = splat(p.residual_scale);
+    const float inv_h = 1.f / (float)h;
+    // a row's gate is loaded while the row before it is worked on
+    auto gate_of = [&](int i) {
+        return p.gate_kind == GATE_TOKEN && i < rows
+                   ? DT<T>::load1(reinterpret_cast<const T*>(p.gate) + (first + i * step) * p.gate_stride) : 1.f;
+    };
+    float token_next = gate_of(0);
+    int64_t at_row = first * h + t * E;  // the thread's place in the outputs
+    for (int i = 0; i < rows; ++i, g.next(), at_row += step * h) {
+        const int64_t row = first + i * step;
+        const float token = token_next;
+        token_next = gate_of(i + 1);
+        const uint32_t in = g.wait(i) + t * 16;
+        float2 x[NV][N], two = splat(0.f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if ((j * threads + t) * E >= h) break;
+            V::get(V::at(in + j * threads * 16), x[j]);
+#pragma unroll
+            for (int k = 0; k < N; ++k) two = fma2(x[j][k], x[j][k], two);
+        }
+        float sum = g.sum(two.x + two.y, threads, false);
+        const float r1 = g.ok ? rsqrtf(fmaf(sum, inv_h, p.eps)) : __int_as_float(0x7fc00000);
+        if (p.rstd_post && t == 0) p.rstd_post[row] = r1;
+        const float2 k1 = splat(r1 * token);
+        two = splat(0.f);
+        T* so = reinterpret_cast<T*>(p.s) + at_row;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (j * threads + t) * E;
+            if (col >= h) break;
+            const uint32_t at = in + j * threads * 16;
+            float2 b[N];
+            V::get(V::at(at + q.slot), b);
+            if (gates) {
+                float2 c[N];
+                V::get(V::at(at + 2 * q.slot), c);
+#pragma unroll
+                for (int k = 0; k < N; ++k) x[j][k] = mul2(x[j][k], c[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) x[j][k] = fma2(mul2(x[j][k], k1), wg[j][k], mul2(b[k], rs));
+            const uint4 s = V::put(x[j]);
+            stg_stream(so + j * threads * E, s);
+            V::get(s, x[j]);  // the stream as stored
+#pragma unroll
+            for (int k = 0; k < N; ++k) two = fma2(x[j][k], x[j][k], two);
+        }
+        sum = g.sum(two.x + two.y, threads, true);  // after it nobody reads the stage
+        if (t == 0 && g.ok && i + q.stages < rows) order(i + q.stages, g.at);
+        const float r2 = rsqrtf(fmaf(sum, inv_h, p.eps));
+        if (p.rstd && t == 0) p.rstd[row] = r2;
+        if constexpr (OUT == SAME) {
+            T* y = reinterpret_cast<T*>(p.y) + at_row;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int col = (j * threads + t) * E;
+                if (col >= h) break;
+#pragma unroll
+                for (int k = 0; k < N; ++k) x[j][k] = mul2(mul2(x[j][k], splat(r2)), w[j][k]);
+                stg_stream(y + j * threads * E, V::put(x[j]));
+            }
+        } else {
+            // as in k1_rmsnorm_kernel, which has the reasons
+            const uint32_t bits = __float_as_uint(r2);
+            const float unit = 0.875f * (r2 == r2 ? __uint_as_float(bits & 0x7f800000u) : r2);
+            const float rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) * (8.f / 7.f);
+            const float least = kAmaxFloor / rest;
+            constexpr int LANES = kFp8Block / E;
+            uint8_t* y = reinterpret_cast<uint8_t*>(p.y) + at_row;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int col = (j * threads + t) * E;
+                float2 (&a)[N] = x[j];
+                float m = 0.f;
+                if (col < h) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        a[k] = mul2(mul2(a[k], splat(unit)), w[j][k]);
+                        m = fmax_nan(m, fmax_nan(fabsf(a[k].x), fabsf(a[k].y)));
+                    }
+                }
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                if (col < h) {
+                    m = fmax_nan(m, least);
+                    const float d = m / kFp8Max;
+                    const Quotient to(d);
+                    uint32_t v[N];
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {  // Quotient's steps, in pairs
+                        const float2 c = mul2(a[k], splat(to.inv));
+                        const float2 e = fma2(fma2(make_float2(-c.x, -c.y), splat(to.step), a[k]), splat(to.inv), c);
+                        v[k] = e4m3x2(e.x, e.y);
+                    }
+                    if constexpr (E == 8)
+                        *reinterpret_cast<uint2*>(y + j * threads * E) =
+                            make_uint2(v[0] | (v[1] << 16), v[2 % N] | (v[3 % N] << 16));
+                    else
+                        *reinterpret_cast<uint32_t*>(y + j * threads * E) = v[0] | (v[1] << 16);
+                    if ((t & (LANES - 1)) == 0) p.scales[row * n_blocks + col / kFp8Block] = d * rest;
+                }
+            }
+        }
+    }
+    if (t == 0) g.drain(rows);
+}
+
+// Per row and column: ds as in the header; with m = x R1 and f = bs wp (gate per column, where there
+// is one),
+//   t = ds f gate (per row or element), dot = sum t m;  dx = R1 (t - m dot / h)
+//   A = sum over rows of ds m gate (per row or element), of which dwp and a column gate's gradient are
+//   multiples: bs gate A and bs wp A.
+// So two sums per column whatever the gate.  PLAIN: both gradients come in, both go out, and the gate
+// is not per element, so that a training step's rows test for none of it.
+template <typename T, int NV, bool PLAIN>
+__global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_ring_kernel(SandwichBwdParams p, Ring q) {
+    using V = Vec<T>;
+    constexpr int E = V::E, N = V::N, H = E / 4;  // H: float4 of a vector
+    extern __shared__ __align__(16) unsigned char raw[];
+    RingGroup g;
+    g.init(raw, q);
+    pdl_wait();
+    pdl_trigger();
+    const int t = g.t, threads = q.threads, h = p.h, bytes = h * (int)sizeof(T);
+    const int64_t step = (int64_t)gridDim.x * q.groups, first = (int64_t)blockIdx.x * q.groups + g.id;
+    const int rows = first < p.n ? (int)((p.n - 1 - first) / step + 1) : 0;
+    const bool has_gy = PLAIN || p.gy, has_gs = PLAIN || p.gs;
+    const T* gates = !PLAIN && p.gate_kind == GATE_FULL ? reinterpret_cast<const T*>(p.gate) : nullptr;
+    // the inputs' places in a stage: s, x, then those of gy, gs and the gate that there are
+    const int at_gs = q.slot * (2 + has_gy), at_gate = at_gs + q.slot * has_gs;
+    auto order = [&](int i, int stage) {
+        const int64_t row = first + i * step;
+        const void* from[5] = {reinterpret_cast<const T*>(p.s) + row * p.s_stride,
+                               reinterpret_cast<const T*>(p.x) + row * p.x_stride,
+                               has_gy ? reinterpret_cast<const T*>(p.gy) + row * p.gy_stride : nullptr,
+                               has_gs ? reinterpret_cast<const T*>(p.gs) + row * p.gs_stride : nullptr,
+                               gates ? gates + row * p.gate_stride : nullptr};
+        order_row(g, q, i, stage, from, bytes);
+    };
+    if (t == 0)
+        for (int i = 0; i < min(rows, q.stages); ++i) order(i, i);
+    // w and f: a thread's 2 NV H pieces of 16 bytes lie side by side, in an order that differs between
+    // the threads of an eighth of a warp, so that they meet no bank twice
+    constexpr int PIECES = 2 * NV * H;
+    const uint32_t weights = g.rings + q.groups * q.stages * g.stage_bytes +
+                             (uint32_t)((t * PIECES + (t * PIECES / 8 & (PIECES - 1))) * 16);
+    static_assert((PIECES & (PIECES - 1)) == 0 && PIECES <= 8, "pieces are told apart by exclusive or");
+    if (g.id == 0) {
+        float2 w[NV][N], f[NV][N], c[NV][N];
+        hold_weight<T, NV, N>(p.w, p.w32, t, threads, h, w);
+        hold_weight<T, NV, N>(p.wp, p.w32, t, threads, h, f);
+        if (p.gate_kind == GATE_COLUMN) hold_weight<T, NV, N>(p.gate, p.w32, t, threads, h, c);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                f[j][k] = mul2(f[j][k], splat(p.branch_scale));
+                if (p.gate_kind == GATE_COLUMN) f[j][k] = mul2(f[j][k], c[j][k]);
+            }
+#pragma unroll
+            for (int b = 0; b < H; ++b) {
+                auto keep = [&](int which, float2 lo, float2 hi) {
+                    sts16(weights ^ (((which * NV + j) * H + b) * 16),
+                          make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y)));
+                };
+                keep(0, w[j][2 * b], w[j][2 * b + 1]);
+                keep(1, f[j][2 * b], f[j][2 * b + 1]);
+            }
+        }
+    }
+    __syncthreads();
+    auto weight = [&](int which, int j, float2 (&v)[N]) {
+#pragma unroll
+        for (int b = 0; b < H; ++b) {
+            const uint4 u = lds16(weights ^ (((which * NV + j) * H + b) * 16));
+            v[2 * b] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+            v[2 * b + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+        }
+    };
+    float2 dw[NV][N], A[NV][N];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < N; ++k) dw[j][k] = A[j][k] = splat(0.f);
+    const float inv_h = 1.f / (float)h;
+    // a row's own values are loaded while the row before it is worked on
+    float next_r1 = 0.f, next_r2 = 0.f, next_token = 1.f;
+    auto fetch = [&](int i) {
+        if (i >= rows) return;
+        const int64_t row = first + i * step;
+        next_r1 = p.rstd_post[row];
+        next_r2 = p.rstd[row];
+        if (p.gate_kind == GATE_TOKEN) next_token = DT<T>::load1(reinterpret_cast<const T*>(p.gate) + row * p.gate_stride);
+    };
+    fetch(0);
+    int64_t at_row = first * h + t * E;  // the thread's place in the outputs
+    for (int i = 0; i < rows; ++i, g.next(), at_row += step * h) {
+        const float r1 = next_r1, token = next_token;
+        float r2 = next_r2;
+        fetch(i + 1);
+        const uint32_t in = g.wait(i) + t * 16;
+        if (!g.ok) r2 = __int_as_float(0x7fc00000);
+        float c2 = 0.f;
+        if (has_gy) {
+            float2 sum = splat(0.f);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if ((j * threads + t) * E >= h) break;
+                const uint32_t at = in + j * threads * 16;
+                float2 a[N], b[N], w[N];
+                V::get(V::at(at + 2 * q.slot), a);
+                V::get(V::at(at), b);
+                weight(0, j, w);
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    a[k] = mul2(a[k], b[k]);
+                    sum = fma2(a[k], w[k], sum);
+                    dw[j][k] = fma2(a[k], splat(r2), dw[j][k]);
+                }
+            }
+            c2 = g.sum((sum.x + sum.y) * r2, threads, false) * inv_h;
+        }
+        float2 dots = splat(0.f);
+        const float2 minus = splat(-r2 * r2 * c2);
+        float2 u[NV][N];
+        uint4 x[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if ((j * threads + t) * E >= h) break;
+            const uint32_t at = in + j * threads * 16;
+            float2 ds[N], a[N], b[N];
+            if (has_gs) {
+                V::get(V::at(at + at_gs), ds);
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) ds[k] = splat(0.f);
+            }
+            if (has_gy) {
+                V::get(V::at(at), a);
+#pragma unroll
+                for (int k = 0; k < N; ++k) ds[k] = fma2(a[k], minus, ds[k]);
+                V::get(V::at(at + 2 * q.slot), a);
+                weight(0, j, b);
+#pragma unroll
+                for (int k = 0; k < N; ++k) ds[k] = fma2(mul2(a[k], b[k]), splat(r2), ds[k]);
+            } else if (!g.ok) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) ds[k] = splat(r2);
+            }
+            if (PLAIN || p.dr) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) a[k] = mul2(ds[k], splat(p.residual_scale));
+                stg_stream(reinterpret_cast<T*>(p.dr) + at_row + j * threads * E, V::put(a));
+            }
+            x[j] = V::at(at + q.slot);
+            V::get(x[j], a);
+            weight(1, j, b);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                a[k] = mul2(a[k], splat(r1));  // m
+                u[j][k] = mul2(ds[k], b[k]);
+                ds[k] = mul2(ds[k], a[k]);     // ds m
+            }
+            if (gates) {  // a gate per element: its gradient, and the products with it
+                V::get(V::at(at + at_gate), b);
+                float2 c[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    c[k] = mul2(u[j][k], a[k]);
+                    u[j][k] = mul2(u[j][k], b[k]);
+                    ds[k] = mul2(ds[k], b[k]);
+                }
+                if (p.dgate) stg_stream(reinterpret_cast<T*>(p.dgate) + at_row + j * threads * E, V::put(c));
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                dots = fma2(u[j][k], a[k], dots);
+                A[j][k] = fma2(ds[k], splat(token), A[j][k]);
+            }
+        }
+        const float dot = g.sum(dots.x + dots.y, threads, has_gy || (i & 1));  // after it nobody reads the stage
+        if (t == 0 && g.ok && i + q.stages < rows) order(i + q.stages, g.at);
+        if (p.dgate && p.gate_kind == GATE_TOKEN && t == 0)
+            DT<T>::store1(reinterpret_cast<T*>(p.dgate) + first + i * step, dot);
+        if (PLAIN || p.dx) {
+            const float2 c1 = splat(-r1 * dot * inv_h);
+            const float2 k1 = splat(r1 * token);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if ((j * threads + t) * E >= h) break;
+                float2 a[N];
+                V::get(x[j], a);
+#pragma unroll
+                for (int k = 0; k < N; ++k) a[k] = mul2(fma2(a[k], c1, u[j][k]), k1);
+                stg_stream(reinterpret_cast<T*>(p.dx) + at_row + j * threads * E, V::put(a));
+            }
+        }
+    }
+    if (t == 0) g.drain(rows);
+    if (!p.sums) return;
+    // the groups' sums, added in their order; the rings have room for one of them from each group
+    float* part = reinterpret_cast<float*>(raw + (g.rings - ring::saddr(raw)));
+    auto add = [&](int k, bool wanted, const float2 (&v)[NV][N], float factor) {
+        if (!wanted) return;
+        __syncthreads();
+        if (g.id > 0) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int col = (j * threads + t) * E;
+                if (col >= h) break;
+#pragma unroll
+                for (int c = 0; c < N; ++c) *reinterpret_cast<float2*>(part + (g.id - 1) * h + col + 2 * c) = v[j][c];
+            }
+        }
+        __syncthreads();
+        if (g.id > 0) return;
+        float* out = p.sums + ((int64_t)k * gridDim.x + blockIdx.x) * h;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (j * threads + t) * E;
+            if (col >= h) break;
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                float2 s = v[j][c];
+                for (int o = 0; o < q.groups - 1; ++o) s = add2(s, *reinterpret_cast<const float2*>(part + o * h + col + 2 * c));
+                *reinterpret_cast<float2*>(out + col + 2 * c) = mul2(s, splat(factor));
+            }
+        }
+    };
+    add(0, p.want & 1, dw, 1.f);
+    add(1, p.want & 6, A, p.branch_scale);
+}
+
+// The blocks' partial sums (blockIdx.y: of dw, or of A), added in a fixed order as in
+// k1_rmsnorm_dw_kernel; A gives dwp (times a gate per column) and that gate's gradient (times wp).
+template <typename W>
+__global__ void __launch_bounds__(512) k1_sandwich_dw_kernel(const float* part, int parts, int h, W* dw, W* dwp, W* dg,
+                                                             const W* wp, const W* gate) {
+    __shared__ float sums[16][33];
+    pdl_wait();
+    pdl_trigger();
     part += (int64_t)blockIdx.y * parts * h;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + lane;
@@ -251,7 +814,12 @@ __global__ void __launch_bounds__(512) k1_sandwich_dw_kernel(const float* part, 
         float t = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) t += sums[i][lane];
-        DT<W>::store1(out + col, t);
+        if (blockIdx.y == 0) {
+            if (dw) DT<W>::store1(dw + col, t);
+        } else {
+            if (dwp) DT<W>::store1(dwp + col, gate ? t * DT<W>::load1(gate + col) : t);
+            if (dg) DT<W>::store1(dg + col, t * DT<W>::load1(wp + col));
+        }
     }
 }
 

@@ -6,6 +6,19 @@
 #include "k1_norm_host.cuh"
 #include "k1_sandwich.cuh"
 
+cudaError_t k1_sandwich_wait_status(unsigned* bits) {
+    unsigned zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(bits, k1::k1_ring_error, sizeof *bits);
+    if (e == cudaSuccess) e = cudaMemcpyToSymbol(k1::k1_ring_error, &zero, sizeof zero);
+    return e;
+}
+
+#ifdef K1_WAIT_TEST
+cudaError_t k1_sandwich_set_withhold(long long withhold) {
+    return cudaMemcpyToSymbol(k1::k1_test_withhold, &withhold, sizeof withhold);
+}
+#endif
+
 namespace {
 
 using k1::norm::GATE_COLUMN;
@@ -37,7 +50,37 @@ cudaError_t with_shape(const NormShape& s, F f) {
     return cudaErrorInvalidValue;
 }
 
-// Checks that forward and backward share; `factor` finite.
+// The ring kernels' layout for rows of vectors of `inputs` tensors, or groups = 0 where they do not
+// serve: few rows (their latency counts, and the ring's set-up), rows shorter than 512 bytes, rows of
+// more than two vectors per thread, or of which a block cannot hold two.  one, two: threads of a block
+// with one and two vectors each.
+constexpr size_t kRingShared = 224 * 1024;
+constexpr int kRingOne = 256;  // vectors of a row that get a thread each
+k1::norm::Ring ring_of(int e, int64_t n, int64_t hidden, int es, int inputs, int weights, int one, int two, int sms) {
+    k1::norm::Ring q = {};
+    const int vecs = (int)(hidden / e);
+    if (e * es != 16 || n <= sms || hidden * es < 512 || vecs > 1024) return q;
+    q.e = e;
+    q.nv = vecs <= kRingOne ? 1 : 2;
+    q.threads = ((vecs + q.nv - 1) / q.nv + 31) / 32 * 32;
+    q.inputs = inputs;
+    q.slot = (int)((hidden * es + 127) / 128 * 128);
+    q.groups = (int)std::min<int64_t>({k1::norm::kMaxRingGroups, (q.nv == 1 ? one : two) / q.threads, (n + sms - 1) / sms});
+    for (; q.groups > 0; --q.groups)
+        for (q.stages = k1::norm::kMaxRingStages; q.stages >= 2; --q.stages)
+            if (ring_smem(q, weights) <= kRingShared) return q;
+    q.groups = 0;
+    return q;
+}
+
+// The instance of a ring kernel: f(NV).
+template <typename F>
+cudaError_t with_ring(const k1::norm::Ring& q, F f) {
+    if (q.nv == 1) return f(std::integral_constant<int, 1>{});
+    return f(std::integral_constant<int, 2>{});
+}
+
+// Checks that forward and backward share.
 int sandwich_check(const char* fn, int dtype, int weight_dtype, int64_t n_rows, int64_t hidden, int gate_kind,
                    float branch_scale, float residual_scale) {
     int rc = norm_check(fn, dtype, weight_dtype, n_rows, hidden);
@@ -115,6 +158,22 @@ int sandwich_forward(const char* fn, int out, const void* x, int64_t x_stride, c
     // of blocks would leave SMs idle
     auto go = [&](auto tag) {
         using T = decltype(tag);
+        constexpr int V = k1::DT<T>::kEPV;
+        const int inputs = gate_kind == GATE_FULL ? 3 : 2;
+        const k1::norm::Ring q = ring_of(sh.e, n, hidden, es, inputs, 0, k1::norm::kRingFwd<V, 1>,
+                                         k1::norm::kRingFwd<V, 2>, sms);
+        if (q.groups > 0)
+            return with_ring(q, [&](auto NV) {
+                auto kern = same ? k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::SAME>
+                                 : k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::FP8>;
+                const int threads = q.groups * q.threads;
+                const size_t smem = ring_smem(q, 0);
+                int per_sm = 0;
+                if (allow_smem(kern, dev, smem) != K1_OK || resident_blocks(kern, dev, threads, smem, &per_sm) != K1_OK)
+                    return cudaErrorInvalidValue;
+                const int64_t grid = std::min<int64_t>((n + q.groups - 1) / q.groups, (int64_t)sms * per_sm);
+                return launch(kern, grid, threads, smem, st, p, q);
+            });
         return with_shape<T>(sh, [&](auto E, auto NV) {
             auto kern = same ? k1::norm::k1_rmsnorm_kernel<T, E, NV, k1::norm::SAME, true>
                              : k1::norm::k1_rmsnorm_kernel<T, E, NV, k1::norm::FP8, true>;
@@ -160,7 +219,7 @@ size_t k1_sandwich_rmsnorm_workspace_bytes(int64_t n_rows, int64_t hidden, int d
         sm_count(device, &sms) != K1_OK)
         return 0;
     return (size_t)std::min<int64_t>(std::max<int64_t>(n_rows, 1), (int64_t)sms * kBwdBlocksPerSm) * (size_t)hidden *
-           3 * sizeof(float);
+           2 * sizeof(float);
 }
 
 int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void* g_stream, int64_t g_stream_stride,
@@ -242,10 +301,28 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
     p.gate_kind = gate_kind;
     p.branch_scale = branch_scale;
     p.residual_scale = residual_scale;
-    const size_t smem = (size_t)hidden * 12;
+    const size_t smem = (size_t)hidden * 8;
     int64_t grid = 0;  // resident blocks, as in the forward
     auto go = [&](auto tag) {
         using T = decltype(tag);
+        constexpr int V = k1::DT<T>::kEPV;
+        const int inputs = 2 + (g_y != nullptr) + (g_stream != nullptr) + (gate_kind == GATE_FULL);
+        const k1::norm::Ring q = ring_of(sh.e, n_rows, hidden, es, inputs, 2, k1::norm::kRingBwd<V, 1>,
+                                         k1::norm::kRingBwd<V, 2>, sms);
+        if (q.groups > 0)
+            return with_ring(q, [&](auto NV) {
+                const bool plain = g_y && g_stream && d_x && d_residual && gate_kind != GATE_FULL;
+                auto kern = plain ? k1::norm::k1_sandwich_bwd_ring_kernel<T, NV, true>
+                                  : k1::norm::k1_sandwich_bwd_ring_kernel<T, NV, false>;
+                const int threads = q.groups * q.threads;
+                const size_t ring = ring_smem(q, 2);
+                int per_sm = 0;
+                if (allow_smem(kern, dev, ring) != K1_OK || resident_blocks(kern, dev, threads, ring, &per_sm) != K1_OK)
+                    return cudaErrorInvalidValue;
+                grid = std::min<int64_t>((n_rows + q.groups - 1) / q.groups,
+                                         (int64_t)sms * std::min(per_sm, kBwdBlocksPerSm));
+                return launch(kern, grid, threads, ring, st, p, q);
+            });
         return with_shape<T>(sh, [&](auto E, auto NV) {
             auto kern = k1::norm::k1_sandwich_bwd_kernel<T, E, NV>;
             int per_sm = 0;
@@ -263,7 +340,7 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
     auto sum = [&](auto tag) {
         using W = decltype(tag);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)((hidden + 31) / 32), d_column ? 3 : 2);
+        cfg.gridDim = dim3((unsigned)((hidden + 31) / 32), want & 6 ? 2 : 1);
         cfg.blockDim = dim3(512);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
@@ -273,7 +350,8 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
         cfg.numAttrs = K1_PDL ? 1 : 0;
         return cudaLaunchKernelEx(&cfg, k1::norm::k1_sandwich_dw_kernel<W>, (const float*)p.sums, (int)grid, (int)hidden,
                                   reinterpret_cast<W*>(d_weight), reinterpret_cast<W*>(d_post_weight),
-                                  reinterpret_cast<W*>(d_column));
+                                  reinterpret_cast<W*>(d_column), reinterpret_cast<const W*>(post_weight),
+                                  reinterpret_cast<const W*>(column));
     };
     return launched(fn, weight_dtype == K1_DTYPE_BF16  ? sum(__nv_bfloat16{})
                         : weight_dtype == K1_DTYPE_F16 ? sum(__half{})
