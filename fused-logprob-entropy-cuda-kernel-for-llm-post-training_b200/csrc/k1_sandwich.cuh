@@ -239,8 +239,7 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
 // into it.  So 100 KB and more per SM are in flight whatever the groups wait for.  A thread has the
 // columns that it would have in the other kernels and sums in the same order, so results are the
 // same bits.  Sums over rows stay in registers and are added over the groups, in their order, at
-// the end.  Backward the weights are in shared memory too, as fp32, so that registers serve three
-// groups.
+// the end; the weights are in shared memory too, as fp32, and not in registers.
 //
 // Every wait is bounded; one that runs out sets bit 0 of the wait status word, the group's rows from
 // there on are NaN, and a block leaves only when the copies that it ordered have landed.
@@ -256,7 +255,7 @@ constexpr int kMaxRingGroups = 15;  // a named barrier each
 constexpr int kMaxRingStages = 4;
 // Threads of a block: what registers allow (a thread holds E NV columns, and backward 2 E NV sums).
 template <int E, int NV>
-constexpr int kRingFwd = E * NV >= 16 ? 512 : 960;
+constexpr int kRingFwd = E * NV >= 16 ? 704 : 960;
 template <int E, int NV>
 constexpr int kRingBwd = E * NV >= 16 ? 512 : 896;
 
@@ -264,10 +263,8 @@ struct RingSmem {
     uint64_t full[kMaxRingGroups * kMaxRingStages];
     float scratch[kMaxRingGroups][2][16];
 };
-// weights: fp32 ones kept beside the rings.
-constexpr size_t ring_smem(const Ring& q, int weights) {
-    return sizeof(RingSmem) + 128 + (size_t)q.groups * q.stages * q.slot * q.inputs +
-           (size_t)weights * q.threads * q.nv * q.e * 4;
+constexpr size_t ring_smem(const Ring& q) {
+    return sizeof(RingSmem) + 128 + (size_t)q.groups * q.stages * q.slot * q.inputs + (size_t)q.threads * q.nv * q.e * 8;
 }
 
 // 16 bytes of shared memory by address (addresses of 32 bits: generic pointers would cost these
@@ -418,6 +415,55 @@ __device__ __forceinline__ void hold_weight(const void* w, bool w32, int t, int 
     }
 }
 
+// The weight w, and f = branch_scale post_weight (times a gate per column), as fp32 in shared memory.  A
+// thread's 2 NV H pieces of 16 bytes (H to a vector) lie side by side, in an order that differs between
+// the threads of an eighth of a warp, so that they meet no bank twice.
+template <typename T, int NV>
+struct Weights {
+    static constexpr int E = DT<T>::kEPV, N = E / 2, H = E / 4, PIECES = 2 * NV * H;
+    static_assert((PIECES & (PIECES - 1)) == 0 && PIECES <= 8, "pieces are told apart by exclusive or");
+    uint32_t at;
+    __device__ __forceinline__ uint32_t piece(int which, int j, int b) const { return at ^ (((which * NV + j) * H + b) * 16); }
+    template <typename P>
+    __device__ __forceinline__ void init(const RingGroup& g, const Ring& q, const P& p) {
+        const int t = g.t;
+        at = g.rings + q.groups * q.stages * g.stage_bytes + (uint32_t)((t * PIECES + (t * PIECES / 8 & (PIECES - 1))) * 16);
+        if (g.id == 0) {
+            float2 w[NV][N], f[NV][N], c[NV][N];
+            hold_weight<T, NV, N>(p.w, p.w32, t, q.threads, p.h, w);
+            hold_weight<T, NV, N>(p.wp, p.w32, t, q.threads, p.h, f);
+            if (p.gate_kind == GATE_COLUMN) hold_weight<T, NV, N>(p.gate, p.w32, t, q.threads, p.h, c);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    f[j][k] = mul2(f[j][k], splat(p.branch_scale));
+                    if (p.gate_kind == GATE_COLUMN) f[j][k] = mul2(f[j][k], c[j][k]);
+                }
+#pragma unroll
+                for (int b = 0; b < H; ++b) {
+                    auto keep = [&](int which, float2 lo, float2 hi) {
+                        sts16(piece(which, j, b), make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y),
+                                                             __float_as_uint(hi.x), __float_as_uint(hi.y)));
+                    };
+                    keep(0, w[j][2 * b], w[j][2 * b + 1]);
+                    keep(1, f[j][2 * b], f[j][2 * b + 1]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // w (0) or f (1) of the thread's vector j
+    __device__ __forceinline__ void get(int which, int j, float2 (&v)[N]) const {
+#pragma unroll
+        for (int b = 0; b < H; ++b) {
+            const uint4 u = lds16(piece(which, j, b));
+            v[2 * b] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+            v[2 * b + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+        }
+    }
+};
+
 template <typename T, int NV, int OUT>
 __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring_kernel(FwdParams p, Ring q) {
     using V = Vec<T>;
@@ -441,22 +487,8 @@ __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring
     };
     if (t == 0)
         for (int i = 0; i < min(rows, q.stages); ++i) order(i, i);
-    // the thread's columns of the weight, and of post_weight times branch_scale and a gate per column
-    float2 w[NV][N], wg[NV][N];
-    hold_weight<T, NV, N>(p.w, p.w32, t, threads, h, w);
-    hold_weight<T, NV, N>(p.wp, p.w32, t, threads, h, wg);
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int k = 0; k < N; ++k) wg[j][k] = mul2(wg[j][k], splat(p.branch_scale));
-    if (p.gate_kind == GATE_COLUMN) {
-        float2 c[NV][N];
-        hold_weight<T, NV, N>(p.gate, p.w32, t, threads, h, c);
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int k = 0; k < N; ++k) wg[j][k] = mul2(wg[j][k], c[j][k]);
-    }
+    Weights<T, NV> weights;
+    weights.init(g, q, p);
     const float2 rs = splat(p.residual_scale);
     const float inv_h = 1.f / (float)h;
     // a row's gate is loaded while the row before it is worked on
@@ -498,8 +530,10 @@ __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring
 #pragma unroll
                 for (int k = 0; k < N; ++k) x[j][k] = mul2(x[j][k], c[k]);
             }
+            float2 f[N];
+            weights.get(1, j, f);
 #pragma unroll
-            for (int k = 0; k < N; ++k) x[j][k] = fma2(mul2(x[j][k], k1), wg[j][k], mul2(b[k], rs));
+            for (int k = 0; k < N; ++k) x[j][k] = fma2(mul2(x[j][k], k1), f[k], mul2(b[k], rs));
             const uint4 s = V::put(x[j]);
             stg_stream(so + j * threads * E, s);
             V::get(s, x[j]);  // the stream as stored
@@ -516,16 +550,20 @@ __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring
             for (int j = 0; j < NV; ++j) {
                 const int col = (j * threads + t) * E;
                 if (col >= h) break;
+                float2 w[N];
+                weights.get(0, j, w);
 #pragma unroll
-                for (int k = 0; k < N; ++k) x[j][k] = mul2(mul2(x[j][k], splat(r2)), w[j][k]);
+                for (int k = 0; k < N; ++k) x[j][k] = mul2(mul2(x[j][k], splat(r2)), w[k]);
                 stg_stream(y + j * threads * E, V::put(x[j]));
             }
         } else {
-            // as in k1_rmsnorm_kernel, which has the reasons
+            // as in k1_rmsnorm_kernel, which has the reasons; the largest value is taken before the factor 7/8,
+            // so that its part in 512 needs no division, and its reciprocal may be rough (the quotient's
+            // Newton step makes up for it; the step is at least 1e-33 and at most 1e36)
             const uint32_t bits = __float_as_uint(r2);
-            const float unit = 0.875f * (r2 == r2 ? __uint_as_float(bits & 0x7f800000u) : r2);
+            const float unit = r2 == r2 ? __uint_as_float(bits & 0x7f800000u) : r2;
             const float rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) * (8.f / 7.f);
-            const float least = kAmaxFloor / rest;
+            const float least = kAmaxFloor * (8.f / 7.f) / rest;
             constexpr int LANES = kFp8Block / E;
             uint8_t* y = reinterpret_cast<uint8_t*>(p.y) + at_row;
 #pragma unroll
@@ -534,23 +572,27 @@ __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring
                 float2 (&a)[N] = x[j];
                 float m = 0.f;
                 if (col < h) {
+                    float2 w[N];
+                    weights.get(0, j, w);
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        a[k] = mul2(mul2(a[k], splat(unit)), w[j][k]);
+                        a[k] = mul2(mul2(a[k], splat(unit)), w[k]);
                         m = fmax_nan(m, fmax_nan(fabsf(a[k].x), fabsf(a[k].y)));
                     }
                 }
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                 if (col < h) {
-                    m = fmax_nan(m, least);
-                    const float d = m / kFp8Max;
-                    const Quotient to(d);
+                    const float d = fmax_nan(m, least) * (1.f / 512.f);
+                    float inv;
+                    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+                    const Quotient to(d, inv);
                     uint32_t v[N];
 #pragma unroll
                     for (int k = 0; k < N; ++k) {  // Quotient's steps, in pairs
-                        const float2 c = mul2(a[k], splat(to.inv));
-                        const float2 e = fma2(fma2(make_float2(-c.x, -c.y), splat(to.step), a[k]), splat(to.inv), c);
+                        const float2 n = mul2(a[k], splat(0.875f));
+                        const float2 c = mul2(n, splat(to.inv));
+                        const float2 e = fma2(fma2(make_float2(-c.x, -c.y), splat(to.step), n), splat(to.inv), c);
                         v[k] = e4m3x2(e.x, e.y);
                     }
                     if constexpr (E == 8)
@@ -576,7 +618,7 @@ __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring
 template <typename T, int NV, bool PLAIN>
 __global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_ring_kernel(SandwichBwdParams p, Ring q) {
     using V = Vec<T>;
-    constexpr int E = V::E, N = V::N, H = E / 4;  // H: float4 of a vector
+    constexpr int E = V::E, N = V::N;
     extern __shared__ __align__(16) unsigned char raw[];
     RingGroup g;
     g.init(raw, q);
@@ -600,44 +642,8 @@ __global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_
     };
     if (t == 0)
         for (int i = 0; i < min(rows, q.stages); ++i) order(i, i);
-    // w and f: a thread's 2 NV H pieces of 16 bytes lie side by side, in an order that differs between
-    // the threads of an eighth of a warp, so that they meet no bank twice
-    constexpr int PIECES = 2 * NV * H;
-    const uint32_t weights = g.rings + q.groups * q.stages * g.stage_bytes +
-                             (uint32_t)((t * PIECES + (t * PIECES / 8 & (PIECES - 1))) * 16);
-    static_assert((PIECES & (PIECES - 1)) == 0 && PIECES <= 8, "pieces are told apart by exclusive or");
-    if (g.id == 0) {
-        float2 w[NV][N], f[NV][N], c[NV][N];
-        hold_weight<T, NV, N>(p.w, p.w32, t, threads, h, w);
-        hold_weight<T, NV, N>(p.wp, p.w32, t, threads, h, f);
-        if (p.gate_kind == GATE_COLUMN) hold_weight<T, NV, N>(p.gate, p.w32, t, threads, h, c);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                f[j][k] = mul2(f[j][k], splat(p.branch_scale));
-                if (p.gate_kind == GATE_COLUMN) f[j][k] = mul2(f[j][k], c[j][k]);
-            }
-#pragma unroll
-            for (int b = 0; b < H; ++b) {
-                auto keep = [&](int which, float2 lo, float2 hi) {
-                    sts16(weights ^ (((which * NV + j) * H + b) * 16),
-                          make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y)));
-                };
-                keep(0, w[j][2 * b], w[j][2 * b + 1]);
-                keep(1, f[j][2 * b], f[j][2 * b + 1]);
-            }
-        }
-    }
-    __syncthreads();
-    auto weight = [&](int which, int j, float2 (&v)[N]) {
-#pragma unroll
-        for (int b = 0; b < H; ++b) {
-            const uint4 u = lds16(weights ^ (((which * NV + j) * H + b) * 16));
-            v[2 * b] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-            v[2 * b + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
-        }
-    };
+    Weights<T, NV> weights;
+    weights.init(g, q, p);
     float2 dw[NV][N], A[NV][N];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -671,7 +677,7 @@ __global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_
                 float2 a[N], b[N], w[N];
                 V::get(V::at(at + 2 * q.slot), a);
                 V::get(V::at(at), b);
-                weight(0, j, w);
+                weights.get(0, j, w);
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
                     a[k] = mul2(a[k], b[k]);
@@ -701,7 +707,7 @@ __global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_
 #pragma unroll
                 for (int k = 0; k < N; ++k) ds[k] = fma2(a[k], minus, ds[k]);
                 V::get(V::at(at + 2 * q.slot), a);
-                weight(0, j, b);
+                weights.get(0, j, b);
 #pragma unroll
                 for (int k = 0; k < N; ++k) ds[k] = fma2(mul2(a[k], b[k]), splat(r2), ds[k]);
             } else if (!g.ok) {
@@ -715,7 +721,7 @@ __global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_
             }
             x[j] = V::at(at + q.slot);
             V::get(x[j], a);
-            weight(1, j, b);
+            weights.get(1, j, b);
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 a[k] = mul2(a[k], splat(r1));  // m

@@ -56,7 +56,7 @@ cudaError_t with_shape(const NormShape& s, F f) {
 // with one and two vectors each.
 constexpr size_t kRingShared = 224 * 1024;
 constexpr int kRingOne = 256;  // vectors of a row that get a thread each
-k1::norm::Ring ring_of(int e, int64_t n, int64_t hidden, int es, int inputs, int weights, int one, int two, int sms) {
+k1::norm::Ring ring_of(int e, int64_t n, int64_t hidden, int es, int inputs, int one, int two, int sms) {
     k1::norm::Ring q = {};
     const int vecs = (int)(hidden / e);
     if (e * es != 16 || n <= sms || hidden * es < 512 || vecs > 1024) return q;
@@ -68,7 +68,7 @@ k1::norm::Ring ring_of(int e, int64_t n, int64_t hidden, int es, int inputs, int
     q.groups = (int)std::min<int64_t>({k1::norm::kMaxRingGroups, (q.nv == 1 ? one : two) / q.threads, (n + sms - 1) / sms});
     for (; q.groups > 0; --q.groups)
         for (q.stages = k1::norm::kMaxRingStages; q.stages >= 2; --q.stages)
-            if (ring_smem(q, weights) <= kRingShared) return q;
+            if (ring_smem(q) <= kRingShared) return q;
     q.groups = 0;
     return q;
 }
@@ -160,14 +160,14 @@ int sandwich_forward(const char* fn, int out, const void* x, int64_t x_stride, c
         using T = decltype(tag);
         constexpr int V = k1::DT<T>::kEPV;
         const int inputs = gate_kind == GATE_FULL ? 3 : 2;
-        const k1::norm::Ring q = ring_of(sh.e, n, hidden, es, inputs, 0, k1::norm::kRingFwd<V, 1>,
+        const k1::norm::Ring q = ring_of(sh.e, n, hidden, es, inputs, k1::norm::kRingFwd<V, 1>,
                                          k1::norm::kRingFwd<V, 2>, sms);
         if (q.groups > 0)
             return with_ring(q, [&](auto NV) {
                 auto kern = same ? k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::SAME>
                                  : k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::FP8>;
                 const int threads = q.groups * q.threads;
-                const size_t smem = ring_smem(q, 0);
+                const size_t smem = ring_smem(q);
                 int per_sm = 0;
                 if (allow_smem(kern, dev, smem) != K1_OK || resident_blocks(kern, dev, threads, smem, &per_sm) != K1_OK)
                     return cudaErrorInvalidValue;
@@ -307,7 +307,7 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
         using T = decltype(tag);
         constexpr int V = k1::DT<T>::kEPV;
         const int inputs = 2 + (g_y != nullptr) + (g_stream != nullptr) + (gate_kind == GATE_FULL);
-        const k1::norm::Ring q = ring_of(sh.e, n_rows, hidden, es, inputs, 2, k1::norm::kRingBwd<V, 1>,
+        const k1::norm::Ring q = ring_of(sh.e, n_rows, hidden, es, inputs, k1::norm::kRingBwd<V, 1>,
                                          k1::norm::kRingBwd<V, 2>, sms);
         if (q.groups > 0)
             return with_ring(q, [&](auto NV) {
@@ -315,7 +315,7 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
                 auto kern = plain ? k1::norm::k1_sandwich_bwd_ring_kernel<T, NV, true>
                                   : k1::norm::k1_sandwich_bwd_ring_kernel<T, NV, false>;
                 const int threads = q.groups * q.threads;
-                const size_t ring = ring_smem(q, 2);
+                const size_t ring = ring_smem(q);
                 int per_sm = 0;
                 if (allow_smem(kern, dev, ring) != K1_OK || resident_blocks(kern, dev, threads, ring, &per_sm) != K1_OK)
                     return cudaErrorInvalidValue;
