@@ -62,9 +62,12 @@ int score_launch(const char* fn, k1::score::FwdParams p, int64_t n_rows, int sms
 
 template <typename T>
 int score_forward(const char* fn, const k1::score::FwdParams& p, int64_t n_rows, int sms, int dev, cudaStream_t st) {
-    if (p.k == 0) return score_launch<T, 256, 8, 3, false>(fn, p, n_rows, sms, dev, st);
-    return n_rows >= 6 * sms ? score_launch<T, 128, 4, 8, true>(fn, p, n_rows, sms, dev, st)
-                             : score_launch<T, 256, 4, 4, true>(fn, p, n_rows, sms, dev, st);
+    // the same work split with and without a list, so that both give the same bits
+    if (n_rows >= 6 * sms)
+        return p.k > 0 ? score_launch<T, 128, 4, 7, true>(fn, p, n_rows, sms, dev, st)
+                       : score_launch<T, 128, 4, 7, false>(fn, p, n_rows, sms, dev, st);
+    return p.k > 0 ? score_launch<T, 256, 4, 4, true>(fn, p, n_rows, sms, dev, st)
+                   : score_launch<T, 256, 4, 4, false>(fn, p, n_rows, sms, dev, st);
 }
 
 template <typename T>
@@ -74,7 +77,7 @@ int score_backward(const char* fn, k1::score::BwdParams p, int64_t n_rows, int s
     constexpr int chunk = UB * kBwdThreads;
     const int64_t vecs = (p.vocab + E - 1) / E + 1;
     int64_t parts = 1;
-    while (n_rows * parts < 32 * sms && vecs >= 2 * parts * chunk) parts *= 2;
+    while (n_rows * parts < 2 * sms && vecs >= 2 * parts * chunk) parts *= 2;
     p.parts = (int)parts;
     p.slice = (int)((vecs + parts - 1) / parts);
     const size_t smem = (size_t)(p.n_ids + p.k) * 12;
