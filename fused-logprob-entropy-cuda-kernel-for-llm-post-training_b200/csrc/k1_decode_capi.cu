@@ -179,14 +179,26 @@ int make_tmap8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
 // memory beside the ring.
 constexpr int64_t kMaxInner = 32768;
 
-template <int TN, typename OutT, bool EPI>
-int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
-           int64_t inner, int sms, int dev, cudaStream_t st) {
-    using S = k1::fp8::Skinny<TN>;
+template <int TN, typename OutT, bool EPI, bool DEEP>
+int skinny_launch(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                  int64_t inner, int split, int dev, cudaStream_t st) {
+    using S = k1::fp8::Skinny<TN, DEEP>;
     CUtensorMap tx, tw;
     int rc = make_tmap8(&tx, x, p.m, inner, ldx, TN, "x");
     if (!rc) rc = make_tmap8(&tw, w, p.n, inner, ldw, k1::fp8::BM, "weight");
     if (rc) return rc;
+    const int64_t tiles = (p.n + 127) / 128, tok = (p.m + TN - 1) / TN;
+    auto kern = k1::fp8::k1_fp8_skinny_kernel<TN, OutT, EPI, DEEP>;
+    const size_t smem = S::smem((p.kb_total + split - 1) / split);
+    rc = allow_smem(kern, dev, smem);
+    if (rc) return rc;
+    const dim3 grid((unsigned)(tiles * tok * split));
+    return launched(fn, launch_cluster(kern, grid, S::THREADS, smem, split, st, tx, tw, p, split));
+}
+
+template <int TN, typename OutT, bool EPI>
+int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
+           int64_t inner, int sms, int dev, cudaStream_t st) {
     const int64_t tiles = (p.n + 127) / 128, tok = (p.m + TN - 1) / TN;
     // K is split over a cluster where a third of the SMs or more would stay without a block,
     // until all have one and while every part keeps two blocks of K.  Measured (us, bf16 out):
@@ -195,12 +207,11 @@ int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx,
     int split = 1;
     if (tiles * tok * 3 < 2 * sms)
         while (split < 8 && tiles * tok * split < sms && p.kb_total >= 4 * split) split *= 2;
-    auto kern = k1::fp8::k1_fp8_skinny_kernel<TN, OutT, EPI>;
-    const size_t smem = S::smem((p.kb_total + split - 1) / split);
-    rc = allow_smem(kern, dev, smem);
-    if (rc) return rc;
-    const dim3 grid((unsigned)(tiles * tok * split));
-    return launched(fn, launch_cluster(kern, grid, S::THREADS, smem, split, st, tx, tw, p, split));
+    // few blocks: a deeper ring, where the scales leave room for it
+    if constexpr (EPI)
+        if (tiles * tok * split <= sms && k1::fp8::Skinny<TN, true>::smem((p.kb_total + split - 1) / split) <= 227 * 1024)
+            return skinny_launch<TN, OutT, EPI, true>(fn, p, x, ldx, w, ldw, inner, split, dev, st);
+    return skinny_launch<TN, OutT, EPI, false>(fn, p, x, ldx, w, ldw, inner, split, dev, st);
 }
 
 // Pairs of the many-token kernel that can be resident at once; its persistent grid must not
