@@ -74,6 +74,7 @@ struct FwdParams {
     float* top_logprobs; // [n, k]
     float* entropy;
     float* lse;
+    float* lse_rest;     // lse before its rounding, less lse; may be NULL
     int cluster;         // blocks per row
     int slice;           // vectors per block
     int groups;          // groups per thread
@@ -708,6 +709,7 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
     const bool fine = !none && part.m < INFINITY && l - l == 0.0;
     if (tid == 0) {
         p.lse[r] = fine ? (float)l : none ? -INFINITY : NAN;
+        if (p.lse_rest) p.lse_rest[r] = fine ? (float)(l - (double)(float)l) : 0.f;
         p.entropy[r] = fine ? (float)(l - s * (double)part.m - s * part.t / part.z) : NAN;
     }
     if (tid < p.n_ids) p.logprobs[r * p.n_ids + tid] = fine ? (float)(s * (double)xid - l) : NAN;
@@ -740,6 +742,7 @@ struct BwdParams {
     const float* g_top;      // [n, k], NULL: none
     int n_ids, k;            // 0 without gradient
     const float* lse;
+    const float* lse_rest;   // NULL: 0
     const float* entropy;
     const float* g_entropy;  // NULL: none
     const float* g_lse;      // NULL: none
@@ -754,7 +757,7 @@ constexpr int UB = 4;
 
 // dL/dx of a vector of logits that no list names.
 struct BwdRow {
-    float s, nl, c0, ge;  // s, -lse, s (g_lse - sum g - g_H H), s g_H
+    float s, nl, nr, c0, ge;  // s, -lse, -lse_rest log2 e, s (g_lse - sum g - g_H (H - lse_rest)), s g_H
 };
 template <typename T>
 __device__ __forceinline__ uint4 grad_vector(uint4 v, const BwdRow& q) {
@@ -764,9 +767,11 @@ __device__ __forceinline__ uint4 grad_vector(uint4 v, const BwdRow& q) {
     float2 g[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
+        // d = s x - lse is rounded by 2^-24 of itself; lse's own rounding, which at a low temperature is
+        // many times that, is made good in the exponent and in c0
         float2 d = fma2(make_float2(x[2 * i], x[2 * i + 1]), splat(q.s), splat(q.nl));
         d = make_float2(fmax_nan(d.x, -1e30f), fmax_nan(d.y, -1e30f));
-        const float2 a = mul2(d, splat(kLog2e));
+        const float2 a = fma2(d, splat(kLog2e), splat(q.nr));
         g[i] = mul2(make_float2(ex2(a.x), ex2(a.y)), fma2(d, splat(-q.ge), splat(q.c0)));
     }
     if constexpr (sizeof(T) == 4)
@@ -826,10 +831,12 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks) k1_score_bwd_kernel(B
     const float lse = p.lse[r], h = p.entropy[r];
     BwdRow q;
     q.s = p.scale;
+    const float rest = p.lse_rest ? p.lse_rest[r] : 0.f;
+    q.nr = -rest * kLog2e;
     q.nl = lse - lse == 0.f ? -lse : NAN;  // a row without a distribution
     q.ge = p.scale * ge;
     // entropy: only where it has a gradient, so that a row without one needs no finite entropy
-    const double c0 = (double)gl - sum - (ge != 0.f ? (double)ge * (double)h : 0.0);
+    const double c0 = (double)gl - sum - (ge != 0.f ? (double)ge * ((double)h - (double)rest) : 0.0);
     q.c0 = (float)((double)p.scale * c0);
     uint4* ov = reinterpret_cast<uint4*>(out - row.shift);
     auto store = [&](int j, uint4 v) {
@@ -880,7 +887,7 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks) k1_score_bwd_kernel(B
             (eq ? mine : others) += (double)gs[o];
         }
         if (!first) continue;
-        const double lp = (double)p.scale * (double)DT<T>::load1(row.p + e) - (double)lse;
+        const double lp = (double)p.scale * (double)DT<T>::load1(row.p + e) - ((double)lse + (double)rest);
         const double pr = exp(lp);
         double g = mine * -expm1(lp) + pr * ((double)gl - others);
         if (ge != 0.f && pr > 0.0) g -= (double)ge * pr * (lp + (double)h);

@@ -91,7 +91,7 @@ extern "C" {
 int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t inner_rows,
                       int64_t inner_stride, int64_t outer_stride, double temperature, const int64_t* token_ids,
                       int64_t n_ids, float* logprobs, int64_t k, int64_t* top_ids, float* top_logprobs,
-                      float* entropy, float* lse, void* stream) {
+                      float* entropy, float* lse, float* lse_rest, void* stream) {
     const char* fn = "k1_token_logprobs";
     int rc = score_check(fn, logits, dtype, n_rows, vocab, inner_rows, inner_stride, outer_stride, temperature, n_ids, k);
     if (rc) return rc;
@@ -115,6 +115,7 @@ int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t voc
     p.top_logprobs = top_logprobs;
     p.entropy = entropy;
     p.lse = lse;
+    p.lse_rest = lse_rest;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (dtype) {
         case K1_DTYPE_BF16: return score_forward<__nv_bfloat16>(fn, p, n_rows, sms, dev, st);
@@ -127,7 +128,7 @@ int k1_token_logprobs_backward(const void* logits, int dtype, int64_t n_rows, in
                                int64_t inner_stride, int64_t outer_stride, double temperature,
                                const int64_t* token_ids, int64_t n_ids, const float* g_logprobs,
                                const int64_t* top_ids, int64_t k, const float* g_top, const float* lse,
-                               const float* entropy, const float* g_entropy, const float* g_lse, void* d_logits,
+                               const float* lse_rest, const float* entropy, const float* g_entropy, const float* g_lse, void* d_logits,
                                int64_t d_stride, void* stream) {
     const char* fn = "k1_token_logprobs_backward";
     int rc = score_check(fn, logits, dtype, n_rows, vocab, inner_rows, inner_stride, outer_stride, temperature, n_ids, k);
@@ -155,6 +156,7 @@ int k1_token_logprobs_backward(const void* logits, int dtype, int64_t n_rows, in
     p.g_top = g_top;
     p.k = g_top ? (int)k : 0;
     p.lse = lse;
+    p.lse_rest = lse_rest;
     p.entropy = entropy;
     p.g_entropy = g_entropy;
     p.g_lse = g_lse;

@@ -1004,7 +1004,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sandwich_rmsnorm_fp8(const at::Te
 // Log-probabilities of given tokens and of the most likely ones
 // ---------------------------------------------------------------------------------------
 struct ScoreOut {
-    at::Tensor logprobs, entropy, lse, top_ids, top;
+    at::Tensor logprobs, entropy, lse, top_ids, top, rest;  // rest: of lse, for a backward
 };
 
 // The rows of logits; without any, a grouping that the C ABI takes.
@@ -1015,7 +1015,7 @@ Rows score_rows(const at::Tensor& logits) {
 }
 
 // ids: [..., K] (K = 1 for a target), undefined: none.
-ScoreOut score_run(const at::Tensor& logits, const at::Tensor& ids, int64_t k, double temperature) {
+ScoreOut score_run(const at::Tensor& logits, const at::Tensor& ids, int64_t k, double temperature, bool want_rest) {
     const Rows L = score_rows(logits);
     c10::cuda::CUDAGuard guard(logits.device());
     const auto lead = logits.sizes().slice(0, logits.dim() - 1);
@@ -1023,18 +1023,21 @@ ScoreOut score_run(const at::Tensor& logits, const at::Tensor& ids, int64_t k, d
     ScoreOut o;
     o.entropy = at::empty(lead, f32);
     o.lse = at::empty(lead, f32);
-    std::vector<int64_t> wide(lead.begin(), lead.end());
-    wide.push_back(k);
+    if (want_rest) o.rest = at::empty(lead, f32);
+    if (k > 0) {
+        std::vector<int64_t> wide(lead.begin(), lead.end());
+        wide.push_back(k);
+        o.top_ids = at::empty(wide, logits.options().dtype(at::kLong));
+        o.top = at::empty(wide, f32);
+    }
     const int64_t n_ids = ids.defined() ? ids.size(-1) : 0;
     if (ids.defined()) o.logprobs = at::empty(ids.sizes(), f32);
-    o.top_ids = at::empty(wide, logits.options().dtype(at::kLong));
-    o.top = at::empty(wide, f32);
     const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
     check_launch(k1_token_logprobs(
         logits.data_ptr(), dtype_code(logits), L.n_rows, L.vocab, L.inner_rows, L.inner_stride, L.outer_stride,
         temperature, ids.defined() ? ids.data_ptr<int64_t>() : nullptr, n_ids, ptr(o.logprobs), k,
-        o.top_ids.data_ptr<int64_t>(), o.top.data_ptr<float>(), o.entropy.data_ptr<float>(), o.lse.data_ptr<float>(),
-        at::cuda::getCurrentCUDAStream().stream()));
+        k > 0 ? o.top_ids.data_ptr<int64_t>() : nullptr, ptr(o.top), o.entropy.data_ptr<float>(), o.lse.data_ptr<float>(),
+        ptr(o.rest), at::cuda::getCurrentCUDAStream().stream()));
     return o;
 }
 
@@ -1043,34 +1046,40 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
                                                   const c10::optional<at::Tensor>& ids_, int64_t k,
                                                   double temperature) {
         const at::Tensor ids = ids_.has_value() ? *ids_ : at::Tensor();
-        ScoreOut o = score_run(logits, ids, k, temperature);
-        ctx->save_for_backward({logits, ids, o.entropy, o.lse, o.top_ids});
+        ScoreOut o = score_run(logits, ids, k, temperature, true);
+        ctx->save_for_backward({logits, ids, o.entropy, o.lse, o.top_ids, o.rest});
         ctx->saved_data["temperature"] = temperature;
         ctx->set_materialize_grads(false);
-        ctx->mark_non_differentiable({o.top_ids});
-        if (ids.defined()) return {o.entropy, o.lse, o.top_ids, o.top, o.logprobs};
-        return {o.entropy, o.lse, o.top_ids, o.top};
+        torch::autograd::variable_list out = {o.entropy, o.lse};
+        if (ids.defined()) out.push_back(o.logprobs);
+        if (k > 0) {
+            ctx->mark_non_differentiable({o.top_ids});
+            out.push_back(o.top_ids);
+            out.push_back(o.top);
+        }
+        return out;
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "the log-probabilities have no second derivative");
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &logits = saved[0], &ids = saved[1], &entropy = saved[2], &lse = saved[3], &top_ids = saved[4];
+        const at::Tensor &logits = saved[0], &ids = saved[1], &entropy = saved[2], &lse = saved[3], &top_ids = saved[4],
+                         &rest = saved[5];
         const at::Tensor none;
         const Rows L = score_rows(logits);
         c10::cuda::CUDAGuard guard(logits.device());
         const auto ready = [](const at::Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; };
-        const at::Tensor g_ent = ready(grads[0]), g_lse = ready(grads[1]), g_top = ready(grads[3]),
-                         g_ids = grads.size() > 4 ? ready(grads[4]) : none;
+        const at::Tensor g_ent = ready(grads[0]), g_lse = ready(grads[1]), g_ids = ids.defined() ? ready(grads[2]) : none,
+                         g_top = top_ids.defined() ? ready(grads.back()) : none;
         if (!g_ent.defined() && !g_lse.defined() && !g_top.defined() && !g_ids.defined()) return {none, none, none, none};
         const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
         at::Tensor d = at::empty(logits.sizes(), logits.options());
         check_launch(k1_token_logprobs_backward(
             logits.data_ptr(), dtype_code(logits), L.n_rows, L.vocab, L.inner_rows, L.inner_stride, L.outer_stride,
             ctx->saved_data["temperature"].toDouble(), ids.defined() ? ids.data_ptr<int64_t>() : nullptr,
-            ids.defined() ? ids.size(-1) : 0, ptr(g_ids), top_ids.data_ptr<int64_t>(), top_ids.size(-1), ptr(g_top),
-            lse.data_ptr<float>(), entropy.data_ptr<float>(), ptr(g_ent), ptr(g_lse), d.data_ptr(), L.vocab,
+            ids.defined() ? ids.size(-1) : 0, ptr(g_ids), top_ids.defined() ? top_ids.data_ptr<int64_t>() : nullptr,
+            top_ids.defined() ? top_ids.size(-1) : 0, ptr(g_top), lse.data_ptr<float>(), ptr(rest), entropy.data_ptr<float>(), ptr(g_ent), ptr(g_lse), d.data_ptr(), L.vocab,
             at::cuda::getCurrentCUDAStream().stream()));
         return {d, none, none, none};
     }
@@ -1080,9 +1089,11 @@ ScoreOut score(const at::Tensor& logits, const at::Tensor& ids_, int64_t k, doub
     TORCH_CHECK(!logits._fw_grad(/*level=*/0).defined(),
                 "the log-probabilities do not support forward AD: they have no jvp");
     const at::Tensor ids = ids_.defined() ? ids_.contiguous() : ids_;
-    if (!at::GradMode::is_enabled() || !logits.requires_grad()) return score_run(logits, ids, k, temperature);
+    if (!at::GradMode::is_enabled() || !logits.requires_grad()) return score_run(logits, ids, k, temperature, false);
     auto out = TokenLogprobs::apply(logits, ids.defined() ? c10::optional<at::Tensor>(ids) : c10::nullopt, k, temperature);
-    return {ids.defined() ? out[4] : at::Tensor(), out[0], out[1], out[2], out[3]};
+    const size_t at = ids.defined() ? 3 : 2;
+    return {ids.defined() ? out[2] : at::Tensor(), out[0], out[1], k > 0 ? out[at] : at::Tensor(),
+            k > 0 ? out[at + 1] : at::Tensor()};
 }
 
 void score_tokens(const at::Tensor& ids, const at::Tensor& logits, const char* what) {

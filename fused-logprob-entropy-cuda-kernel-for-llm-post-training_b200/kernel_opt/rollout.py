@@ -68,6 +68,8 @@ class RolloutHead:
         if lm_head_bias is not None and lm_head_bias.shape != lm_head_weight.shape[:1]:
             raise ValueError(f"lm_head_bias must be [V] for lm_head_weight {tuple(lm_head_weight.shape)}, got "
                              f"{tuple(lm_head_bias.shape)}")
+        if lm_head_bias is not None and lm_head_bias.dtype not in (self.logits_dtype, torch.float32):
+            raise ValueError(f"lm_head_bias must be {self.logits_dtype} or float32, got {lm_head_bias.dtype}")
         names = ["norm_weight", "weight", "weight_scales", "post_norm_weight", "bias"]
         new = [norm_weight.detach(), *quantize_fp8_blocks(lm_head_weight.detach()),
                *(None if t is None else t.detach() for t in (post_norm_weight, lm_head_bias))]

@@ -496,11 +496,11 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
  *     logprobs[i]     = y[token_ids[i]] - l    (an id outside [0, vocab) reads y = 0: -l)
  *     top_ids         = the k largest x, larger first, the lowest index first among equals
  *     top_logprobs[i] = y[top_ids[i]] - l
- *     entropy         = -sum p log p,  lse = l
+ *     entropy         = -sum p log p,  lse = fp32(l),  lse_rest = l - lse (NULL: not wanted)
  * logits: rows as in k1_fused_logprob_entropy_v1 (vocab below 2^30, n_rows up to 2^27).
  * token_ids, logprobs: n_rows x n_ids, n_ids in [0, 1024]; top_ids, top_logprobs: n_rows x k, k in
- * [0, min(128, vocab)]; contiguous.  temperature in [1e-30, 1e30].  Values at or below -1e38
- * count as masked (probability 0, after all others in the order of x).  A row with a NaN or +inf,
+ * [0, min(128, vocab)]; contiguous.  temperature in [1e-30, 1e30].  Values at or below about
+ * -1e38 count as masked (probability 0, after all others in the order of x).  A row with a NaN or +inf,
  * or with every value masked, has no distribution: top_ids -1, every output NaN (lse -inf where
  * all is masked).  No workspace.
  */
@@ -508,12 +508,13 @@ int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t voc
                       int64_t inner_rows, int64_t inner_stride, int64_t outer_stride,
                       double temperature, const int64_t* token_ids, int64_t n_ids, float* logprobs,
                       int64_t k, int64_t* top_ids, float* top_logprobs, float* entropy, float* lse,
-                      void* stream);
+                      float* lse_rest, void* stream);
 
 /*
  * Backward of k1_token_logprobs: d_logits (the logits' dtype, rows d_stride >= vocab elements
- * apart, not the logits' own memory) from the saved lse and entropy and the gradients of the
- * outputs, each of which may be NULL (none).  Rounded once.  A token that a row's lists name
+ * apart, not the logits' own memory) from the saved lse, lse_rest (NULL: 0; a probability then
+ * errs by 2^-24 |lse| of itself) and entropy and the gradients of the outputs, each of which may
+ * be NULL (none).  Rounded once.  A token that a row's lists name
  * several times gets all their gradients; ids outside [0, vocab) get none of their own.  A row
  * whose gradients are all zero gets zeros, whatever its logits hold.
  */
@@ -521,9 +522,9 @@ int k1_token_logprobs_backward(const void* logits, int dtype, int64_t n_rows, in
                                int64_t inner_rows, int64_t inner_stride, int64_t outer_stride,
                                double temperature, const int64_t* token_ids, int64_t n_ids,
                                const float* g_logprobs, const int64_t* top_ids, int64_t k,
-                               const float* g_top, const float* lse, const float* entropy,
-                               const float* g_entropy, const float* g_lse, void* d_logits,
-                               int64_t d_stride, void* stream);
+                               const float* g_top, const float* lse, const float* lse_rest,
+                               const float* entropy, const float* g_entropy, const float* g_lse,
+                               void* d_logits, int64_t d_stride, void* stream);
 
 #ifdef __cplusplus
 }

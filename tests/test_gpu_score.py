@@ -186,12 +186,14 @@ def check_gradient(x, d, ids, g_ids, g_entropy, g_lse, temperature):
     at = torch.where(inside, ids, 0)
     along = torch.where(p > 0, logp, 0.0)
     want = p * (gl[:, None] - g.sum(1, keepdim=True) - ge[:, None] * (along + h[:, None]))
-    size = p * (gl.abs()[:, None] + g.abs().sum(1, keepdim=True) + ge.abs()[:, None] * (along.abs() + h[:, None]))
+    factor = gl.abs()[:, None] + g.abs().sum(1, keepdim=True) + ge.abs()[:, None] * (along.abs() + h[:, None])
+    size = p * factor
     want.scatter_add_(1, at, g * inside)
     size.scatter_add_(1, at, g.abs() * inside)
     s = scale_of(temperature)
     err = (d.double() - s * want).abs()
-    tol = U[x.dtype] * (s * want).abs() + 2e-5 * s * size + TINY[x.dtype]
+    # a probability below fp32's normal numbers (2^-126) is taken as 0: an error of 2^-126 times its factor
+    tol = U[x.dtype] * (s * want).abs() + 2e-5 * s * size + TINY[x.dtype] + 2.0 ** -126 * s * factor
     bad = ~(err <= tol)
     assert not bad.any(), (float((err - tol)[bad].max()), int(bad.sum()))
 
@@ -216,6 +218,23 @@ def test_top_gradient(dtype, n, v, k, temperature, which):
     g_ids = torch.cat([gs["logprob"][:, None] if "logprob" in gs else zero,
                        gs["top"] if "top" in gs else zero.expand(n, k)], 1)
     check_gradient(x.detach(), d, torch.cat([targets[:, None], ids], 1), g_ids, gs.get("entropy"), gs.get("lse"), temperature)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("temperature", [1e-4, 0.01, 0.1, 50.0])
+def test_gradient_at_far_temperatures(dtype, temperature):
+    # lse is thousands of times the logits' spread here: its rounding to fp32 alone would put
+    # probabilities off by 2^-24 |lse|, 4e-3 and more at 1e-4
+    x = logits_of(4, 5001, dtype, spread=4.0)
+    x[0, :40] = x[0].max()          # equal largest ones share the mass
+    x[1, 7] = x[1].max()
+    x = x.requires_grad_(True)
+    ids = torch.arange(12, device="cuda").expand(4, 12)
+    lp, entropy, lse = kernel_opt.fused_token_logprobs(x, ids, temperature)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    gi, ge, gl = 0.3 * torch.randn(4, 12, generator=g, device="cuda"), *(0.3 * torch.randn(2, 4, generator=g, device="cuda"))
+    d, = torch.autograd.grad((lp, entropy, lse), x, (gi, ge, gl))
+    check_gradient(x.detach(), d, ids, gi, ge, gl, temperature)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -309,7 +328,8 @@ def test_only_what_is_asked_has_a_gradient():
     with pytest.raises(RuntimeError, match="forward AD"):
         import torch.autograd.forward_ad as fw
         with fw.dual_level():
-            kernel_opt.fused_token_logprobs(fw.make_dual(x.detach(), torch.ones_like(x)), torch.zeros(4, 1, dtype=torch.int64, device="cuda"))
+            dual = fw.make_dual(x.detach(), torch.ones_like(x))
+            kernel_opt.fused_token_logprobs(dual, torch.zeros(4, 1, dtype=torch.int64, device="cuda"))
 
 
 def test_empty():

@@ -18,20 +18,20 @@ def lib():
     lib = ctypes.CDLL(CAPI_LIB)
     lib.k1_last_error.restype = ctypes.c_char_p
     rows = [p, c_int, i64, i64, i64, i64, i64, c_double]
-    lib.k1_token_logprobs.argtypes = rows + [p, i64, p, i64, p, p, p, p, p]
-    lib.k1_token_logprobs_backward.argtypes = rows + [p, i64, p, p, i64, p, p, p, p, p, p, i64, p]
+    lib.k1_token_logprobs.argtypes = rows + [p, i64, p, i64, p, p, p, p, p, p]
+    lib.k1_token_logprobs_backward.argtypes = rows + [p, i64, p, p, i64, p, p, p, p, p, p, p, i64, p]
     return lib
 
 
 def forward(lib, x=1024, d=BF16, n=4, v=1000, inner=4, t=1.0, ids=2048, n_ids=1, lp=4096, k=5, top=8192, tl=8192,
             out=16384):
-    return lib.k1_token_logprobs(x, d, n, v, inner, v, 0, t, ids, n_ids, lp, k, top, tl, out, out, None)
+    return lib.k1_token_logprobs(x, d, n, v, inner, v, 0, t, ids, n_ids, lp, k, top, tl, out, out, None, None)
 
 
 def backward(lib, x=1024, d=BF16, n=4, v=1000, t=1.0, ids=2048, n_ids=1, g=4096, top=8192, k=5, gt=4096, saved=16384,
              dx=65536, stride=1000):
-    return lib.k1_token_logprobs_backward(x, d, n, v, 4, v, 0, t, ids, n_ids, g, top, k, gt, saved, saved, None, None,
-                                          dx, stride, None)
+    return lib.k1_token_logprobs_backward(x, d, n, v, 4, v, 0, t, ids, n_ids, g, top, k, gt, saved, None, saved, None,
+                                          None, dx, stride, None)
 
 
 def test_refuses(lib):
