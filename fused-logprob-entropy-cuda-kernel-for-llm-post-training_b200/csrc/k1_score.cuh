@@ -18,7 +18,7 @@
 // group of its vectors (one chunk's 8 usually), which the sums need anyway.  Then
 //   T0, the k-th largest of the threads' maxima cut to 16 bits, is a bound that at least k
 //   elements reach, and usually few more;
-//   the groups that reach T0 are read again (from L2, some k x 128 bytes) and their elements that
+//   the groups that reach T0 are read again (from L2, some k x 64 bytes) and their elements that
 //   do go to a list of 64-bit keys (value, then lowest index), each key's rank in the list is its
 //   place.
 // Where that overflows (many equal values, masks that leave fewer than k, rows whose large values
@@ -26,6 +26,7 @@
 // pass and takes the equal ones in index order.  Either way the result is exact.
 #pragma once
 
+#include <cstddef>
 #include <type_traits>
 
 #include "k1_common.cuh"
@@ -36,7 +37,7 @@ namespace score {
 
 constexpr int kMaxGroups = 32;   // maxima per thread
 constexpr int kKeys = 256;       // maxima that the bound is found among
-constexpr int kCand = 1024;      // entries of the list
+constexpr int kCand = 512;       // entries of the list
 constexpr int kMaxTop = 128;     // largest k
 constexpr int kMaxIds = 1024;    // given tokens per row
 constexpr int kMaxCluster = 8;
@@ -290,29 +291,44 @@ __device__ __forceinline__ uint64_t entry_of(float x, int64_t e) {
     return ((uint64_t)key_of(x) << 32) | (uint32_t)~(uint32_t)e;
 }
 
+// Shared memory is kept small: what it leaves is L1, through which the loads in flight go (with 26
+// instead of 24 KB per block, 182 instead of 168 per SM, 1024 x 128256 bf16 with gradient took 165 us
+// instead of 151; with all of it as shared memory, 2048 x 151936 took 372 instead of 323).
 template <int TH>
-struct FwdSmem {
+struct FwdSums {
     static constexpr int W = TH / 32;
-    unsigned wmax[W];         // keys of the warps' maxima
     double wz[W], wt[W];
+    unsigned wmax[W];         // keys of the warps' maxima
+};
+// Only where a list is wanted; behind it the groups' maxima, [groups][TH], as the upper 16 bits of keys.
+struct FwdList {
     int n_cand;
     unsigned bound;           // T0's key, its upper 16 bits
-    unsigned prefix, need, scan[W];
+    unsigned prefix, need, scan[8];
+    int n_list;
     uint16_t keys[kKeys];
-    unsigned hist[256];
-    uint64_t cand[kCand];
+    uint16_t list[kCand];
+    union {
+        uint64_t cand[kCand];
+        unsigned hist[256];   // while the list is empty
+    };
 };
 // Of a cluster's first block, written by all: their sums and their lists.
 struct Meet {
     RowPartial part[kMaxCluster];
     int n[kMaxCluster];
-    uint64_t list[kMaxCluster][kMaxTop];
+    uint64_t list[kMaxCluster][kMaxTop];  // only where a list is wanted
 };
+template <int TH, bool TOP>
+constexpr size_t fwd_smem(int cluster, int groups) {
+    return sizeof(FwdSums<TH>) + (cluster > 1 ? (TOP ? sizeof(Meet) : offsetof(Meet, list)) : 0) +
+           (TOP ? sizeof(FwdList) + (size_t)groups * TH * 2 : 0);
+}
 
 // The block's list by exact selection: the kk-th largest key by histograms, what lies above it,
 // and the first ones in index order among what equals it.
 template <typename T, int TH>
-__device__ __noinline__ void select_exact(const Row<T>& row, int j0, int j1, int kk, FwdSmem<TH>& sm) {
+__device__ __noinline__ void select_exact(const Row<T>& row, int j0, int j1, int kk, FwdList& sm) {
     constexpr int E = DT<T>::kEPV;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto each = [&](int j, auto&& f) {
@@ -396,7 +412,7 @@ __device__ __noinline__ void select_exact(const Row<T>& row, int j0, int j1, int
 // T0: a bound that kk of the threads' maxima reach and, to 16 bits, no more than their equals do (one
 // warp).
 template <int TH>
-__device__ __forceinline__ void find_bound(int kk, FwdSmem<TH>& sm) {
+__device__ __forceinline__ void find_bound(int kk, FwdList& sm) {
     const int lane = threadIdx.x & 31;
     unsigned mine[kKeys / 32], top = 0, low = 0xffffu;
 #pragma unroll
@@ -425,62 +441,78 @@ __device__ __forceinline__ void find_bound(int kk, FwdSmem<TH>& sm) {
     if (lane == 0) sm.bound = t;
 }
 
-// The elements of the part that reach T0 go to sm.cand: their groups are read again, U lanes to a
-// group.  Every warp sees to its own threads' groups.
+// The elements of the part that reach T0 go to sm.cand: their groups are listed, and the groups'
+// vectors read again, dealt to all threads (lists that overflow are left to select_exact: n_cand says
+// so).  Up to four loads per thread are in flight at once: with each warp reading its own threads'
+// groups one after the other, k = 64 of 50264 took 11300 cycles here.
 template <typename T, int TH, int U>
-__device__ __forceinline__ void gather(const Row<T>& row, int j0, int j1, float thread_max, const FwdParams& p,
-                                       const float* gmax, unsigned bound, FwdSmem<TH>& sm) {
-    constexpr int E = DT<T>::kEPV;
-    const int tid = threadIdx.x, lane = tid & 31;
+__device__ __forceinline__ void gather(const Row<T>& row, int j0, int j1, unsigned thread_key, const FwdParams& p,
+                                       const uint16_t* gmax, unsigned bound, FwdList& sm) {
+    constexpr int E = DT<T>::kEPV, B = 4;
+    const int tid = threadIdx.x;
     const float t0 = value_of(bound << 16);
-    unsigned mine = 0;  // this thread's groups
-    if (bound == 0) {
-        mine = p.groups < 32 ? (1u << p.groups) - 1u : ~0u;
-    } else if (thread_max >= t0) {
+    if (bound != 0) {
+        if (thread_key >= bound) {
+            unsigned mine = 0;  // this thread's groups
 #pragma unroll 4
-        for (int g = 0; g < p.groups; ++g) mine |= (gmax[g * TH + tid] >= t0 ? 1u : 0u) << g;
-    }
-    unsigned any = __ballot_sync(0xffffffffu, mine != 0);
-    while (any) {
-        int of = -1, group = 0;
-#pragma unroll
-        for (int s = 0; s < 32 / U; ++s) {
-            if (!any) break;
-            const int l = __ffs((int)any) - 1;
-            const unsigned m = __shfl_sync(0xffffffffu, mine, l);
-            if (lane == l) mine &= mine - 1;
-            if ((m & (m - 1)) == 0) any &= any - 1;
-            if (lane / U == s) {
-                of = l;
-                group = __ffs((int)m) - 1;
-            }
+            for (int g = 0; g < p.groups; ++g) mine |= (gmax[g * TH + tid] >= bound ? 1u : 0u) << g;
+            int at = atomicAdd(&sm.n_list, __popc(mine));
+            for (; mine; mine &= mine - 1, ++at)
+                if (at < kCand) sm.list[at] = (uint16_t)((__ffs((int)mine) - 1) * TH + tid);
         }
-        if (of >= 0) {
-            int j = j0 + (group * p.group_chunks * U + lane % U) * TH + (tid - lane) + of;
-            for (int c = 0; c < p.group_chunks && j < j1; ++c, j += U * TH) {
-                uint4 v[1];
-                row.template load<1>(v, j, 0, j1);
-                float x[E];
-                unpack<T>(v[0], x);
-                unsigned hit = 0;
+        __syncthreads();
+    }
+    const int per = p.group_chunks * U;
+    const int n_list = bound != 0 ? sm.n_list : 0;
+    const int tasks = bound == 0 ? j1 - j0 : n_list <= kCand ? n_list * per : 0;
+    if (n_list > kCand && tid == 0) sm.n_cand = kCand + 1;
+    for (int i = tid; i < tasks; i += B * TH) {
+        uint4 v[B];
+        int j[B];
 #pragma unroll
-                for (int q = 0; q < E; ++q) hit |= (bound == 0 || x[q] >= t0 ? 1u : 0u) << q;
-                if (j < row.lo || j >= row.hi)
-#pragma unroll
-                    for (int q = 0; q < E; ++q)
-                        if (!row.inside(row.at(j, q))) hit &= ~(1u << q);
-                if (hit) {
-                    int at = atomicAdd(&sm.n_cand, __popc(hit));
-#pragma unroll
-                    for (int q = 0; q < E; ++q)
-                        if (hit >> q & 1) {
-                            if (at < kCand) sm.cand[at] = entry_of(x[q], row.at(j, q));
-                            ++at;
-                        }
+        for (int q = 0; q < B; ++q) {
+            const int task = i + q * TH;
+            j[q] = j1;
+            if (task < tasks) {
+                if (bound == 0) {
+                    j[q] = j0 + task;
+                } else {
+                    const int entry = sm.list[task / per];
+                    j[q] = j0 + (entry / TH * per + task % per) * TH + entry % TH;
                 }
             }
         }
-        __syncwarp();
+        // whole vectors first, all in flight together; the row's first and last are put together after
+#pragma unroll
+        for (int q = 0; q < B; ++q) {
+            v[q] = make_uint4(0, 0, 0, 0);
+            if (j[q] < j1 && j[q] >= row.lo && j[q] < row.hi) v[q] = ldg_stream(row.base + j[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < B; ++q)
+            if (j[q] < j1 && (j[q] < row.lo || j[q] >= row.hi)) v[q] = row.partial(j[q]);
+#pragma unroll
+        for (int q = 0; q < B; ++q) {
+            if (j[q] >= j1) continue;
+            float x[E];
+            unpack<T>(v[q], x);
+            unsigned hit = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) hit |= (bound == 0 || x[e] >= t0 ? 1u : 0u) << e;
+            if (j[q] < row.lo || j[q] >= row.hi)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (!row.inside(row.at(j[q], e))) hit &= ~(1u << e);
+            if (hit) {
+                int at = atomicAdd(&sm.n_cand, __popc(hit));
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (hit >> e & 1) {
+                        if (at < kCand) sm.cand[at] = entry_of(x[e], row.at(j[q], e));
+                        ++at;
+                    }
+            }
+        }
     }
 }
 
@@ -503,9 +535,10 @@ __device__ __forceinline__ void st_cluster32(uint32_t addr, uint32_t v) {
 template <typename T, int TH, int U, int MINB, bool TOP>
 __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char raw[];
-    FwdSmem<TH>& sm = *reinterpret_cast<FwdSmem<TH>*>(raw);
-    Meet& meet = *reinterpret_cast<Meet*>(raw + sizeof(FwdSmem<TH>));  // only in a cluster
-    float* gmax = reinterpret_cast<float*>(raw + sizeof(FwdSmem<TH>) + (p.cluster > 1 ? sizeof(Meet) : 0));  // [groups][TH]
+    FwdSums<TH>& sums = *reinterpret_cast<FwdSums<TH>*>(raw);
+    Meet& meet = *reinterpret_cast<Meet*>(raw + sizeof(FwdSums<TH>));  // only in a cluster
+    FwdList& sm = *reinterpret_cast<FwdList*>(raw + sizeof(FwdSums<TH>) + (p.cluster > 1 ? sizeof(Meet) : 0));
+    uint16_t* gmax = reinterpret_cast<uint16_t*>(&sm + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = p.cluster > 1 ? (int)ring::cluster_rank() : 0;
     const int64_t r = p.cluster > 1 ? blockIdx.x / p.cluster : blockIdx.x;
@@ -520,8 +553,8 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
 
     State st;
     st.init();
-    float own = -INFINITY;  // the thread's maximum
-    float odd = -INFINITY;  // the maximum of the groups of odd number, where threads give two keys
+    unsigned own = 0, odd = 0;  // keys of the thread's maximum, and of that of its groups of odd number
+    auto key16 = [](float m) { return key_of(m) >> 16; };
     {
         int g = 0, left = p.group_chunks;
         float gm = -INFINITY;
@@ -542,11 +575,12 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
             fetch(j + U * TH);  // in flight while this chunk is added
             const float mc = add_chunk<T, U>(v, st, c);
             if constexpr (TOP) {
-                own = fmax_nan(own, mc);
                 gm = fmax_nan(gm, mc);
                 if (--left == 0 || j + U * TH >= j1) {
-                    gmax[g * TH + tid] = gm;
-                    if (TH < kKeys && (g & 1)) odd = fmax_nan(odd, gm);
+                    const unsigned key = key16(gm);
+                    gmax[g * TH + tid] = (uint16_t)key;
+                    own = max(own, key);
+                    if (g & 1) odd = max(odd, key);
                     ++g;
                     left = p.group_chunks;
                     gm = -INFINITY;
@@ -554,15 +588,16 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
             }
         }
         if constexpr (TOP) {
-            for (; g < p.groups; ++g) gmax[g * TH + tid] = -INFINITY;
-            auto key16 = [](float m) { return m > Floor<T>::value ? (uint16_t)(key_of(m) >> 16) : (uint16_t)0; };
+            for (; g < p.groups; ++g) gmax[g * TH + tid] = 0;
+            // one key per thread, or two where that makes too few; what is masked bounds nothing
+            auto real = [&](unsigned key) { return key > key16(Floor<T>::value) ? (uint16_t)key : (uint16_t)0; };
             if constexpr (TH < kKeys) {
-                float even = -INFINITY;
-                for (int q = 0; q < p.groups; q += 2) even = fmax_nan(even, gmax[q * TH + tid]);
-                sm.keys[tid] = key16(even);
-                sm.keys[TH + tid] = key16(odd);
+                unsigned even = 0;
+                for (int q = 0; q < p.groups; q += 2) even = max(even, (unsigned)gmax[q * TH + tid]);
+                sm.keys[tid] = real(even);
+                sm.keys[TH + tid] = real(odd);
             } else {
-                sm.keys[tid] = key16(own);
+                sm.keys[tid] = real(own);
             }
         }
     }
@@ -572,14 +607,14 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
 
     // the block's sums, relative to its maximum; one warp looks for the bound meanwhile
     const bool empty = st.m <= Floor<T>::value;
-    if (lane == 0) sm.wmax[warp] = key_of(empty ? -INFINITY : st.m);
-    if (TOP && tid == 0) sm.n_cand = 0;
+    if (lane == 0) sums.wmax[warp] = key_of(empty ? -INFINITY : st.m);
+    if (TOP && tid == 0) sm.n_cand = sm.n_list = 0;
     __syncthreads();
     RowPartial part;
     {
-        unsigned m = sm.wmax[0];
+        unsigned m = sums.wmax[0];
 #pragma unroll
-        for (int i = 1; i < TH / 32; ++i) m = max(m, sm.wmax[i]);
+        for (int i = 1; i < TH / 32; ++i) m = max(m, sums.wmax[i]);
         part.m = value_of(m);
         double z = 0.0, t = 0.0;
         if (!empty) {
@@ -591,8 +626,8 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
         z = warp_sum(z);
         t = warp_sum(t);
         if (lane == 0) {
-            sm.wz[warp] = z;
-            sm.wt[warp] = t;
+            sums.wz[warp] = z;
+            sums.wt[warp] = t;
         }
     }
     // elements of the part, and the entries wanted of it
@@ -604,8 +639,8 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
     part.z = part.t = 0.0;
 #pragma unroll
     for (int i = 0; i < TH / 32; ++i) {
-        part.z += sm.wz[i];
-        part.t += sm.wt[i];
+        part.z += sums.wz[i];
+        part.t += sums.wt[i];
     }
     part.pad = 0.f;
     // a NaN or +inf somewhere: no list either, what cannot be ordered must not reach one

@@ -54,7 +54,7 @@ int score_launch(const char* fn, k1::score::FwdParams p, int64_t n_rows, int sms
     p.group_chunks = (chunks + kMaxGroups - 1) / kMaxGroups;
     p.groups = (chunks + p.group_chunks - 1) / p.group_chunks;
     auto kern = k1_score_kernel<T, TH, U, MINB, TOP>;
-    const size_t smem = sizeof(FwdSmem<TH>) + (cluster > 1 ? sizeof(Meet) : 0) + (TOP ? (size_t)p.groups * TH * 4 : 0);
+    const size_t smem = fwd_smem<TH, TOP>(cluster, p.groups);
     int rc = allow_smem(kern, dev, smem);
     if (rc) return rc;
     return launched(fn, launch_cluster(kern, dim3((unsigned)(n_rows * cluster)), TH, smem, cluster, st, p));
