@@ -232,7 +232,8 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
 // ------------------------------------------------------------------------------------
 // The kernels above and in k1_norm.cuh load a row, reduce it twice and store it, and nothing is in flight
 // meanwhile but other blocks' loads, of which registers allow two or three blocks per SM (75 us
-// forward and 128 backward at 8192 x 3584 bf16; the bytes alone take 36 and 55).  Here a block is a few
+// forward and 128 backward at 8192 x 3584 bf16; the bytes alone take 36 and 55, these kernels 44 and 68,
+// and 56 forward with 8-bit output).  Here a block is a few
 // groups of threads, each with rows and a ring of stages of its own: a stage holds one row of every
 // input, a bulk copy each, counted on the stage's mbarrier.  When a group has read a stage (which the
 // row's second reduction, a barrier of the group, tells), one thread orders the group's next row
@@ -373,7 +374,9 @@ __device__ __forceinline__ void order_row(const RingGroup& g, const Ring& q, int
         }
 }
 
-// Vectors as pairs of fp32 numbers: instructions per element are what these kernels run out of first.
+// Vectors as pairs of fp32 numbers: instructions are what these kernels run out of first (22 per element
+// forward and 34 backward, counting all that a row costs; with generic addresses, single conversions and
+// every option tested per row it was 48 and 86, and bound by that).
 template <typename T>
 struct Vec {
     static constexpr int E = DT<T>::kEPV, N = E / 2;

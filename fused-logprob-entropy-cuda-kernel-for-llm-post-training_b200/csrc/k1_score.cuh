@@ -24,6 +24,12 @@
 // Where that overflows (many equal values, masks that leave fewer than k, rows whose large values
 // lie in few threads' columns) the block finds the k-th largest value by histograms of 8 bits a
 // pass and takes the equal ones in index order.  Either way the result is exact.
+//
+// Forward and backward are bound by traffic where rows are many and wide; small calls by latency, and
+// lists by the chain of short phases behind a row's last load.  Measured on B200 (us, with the call):
+// 2048 x 151936 bf16, 32 given tokens, forward 108 (5.8 TB/s) and backward 211 (5.9 TB/s), 323 to 335
+// together; 1024 x 128256 bf16 top 8 with gradient 148; 512 x 152064 bf16 top 20 38 to 39 (32 without a
+// list, its bytes 24); 1023 x 50257 fp16 top 64 33 (22 without, 16); one row of 151936 top 20 11.
 #pragma once
 
 #include <cstddef>
