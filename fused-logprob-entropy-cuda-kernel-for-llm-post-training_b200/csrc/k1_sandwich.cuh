@@ -256,7 +256,7 @@ constexpr int kMaxRingGroups = 15;  // a named barrier each
 constexpr int kMaxRingStages = 4;
 // Threads of a block: what registers allow (a thread holds E NV columns, and backward 2 E NV sums).
 template <int E, int NV>
-constexpr int kRingFwd = E * NV >= 16 ? 704 : 960;
+constexpr int kRingFwd = E * NV >= 16 ? 896 : 960;
 template <int E, int NV>
 constexpr int kRingBwd = E * NV >= 16 ? 512 : 896;
 
@@ -802,11 +802,12 @@ __global__ void __launch_bounds__(kRingBwd<DT<T>::kEPV, NV>, 1) k1_sandwich_bwd_
 }
 
 // The blocks' partial sums (blockIdx.y: of dw, or of A), added in a fixed order as in
-// k1_rmsnorm_dw_kernel; A gives dwp (times a gate per column) and that gate's gradient (times wp).
+// k1_rmsnorm_dw_kernel, by 32 warps so that one batch of loads covers them.  A gives dwp (times a gate per
+// column) and that gate's gradient (times wp).
 template <typename W>
-__global__ void __launch_bounds__(512) k1_sandwich_dw_kernel(const float* part, int parts, int h, W* dw, W* dwp, W* dg,
+__global__ void __launch_bounds__(1024) k1_sandwich_dw_kernel(const float* part, int parts, int h, W* dw, W* dwp, W* dg,
                                                              const W* wp, const W* gate) {
-    __shared__ float sums[16][33];
+    __shared__ float sums[32][33];
     pdl_wait();
     pdl_trigger();
     part += (int64_t)blockIdx.y * parts * h;
@@ -815,14 +816,14 @@ __global__ void __launch_bounds__(512) k1_sandwich_dw_kernel(const float* part, 
     float v = 0.f;
     if (col < h) {
 #pragma unroll 8
-        for (int i = warp; i < parts; i += 16) v += part[(int64_t)i * h + col];
+        for (int i = warp; i < parts; i += 32) v += part[(int64_t)i * h + col];
     }
     sums[warp][lane] = v;
     __syncthreads();
     if (warp == 0 && col < h) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += sums[i][lane];
+        for (int i = 0; i < 32; ++i) t += sums[i][lane];
         if (blockIdx.y == 0) {
             if (dw) DT<W>::store1(dw + col, t);
         } else {

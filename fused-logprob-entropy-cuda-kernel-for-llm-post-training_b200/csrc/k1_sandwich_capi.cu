@@ -341,7 +341,7 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
         using W = decltype(tag);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)((hidden + 31) / 32), want & 6 ? 2 : 1);
-        cfg.blockDim = dim3(512);
+        cfg.blockDim = dim3(1024);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -17,7 +17,8 @@ pytestmark = pytest.mark.gpu
 
 E = 2.0 ** -24
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: E}
-TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0}
+# half the spacing of the smallest numbers a type holds
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
