@@ -232,8 +232,8 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
 // ------------------------------------------------------------------------------------
 // The kernels above and in k1_norm.cuh load a row, reduce it twice and store it, and nothing is in flight
 // meanwhile but other blocks' loads, of which registers allow two or three blocks per SM (75 us
-// forward and 128 backward at 8192 x 3584 bf16; the bytes alone take 36 and 55, these kernels 44 and 68,
-// and 56 forward with 8-bit output).  Here a block is a few
+// forward and 128 backward at 8192 x 3584 bf16; the bytes alone take 36 and 55, these kernels 39 and 68,
+// and 53 forward with 8-bit output).  Here a block is a few
 // groups of threads, each with rows and a ring of stages of its own: a stage holds one row of every
 // input, a bulk copy each, counted on the stage's mbarrier.  When a group has read a stage (which the
 // row's second reduction, a barrier of the group, tells), one thread orders the group's next row
@@ -255,8 +255,10 @@ struct Ring {
 constexpr int kMaxRingGroups = 15;  // a named barrier each
 constexpr int kMaxRingStages = 4;
 // Threads of a block: what registers allow (a thread holds E NV columns, and backward 2 E NV sums).
-template <int E, int NV>
-constexpr int kRingFwd = E * NV >= 16 ? 896 : 960;
+// Forward, rows of which that many threads hold one only (LONG) have 1024 for two, which is worth the
+// 64 registers: 3584 x 8192 bf16 46 to 44 us and 58 to 51 with 8-bit output; at 7168 x 4096 44 instead of 42.6.
+template <int E, int NV, bool LONG = false>
+constexpr int kRingFwd = LONG ? 1024 : E * NV >= 16 ? 896 : 960;
 template <int E, int NV>
 constexpr int kRingBwd = E * NV >= 16 ? 512 : 896;
 
@@ -467,8 +469,8 @@ struct Weights {
     }
 };
 
-template <typename T, int NV, int OUT>
-__global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV>, 1) k1_sandwich_ring_kernel(FwdParams p, Ring q) {
+template <typename T, int NV, int OUT, bool LONG>
+__global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV, LONG>, 1) k1_sandwich_ring_kernel(FwdParams p, Ring q) {
     using V = Vec<T>;
     constexpr int E = V::E, N = V::N;
     extern __shared__ __align__(16) unsigned char raw[];

@@ -160,12 +160,17 @@ int sandwich_forward(const char* fn, int out, const void* x, int64_t x_stride, c
         using T = decltype(tag);
         constexpr int V = k1::DT<T>::kEPV;
         const int inputs = gate_kind == GATE_FULL ? 3 : 2;
+        const bool lng = hidden / V > k1::norm::kRingFwd<V, 2>;  // two such groups have more threads
         const k1::norm::Ring q = ring_of(sh.e, n, hidden, es, inputs, k1::norm::kRingFwd<V, 1>,
-                                         k1::norm::kRingFwd<V, 2>, sms);
+                                         lng ? k1::norm::kRingFwd<V, 2, true> : k1::norm::kRingFwd<V, 2>, sms);
         if (q.groups > 0)
             return with_ring(q, [&](auto NV) {
-                auto kern = same ? k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::SAME>
-                                 : k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::FP8>;
+                auto kern = same ? k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::SAME, false>
+                                 : k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::FP8, false>;
+                if constexpr (NV == 2)
+                    if (lng)
+                        kern = same ? k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::SAME, true>
+                                    : k1::norm::k1_sandwich_ring_kernel<T, NV, k1::norm::FP8, true>;
                 const int threads = q.groups * q.threads;
                 const size_t smem = ring_smem(q);
                 int per_sm = 0;
