@@ -233,14 +233,15 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
 // The kernels above and in k1_norm.cuh load a row, reduce it twice and store it, and nothing is in flight
 // meanwhile but other blocks' loads, of which registers allow two or three blocks per SM (75 us
 // forward and 128 backward at 8192 x 3584 bf16; the bytes alone take 36 and 55, these kernels 39 and 68,
-// and 53 forward with 8-bit output).  Here a block is a few
-// groups of threads, each with rows and a ring of stages of its own: a stage holds one row of every
-// input, a bulk copy each, counted on the stage's mbarrier.  When a group has read a stage (which the
-// row's second reduction, a barrier of the group, tells), one thread orders the group's next row
-// into it.  So 100 KB and more per SM are in flight whatever the groups wait for.  A thread has the
-// columns that it would have in the other kernels and sums in the same order, so results are the
-// same bits.  Sums over rows stay in registers and are added over the groups, in their order, at
-// the end; the weights are in shared memory too, as fp32, and not in registers.
+// and 53 forward with 8-bit output).  Here a block is a few groups of threads, each with rows and a ring
+// of stages of its own: a stage holds one row of every input, a bulk copy each, counted on the stage's
+// mbarrier.  When a group has read a stage (which the row's second reduction, a barrier of the group,
+// tells), one thread orders the group's next row into it.  So 100 KB and more per SM are in flight
+// whatever the groups wait for.  Columns are summed in pairs, so a row's last bits may differ from those
+// of the other kernels, which keep the order of the norms without POST (from the stored stream on their
+// y is the residual norm's): one by one the sums would cost the packed arithmetic.  Sums over rows stay
+// in registers and are added over the groups, in their order, at the end; the weights are in shared
+// memory too, as fp32, and not in registers.
 //
 // Every wait is bounded; one that runs out sets bit 0 of the wait status word, the group's rows from
 // there on are NaN, and a block leaves only when the copies that it ordered have landed.

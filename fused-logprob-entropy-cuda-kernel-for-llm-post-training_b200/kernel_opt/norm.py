@@ -47,7 +47,9 @@ def fused_sandwich_rmsnorm(x: torch.Tensor, residual: torch.Tensor, post_weight:
     both fp32.  gate: None, [H] of the weights' dtype, or x's leading dimensions with H or 1 columns in
     x's dtype (other shapes: expand them).  branch_scale, residual_scale: finite numbers.
     Differentiable (once, backwards) in x, residual, both weights and the gate, through y and the
-    stream."""
+    stream.  Rows of few and of many (more than the device has SMs) are summed in different orders,
+    so a row's last bits may depend on which of the two it is in; within either they do not depend
+    on the other rows, and the same call gives the same bits."""
     return _C.sandwich_rmsnorm(x, residual, post_weight, weight, gate, branch_scale, residual_scale, eps)
 
 

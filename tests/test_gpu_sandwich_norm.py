@@ -294,3 +294,23 @@ def test_captured_and_on_another_stream():
         torch.cuda.synchronize()
         for a, b in zip(held, step()):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("n,h", [(700, 256), (460, 1000), (450, 2048), (501, 3584), (333, 4096), (300, 5120), (299, 8192)])
+def test_more_rows_than_sms(dtype, gate, n, h):
+    t, gy, gs = inputs(n, h, dtype, gate)
+    y, stream, got = run(t, gy, gs, 0.7, 0.9)
+    check_forward(t, y, stream, 0.7, 0.9)
+    check_grads(t, stream, gy, gs, got, 0.7, 0.9)
+    q, scales, s8 = kernel_opt.fused_sandwich_rmsnorm_fp8(**t, branch_scale=0.7, residual_scale=0.9, eps=EPS)
+    assert torch.equal(s8, stream)
+    s = stream.double()
+    v = s / (s.square().mean(-1, keepdim=True) + EPS).sqrt() * t["weight"].double()
+    step = scales.double().repeat_interleave(128, 1)[:, :h]
+    top = torch.nn.functional.pad(v.abs(), (0, -h % 128)).unflatten(-1, (-1, 128)).amax(-1) / 448
+    # the norm's own error (see check_forward) and four more roundings
+    within(scales, top, 44 * E * top, "scales")
+    # half a step of e4m3 (2^-4 of the value, or 2^-10 where it is subnormal), and the same
+    within(q.double() * step, v, torch.maximum(v.abs() / 16, step / 1024) * (1 + 100 * E) + 100 * E * v.abs(), "q")
