@@ -33,8 +33,8 @@ CAPI_UNITS = {
     "k1_decode_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_tc.cuh",
                           "k1_norm.cuh", "k1_norm_host.cuh", "k1_fp8_linear.cuh", "k1_sample.cuh",
                           "k1_sample_math.cuh"],
-    "k1_sandwich_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_norm.cuh", "k1_norm_host.cuh",
-                            "k1_sandwich.cuh"],
+    "k1_sandwich_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_norm.cuh",
+                            "k1_norm_host.cuh", "k1_sandwich.cuh"],
     "k1_score_capi.cu": ["k1_host.cuh", "k1_common.cuh", "k1_sync.cuh", "k1_score.cuh"],
 }
 OBJDIR = os.path.join(HERE, "build")
