@@ -243,8 +243,10 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
 // in registers and are added over the groups, in their order, at the end; the weights are in shared
 // memory too, as fp32, and not in registers.
 //
-// Every wait is bounded; one that runs out sets bit 0 of the wait status word, the group's rows from
-// there on are NaN, and a block leaves only when the copies that it ordered have landed.
+// Every wait is bounded; one that runs out, be it for one thread of a group alone, sets bit 0 of the wait
+// status word.  That thread brings NaN into the sums over the row and over its columns: from there on the
+// group's rows are NaN (backward without a gradient of y: dx, a gate's per row, and the columns of the threads
+// that saw nothing land).  A block leaves only when the copies that it ordered have landed.
 struct Ring {
     int groups, threads;  // groups per block, threads per group
     int e, nv;            // elements of a vector, vectors per thread
@@ -281,6 +283,12 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
 __device__ __forceinline__ void sts16(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+
+#ifdef K1_WAIT_TEST
+// Test only: one thread of block 0's first group takes the group's row of this number, and all after it,
+// for rows whose wait ran out; the others see them land.  -1: off.
+static __device__ long long k1_test_lone = -1;
+#endif
 
 // One group's view of its ring (shared-memory addresses).
 struct RingGroup {
@@ -323,6 +331,13 @@ struct RingGroup {
     // The current stage holds row i of the group (or the wait ran out, now or before).
     __device__ __forceinline__ uint32_t wait(int i) {
         if (ok && !(ok = wait_for(at, parity))) failed = i;
+#ifdef K1_WAIT_TEST
+        if (ok && k1_test_lone == i && blockIdx.x == 0 && threadIdx.x == 5) {
+            ok = false;
+            failed = i;
+            atomicOr(&k1_ring_error, 1u);
+        }
+#endif
         return stages + at * stage_bytes;
     }
     __device__ __forceinline__ void next() {
@@ -517,8 +532,9 @@ __global__ void __launch_bounds__(kRingFwd<DT<T>::kEPV, NV, LONG>, 1) k1_sandwic
 #pragma unroll
             for (int k = 0; k < N; ++k) two = fma2(x[j][k], x[j][k], two);
         }
+        if (!g.ok) two.x = __int_as_float(0x7fc00000);  // one thread's wait ran out: the row is lost to all
         float sum = g.sum(two.x + two.y, threads, false);
-        const float r1 = g.ok ? rsqrtf(fmaf(sum, inv_h, p.eps)) : __int_as_float(0x7fc00000);
+        const float r1 = rsqrtf(fmaf(sum, inv_h, p.eps));
         if (p.rstd_post && t == 0) p.rstd_post[row] = r1;
         const float2 k1 = splat(r1 * token);
         two = splat(0.f);

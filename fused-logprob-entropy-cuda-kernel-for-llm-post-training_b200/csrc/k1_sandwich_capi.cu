@@ -17,6 +17,11 @@ cudaError_t k1_sandwich_wait_status(unsigned* bits) {
 cudaError_t k1_sandwich_set_withhold(long long withhold) {
     return cudaMemcpyToSymbol(k1::k1_test_withhold, &withhold, sizeof withhold);
 }
+
+// Not part of the product: see k1_test_lone.
+extern "C" int k1_test_set_lone(long long row) {
+    return cudaMemcpyToSymbol(k1::norm::k1_test_lone, &row, sizeof row) == cudaSuccess ? K1_OK : K1_ERR_CUDA;
+}
 #endif
 
 namespace {
