@@ -698,6 +698,27 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8_blocks(const at::Tensor& w) {
     return {q, scales};
 }
 
+// Whether a and b, both [M, N] of one type with unit stride along N, are the same elements.
+bool same_rows(const at::Tensor& a, const at::Tensor& b) {
+    return a.data_ptr() == b.data_ptr() && (a.size(0) == 1 || a.stride(0) == b.stride(0));
+}
+
+// Whether they share memory.  Column blocks of one buffer lie between each other's rows, so the rows' own
+// ranges count, not the tensors'; b's rows do not overlap (stride(0) >= N).
+bool rows_meet(const at::Tensor& a, const at::Tensor& b) {
+    const int64_t M = a.size(0), es = a.element_size(), width = a.size(1) * es;
+    const auto start = [](const at::Tensor& t) { return (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    const int64_t sa = M > 1 ? a.stride(0) * es : 0, sb = M > 1 ? b.stride(0) * es : width;
+    const int64_t a0 = start(a), b0 = start(b);
+    if (a0 + (M - 1) * sa + width <= b0 || b0 + (M - 1) * sb + width <= a0) return false;
+    for (int64_t i = 0; i < M; ++i) {
+        const int64_t at = a0 + i * sa - b0;  // the first row of b that ends behind it
+        const int64_t j = at < width ? 0 : (at - width) / sb + 1;
+        if (j < M && j * sb < at + width) return true;
+    }
+    return false;
+}
+
 at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
                       const at::Tensor& weight_scales, at::ScalarType out_dtype, const c10::optional<at::Tensor>& out,
                       const c10::optional<at::Tensor>& bias_, const c10::optional<std::string>& activation,
@@ -756,16 +777,9 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scales, const at:
         residual = rows2d(*residual_);
         // broadcast rows (and what torch lets overlap) are laid out
         if (M > 1 && residual.stride(0) < N) residual = residual.contiguous();
-        if (out.has_value() && M > 0 && N > 0) {
-            const auto range = [&](const at::Tensor& t) {
-                const char* at = (const char*)t.data_ptr();
-                return std::make_pair(at, at + ((M - 1) * (M > 1 ? t.stride(0) : 0) + N) * t.element_size());
-            };
-            const auto a = range(y), b = range(residual);
-            const bool same = a.first == b.first && (M == 1 || y.stride(0) == residual.stride(0));
-            TORCH_CHECK_VALUE(same || a.second <= b.first || b.second <= a.first,
+        if (out.has_value() && M > 0 && N > 0)
+            TORCH_CHECK_VALUE(same_rows(y, residual) || !rows_meet(y, residual),
                               "residual must be the output itself or lie apart from it");
-        }
     }
     check_launch(k1_fp8_linear_epilogue(
         x2.data_ptr(), M > 1 ? x2.stride(0) : K, xs.data_ptr<float>(), w2.data_ptr(), N > 1 ? w2.stride(0) : K,
