@@ -60,10 +60,12 @@ int score_launch(const char* fn, k1::score::FwdParams p, int64_t n_rows, int sms
     return launched(fn, launch_cluster(kern, dim3((unsigned)(n_rows * cluster)), TH, smem, cluster, st, p));
 }
 
+// Threads of a row's block (the same with and without a list, so that both give the same bits).
+int score_threads(int64_t n_rows, int sms) { return n_rows >= 6 * sms ? 128 : 256; }
+
 template <typename T>
 int score_forward(const char* fn, const k1::score::FwdParams& p, int64_t n_rows, int sms, int dev, cudaStream_t st) {
-    // the same work split with and without a list, so that both give the same bits
-    if (n_rows >= 6 * sms)
+    if (score_threads(n_rows, sms) == 128)
         return p.k > 0 ? score_launch<T, 128, 4, 7, true>(fn, p, n_rows, sms, dev, st)
                        : score_launch<T, 128, 4, 7, false>(fn, p, n_rows, sms, dev, st);
     return p.k > 0 ? score_launch<T, 256, 4, 4, true>(fn, p, n_rows, sms, dev, st)
@@ -87,6 +89,11 @@ int score_backward(const char* fn, k1::score::BwdParams p, int64_t n_rows, int s
 }  // namespace
 
 extern "C" {
+
+#ifdef K1_WAIT_TEST
+// Not part of the product: the threads of a row's block, for tests that mean one kernel of them.
+int k1_test_score_threads(int64_t n_rows, int sms) { return score_threads(n_rows, sms); }
+#endif
 
 int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t inner_rows,
                       int64_t inner_stride, int64_t outer_stride, double temperature, const int64_t* token_ids,

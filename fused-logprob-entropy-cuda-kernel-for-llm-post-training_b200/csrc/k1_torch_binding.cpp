@@ -867,7 +867,10 @@ Sandwich sandwich_inputs(const at::Tensor& x, const at::Tensor& residual, const 
         TORCH_CHECK_VALUE(gate.device() == x.device(), "gate must be on x's device");
         const int64_t H = x.size(-1);
         const bool rows = gate.dim() == x.dim() && gate.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
-        if (gate.dim() == 1 && gate.size(0) == H) {
+        // a gate [H] beside a single row [H] may be either: its type says which (column where both fit)
+        const bool element = x.dim() == 1 && gate.scalar_type() != weight.scalar_type() &&
+                             gate.scalar_type() == x.scalar_type();
+        if (gate.dim() == 1 && gate.size(0) == H && !element) {
             a.kind = K1_GATE_COLUMN;
             TORCH_CHECK(gate.scalar_type() == weight.scalar_type(), "a gate per column must have the weights' dtype");
         } else {

@@ -45,7 +45,7 @@ def fused_sandwich_rmsnorm(x: torch.Tensor, residual: torch.Tensor, post_weight:
 
     x, residual: [..., H] as in `fused_residual_rmsnorm`; post_weight, weight: [H] of x's dtype or
     both fp32.  gate: None, [H] of the weights' dtype, or x's leading dimensions with H or 1 columns in
-    x's dtype (other shapes: expand them).  branch_scale, residual_scale: finite numbers.
+    x's dtype (other shapes: expand them; beside a single row [H] its dtype says which it is).  branch_scale, residual_scale: finite numbers.
     Differentiable (once, backwards) in x, residual, both weights and the gate, through y and the
     stream.  Rows of few and of many (more than the device has SMs) are summed in different orders,
     so a row's last bits may depend on which of the two it is in; within either they do not depend
