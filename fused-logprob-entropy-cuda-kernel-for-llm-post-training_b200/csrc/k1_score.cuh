@@ -793,6 +793,9 @@ struct BwdParams {
     int slice;               // vectors per block
 };
 
+// A log-probability whose weight is 0 in fp32, whatever lse_rest (at most 64 where it matters) adds.
+constexpr float kNoWeight = -1024.f;
+
 constexpr int kBwdThreads = 256;
 constexpr int UB = 4;
 
@@ -811,7 +814,8 @@ __device__ __forceinline__ uint4 grad_vector(uint4 v, const BwdRow& q) {
         // d = s x - lse is rounded by 2^-24 of itself; lse's own rounding, which at a low temperature is
         // many times that, is made good in the exponent and in c0
         float2 d = fma2(make_float2(x[2 * i], x[2 * i + 1]), splat(q.s), splat(q.nl));
-        d = make_float2(fmax_nan(d.x, -1e30f), fmax_nan(d.y, -1e30f));
+        // far below the maximum the weight is 0; d stays small, so that its product with s g_H is finite
+        d = make_float2(fmax_nan(d.x, kNoWeight), fmax_nan(d.y, kNoWeight));
         const float2 a = fma2(d, splat(kLog2e), splat(q.nr));
         g[i] = mul2(make_float2(ex2(a.x), ex2(a.y)), fma2(d, splat(-q.ge), splat(q.c0)));
     }
