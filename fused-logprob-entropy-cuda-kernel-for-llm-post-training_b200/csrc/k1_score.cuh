@@ -652,7 +652,8 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
     // a NaN or +inf somewhere: no list either, what cannot be ordered must not reach one
     const bool sound = part.m < INFINITY;
     const double s = (double)p.scale;
-    double l = s * (double)part.m + (p.cluster > 1 ? 0.0 : log(part.z));
+    // log-probabilities are s (x - m) - log Z: beside s m, which a low temperature makes large, log Z would be lost
+    double log_z = p.cluster > 1 ? 0.0 : log(part.z);
     int n = 0;
     if constexpr (TOP) {
         if (sound && kk > 0) {
@@ -669,9 +670,10 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
         }
     }
 
+    auto logprob = [&](float x) { return (float)(s * ((double)x - (double)part.m) - log_z); };
     auto emit = [&](int place, uint64_t key) {
         p.top_ids[r * p.k + place] = (int64_t)(uint32_t)~(uint32_t)key;
-        p.top_logprobs[r * p.k + place] = (float)(s * (double)value_of((uint32_t)(key >> 32)) - l);
+        p.top_logprobs[r * p.k + place] = logprob(value_of((uint32_t)(key >> 32)));
     };
     if (p.cluster == 1) {
         if constexpr (TOP)
@@ -716,7 +718,7 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
             }
         }
         part.m = M;
-        l = s * (double)M + log(part.z);
+        log_z = log(part.z);
         if constexpr (TOP) {
             if (M < INFINITY)
                 for (int i = tid; i < p.cluster * p.k; i += TH) {
@@ -747,17 +749,18 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
 
     // the row's values
     const bool none = part.m == -INFINITY;  // nothing above the floor
+    const double l = s * (double)part.m + log_z;
     const bool fine = !none && part.m < INFINITY && l - l == 0.0;
     if (tid == 0) {
         p.lse[r] = fine ? (float)l : none ? -INFINITY : NAN;
         if (p.lse_rest) p.lse_rest[r] = fine ? (float)(l - (double)(float)l) : 0.f;
-        p.entropy[r] = fine ? (float)(l - s * (double)part.m - s * part.t / part.z) : NAN;
+        p.entropy[r] = fine ? (float)(log_z - s * part.t / part.z) : NAN;
     }
-    if (tid < p.n_ids) p.logprobs[r * p.n_ids + tid] = fine ? (float)(s * (double)xid - l) : NAN;
+    if (tid < p.n_ids) p.logprobs[r * p.n_ids + tid] = fine ? logprob(xid) : NAN;
     for (int i = tid + TH; i < p.n_ids; i += TH) {
         const int64_t e = p.ids[r * p.n_ids + i];
         const float x = row.inside(e) ? DT<T>::load1(row.p + e) : 0.f;
-        p.logprobs[r * p.n_ids + i] = fine ? (float)(s * (double)x - l) : NAN;
+        p.logprobs[r * p.n_ids + i] = fine ? logprob(x) : NAN;
     }
     if constexpr (TOP) {
         if (fine) return;
@@ -799,6 +802,11 @@ constexpr float kNoWeight = -1024.f;
 constexpr int kBwdThreads = 256;
 constexpr int UB = 4;
 
+// From this |lse| on, the values next to a row's maximum m lie 2^-24 |m| s >= 128 or more below it: their
+// weight is 0 in fp32, and those equal to m share it all.  lse and lse_rest together then no longer hold log Z, but
+// they hold m (log Z is at most 21, less than half of fp32's spacing at s m), and the entropy is log Z.
+constexpr float kOnlyMax = 2147483648.f;  // 2^31
+
 // dL/dx of a vector of logits that no list names.
 struct BwdRow {
     float s, nl, nr, c0, ge;  // s, -lse, -lse_rest log2 e, s (g_lse - sum g - g_H (H - lse_rest)), s g_H
@@ -825,6 +833,23 @@ __device__ __forceinline__ uint4 grad_vector(uint4 v, const BwdRow& q) {
     else
         return make_uint4(DT<T>::from_f2(g[0]), DT<T>::from_f2(g[1]), DT<T>::from_f2(g[2 % (E / 2)]),
                           DT<T>::from_f2(g[3 % (E / 2)]));
+}
+
+// Such a row's maximum, and vectors [j0, j1) of its gradient (each element as one: such rows are rare).
+__device__ __forceinline__ float only_max_of(float lse, float rest, float scale) {
+    return (float)(((double)lse + (double)rest) / (double)scale);
+}
+template <typename T>
+__device__ __noinline__ void grad_only_max(const T* p, int64_t vocab, T* out, int j0, int j1, float m, float equal) {
+    constexpr int E = DT<T>::kEPV;
+    const Row<T> row(p, vocab);
+    for (int j = j0 + threadIdx.x; j < j1; j += kBwdThreads) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int64_t e = row.at(j, i);
+            if (row.inside(e)) DT<T>::store1(out + e, DT<T>::load1(p + e) == m ? equal : 0.f);
+        }
+    }
 }
 
 constexpr int kBwdBlocks = 4;
@@ -901,7 +926,11 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks) k1_score_bwd_kernel(B
         for (int j = j0 + tid; j < j1; j += TH) store(j, make_uint4(0, 0, 0, 0));
         return;
     }
-    for (int j = j0; j < j1; j += UB * TH) {
+    const bool only_max = fabsf(lse) >= kOnlyMax && lse - lse == 0.f;  // a low temperature
+    if (only_max)
+        grad_only_max<T>(row.p, p.vocab, out, j0, j1, only_max_of(lse, rest, p.scale),
+                         (float)((double)p.scale * exp(-(double)h) * ((double)gl - sum)));
+    for (int j = only_max ? j1 : j0; j < j1; j += UB * TH) {
         if (whole(j)) {
             uint4 o[UB];
 #pragma unroll
@@ -932,7 +961,10 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdBlocks) k1_score_bwd_kernel(B
             (eq ? mine : others) += (double)gs[o];
         }
         if (!first) continue;
-        const double lp = (double)p.scale * (double)DT<T>::load1(row.p + e) - ((double)lse + (double)rest);
+        const float x = DT<T>::load1(row.p + e);
+        const double lp = !only_max ? (double)p.scale * (double)x - ((double)-q.nl + (double)rest)
+                          : x == only_max_of(lse, rest, p.scale) ? -(double)h
+                                                                 : -INFINITY;
         const double pr = exp(lp);
         double g = mine * -expm1(lp) + pr * ((double)gl - others);
         if (ge != 0.f && pr > 0.0) g -= (double)ge * pr * (lp + (double)h);

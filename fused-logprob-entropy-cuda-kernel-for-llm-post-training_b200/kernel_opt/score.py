@@ -28,8 +28,9 @@ def fused_top_logprobs(logits: torch.Tensor, targets: torch.Tensor | None, k: in
 
     Differentiable (once, backwards) in logits through all but top_ids.  Logits at or below about
     -1e38 are masked: probability 0, after all others.  A row with a NaN or +inf, or with every logit
-    masked, gives ids -1 and NaN (lse -inf where all are masked).  A row whose upstream gradients
-    are all zero gets a zero gradient whatever it holds."""
+    masked, gives ids -1 and NaN (lse -inf where all are masked).  Where a low temperature puts lse
+    beyond fp32's range it is infinite and the gradient NaN.  A row whose upstream gradients are all
+    zero gets a zero gradient whatever it holds."""
     return _C.top_logprobs(logits, targets, k, temperature)
 
 

@@ -502,7 +502,8 @@ int k1_sandwich_rmsnorm_backward(const void* g_y, int64_t g_y_stride, const void
  * [0, min(128, vocab)]; contiguous.  temperature in [1e-30, 1e30].  Values at or below about
  * -1e38 count as masked (probability 0, after all others in the order of x).  A row with a NaN or +inf,
  * or with every value masked, has no distribution: top_ids -1, every output NaN (lse -inf where
- * all is masked).  No workspace.
+ * all is masked).  An lse beyond fp32's range (logits far from 0 at a low temperature) is infinite;
+ * everything else of the forward is right there, and the backward gives NaN.  No workspace.
  */
 int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
                       int64_t inner_rows, int64_t inner_stride, int64_t outer_stride,
@@ -513,7 +514,7 @@ int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t voc
 /*
  * Backward of k1_token_logprobs: d_logits (the logits' dtype, rows d_stride >= vocab elements
  * apart, not the logits' own memory) from the saved lse, lse_rest (NULL: 0; a probability then
- * errs by 2^-24 |lse| of itself) and entropy and the gradients of the outputs, each of which may
+ * errs by 2^-24 |lse| of itself, so pass it where |lse| may be large) and entropy and the gradients of the outputs, each of which may
  * be NULL (none).  Rounded once.  A token that a row's lists name
  * several times gets all their gradients; ids outside [0, vocab) get none of their own.  A row
  * whose gradients are all zero gets zeros, whatever its logits hold.
