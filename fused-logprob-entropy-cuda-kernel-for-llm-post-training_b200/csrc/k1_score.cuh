@@ -68,6 +68,10 @@ struct Floor<float> {
     static constexpr float value = -1.0e38f;
 };
 
+// Differences of values that fp32 has no number for are held to this in sums: of a masked value and a maximum
+// above 2.4e38, say, whose weight, 0, times an infinity would be NaN.
+constexpr float kFar = -3.0e38f;
+
 struct FwdParams {
     const void* logits;
     RowLayout lay;
@@ -268,6 +272,24 @@ struct Row {
         }
     }
 };
+
+// A thread's sum of e d once more, relative to the part's maximum and with differences held to kFar: for logits
+// beyond 1e31, where a difference (or an earlier reference's) was beyond fp32 and the sum is NaN.  Out of the
+// way of all others: held in the loop itself, lists took 1 % longer.
+template <typename T, int TH>
+__device__ __noinline__ double far_sum(const T* p, int64_t vocab, int j0, int j1, float m, float c) {
+    constexpr int E = DT<T>::kEPV;
+    const Row<T> row(p, vocab);
+    double t = 0.0;
+    for (int j = j0 + threadIdx.x; j < j1; j += TH)
+        for (int i = 0; i < E; ++i) {
+            const int64_t e = row.at(j, i);
+            if (!row.inside(e)) continue;
+            const float d = fmax_nan(fmax_nan(DT<T>::load1(p + e), Floor<T>::value) - m, kFar);
+            t += (double)ex2(d * c) * (double)d;
+        }
+    return t;
+}
 
 template <typename T>
 __device__ __forceinline__ void unpack(uint4 v, float (&f)[DT<T>::kEPV]) {
@@ -624,7 +646,7 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
         part.m = value_of(m);
         double z = 0.0, t = 0.0;
         if (!empty) {
-            const float dm = st.m - part.m;
+            const float dm = fmax_nan(st.m - part.m, kFar);
             const double f = dm == 0.f ? 1.f : ex2(dm * c);
             z = f * st.z64();
             t = f * st.t64() + f * (double)dm * st.z64();
@@ -649,6 +671,16 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
         part.t += sums.wt[i];
     }
     part.pad = 0.f;
+    if constexpr (!std::is_same<T, __half>::value) {  // whose values lie close enough
+        if (isnan(part.t) && part.m - part.m == 0.f) {  // uniform
+            const double t = warp_sum(far_sum<T, TH>(row.p, p.vocab, j0, j1, part.m, c));
+            __syncthreads();
+            if (lane == 0) sums.wt[warp] = t;
+            __syncthreads();
+            part.t = 0.0;
+            for (int i = 0; i < TH / 32; ++i) part.t += sums.wt[i];
+        }
+    }
     // a NaN or +inf somewhere: no list either, what cannot be ordered must not reach one
     const bool sound = part.m < INFINITY;
     const double s = (double)p.scale;
@@ -711,7 +743,7 @@ __global__ void __launch_bounds__(TH, MINB) k1_score_kernel(FwdParams p) {
         for (int q = 0; q < p.cluster; ++q) {
             const float m = meet.part[q].m;
             if (m != -INFINITY) {
-                const float dm = m - M;
+                const float dm = fmax_nan(m - M, kFar);
                 const double f = dm == 0.f ? 1.f : ex2(dm * c);
                 part.z += f * meet.part[q].z;
                 part.t += f * meet.part[q].t + f * (double)dm * meet.part[q].z;
