@@ -196,21 +196,36 @@ int skinny_launch(const char* fn, const k1::fp8::Params& p, const void* x, int64
     return launched(fn, launch_cluster(kern, grid, S::THREADS, smem, split, st, tx, tw, p, split));
 }
 
+// Parts of K, each a block of a cluster.  K is split where a third of the SMs or more would stay without a
+// block, until all have one and while every part keeps two blocks of K.  Measured (us, bf16 out):
+// 100 x 3584 x 4096 in 64 / 128 / 256 parts - / 14.0 / 12.0; 200 x 3584 x 3584 in 112 / 224
+// 15.1 / 18.7; 936 x 800 x 1978 in 240 / 480 8.7 / 22.9.
+int linear_split(int64_t blocks, int kb_total, int sms) {
+    int split = 1;
+    if (blocks * 3 < 2 * sms)
+        while (split < 8 && blocks * split < sms && kb_total >= 4 * split) split *= 2;
+    return split;
+}
+
+// Whether a product with an epilogue takes the deeper ring: unsplit blocks of 16 tokens, no more than a block
+// per SM, and more of K than the other ring holds.  Measured (us, bf16 out with bias, 4 stages / 9): 16 x 3584 x
+// 14336 14.4 / 12.8, one token of it 13.7 / 12.2, 16 x 28672 x 14336 81.0 / 69.5, 3 x 1024 x 15000 6.5 / 6.2; but
+// of 4 blocks of K, 16 x 512 x 12800, 4.2 / 4.4, of 32 tokens 16.4 / 16.3, of 64 18.6 / 19.3, 64 x 28672 x 2048
+// 29.3 / 38.8, and with K split 16 x 1040 x 4100 6.2 / 6.7, 37 x 2048 x 1000 6.4 / 6.6.
+bool deep_ring(int tokens_per_block, int64_t blocks, int kb_total, int split, int sms) {
+    return tokens_per_block == 16 && split == 1 && blocks <= sms && kb_total > 4;
+}
+
 template <int TN, typename OutT, bool EPI>
 int skinny(const char* fn, const k1::fp8::Params& p, const void* x, int64_t ldx, const void* w, int64_t ldw,
            int64_t inner, int sms, int dev, cudaStream_t st) {
-    const int64_t tiles = (p.n + 127) / 128, tok = (p.m + TN - 1) / TN;
-    // K is split over a cluster where a third of the SMs or more would stay without a block,
-    // until all have one and while every part keeps two blocks of K.  Measured (us, bf16 out):
-    // 100 x 3584 x 4096 in 64 / 128 / 256 parts - / 14.0 / 12.0; 200 x 3584 x 3584 in 112 / 224
-    // 15.1 / 18.7; 936 x 800 x 1978 in 240 / 480 8.7 / 22.9.
-    int split = 1;
-    if (tiles * tok * 3 < 2 * sms)
-        while (split < 8 && tiles * tok * split < sms && p.kb_total >= 4 * split) split *= 2;
-    // few blocks: a deeper ring, where the scales leave room for it
-    if constexpr (EPI)
-        if (tiles * tok * split <= sms && k1::fp8::Skinny<TN, true>::smem((p.kb_total + split - 1) / split) <= 227 * 1024)
+    const int64_t blocks = (p.n + 127) / 128 * ((p.m + TN - 1) / TN);
+    const int split = linear_split(blocks, p.kb_total, sms);
+    if constexpr (EPI && TN == 16) {
+        static_assert(k1::fp8::Skinny<TN, true>::smem(kMaxInner / 128) <= 227 * 1024, "room for the scales of the longest rows");
+        if (deep_ring(TN, blocks, p.kb_total, split, sms))
             return skinny_launch<TN, OutT, EPI, true>(fn, p, x, ldx, w, ldw, inner, split, dev, st);
+    }
     return skinny_launch<TN, OutT, EPI, false>(fn, p, x, ldx, w, ldw, inner, split, dev, st);
 }
 
@@ -341,6 +356,13 @@ extern "C" {
 // Which kernel a product takes on a device of `sms` SMs, so that a test knows which one it tests.
 int k1_test_linear_kernel(int64_t tokens, int64_t inner, int64_t outer, int sms) {
     return linear_kernel(tokens, outer, (int)((inner + 127) / 128), sms);
+}
+// Whether, with an epilogue, it takes the deeper ring.
+int k1_test_linear_deep(int64_t tokens, int64_t inner, int64_t outer, int sms) {
+    const int kb_total = (int)((inner + 127) / 128), tn = linear_kernel(tokens, outer, kb_total, sms);
+    if (tn == 0) return 0;
+    const int64_t blocks = (outer + 127) / 128 * ((tokens + tn - 1) / tn);
+    return deep_ring(tn, blocks, kb_total, linear_split(blocks, kb_total, sms), sms);
 }
 #endif
 

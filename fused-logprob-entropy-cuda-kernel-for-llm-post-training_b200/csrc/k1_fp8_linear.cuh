@@ -213,8 +213,8 @@ __device__ __forceinline__ float residual_of(const Params& p, int64_t row, int64
 // ------------------------------------------------------------------------------------
 // Few tokens
 // ------------------------------------------------------------------------------------
-// DEEP: a ring of 9 stages instead of 4, for launches of no more than a block per SM, where one ring has
-// to keep the weight coming (16 x 3584 x 14336: 14.1 -> 12.9 us).
+// DEEP: a ring of 9 stages instead of 4, for launches of no more than a block of 16 tokens per SM, where one
+// ring has to keep the weight coming (figures at the rule, deep_ring in k1_decode_capi.cu).
 template <int TN, bool DEEP = false>
 struct Skinny {
     static constexpr int W_BYTES = BM * BK;           // 16 KB
