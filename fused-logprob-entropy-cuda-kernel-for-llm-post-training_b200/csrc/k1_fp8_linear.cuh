@@ -167,7 +167,10 @@ struct Params {
 enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
 
 // The activation in fp32, in forms that keep relative accuracy in the tails that go to 0.  What is
-// rounded to 16 bits takes the fast exponential and quotient (both right to about 2^-21 there).
+// rounded to 16 bits takes the fast exponential, whose result errs by 2 + 1.17 |u| units of 2^-23 (2^-22 at 0,
+// below 2^-16 at |u| = 88, where half a step of bf16 is 2^-9 and of fp16 2^-12 of the value), and the fast
+// quotient (2 units).  Below u = -87.3 that quotient is 0: the value is less than 1e-36 there, which is 0 in fp16
+// and in bf16 next to nothing of what a residual or a following product adds to it.
 template <int ACT, bool FAST>
 __device__ __forceinline__ float activate(float v) {
     if constexpr (ACT == ACT_RELU) {

@@ -1,19 +1,23 @@
-// k1_sandwich.cuh -- gradient of the norms around a block's end: the norm of the block's output,
-// its gate and scales, the residual addition, and the norm in front of the next block.
+// k1_sandwich.cuh -- the norms around a block's end: the norm of the block's output, its gate and
+// scales, the residual addition, and the norm in front of the next block; and their gradient.
 //
 //   R1 = 1 / sqrt(mean(x^2) + eps),  m = x R1,  b = m wp gate
 //   s = T(rs r + bs b)                            the residual stream, as stored
 //   R2 = 1 / sqrt(mean(s^2) + eps),  n = s R2,  y = T(n w)
-//   (the forward is k1_rmsnorm_kernel with POST: k1_norm.cuh)
+//   (k1_sandwich_ring_kernel below for many rows of whole vectors, else k1_rmsnorm_kernel with POST:
+//   k1_norm.cuh)
 //
 //   ds = R2 (gy w - n c2) + gs,  c2 = mean(gy w n);      dr = T(rs ds),  dw = sum over rows of gy n
 //   u = bs ds;  dgate = u m wp (summed over rows, or over the row, where the gate is broadcast)
 //   t = u gate wp,  c1 = mean(t m);  dx = T(R1 (t - m c1)),  dwp = sum over rows of u gate m
 //
-// ds stays in fp32 from the stream's gradient to the branch's.  Layout as in the norm's own backward:
-// a block of threads owns a row at a time, a thread the same columns for every row.  Sums over rows
-// (up to three per column) are kept in shared memory, where only their thread touches them, and
-// written as one partial row per block; a second kernel adds the blocks' partials in block order.
+// ds stays in fp32 from the stream's gradient to the branch's.  Sums over rows are two per column whatever
+// the gate, since dwp and a column gate's gradient are multiples of one.
+//
+// k1_sandwich_bwd_kernel, for few rows and for widths without whole vectors: layout as in the norm's own
+// backward, a block of threads owns a row at a time, a thread the same columns for every row.  The
+// sums over rows are kept in shared memory, where only their thread touches them, and written as one partial
+// row per block; a second kernel adds the blocks' partials in block order.
 // Bound by traffic: gy, gs, s, x in, dr, dx out (and a gate per element in, its gradient out).
 #pragma once
 
@@ -236,8 +240,9 @@ __global__ void __launch_bounds__(kThreads<E>) k1_sandwich_bwd_kernel(SandwichBw
 // and 53 forward with 8-bit output).  Here a block is a few groups of threads, each with rows and a ring
 // of stages of its own: a stage holds one row of every input, a bulk copy each, counted on the stage's
 // mbarrier.  When a group has read a stage (which the row's second reduction, a barrier of the group,
-// tells), one thread orders the group's next row into it.  So 100 KB and more per SM are in flight
-// whatever the groups wait for.  Columns are summed in pairs, so a row's last bits may differ from those
+// tells), one thread orders the group's next row into it.  So 112 to 168 KB per SM are in flight
+// whatever the groups wait for (bf16, forward with two inputs and backward with four; 96 forward at 2048, and 60
+// and 120 at 256, the shortest rows).  Columns are summed in pairs, so a row's last bits may differ from those
 // of the other kernels, which keep the order of the norms without POST (from the stored stream on their
 // y is the residual norm's): one by one the sums would cost the packed arithmetic.  Sums over rows stay
 // in registers and are added over the groups, in their order, at the end; the weights are in shared

@@ -28,8 +28,13 @@
 // Forward and backward are bound by traffic where rows are many and wide; small calls by latency, and
 // lists by the chain of short phases behind a row's last load.  Measured on B200 (us, with the call):
 // 2048 x 151936 bf16, 32 given tokens, forward 108 (5.8 TB/s) and backward 211 (5.9 TB/s), 323 to 335
-// together; 1024 x 128256 bf16 top 8 with gradient 148; 512 x 152064 bf16 top 20 38 to 39 (32 without a
-// list, its bytes 24); 1023 x 50257 fp16 top 64 33 (22 without, 16); one row of 151936 top 20 11.
+// together; 1024 x 128256 bf16 top 8 with gradient 149 to 153; 512 x 152064 bf16 top 20 38 to 39 (32 without a
+// list, its bytes 24); 1023 x 50257 fp16 top 64 32 to 33 (22 without, 16); one row of 151936 top 20 11.
+//
+// Two ways are slow, and right.  A list where a mask leaves fewer than k in a block's part takes the exact
+// selection: 512 x 152064 bf16 with 50 tokens left 480.  The backward stores single elements where a row of the
+// gradient starts at another place of a 16-byte vector than its logits (a window of a wider head, odd
+// vocabularies): 1024 x 50257 of 50304 columns 162, all columns of 50257 45.
 #pragma once
 
 #include <cstddef>

@@ -135,8 +135,8 @@ int k1_token_logprobs_backward(const void* logits, int dtype, int64_t n_rows, in
                                int64_t inner_stride, int64_t outer_stride, double temperature,
                                const int64_t* token_ids, int64_t n_ids, const float* g_logprobs,
                                const int64_t* top_ids, int64_t k, const float* g_top, const float* lse,
-                               const float* lse_rest, const float* entropy, const float* g_entropy, const float* g_lse, void* d_logits,
-                               int64_t d_stride, void* stream) {
+                               const float* lse_rest, const float* entropy, const float* g_entropy,
+                               const float* g_lse, void* d_logits, int64_t d_stride, void* stream) {
     const char* fn = "k1_token_logprobs_backward";
     int rc = score_check(fn, logits, dtype, n_rows, vocab, inner_rows, inner_stride, outer_stride, temperature, n_ids, k);
     if (rc) return rc;

@@ -1096,7 +1096,8 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
             logits.data_ptr(), dtype_code(logits), L.n_rows, L.vocab, L.inner_rows, L.inner_stride, L.outer_stride,
             ctx->saved_data["temperature"].toDouble(), ids.defined() ? ids.data_ptr<int64_t>() : nullptr,
             ids.defined() ? ids.size(-1) : 0, ptr(g_ids), top_ids.defined() ? top_ids.data_ptr<int64_t>() : nullptr,
-            top_ids.defined() ? top_ids.size(-1) : 0, ptr(g_top), lse.data_ptr<float>(), ptr(rest), entropy.data_ptr<float>(), ptr(g_ent), ptr(g_lse), d.data_ptr(), L.vocab,
+            top_ids.defined() ? top_ids.size(-1) : 0, ptr(g_top), lse.data_ptr<float>(), ptr(rest),
+            entropy.data_ptr<float>(), ptr(g_ent), ptr(g_lse), d.data_ptr(), L.vocab,
             at::cuda::getCurrentCUDAStream().stream()));
         return {d, none, none, none};
     }

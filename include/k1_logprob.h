@@ -106,7 +106,7 @@ size_t k1_forward_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int 
  *   logprob, entropy, lse : n_rows fp32 each, contiguous (written)
  * One streaming read of the logits; every thread block gets an equal share of the
  * flattened row x vocab range, so few rows (split-vocab) and many rows use the same
- * kernel.
+ * kernel.  Finite logits may be up to 1e31 in size; above, the entropy (and its gradient) may be NaN.
  */
 int k1_fused_logprob_entropy_v1(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
                                 int64_t inner_rows, int64_t inner_stride, int64_t outer_stride,
@@ -514,8 +514,8 @@ int k1_token_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t voc
 /*
  * Backward of k1_token_logprobs: d_logits (the logits' dtype, rows d_stride >= vocab elements
  * apart, not the logits' own memory) from the saved lse, lse_rest (NULL: 0; a probability then
- * errs by 2^-24 |lse| of itself, so pass it where |lse| may be large) and entropy and the gradients of the outputs, each of which may
- * be NULL (none).  Rounded once.  A token that a row's lists name
+ * errs by 2^-24 |lse| of itself, so pass it where |lse| may be large) and entropy and the gradients
+ * of the outputs, each of which may be NULL (none).  Rounded once.  A token that a row's lists name
  * several times gets all their gradients; ids outside [0, vocab) get none of their own.  A row
  * whose gradients are all zero gets zeros, whatever its logits hold.
  */
